@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define MLLM_ABI_VERSION 5
+#define MLLM_ABI_VERSION 6
 
 #define MLLM_OK 0
 #define MLLM_ERR_INVALID (-1)
@@ -37,6 +37,11 @@ extern "C" {
 #define MLLM_DTYPE_F32 0
 #define MLLM_DTYPE_F16 1
 #define MLLM_DTYPE_BF16 2
+
+/* pool types: elements of `dtype`, fp8 e4m3fn with one scale per tensor, 4 bits with block scales */
+#define MLLM_POOL_16BIT 0
+#define MLLM_POOL_FP8 1
+#define MLLM_POOL_FP4 2
 
 /* ABI version of the loaded library (MLLM_ABI_VERSION at build time). */
 int mllm_abi_version(void);
@@ -267,7 +272,8 @@ typedef struct mllm_layer_step {
   int32_t pages_per_split, q_tile_tokens;
   int32_t num_heads, num_kv_heads, head_dim, block_size;
   int32_t dtype;               /* q, k, v, cos, sin, q_rot, out: MLLM_DTYPE_BF16 or MLLM_DTYPE_F16 */
-  int32_t kv_fp8;              /* 0: pools of `dtype`; 1: fp8 e4m3fn pools with k_scale / v_scale */
+  int32_t kv_fp8;              /* MLLM_POOL_*: 0 pools of `dtype`; 1 fp8 e4m3fn pools with k_scale / v_scale; 2 4-bit pools
+                                  (mllm_attention_forward_pool) */
   float softmax_scale;
 } mllm_layer_step;
 
@@ -412,6 +418,110 @@ int mllm_paged_prefill_fp8(const void* q, int64_t q_stride_tok, int64_t q_stride
                            int32_t num_prefill_work, int32_t q_tile_tokens, float softmax_scale, int32_t dtype,
                            float k_scale, float v_scale, void* out, int64_t out_stride_tok, int64_t out_stride_head,
                            void* stream);
+
+/*
+ * 4-bit KV pool.  No counterpart in the reference's code; a further step of its planned quantized KV cache
+ * (docs/distributed_inference_plan.md:310): 136 bytes per token and head of 128 dims for K and V together, against 256
+ * in fp8 and 512 in 16 bits.  OCP microscaling: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives), two to a byte with
+ * the even dim in the low half, and one e8m0 scale for 32 consecutive dims of a token and head.
+ *   codes     [num_blocks, block_size, Hkv, Dh / 2] bytes
+ *   k_scales  [num_blocks, block_size, Hkv, Dh / 32] bytes
+ *   v_scales  [num_blocks, Hkv, Dh / 32, block_size] bytes
+ *   value = e2m1(code) * 2^(scale - 127); scale 255: NaN
+ * A block is stored under the least power of two below which its largest magnitude rounds to at most 6 (its magnitude is
+ * less than 7 times the scale), kept within the exponents whose values the 16-bit type holds (bf16: 1 .. 252, fp16:
+ * 104 .. 140; above, magnitudes saturate), each element rounded to the nearest code with ties to even.  A block that
+ * holds an infinity or a NaN gets scale 255.  Every step is exact but the rounding.  A pool is written and read with one
+ * 16-bit type: fp16 does not hold every block that bf16 rows fill.
+ */
+
+/* KV append into a 4-bit pool: rows and slots as mllm_kv_append_fp8, head_dim a multiple of 32.  Tokens that share a slot leave
+ * it undefined. */
+int mllm_kv_append_fp4(const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                       int64_t v_stride_tok, int64_t v_stride_head, int32_t src_dtype, void* k_cache, void* v_cache,
+                       void* k_scales, void* v_scales, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+                       int32_t head_dim, const int64_t* slot_mapping, int64_t num_tokens, void* stream);
+
+/* Rows slots[num_slots] of a 4-bit pool as values of `dtype`: k_out, v_out [num_slots, Hkv, Dh], contiguous.  A slot outside the
+ * pool reads as zeros. */
+int mllm_kv_read_fp4(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+                     int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                     const int64_t* slots, int64_t num_slots, int32_t dtype, void* k_out, void* v_out, void* stream);
+
+/* mllm_paged_decode over a 4-bit pool; mllm_merge_splits combines its partials unchanged.  Codes and scales 16-byte aligned. */
+int mllm_paged_decode_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                          const void* v_cache, const void* k_scales, const void* v_scales, int64_t num_blocks,
+                          int32_t block_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                          const int32_t* kv_indices, const int32_t* decode_work, int32_t num_decode_work,
+                          int32_t num_merge_work, int32_t pages_per_split, float softmax_scale, int32_t dtype,
+                          void* out, int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* mllm_paged_prefill over a 4-bit pool. */
+int mllm_paged_prefill_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                           const void* v_cache, const void* k_scales, const void* v_scales, int64_t num_blocks,
+                           int32_t block_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                           const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                           const int32_t* seq_lens, const int32_t* prefill_work, int32_t num_prefill_work,
+                           int32_t q_tile_tokens, float softmax_scale, int32_t dtype, void* out,
+                           int64_t out_stride_tok, int64_t out_stride_head, void* stream);
+
+/* The arguments of mllm_qk_norm_rope_kv_append: those of mllm_rope_kv_append / _fp8, the pool's type and block scales. */
+typedef struct mllm_rope_append {
+  const void *q, *k, *v;       /* [N, heads, Dh], element strides (tok, head), rows 16-byte aligned */
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head;
+  const void *cos, *sin;       /* [N, Dh] rows */
+  int64_t cs_stride_tok;
+  void* q_out;
+  int64_t q_out_stride_tok, q_out_stride_head;
+  void *k_cache, *v_cache;
+  void *k_scales, *v_scales;   /* MLLM_POOL_FP4 */
+  float k_scale, v_scale;      /* MLLM_POOL_FP8 */
+  int64_t num_blocks;
+  const int64_t* slot_mapping; /* [N]; slots outside the pool are not written */
+  int64_t num_tokens;
+  int32_t block_size, num_heads, num_kv_heads, head_dim;
+  int32_t dtype;               /* q, k, v, cos, sin, norms, q_out */
+  int32_t pool;                /* MLLM_POOL_* */
+} mllm_rope_append;
+
+/*
+ * RMSNorm of each query and key head (weights q_norm, k_norm [Dh]) with the model's RoPE and the append in one launch; no
+ * counterpart in the reference, whose q and k are not normed:
+ *   y = x * rsqrt(mean(x^2) + eps) * w,  q_out / pool row = y * cos + rotate_half(y) * sin,  v copied (or quantized)
+ * in fp32 with one rounding to `dtype`; fp8 and 4-bit pools quantize the rounded k and v as their appends do.  Without norms
+ * (both NULL, 4-bit pools only): mllm_rope_kv_append's rotation.  head_dim a multiple of 16 (4-bit pools: 64), at most 1024.
+ */
+int mllm_qk_norm_rope_kv_append(const mllm_rope_append* args, const void* q_norm, const void* k_norm, float eps,
+                                void* stream);
+
+/* The same on contiguous tensors, without a pool: q [B, H, T, Dh], k [B, Hkv, T, Dh] with element strides (batch, head,
+ * token), cos / sin rows with strides (batch, token) -> q_out, k_out, contiguous [B, heads, T, Dh]. */
+int mllm_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
+                      int64_t k_st, const void* cos, const void* sin, int64_t cs_sb, int64_t cs_st, const void* q_norm,
+                      const void* k_norm, float eps, int32_t batch, int32_t seq, int32_t num_heads,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void* q_out, void* k_out, void* stream);
+
+/* A layer's pools and head norms, for the entry points below. */
+typedef struct mllm_layer_pool {
+  void *k_cache, *v_cache;
+  void *k_scales, *v_scales;      /* 4-bit pools */
+  float k_scale, v_scale;         /* fp8 pools; 1 otherwise */
+  const void *q_norm, *k_norm;    /* head norm weights [Dh], or both NULL; they need cos and sin */
+  float norm_eps;
+} mllm_layer_pool;
+
+/* mllm_attention_forward and mllm_decoder_layer over any pool type, with head norms where given (mllm_qk_norm_rope_kv_append). */
+int mllm_attention_forward_pool(const mllm_layer_step* step, const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                                int64_t v_stride_tok, int64_t v_stride_head, const void* cos, const void* sin,
+                                int64_t cs_stride_tok, void* q_rot, const mllm_layer_pool* pool, void* out,
+                                void* stream);
+int mllm_decoder_layer_pool(const mllm_layer_step* step, const void* x, int64_t hidden, const void* norm1, float eps1,
+                            const void* wq, const void* wk, const void* wv, const void* wo, const void* norm2,
+                            float eps2, const void* gate, const void* up, const void* down, int64_t ffn,
+                            const void* cos, const void* sin, int64_t cs_stride_tok, const mllm_layer_pool* pool,
+                            void* scratch, int64_t scratch_bytes, void* out, void* stream);
 
 #ifdef __cplusplus
 }

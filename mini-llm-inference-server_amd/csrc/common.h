@@ -108,6 +108,74 @@ __device__ __forceinline__ u32x4 fp8x8_to(uint32_t w0, uint32_t w1) {
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
+// ---------------------------------------------------------------- 4-bit KV pool (OCP MX: e2m1 codes, e8m0 scales)
+// A code is 1 sign, 2 exponent (bias 1) and 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, two codes to
+// a byte with the even dim in the low half.  32 consecutive dims of a token and head share one power-of-two scale
+// 2^(e - 127), stored as its exponent e; 255 marks a block that held an infinity or a NaN and reads as NaN.
+
+struct FP4 {};  // pool storage tag
+constexpr int kFp4Block = 32;  // dims per scale
+
+// Scale exponents whose values, up to 6 2^(e - 127), the 16-bit type holds exactly.
+template <typename T>
+struct Fp4Range;
+template <>
+struct Fp4Range<BF16> {
+  static constexpr int lo = 1, hi = 252;
+};
+template <>
+struct Fp4Range<F16> {
+  static constexpr int lo = 104, hi = 140;
+};
+
+// The scale exponent of a block whose largest magnitude is `amax` (fp32, not negative): the least power of two under
+// which amax rounds to at most 6, i.e. lies below 7.  floor(log2 amax) - 2 puts it in [4, 8); adding a quarter of
+// the mantissa carries into the exponent from 1.75 on.  With floor alone amax in [7, 8) would saturate, up to a quarter off.
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_scale_exp(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u >= 0x7f800000u) return 255u;
+  const int e = (int)((u + 0x200000u) >> 23) - 2;
+  return (uint32_t)min(max(e, Fp4Range<T>::lo), Fp4Range<T>::hi);
+}
+// The conversions' scale operand: they read bits 30:23 only, and take 255 as NaN.
+__device__ __forceinline__ float e8m0_to_f32(uint32_t e) { return __uint_as_float(e << 23); }
+
+// Eight e2m1 codes (one dword) -> eight 16-bit values, exact within Fp4Range.
+template <typename T>
+__device__ __forceinline__ u32x4 fp4x8_to(uint32_t w, float scale);
+template <>
+__device__ __forceinline__ u32x4 fp4x8_to<BF16>(uint32_t w, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+template <>
+__device__ __forceinline__ u32x4 fp4x8_to<F16>(uint32_t w, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+}
+// Eight 16-bit values -> eight codes of x / scale, to nearest with ties to even, saturated at 6.
+template <typename T>
+__device__ __forceinline__ uint32_t fp4x8_from(u32x4 x, float scale);
+template <>
+__device__ __forceinline__ uint32_t fp4x8_from<BF16>(u32x4 x, float scale) {
+  uint32_t r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf16x2, (uint32_t)x[0]), scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, (uint32_t)x[1]), scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, (uint32_t)x[2]), scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, (uint32_t)x[3]), scale, 3);
+}
+template <>
+__device__ __forceinline__ uint32_t fp4x8_from<F16>(u32x4 x, float scale) {
+  uint32_t r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(0u, __builtin_bit_cast(f16x2, (uint32_t)x[0]), scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, (uint32_t)x[1]), scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, (uint32_t)x[2]), scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, (uint32_t)x[3]), scale, 3);
+}
+
 // Packs two floats into one dword of 16-bit values (lo in bits 0-15), rounding to nearest even with
 // the hardware conversion (v_cvt_pk_bf16_f32 / v_cvt_pk_f16_f32 on gfx950).  For the attention
 // kernels' P tiles and outputs; KV append keeps the bit-level conversion above, whose NaN encoding

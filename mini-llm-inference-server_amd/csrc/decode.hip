@@ -31,12 +31,11 @@
 #include <mutex>
 #include <string>
 
-#include "common.h"
+#include "decode_common.h"
 
 namespace mllm {
 namespace {
 
-constexpr int kHeadDim = 128;
 constexpr int kWaves = 4;  // KV heads per workgroup of the decode kernel on small steps
 // Whole-page decode (16-bit pools): one workgroup of 8 wavefronts reads all 8 KV heads of a bin's pages,
 // each 16-token page of the pool one contiguous 32 KB run, at 2 wavefronts per SIMD: one workgroup per CU.
@@ -81,21 +80,6 @@ struct DecodeArgs {
   float2* part_ml;
 };
 
-template <bool NT>
-__device__ __forceinline__ u32x4 ldkv(const char* p) {
-  if constexpr (NT)
-    return ld16_nt(p);
-  else
-    return ld16(p);
-}
-template <bool NT>
-__device__ __forceinline__ u32x2 ldkv8(const char* p) {
-  if constexpr (NT)
-    return __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
-  else
-    return ld8(p);
-}
-
 // The registers of one loaded 16-token tile, as the pool stores it.
 template <bool F8>
 struct TileRegs {  // 16-bit pool: K row c at dims 32 kk + 8 g .. +7; V rows 4 g + i at dims 8 c .. 8 c + 7
@@ -112,35 +96,6 @@ struct TileRegs<true> {  // fp8 pool: K row c at dims 64 h + 16 g .. +15; V rows
 template <bool F8>
 __device__ __forceinline__ int qk_dim0(int kk, int g) {
   return F8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
-}
-
-// The next 16-token tile to load: its page within the segment and its 16-token slice of that page (tiles
-// are loaded in order, once each, so a counter replaces a division by the tiles per page).
-struct LoadCursor {
-  int page = 0, sub = 0;
-  __device__ __forceinline__ void advance(int tpp) {
-    if (++sub == tpp) {
-      sub = 0;
-      ++page;
-    }
-  }
-};
-
-// A segment's page ids, one per lane in three registers: pages 0-63, 64-127 and 128-191 of the segment
-// (a bin holds at most kMaxSplitPages pages).
-constexpr int kMaxSplitPages = 192;
-struct PageIds {
-  int r[3];
-};
-__device__ __forceinline__ PageIds load_page_ids(const int32_t* kv_indices, const int4& r0, int lane) {
-  PageIds p;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) p.r[i] = lane + 64 * i < r0.y ? kv_indices[r0.x + 64 * i + lane] : 0;
-  return p;
-}
-// Page `page` (wave-uniform) of the segment.
-__device__ __forceinline__ int page_id(const PageIds& p, int page) {
-  return __builtin_amdgcn_readlane(page < 64 ? p.r[0] : (page < 128 ? p.r[1] : p.r[2]), page & 63);
 }
 
 // Loads the 16-token tile at `at` of this wave's page range (lane (c, g); kbase/vbase: this head's bytes
@@ -231,24 +186,6 @@ __device__ __forceinline__ void consume_tile(const u32x4 (&ka)[4], u32x4 (&va)[4
     const u32x2 vfrag = u32x2{pick_halves(va[0][dw], hf, va[1][dw], hf), pick_halves(va[2][dw], hf, va[3][dw], hf)};
     o[m] = Mfma<T>::m16x16x16(vfrag, pfrag, o[m]);
   }
-}
-
-// The records of one segment of a bin (the plan's layout): r0 = {first page in kv_indices, pages, first
-// page within the row, row length}, r1 = {q row, partial slot or -1, sequence, 0}.
-struct SegRec {
-  int4 r0, r1;
-};
-// The plan is read through the constant address space: it does not change during the launch, so its
-// uniform records become scalar loads, which the wave waits for with lgkmcnt apart from the vector
-// loads of K, V and q (read as global memory, a record would be a vector load, and waiting for it would
-// wait for every vector load issued before it).
-typedef const __attribute__((address_space(4))) int PlanInt;
-__device__ __forceinline__ int4 plan_rec(const int4* work, int i) {
-  const PlanInt* p = (const PlanInt*)(work + i);
-  return make_int4(p[0], p[1], p[2], p[3]);
-}
-__device__ __forceinline__ SegRec seg_rec(const int4* segs, int g) {
-  return SegRec{plan_rec(segs, 2 * g), plan_rec(segs, 2 * g + 1)};
 }
 
 // One wavefront per (bin, KV head) streams the bin's segments back to back, one 16-token tile ahead.
@@ -694,14 +631,6 @@ constexpr int kOccupancyPair = MLLM_DECODE_PAIR_OCC;
 __host__ __device__ constexpr bool pair_heads(int num_kv_heads, int group) {
   return num_kv_heads % 2 == 0 && 2 * group <= 16;
 }
-
-// Bins a plan of n_work records can hold: a header, then per bin one record and at least one segment
-// of two records.  The grid covers that many bins; the workgroups past the step's own exit at once.
-constexpr int max_bins(int n_work) { return n_work >= 4 ? (n_work - 1) / 3 : 0; }
-// Partial slots a plan of n_work records can use: a cut row takes one slot per segment, and the segments
-// take two records each after the header, so slots <= segments <= (n_work - 1) / 2.  The workspace holds
-// that many slots: acc[slot][head][Dh], then (m, l)[slot][head].
-constexpr int partial_slots(int n_work) { return n_work >= 1 ? (n_work - 1) / 2 : 0; }
 
 template <typename T, bool F8>
 int launch(const DecodeArgs& a, int n_work, int pages_per_split, hipStream_t st) {

@@ -11,39 +11,10 @@
 // and one for V; a thread quantizes 16 elements into one 16-byte pool chunk.
 #include <type_traits>
 
-#include "common.h"
+#include "kv_common.h"
 
 namespace mllm {
 namespace {
-
-template <typename T>
-__device__ __forceinline__ float to_f32(uint16_t b) {
-  if constexpr (std::is_same<T, BF16>::value)
-    return bf16_bits_to_f32(b);
-  else
-    return f16_bits_to_f32(b);
-}
-template <typename T>
-__device__ __forceinline__ uint16_t from_f32(float f) {
-  if constexpr (std::is_same<T, BF16>::value)
-    return f32_to_bf16_bits(f);
-  else
-    return f32_to_f16_bits(f);
-}
-
-// Four 16-bit values (two dwords) -> four e4m3fn bytes of x * inv.
-template <typename T>
-__device__ __forceinline__ uint32_t quant4(uint32_t w0, uint32_t w1, float inv) {
-  return f32_to_e4m3fn_bits(to_f32<T>((uint16_t)w0) * inv) |
-         (f32_to_e4m3fn_bits(to_f32<T>((uint16_t)(w0 >> 16)) * inv) << 8) |
-         (f32_to_e4m3fn_bits(to_f32<T>((uint16_t)w1) * inv) << 16) |
-         (f32_to_e4m3fn_bits(to_f32<T>((uint16_t)(w1 >> 16)) * inv) << 24);
-}
-// Eight 16-bit values (16 bytes) -> eight e4m3fn bytes.
-template <typename T>
-__device__ __forceinline__ u32x2 quant8(u32x4 x, float inv) {
-  return u32x2{quant4<T>(x[0], x[1], inv), quant4<T>(x[2], x[3], inv)};
-}
 
 __global__ __launch_bounds__(256) void kv_append_vec_kernel(const char* __restrict__ k, int64_t k_st, int64_t k_sh,
                                                            const char* __restrict__ v, int64_t v_st, int64_t v_sh,
@@ -248,22 +219,6 @@ extern "C" int mllm_kv_append_fp8(const void* k, int64_t k_stride_tok, int64_t k
 
 namespace mllm {
 namespace {
-
-// round(round(x c) + round(r s)) in the 16-bit type.  The rounded products pass through an empty asm:
-// for fp16 the compiler narrows these float ops to native half arithmetic and would otherwise fuse the
-// first product into the sum's fma, skipping that product's own rounding.
-template <typename T>
-__device__ __forceinline__ uint16_t rot1(uint16_t x, uint16_t c, float r, uint16_t s) {
-  float a = to_f32<T>(from_f32<T>(to_f32<T>(x) * to_f32<T>(c)));
-  float b = to_f32<T>(from_f32<T>(r * to_f32<T>(s)));
-  asm volatile("" : "+v"(a), "+v"(b));
-  return from_f32<T>(a + b);
-}
-
-union Chunk {
-  u32x4 v;
-  uint16_t e[8];
-};
 
 // Q8: the pool is e4m3fn: the rotated k (rounded to T, as the unfused sequence stores it before the
 // append) and v are quantized with k_inv / v_inv, 8 bytes per half row instead of 16.

@@ -35,6 +35,8 @@
 // is folded into the softmax scale and v_scale into the output.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace mllm {
@@ -59,6 +61,7 @@ struct PrefillArgs {
   const int4* work;  // the plan's prefill records, two int4 each (see the kernel)
   float scale_log2;  // softmax scale x k_scale x log2(e)
   float v_scale;     // output scale of an fp8 pool
+  const uint8_t *ks, *vs;  // block scales of a 4-bit pool (kv_fp4.hip)
   uint16_t* out;
   int64_t o_st, o_sh;
 };
@@ -105,27 +108,68 @@ __device__ __forceinline__ void dma_tile(const char* pool, const PrefillArgs& a,
   }
 }
 
-// fp8 pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7, 128 bytes each) is one 16-byte load
-// per lane: row 8 w + l / 8, dims 16 (l % 8) .. +15.  off: the lane's offset from the group base for a
-// full tile.  Keys past `last` load the row of `last`, as in dma_tile.
-__device__ __forceinline__ u32x4 stage_load(const char* pool, const PrefillArgs& a, int blk, int kv0, int last,
-                                            int kv_end, int w, unsigned off, unsigned head_bytes, int lane) {
-  if (kv0 + kBN <= kv_end) return ld16(group_base(pool, a, blk, kv0 + 16 * (w >> 1)) + off);
-  const int r = 8 * w + (lane >> 3);
-  const unsigned slot_bytes = (unsigned)(min(kv0 + r, last) & (a.bs - 1)) * (unsigned)a.row_bytes;
-  return ld16(group_base(pool, a, blk, 0) + (slot_bytes + head_bytes + 16u * (lane & 7)));
+// What the pool holds, and with it the way of a tile into LDS: DMA, or through registers to be widened.
+enum Pool { kPool16 = 0, kPoolFp8 = 1, kPoolFp4 = 2 };
+constexpr int head_row_bytes(int pool) { return pool == kPool16 ? 2 * kHeadDim : (pool == kPoolFp8 ? kHeadDim : kHeadDim / 2); }
+
+// One lane's 16 values of a tile on their way through registers.
+template <int POOL>
+struct Staged {
+  u32x4 x;
+};
+template <>
+struct Staged<kPoolFp4> {
+  u32x2 x;
+  uint32_t e;  // their block's scale
+};
+
+// fp8 and 4-bit pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7) is one load of 16 values per
+// lane: row 8 w + l / 8, dims 16 (l % 8) .. +15.  off: the lane's offset from the group base for a full
+// tile.  Keys past `last` load the row of `last`, as in dma_tile.
+template <int POOL, bool IS_V>
+__device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const PrefillArgs& a, int blk, int kv0, int last,
+                                                   int kv_end, int w, unsigned off, unsigned head_bytes, int lane) {
+  constexpr unsigned kLane = POOL == kPoolFp8 ? 16 : 8;  // bytes of 16 values
+  const int key0 = kv0 + 16 * (w >> 1);
+  const char* p;
+  int tok;  // the row within its block
+  if (kv0 + kBN <= kv_end) {
+    p = group_base(pool, a, blk, key0) + off;
+    tok = (key0 & (a.bs - 1)) + 8 * (w & 1) + (lane >> 3);
+  } else {
+    tok = min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);
+    p = group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
+  }
+  if constexpr (POOL != kPoolFp4) {
+    return {ld16(p)};
+  } else {
+    constexpr int kBlocks = kHeadDim / kFp4Block;
+    const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
+    const uint64_t page = (uint64_t)b * (unsigned)(a.Hkv * kBlocks * a.bs);
+    const unsigned col = head_bytes / (kHeadDim / 2) * kBlocks + ((lane & 7) >> 1);  // the head's dim block
+    const uint8_t* sp = IS_V ? a.vs + page + (col * (unsigned)a.bs + tok) : a.ks + page + ((unsigned)(tok * a.Hkv * kBlocks) + col);
+    return {ld8(p), *sp};
+  }
 }
 
-// Widens a lane's 16 fp8 values to two 16-byte chunks of 16-bit values (logical chunks 2 (l % 8) and
+// Widens a lane's 16 values to two 16-byte chunks of 16-bit values (logical chunks 2 (l % 8) and
 // 2 (l % 8) + 1 of row 8 w + l / 8) and writes them at their swizzled places in the LDS tile.
-template <typename T, bool IS_V>
-__device__ __forceinline__ void stage_store(u32x4 x, int w, int lane, char* slot) {
+template <typename T, bool IS_V, int POOL>
+__device__ __forceinline__ void stage_store(const Staged<POOL>& s, int w, int lane, char* slot) {
   const int r = 8 * w + (lane >> 3);
   const int c0 = 2 * (lane & 7);
   const int sw = IS_V ? 4 * (r & 3) : (r & 15);
   char* row = slot + r * kRowBytes;
-  *reinterpret_cast<u32x4*>(row + 16 * (c0 ^ sw)) = fp8x8_to<T>(x[0], x[1]);
-  *reinterpret_cast<u32x4*>(row + 16 * ((c0 + 1) ^ sw)) = fp8x8_to<T>(x[2], x[3]);
+  u32x4 lo, hi;
+  if constexpr (POOL != kPoolFp4) {
+    lo = fp8x8_to<T>(s.x[0], s.x[1]);
+    hi = fp8x8_to<T>(s.x[2], s.x[3]);
+  } else {
+    lo = fp4x8_to<T>(s.x[0], e8m0_to_f32(s.e));
+    hi = fp4x8_to<T>(s.x[1], e8m0_to_f32(s.e));
+  }
+  *reinterpret_cast<u32x4*>(row + 16 * (c0 ^ sw)) = lo;
+  *reinterpret_cast<u32x4*>(row + 16 * ((c0 + 1) ^ sw)) = hi;
 }
 
 // ---------------------------------------------------------------- MFMA operands from LDS
@@ -341,7 +385,7 @@ __device__ __forceinline__ void softmax_two(STile& s0, STile& s1, u32x4 (&pf0)[2
   l_run += sum_xor32((s4[0] + s4[1]) + (s4[2] + s4[3]));
 }
 
-template <typename T, bool F8>
+template <typename T, int POOL>
 __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
   const int tid = threadIdx.x;
@@ -370,14 +414,14 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
   const int wave_qp_lo = cached + t0 + wave * tpw;
   const float c = a.scale_log2;
 
-  const unsigned head_bytes = (unsigned)(kvh * kHeadDim * (F8 ? 1 : 2));
+  const unsigned head_bytes = (unsigned)(kvh * head_row_bytes(POOL));
   const int r0 = 8 * wave + (lane >> 4), r1 = r0 + 4;
   const unsigned rb = (unsigned)a.row_bytes;
   const unsigned koff0 = (unsigned)(r0 & 15) * rb + head_bytes + 16u * k_chunk(r0, lane);
   const unsigned koff1 = (unsigned)(r1 & 15) * rb + head_bytes + 16u * k_chunk(r1, lane);
   const unsigned voff0 = (unsigned)(r0 & 15) * rb + head_bytes + 16u * v_chunk(r0, lane);
   const unsigned voff1 = (unsigned)(r1 & 15) * rb + head_bytes + 16u * v_chunk(r1, lane);
-  const unsigned soff = (unsigned)(8 * (wave & 1) + (lane >> 3)) * rb + head_bytes + 16u * (lane & 7);  // fp8
+  const unsigned soff = (unsigned)(8 * (wave & 1) + (lane >> 3)) * rb + head_bytes + (POOL == kPoolFp4 ? 8u : 16u) * (lane & 7);  // fp8, fp4
   const unsigned kread = (unsigned)(n * kRowBytes + 16 * (h ^ (n & 1)) + 32 * ((n & 15) >> 1));
   const unsigned vread = (unsigned)(kVBase + 1024 * h + 320 * ((lane >> 2) & 3) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 
@@ -406,14 +450,14 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
 
   // prologue: K(0..3), V(0..1), then Q; all of them have landed after the first barrier (fp8 pools: all
   // six tiles loaded into registers first, then widened into LDS)
-  if constexpr (F8) {
-    u32x4 kx[4], vx[2];
+  if constexpr (POOL != kPool16) {
+    Staged<POOL> kx[4], vx[2];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t < ntiles) {
         const int b = blk_direct(t);
-        kx[t] = stage_load(kc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
-        if (t < 2) vx[t] = stage_load(vc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
+        kx[t] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
+        if (t < 2) vx[t] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
       }
     }
 #pragma unroll
@@ -458,7 +502,7 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
 
   // fp8 pools: V(2j+2), V(2j+3) pass through registers during the even phase and K(2j+4), K(2j+5) during
   // the odd one, each widened into LDS at the end of its phase
-  u32x4 st_a = {0, 0, 0, 0}, st_b = {0, 0, 0, 0};
+  Staged<POOL> st_a = {}, st_b = {};
   int k0b = 0, k1b = 0;
   for (int p = 0; p < 2 * npairs; ++p) {
     const int j = p >> 1;
@@ -472,9 +516,9 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
         wbase = ta + 4;
         load_ids(wbase, wsel);
       }
-      if constexpr (F8) {
-        if (ta + 2 < ntiles) st_a = stage_load(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, head_bytes, lane);
-        if (ta + 3 < ntiles) st_b = stage_load(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+      if constexpr (POOL != kPool16) {
+        if (ta + 2 < ntiles) st_a = stage_load<POOL, true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+        if (ta + 3 < ntiles) st_b = stage_load<POOL, true>(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, head_bytes, lane);
       } else {
         if (ta + 2 < ntiles)
           dma_tile<true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, voff0, voff1, head_bytes, lane, v_slot(ta + 2));
@@ -485,14 +529,14 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
         if (ta + 5 < ntiles)
           dma_tile<false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, koff0, koff1, head_bytes, lane, k_slot(ta + 5));
       }
-    } else if constexpr (F8) {
-      if (ta + 4 < ntiles) st_a = stage_load(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, head_bytes, lane);
-      if (ta + 5 < ntiles) st_b = stage_load(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+    } else if constexpr (POOL != kPool16) {
+      if (ta + 4 < ntiles) st_a = stage_load<POOL, false>(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+      if (ta + 5 < ntiles) st_b = stage_load<POOL, false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, head_bytes, lane);
     }
     if ((p & 1) == grp) {  // matrix phase of pair j
       __builtin_amdgcn_s_setprio(1);
       // all four products of the pair (fp8 pools keep two tiles of staging registers: no single ring)
-      const bool full = !F8 && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
+      const bool full = POOL == kPool16 && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
       if (full) {
         matrix_phase_pair<T>(lds, vread + (ta & (kRingV - 1)) * kTileBytes, kread + ((ta + 2) & (kRingK - 1)) * kTileBytes,
                              vread + ((ta + 1) & (kRingV - 1)) * kTileBytes, kread + ((ta + 3) & (kRingK - 1)) * kTileBytes,
@@ -518,7 +562,7 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
       if (tn < ntiles && tn * kBN <= wave_qp_hi)
         softmax_two<T>(st0, st1, pf0, pf1, oacc, m_run, l_run, tn * kBN, qp, wave_qp_lo, h, c);
     }
-    if constexpr (F8) {  // the staged tiles' slots were freed by the barrier that ended phase 2j-1
+    if constexpr (POOL != kPool16) {  // the staged tiles' slots were freed by the barrier that ended phase 2j-1
       if ((p & 1) == 0) {
         if (ta + 2 < ntiles) stage_store<T, true>(st_a, wu, lane, v_slot(ta + 2));
         if (ta + 3 < ntiles) stage_store<T, true>(st_b, wu, lane, v_slot(ta + 3));
@@ -538,7 +582,7 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
     }
   }
 
-  const float inv = (F8 ? a.v_scale : 1.f) / l_run;
+  const float inv = (POOL == kPoolFp8 ? a.v_scale : 1.f) / l_run;
   char* ost = lds + wave * (32 * kRowBytes);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -657,7 +701,7 @@ __device__ __forceinline__ void softmax_one(STile& s, u32x4 (&pf)[2][2], f32x16 
 
 typedef const __attribute__((address_space(4))) int32_t ConstI32;
 
-template <typename T, bool F8>
+template <typename T, int POOL>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill4w_kernel(
     const PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes4];
@@ -685,7 +729,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wave_qp_lo = cached + t0 + wave * tpw;
   const float c = a.scale_log2;
 
-  const unsigned head_bytes = (unsigned)(kvh * kHeadDim * (F8 ? 1 : 2));
+  const unsigned head_bytes = (unsigned)(kvh * head_row_bytes(POOL));
   const unsigned rb = (unsigned)a.row_bytes;
   unsigned koff[4], voff[4];
 #pragma unroll
@@ -695,25 +739,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     voff[i] = (unsigned)r * rb + head_bytes + 16u * v_chunk(r, lane);
   }
   // fp8: this wavefront's rows as two 8-row shares (those of wavefront 2 w + i of the 8-wavefront layout)
-  const unsigned soff0 = (unsigned)(lane >> 3) * rb + head_bytes + 16u * (lane & 7), soff1 = soff0 + 8 * rb;
-  auto stage2 = [&](const char* pool, int b, int t, u32x4 (&x)[2]) {
-    x[0] = stage_load(pool, a, b, t * kBN, last, kv_end, 2 * wu, soff0, head_bytes, lane);
-    x[1] = stage_load(pool, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, head_bytes, lane);
+  const unsigned soff0 = (unsigned)(lane >> 3) * rb + head_bytes + (POOL == kPoolFp4 ? 8u : 16u) * (lane & 7), soff1 = soff0 + 8 * rb;
+  const char* kc = reinterpret_cast<const char*>(a.kc);
+  const char* vc = reinterpret_cast<const char*>(a.vc);
+  typedef Staged<POOL> Staged2[2];
+  auto stage_k = [&](int b, int t, Staged2& x) {
+    x[0] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, head_bytes, lane);
+    x[1] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, head_bytes, lane);
   };
-  auto store2 = [&](bool is_v, const u32x4 (&x)[2], char* slot) {
-    if (is_v) {
-      stage_store<T, true>(x[0], 2 * wu, lane, slot);
-      stage_store<T, true>(x[1], 2 * wu + 1, lane, slot);
-    } else {
-      stage_store<T, false>(x[0], 2 * wu, lane, slot);
-      stage_store<T, false>(x[1], 2 * wu + 1, lane, slot);
-    }
+  auto stage_v = [&](int b, int t, Staged2& x) {
+    x[0] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, head_bytes, lane);
+    x[1] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, head_bytes, lane);
+  };
+  auto store_k = [&](const Staged2& x, char* slot) {
+    stage_store<T, false>(x[0], 2 * wu, lane, slot);
+    stage_store<T, false>(x[1], 2 * wu + 1, lane, slot);
+  };
+  auto store_v = [&](const Staged2& x, char* slot) {
+    stage_store<T, true>(x[0], 2 * wu, lane, slot);
+    stage_store<T, true>(x[1], 2 * wu + 1, lane, slot);
   };
   const unsigned kread = (unsigned)(n * kRowBytes + 16 * (h ^ (n & 1)) + 32 * ((n & 15) >> 1));
   const unsigned vread = (unsigned)(kVBase4 + 1024 * h + 320 * ((lane >> 2) & 3) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 
-  const char* kc = reinterpret_cast<const char*>(a.kc);
-  const char* vc = reinterpret_cast<const char*>(a.vc);
   auto k_slot = [&](int t) { return lds + (t % kRingK4) * kTileBytes; };
   auto v_slot = [&](int t) { return lds + kVBase4 + (t & (kRingV4 - 1)) * kTileBytes; };
   // block id of this wavefront's 16-key group of tile t (clamped into the row: always a valid entry)
@@ -728,17 +776,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   // prologue: K(0..2), V(0), then Q; all landed after the first barrier
   int i1 = blk(1), i2 = blk(2), i3 = blk(3);  // ids of tiles j + 1 .. j + 3 at step j = 0
-  if constexpr (F8) {
+  if constexpr (POOL != kPool16) {
     const int b0 = blk(0);
-    u32x4 k0[2], v0[2], k1[2], k2[2];
-    stage2(kc, b0, 0, k0);
-    stage2(vc, b0, 0, v0);
-    if (1 < ntiles) stage2(kc, i1, 1, k1);
-    if (2 < ntiles) stage2(kc, i2, 2, k2);
-    store2(false, k0, k_slot(0));
-    store2(true, v0, v_slot(0));
-    if (1 < ntiles) store2(false, k1, k_slot(1));
-    if (2 < ntiles) store2(false, k2, k_slot(2));
+    Staged2 k0, v0, k1, k2;
+    stage_k(b0, 0, k0);
+    stage_v(b0, 0, v0);
+    if (1 < ntiles) stage_k(i1, 1, k1);
+    if (2 < ntiles) stage_k(i2, 2, k2);
+    store_k(k0, k_slot(0));
+    store_v(v0, v_slot(0));
+    if (1 < ntiles) store_k(k1, k_slot(1));
+    if (2 < ntiles) store_k(k2, k_slot(2));
   } else {
     const int b0 = blk(0);
     dma_tile4<false>(kc, a, b0, 0, last, kv_end, wu, koff, head_bytes, lane, k_slot(0));
@@ -768,12 +816,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   barrier_lds();  // K(0) has been read: step 0 loads K(3) into its slot
 
-  u32x4 sv[2] = {}, sk[2] = {};  // fp8: V(j+1) and K(j+3) on their way through registers
+  Staged2 sv = {}, sk = {};  // fp8, fp4: V(j+1) and K(j+3) on their way through registers
   for (int j = 0; j < ntiles; ++j) {
     const bool v_ahead = j + 1 < ntiles, k_ahead = j + 3 < ntiles;
-    if constexpr (F8) {
-      if (v_ahead) stage2(vc, i1, j + 1, sv);
-      if (k_ahead) stage2(kc, i3, j + 3, sk);
+    if constexpr (POOL != kPool16) {
+      if (v_ahead) stage_v(i1, j + 1, sv);
+      if (k_ahead) stage_k(i3, j + 3, sk);
     } else {
       if (v_ahead)
         dma_tile4<true>(vc, a, i1, (j + 1) * kBN, last, kv_end, wu, voff, head_bytes, lane, v_slot(j + 1));
@@ -795,9 +843,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     __builtin_amdgcn_s_setprio(0);
     if (do_s) softmax_one<T>(st, pf, oacc, m_run, l_run, (j + 1) * kBN, qp, wave_qp_lo, h, c);
-    if constexpr (F8) {  // widened into the slots of V(j-1) and K(j), both last read in step j-1
-      if (v_ahead) store2(true, sv, v_slot(j + 1));
-      if (k_ahead) store2(false, sk, k_slot(j + 3));
+    if constexpr (POOL != kPool16) {  // widened into the slots of V(j-1) and K(j), both last read in step j-1
+      if (v_ahead) store_v(sv, v_slot(j + 1));
+      if (k_ahead) store_k(sk, k_slot(j + 3));
       barrier_lds();
     } else if (k_ahead) {  // every load but K(j+3) has landed, and every wavefront is done with V(j), K(j+1)
       barrier_vm<4>();
@@ -808,7 +856,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   // output: each wavefront's 32 x 128 block transposed through its 8 KB of the K ring (no DMA is in flight
   // and every wavefront is past its last read of the rings), then whole 16-byte chunks per row
-  const float inv = (F8 ? a.v_scale : 1.f) / l_run;
+  const float inv = (POOL == kPoolFp8 ? a.v_scale : 1.f) / l_run;
   char* ost = lds + wave * (32 * kRowBytes);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -841,9 +889,10 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
                                   const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* seq_lens,
                                   const int32_t* prefill_work, int32_t num_prefill_work, int32_t q_tile_tokens,
                                   float softmax_scale, int32_t dtype, void* out, int64_t out_stride_tok,
-                                  int64_t out_stride_head, bool fp8, float k_scale, float v_scale, void* stream) {
+                                  int64_t out_stride_head, int pool, float k_scale, float v_scale, const void* k_scales,
+                  const void* v_scales, void* stream) {
   using namespace mllm;
-  const std::string fn = fp8 ? "mllm_paged_prefill_fp8" : "mllm_paged_prefill";
+  const std::string fn = pool == kPoolFp4 ? "mllm_paged_prefill_fp4" : (pool == kPoolFp8 ? "mllm_paged_prefill_fp8" : "mllm_paged_prefill");
   MLLM_REQUIRE(dtype == MLLM_DTYPE_BF16 || dtype == MLLM_DTYPE_F16, MLLM_ERR_UNSUPPORTED,
                fn + ": dtype must be bfloat16 or float16");
   MLLM_REQUIRE(head_dim == kHeadDim, MLLM_ERR_UNSUPPORTED, fn + ": head_dim must be 128");
@@ -860,7 +909,8 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
                fn + ": q_tile_tokens must be 256 / (H / Hkv) or 128 / (H / Hkv)");
   MLLM_REQUIRE(num_prefill_work >= 0, MLLM_ERR_INVALID, fn + ": negative count");
   if (num_prefill_work == 0) return MLLM_OK;
-  MLLM_REQUIRE(q && k_cache && v_cache && out && qo_indptr && kv_indptr && kv_indices && seq_lens && prefill_work,
+  MLLM_REQUIRE(q && k_cache && v_cache && out && qo_indptr && kv_indptr && kv_indices && seq_lens && prefill_work &&
+                   (pool != kPoolFp4 || (k_scales && v_scales)),
                MLLM_ERR_INVALID, fn + ": null pointer");
   const bool aligned = ((uintptr_t)q % 16 == 0) && ((uintptr_t)out % 16 == 0) && ((uintptr_t)k_cache % 16 == 0) &&
                        ((uintptr_t)v_cache % 16 == 0) && (q_stride_tok * 2) % 16 == 0 &&
@@ -877,7 +927,7 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
   a.kc = static_cast<const uint16_t*>(k_cache);
   a.vc = static_cast<const uint16_t*>(v_cache);
   a.num_blocks = num_blocks;
-  a.row_bytes = num_kv_heads * head_dim * (fp8 ? 1 : 2);
+  a.row_bytes = num_kv_heads * head_row_bytes(pool);
   a.page_bytes = (unsigned)((int64_t)block_size * a.row_bytes);
   a.bs = block_size;
   a.bs_shift = __builtin_ctz((unsigned)block_size);
@@ -887,34 +937,33 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
   a.work = reinterpret_cast<const int4*>(prefill_work);
   a.scale_log2 = softmax_scale * k_scale * kLog2e;
   a.v_scale = v_scale;
+  a.ks = static_cast<const uint8_t*>(k_scales);
+  a.vs = static_cast<const uint8_t*>(v_scales);
   a.out = static_cast<uint16_t*>(out);
   a.o_st = out_stride_tok;
   a.o_sh = out_stride_head;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)num_prefill_work * (unsigned)num_kv_heads;
-  if (four_waves) {  // 128-row items: 4-wavefront workgroups, two per CU
-    if (dtype == MLLM_DTYPE_BF16) {
-      if (fp8)
-        prefill4w_kernel<BF16, true><<<grid, 256, 0, st>>>(a);
-      else
-        prefill4w_kernel<BF16, false><<<grid, 256, 0, st>>>(a);
-    } else {
-      if (fp8)
-        prefill4w_kernel<F16, true><<<grid, 256, 0, st>>>(a);
-      else
-        prefill4w_kernel<F16, false><<<grid, 256, 0, st>>>(a);
-    }
-  } else if (dtype == MLLM_DTYPE_BF16) {
-    if (fp8)
-      prefill128_kernel<BF16, true><<<grid, 512, 0, st>>>(a);
+  auto launch = [&](auto tag, auto kind) {
+    using T = decltype(tag);
+    constexpr int POOL = decltype(kind)::value;
+    if (four_waves)  // 128-row items: 4-wavefront workgroups, two per CU
+      prefill4w_kernel<T, POOL><<<grid, 256, 0, st>>>(a);
     else
-      prefill128_kernel<BF16, false><<<grid, 512, 0, st>>>(a);
-  } else {
-    if (fp8)
-      prefill128_kernel<F16, true><<<grid, 512, 0, st>>>(a);
+      prefill128_kernel<T, POOL><<<grid, 512, 0, st>>>(a);
+  };
+  auto of_type = [&](auto kind) {
+    if (dtype == MLLM_DTYPE_BF16)
+      launch(BF16{}, kind);
     else
-      prefill128_kernel<F16, false><<<grid, 512, 0, st>>>(a);
-  }
+      launch(F16{}, kind);
+  };
+  if (pool == kPoolFp4)
+    of_type(std::integral_constant<int, kPoolFp4>{});
+  else if (pool == kPoolFp8)
+    of_type(std::integral_constant<int, kPoolFp8>{});
+  else
+    of_type(std::integral_constant<int, kPool16>{});
   return check_launch(fn.c_str());
 }
 
@@ -930,7 +979,7 @@ extern "C" int mllm_paged_prefill(const void* q, int64_t q_stride_tok, int64_t q
   return paged_prefill(q, q_stride_tok, q_stride_head, k_cache, v_cache, num_blocks, block_size, num_heads,
                        num_kv_heads, head_dim, qo_indptr, kv_indptr, kv_indices, seq_lens, prefill_work,
                        num_prefill_work, q_tile_tokens, softmax_scale, dtype, out, out_stride_tok, out_stride_head,
-                       false, 1.f, 1.f, stream);
+                       mllm::kPool16, 1.f, 1.f, nullptr, nullptr, stream);
 }
 
 extern "C" int mllm_paged_prefill_fp8(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
@@ -943,5 +992,19 @@ extern "C" int mllm_paged_prefill_fp8(const void* q, int64_t q_stride_tok, int64
   return paged_prefill(q, q_stride_tok, q_stride_head, k_cache, v_cache, num_blocks, block_size, num_heads,
                        num_kv_heads, head_dim, qo_indptr, kv_indptr, kv_indices, seq_lens, prefill_work,
                        num_prefill_work, q_tile_tokens, softmax_scale, dtype, out, out_stride_tok, out_stride_head,
-                       true, k_scale, v_scale, stream);
+                       mllm::kPoolFp8, k_scale, v_scale, nullptr, nullptr, stream);
+}
+
+extern "C" int mllm_paged_prefill_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                      const void* v_cache, const void* k_scales, const void* v_scales,
+                                      int64_t num_blocks, int32_t block_size, int32_t num_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                      const int32_t* kv_indices, const int32_t* seq_lens, const int32_t* prefill_work,
+                                      int32_t num_prefill_work, int32_t q_tile_tokens, float softmax_scale,
+                                      int32_t dtype, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                                      void* stream) {
+  return paged_prefill(q, q_stride_tok, q_stride_head, k_cache, v_cache, num_blocks, block_size, num_heads,
+                       num_kv_heads, head_dim, qo_indptr, kv_indptr, kv_indices, seq_lens, prefill_work,
+                       num_prefill_work, q_tile_tokens, softmax_scale, dtype, out, out_stride_tok, out_stride_head,
+                       mllm::kPoolFp4, 1.f, 1.f, k_scales, v_scales, stream);
 }

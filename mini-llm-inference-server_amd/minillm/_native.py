@@ -16,7 +16,8 @@ LIB_PATH = Path(os.environ.get("MLLM_HIP_LIB", Path(__file__).resolve().parent /
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, -1, -2, -3
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-ABI_VERSION = 5
+ABI_VERSION = 6
+POOL_16BIT, POOL_FP8, POOL_FP4 = 0, 1, 2
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -33,6 +34,26 @@ class LayerStep(ctypes.Structure):
                 ("num_merge_work", _i32), ("num_prefill_work", _i32), ("pages_per_split", _i32),
                 ("q_tile_tokens", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
                 ("block_size", _i32), ("dtype", _i32), ("kv_fp8", _i32), ("softmax_scale", _f32)]
+
+
+class RopeAppend(ctypes.Structure):
+    """mllm_rope_append: the arguments of mllm_qk_norm_rope_kv_append."""
+
+    _fields_ = [("q", _p), ("k", _p), ("v", _p), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("k_stride_tok", _i64),
+                ("k_stride_head", _i64), ("v_stride_tok", _i64), ("v_stride_head", _i64), ("cos", _p), ("sin", _p),
+                ("cs_stride_tok", _i64), ("q_out", _p), ("q_out_stride_tok", _i64), ("q_out_stride_head", _i64),
+                ("k_cache", _p), ("v_cache", _p), ("k_scales", _p), ("v_scales", _p), ("k_scale", _f32),
+                ("v_scale", _f32), ("num_blocks", _i64), ("slot_mapping", _p), ("num_tokens", _i64),
+                ("block_size", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+                ("dtype", _i32), ("pool", _i32)]
+
+
+class LayerPool(ctypes.Structure):
+    """mllm_layer_pool: a layer's pools and head norms."""
+
+    _fields_ = [("k_cache", _p), ("v_cache", _p), ("k_scales", _p), ("v_scales", _p), ("k_scale", _f32),
+                ("v_scale", _f32), ("q_norm", _p), ("k_norm", _p), ("norm_eps", _f32)]
+
 
 # symbol -> (restype, argtypes); the exact list include/minillm_hip.h declares
 SIGNATURES = {
@@ -85,6 +106,21 @@ SIGNATURES = {
     "mllm_paged_decode_fp8": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                              _i32, _p, _i32, _i32, _f32, _i32, _f32, _f32, _p, _i64, _i64, _p, _i64,
                                              _p]),
+    # 4-bit pools (e2m1 codes, e8m0 block scales), head norms
+    "mllm_kv_append_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
+                                          _i64, _p]),
+    "mllm_kv_read_fp4": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p]),
+    "mllm_paged_decode_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _i32,
+                                             _i32, _i32, _f32, _i32, _p, _i64, _i64, _p, _i64, _p]),
+    "mllm_paged_prefill_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p,
+                                              _p, _i32, _i32, _f32, _i32, _p, _i64, _i64, _p]),
+    "mllm_qk_norm_rope_kv_append": (ctypes.c_int, [_p, _p, _p, _f32, _p]),
+    "mllm_qk_norm_rope": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _f32, _i32,
+                                         _i32, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "mllm_attention_forward_pool": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p,
+                                                   _p, _p, _p]),
+    "mllm_decoder_layer_pool": (ctypes.c_int, [_p, _p, _i64, _p, _f32, _p, _p, _p, _p, _p, _f32, _p, _p, _p, _i64, _p, _p,
+                                               _i64, _p, _p, _i64, _p, _p]),
     "mllm_paged_prefill_fp8": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                               _i32, _i32, _f32, _i32, _f32, _f32, _p, _i64, _i64, _p]),
 }

@@ -16,6 +16,13 @@ A pool of dtype torch.float8_e4m3fn (the reference's planned fp8 KV cache, M9b i
 docs/distributed_inference_plan.md:310) selects the `_fp8` entry points: the append stores
 e4m3fn(x * (1 / scale)) and attention reads value * scale, with per-tensor `k_scale` / `v_scale` passed
 to `forward`; q, k, v and the output stay bf16 / fp16.
+
+A pool of dtype torch.float4_e2m1fn_x2 ([num_blocks, block_size, Hkv, Dh / 2], two codes to a byte) selects the `_fp4`
+entry points; `k_scale` and `v_scale` are then the pool's block scales, torch.float8_e8m0fnu tensors (PagedKVCache keeps
+them; include/minillm_hip.h has the format).
+
+`forward_rotary` and `rope_append` take `qk_norm=(q weight, k weight, eps)`: RMSNorm of every query and key head in the
+launch that rotates and appends (`mllm_qk_norm_rope_kv_append`), into any of the pools.
 """
 
 from __future__ import annotations
@@ -75,8 +82,16 @@ SMALL_BIN_PAGES = 16  # the 4-wavefront launch adds workgroups per CU before its
 MIN_SPLIT_PAGES = 2  # the smallest bin the heuristic picks (16-bit pools)
 
 
+def fp4_heads(num_heads: int, num_kv_heads: int) -> int:
+    """KV heads a wavefront of mllm_paged_decode_fp4 takes (the library's rule)."""
+    group = num_heads // num_kv_heads
+    if num_kv_heads % 4 == 0 and 4 * group <= 16:
+        return 4
+    return 2 if num_kv_heads % 2 == 0 and 2 * group <= 16 else 1
+
+
 def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None = None, kv_fp8: bool = False,
-                    num_cus: int = FULL_CHIP_CUS, whole_pages: bool = True) -> int:
+                    num_cus: int = FULL_CHIP_CUS, whole_pages: bool = True, kv_fp4: bool = False) -> int:
     """Pages per decode bin for a step of `decode_pages` decode pages on a device of `num_cus` CUs.
 
     16-bit pools with KV heads in groups of 8 (`whole_pages`): one whole-page workgroup per CU, Hkv / 8 per
@@ -104,6 +119,11 @@ def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None 
     forced = os.environ.get("MLLM_PAGES_PER_SPLIT")
     if forced:
         return max(1, min(MAX_SPLIT_PAGES, int(forced)))
+    if kv_fp4:  # one round of the resident wavefronts, 2 per SIMD
+        per_bin = num_kv_heads // fp4_heads(num_heads or 4 * num_kv_heads, num_kv_heads)
+        per_round = max(1, num_cus * 4 * 2 // per_bin)
+        rounds = max(1, math.ceil(decode_pages / (MAX_SPLIT_PAGES * per_round)))
+        return max(MIN_SPLIT_PAGES, min(MAX_SPLIT_PAGES, math.ceil(decode_pages / (rounds * per_round))))
     if whole_pages and not kv_fp8 and num_kv_heads % WHOLE_PAGE_WAVES == 0 and decode_pages > 0:
         per_round = max(1, num_cus // (num_kv_heads // WHOLE_PAGE_WAVES))
         rounds = math.ceil(decode_pages / (MAX_SPLIT_PAGES * per_round))
@@ -123,13 +143,14 @@ def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None 
 
 
 def decode_records_bound(max_pages: int, rows: int, num_kv_heads: int, num_heads: int | None = None,
-                         kv_fp8: bool = False, num_cus: int = FULL_CHIP_CUS, pad_pages: int = 0) -> int:
+                         kv_fp8: bool = False, num_cus: int = FULL_CHIP_CUS, pad_pages: int = 0,
+                         kv_fp4: bool = False) -> int:
     """The most decode plan records a step of `rows` rows and at most `max_pages` decode pages needs at the
     bin size pages_per_split picks for its page count (plus `pad_pages` pages of padding rows, which do not
     change that size)."""
     best = 0
     for t in range(1, max_pages + 1):
-        c = pages_per_split(t, num_kv_heads, num_heads, kv_fp8, num_cus)
+        c = pages_per_split(t, num_kv_heads, num_heads, kv_fp8, num_cus, kv_fp4=kv_fp4)
         best = max(best, decode_plan_size(t + pad_pages, rows, c)[0])
     return best
 
@@ -227,6 +248,51 @@ def is_fp8(pool: torch.Tensor) -> bool:
     return pool.dtype == FP8
 
 
+FP4 = torch.float4_e2m1fn_x2  # two e2m1 codes to an element
+SCALES4 = torch.float8_e8m0fnu  # their block scales
+FP4_BLOCK = 32  # dims per scale
+
+
+def pool_type(pool: torch.Tensor) -> int:
+    """The library's MLLM_POOL_* of a pool."""
+    if pool.dtype == FP4:
+        return _native.POOL_FP4
+    return _native.POOL_FP8 if pool.dtype == FP8 else _native.POOL_16BIT
+
+
+def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
+    """ValueError unless k_scale and v_scale are the block scales of a 4-bit pool."""
+    nb, bs, hkv, half = k_cache.shape
+    blocks = 2 * half // FP4_BLOCK
+    for name, t, shape in (("k_scale", k_scale, (nb, bs, hkv, blocks)), ("v_scale", v_scale, (nb, hkv, blocks, bs))):
+        if not isinstance(t, torch.Tensor) or t.dtype != SCALES4:
+            raise ValueError(f"with a 4-bit pool, {name} is its float8_e8m0fnu tensor of block scales")
+        if t.shape != shape or not t.is_contiguous() or t.device != k_cache.device:
+            raise ValueError(f"{name} must be contiguous {list(shape)} on the pool's device")
+
+
+def check_norms(qk_norm, q: torch.Tensor) -> None:
+    """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's."""
+    wq, wk, eps = qk_norm
+    for w in (wq, wk):
+        if w.shape != (q.shape[-1],) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous():
+            raise ValueError(f"the head norms' weights must be contiguous [Dh] = [{q.shape[-1]}] in q's type, on its device")
+    if not 0 <= eps < math.inf:
+        raise ValueError("the head norms' eps must be finite and not negative")
+
+
+def layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm) -> _native.LayerPool:
+    """The mllm_layer_pool of a layer's checked pools, scales and head norms."""
+    pool = _native.LayerPool(k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), k_scale=1.0, v_scale=1.0)
+    if k_cache.dtype == FP4:
+        pool.k_scales, pool.v_scales = k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        pool.k_scale, pool.v_scale = k_scale, v_scale
+    if qk_norm is not None:
+        pool.q_norm, pool.k_norm, pool.norm_eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
+    return pool
+
+
 class HipBackend(AttentionBackend):
     name = "hip"
     # The model hands q and k to `forward_rotary` before RoPE when this is set (LlamaAttention checks it),
@@ -245,8 +311,9 @@ class HipBackend(AttentionBackend):
     def __init__(self) -> None:
         self._lib = _native.lib()
         self._attention_forward = self._lib.fn("mllm_attention_forward")
+        self._attention_forward_pool = self._lib.fn("mllm_attention_forward_pool")
         self._planned = None  # the AttentionMetadata the plan was last built for
-        self._planned_fp8 = False  # and the pool type it was built for
+        self._planned_pool = _native.POOL_16BIT  # and the pool type it was built for
         self._plan: StepPlan | None = None
         self._workspace: torch.Tensor | None = None
         self._side: dict = {}  # device -> the stream mixed steps run their prefill launch on
@@ -268,19 +335,26 @@ class HipBackend(AttentionBackend):
         prefill goes to a second stream."""
         if not self.overlap_mixed:
             return False
-        plan = self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, is_fp8(k_cache))
+        plan = self._plan_for(meta, q, k_cache)
         return bool(plan.num_decode and plan.num_prefill) and not torch.cuda.is_current_stream_capturing()
 
     def run_layer(self, q, k, v, k_cache, v_cache, meta, out, cos=None, sin=None, q_rot=None,
-                  k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+                  k_scale=1.0, v_scale=1.0, qk_norm=None) -> None:
         """The layer's whole path in one host call (mllm_attention_forward): KV append (with cos and sin, the
         RoPE of q and k fused into it and the rotated q written to q_rot), decode + merge, prefill, on the
         current stream.  The arguments are the checked ones of `forward` / `forward_rotary`; q_rot and out
         are contiguous [N, H, Dh]."""
-        fp8 = is_fp8(k_cache)
-        plan = self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, fp8)
-        step = self._layer_step(plan, meta, q.shape[0], q.shape[1], q.dtype, k_cache, fp8)
+        plan = self._plan_for(meta, q, k_cache)
+        step = self._layer_step(plan, meta, q.shape[0], q.shape[1], q.shape[2], q.dtype, k_cache)
         rot = cos is not None
+        if k_cache.dtype == FP4 or qk_norm is not None:
+            pool = layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm)
+            self._lib.check(self._attention_forward_pool(
+                step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                v.stride(0), v.stride(1), cos.data_ptr() if rot else None, sin.data_ptr() if rot else None,
+                cos.stride(0) if rot else 0, q_rot.data_ptr() if rot else None, ctypes.addressof(pool), out.data_ptr(),
+                _native.stream_ptr(q.device)))
+            return
         self._lib.check(self._attention_forward(
             step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
             v.stride(0), v.stride(1), cos.data_ptr() if rot else None, sin.data_ptr() if rot else None,
@@ -290,18 +364,19 @@ class HipBackend(AttentionBackend):
     def layer_step(self, meta, n: int, num_heads: int, dtype, k_cache) -> int:
         """Address of the step's mllm_layer_step for rows of `num_heads` query heads in `dtype` and these pools (the
         plan is built on the first call with `meta`)."""
-        fp8 = is_fp8(k_cache)
-        plan = self.plan(meta, num_heads, k_cache.shape[2], k_cache.shape[3], k_cache.device, fp8)
-        return self._layer_step(plan, meta, n, num_heads, dtype, k_cache, fp8)
+        dh = k_cache.shape[3] * (2 if k_cache.dtype == FP4 else 1)
+        plan = self.plan(meta, num_heads, k_cache.shape[2], dh, k_cache.device, pool=pool_type(k_cache))
+        return self._layer_step(plan, meta, n, num_heads, dh, dtype, k_cache)
 
-    def _layer_step(self, plan: StepPlan, meta, n: int, num_heads: int, dtype, k_cache, fp8: bool) -> int:
+    def _layer_step(self, plan: StepPlan, meta, n: int, num_heads: int, dh: int, dtype, k_cache) -> int:
         """Address of the plan's mllm_layer_step for these pools and this workspace."""
         ws = self._workspace
-        key = (k_cache.shape[0], k_cache.shape[1], dtype, fp8, ws.data_ptr() if ws is not None else 0)
+        pool = pool_type(k_cache)
+        key = (k_cache.shape[0], k_cache.shape[1], dtype, pool, ws.data_ptr() if ws is not None else 0)
         if plan.layer_key == key:
             return plan.layer_addr
         ws = self._workspace_for(plan.workspace_bytes, k_cache.device)
-        num_blocks, bs, hkv, dh = k_cache.shape
+        num_blocks, bs, hkv, _ = k_cache.shape
         step = _native.LayerStep(
             num_blocks=num_blocks, num_tokens=n, slot_mapping=meta.slot_mapping.data_ptr(),
             qo_indptr=plan.meta_ptrs[0], kv_indptr=plan.meta_ptrs[1], kv_indices=plan.meta_ptrs[2],
@@ -309,10 +384,10 @@ class HipBackend(AttentionBackend):
             prefill_work=_ptr(plan.prefill_work), workspace=_ptr(ws), workspace_bytes=plan.workspace_bytes,
             num_decode_work=plan.num_decode, num_merge_work=plan.num_merge, num_prefill_work=plan.num_prefill,
             pages_per_split=plan.pages_per_split, q_tile_tokens=plan.q_tile, num_heads=num_heads,
-            num_kv_heads=hkv, head_dim=dh, block_size=bs, dtype=_native.dtype_code(dtype), kv_fp8=int(fp8),
+            num_kv_heads=hkv, head_dim=dh, block_size=bs, dtype=_native.dtype_code(dtype), kv_fp8=pool,
             softmax_scale=dh ** -0.5)
         plan.layer_step, plan.layer_addr = step, ctypes.addressof(step)
-        plan.layer_key = (num_blocks, bs, dtype, fp8, ws.data_ptr() if ws is not None else 0)
+        plan.layer_key = (num_blocks, bs, dtype, pool, ws.data_ptr() if ws is not None else 0)
         return plan.layer_addr
 
     def _check(self, q, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0):
@@ -320,6 +395,8 @@ class HipBackend(AttentionBackend):
         if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
             raise ValueError("k_cache and v_cache must both be [num_blocks, block_size, Hkv, Dh]")
         _, bs, hkv, dh_c = k_cache.shape
+        if k_cache.dtype == FP4:
+            dh_c *= 2
         if k.shape != (n, hkv, dh) or v.shape != (n, hkv, dh) or dh_c != dh:
             raise ValueError(f"k/v must be [N, Hkv, Dh] = [{n}, {hkv}, {dh}] to match q and the pool")
         if bs != meta.block_size:
@@ -330,28 +407,35 @@ class HipBackend(AttentionBackend):
             raise ValueError("the KV pools must be contiguous")
         if v_cache.dtype != k_cache.dtype:
             raise ValueError("k_cache and v_cache must share one dtype")
-        if is_fp8(k_cache):
+        if is_fp8(k_cache) or k_cache.dtype == FP4:
             if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-                raise ValueError("with an fp8 pool, q, k and v must share one dtype, bfloat16 or float16")
+                raise ValueError(f"with {'an fp8' if is_fp8(k_cache) else 'a 4-bit'} pool, q, k and v must share one "
+                                 f"dtype, bfloat16 or float16")
+        if k_cache.dtype == FP4:
+            check_scales(k_cache, k_scale, v_scale)
+        elif is_fp8(k_cache):
             if not (0 < k_scale < math.inf and 0 < v_scale < math.inf):
                 raise ValueError("k_scale and v_scale must be positive and finite")
         else:
             if q.dtype != k_cache.dtype:
                 raise ValueError("q and the pools must share one dtype")
-            if k_scale != 1.0 or v_scale != 1.0:
+            if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_scale != 1.0 or v_scale != 1.0:
                 raise ValueError("k_scale / v_scale apply to fp8 pools only")
         if n != meta.query_start_loc[-1]:
             raise ValueError(f"q has {n} tokens, the metadata describes {meta.query_start_loc[-1]}")
         return tuple(t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
 
-    def forward_rotary(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale: float = 1.0, v_scale: float = 1.0):
+    def forward_rotary(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0, qk_norm=None):
         """`forward` with the model's RoPE folded in: q and k arrive before the rotation (reference
         src/minillm/model/llama.py:110 applies it right before the backend call), with the step's
         cos / sin rows [N, Dh].  One launch rotates q and k, appends the rotated k and v to the pool and
-        writes the rotated q, bit for bit what apply_rotary followed by `forward` produces."""
+        writes the rotated q, bit for bit what apply_rotary followed by `forward` produces.  With `qk_norm`
+        every head of q and k is normed before the rotation, in fp32 with one rounding after it."""
         q, k, v = self._check(q, k, v, k_cache, v_cache, meta, k_scale, v_scale)
+        if qk_norm is not None:
+            check_norms(qk_norm, q)
         if self._split_launches(q, k_cache, meta):
-            q_rot = self.rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale)
+            q_rot = self.rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm)
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             self.attend(q_rot, k_cache, v_cache, meta, out, k_scale, v_scale)
             return out
@@ -364,11 +448,14 @@ class HipBackend(AttentionBackend):
             cos, sin = cos.contiguous(), sin.contiguous()
         q_rot = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
         out = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
-        self.run_layer(q, k, v, k_cache, v_cache, meta, out, cos, sin, q_rot, k_scale, v_scale)
+        self.run_layer(q, k, v, k_cache, v_cache, meta, out, cos, sin, q_rot, k_scale, v_scale, qk_norm)
         return out
 
-    def rope_append(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale: float = 1.0, v_scale: float = 1.0):
-        """Rotary embedding of q and k plus the KV append (`mllm_rope_kv_append`); returns the rotated q."""
+    def rope_append(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0, qk_norm=None):
+        """Rotary embedding of q and k plus the KV append (`mllm_rope_kv_append`); returns the rotated q.  With
+        `qk_norm` the heads of q and k are normed first (`mllm_qk_norm_rope_kv_append`)."""
+        if k_cache.dtype == FP4 or qk_norm is not None:
+            return self._norm_rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm)
         n, h, dh = q.shape
         num_blocks, bs, hkv, _ = k_cache.shape
         if cos.shape != (n, dh) or sin.shape != (n, dh):
@@ -388,9 +475,51 @@ class HipBackend(AttentionBackend):
             self._lib.call("mllm_rope_kv_append", *args, _native.stream_ptr(q.device))
         return q_rot
 
-    def append(self, k, v, k_cache, v_cache, meta, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    def _norm_rope_append(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm):
+        q, k, v = self._check(q, k, v, k_cache, v_cache, meta, k_scale, v_scale)
+        n, h, dh = q.shape
+        num_blocks, bs, hkv, _ = k_cache.shape
+        if cos.shape != (n, dh) or sin.shape != (n, dh):
+            raise ValueError(f"cos and sin must be [N, Dh] = [{n}, {dh}]")
+        if cos.dtype != q.dtype or sin.dtype != q.dtype:
+            raise ValueError("q, cos and sin must share one dtype")
+        if cos.stride(-1) != 1 or sin.stride() != cos.stride():
+            cos, sin = cos.contiguous(), sin.contiguous()
+        wq = wk = None
+        eps = 0.0
+        if qk_norm is not None:
+            check_norms(qk_norm, q)
+            wq, wk, eps = qk_norm
+        q_rot = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
+        pool, fp4 = pool_type(k_cache), k_cache.dtype == FP4
+        args = _native.RopeAppend(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride_tok=q.stride(0), q_stride_head=q.stride(1),
+            k_stride_tok=k.stride(0), k_stride_head=k.stride(1), v_stride_tok=v.stride(0), v_stride_head=v.stride(1),
+            cos=cos.data_ptr(), sin=sin.data_ptr(), cs_stride_tok=cos.stride(0), q_out=q_rot.data_ptr(),
+            q_out_stride_tok=h * dh, q_out_stride_head=dh, k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
+            k_scales=k_scale.data_ptr() if fp4 else None, v_scales=v_scale.data_ptr() if fp4 else None,
+            k_scale=1.0 if fp4 else k_scale, v_scale=1.0 if fp4 else v_scale, num_blocks=num_blocks,
+            slot_mapping=meta.slot_mapping.data_ptr(), num_tokens=n, block_size=bs, num_heads=h, num_kv_heads=hkv,
+            head_dim=dh, dtype=_native.dtype_code(q.dtype), pool=pool)
+        self._lib.call("mllm_qk_norm_rope_kv_append", ctypes.addressof(args), None if wq is None else wq.data_ptr(),
+                       None if wk is None else wk.data_ptr(), eps, _native.stream_ptr(q.device))
+        return q_rot
+
+    def append(self, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0) -> None:
         """KV append (reference write_kv, paged_torch_ref.py:23-28): one launch for K and V."""
         num_blocks, bs, hkv, dh = k_cache.shape
+        if k_cache.dtype == FP4:
+            if k.shape != (k.shape[0], hkv, 2 * dh) or v.shape != k.shape or v.dtype != k.dtype:
+                raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {2 * dh}] of one dtype")
+            if meta.slot_mapping.numel() != k.shape[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+                raise ValueError("the pools must be alike and the metadata describe k's tokens")
+            check_scales(k_cache, k_scale, v_scale)
+            k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
+            self._lib.call("mllm_kv_append_fp4", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                           v.stride(1), _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
+                           k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh,
+                           meta.slot_mapping.data_ptr(), k.shape[0], _native.stream_ptr(k_cache.device))
+            return
         if is_fp8(k_cache):
             self._lib.call("mllm_kv_append_fp8", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                            v.stride(1), _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -413,15 +542,24 @@ class HipBackend(AttentionBackend):
         capture records that build, so every replay re-plans from the staged metadata)."""
         self._planned = None
 
-    def plan(self, meta, num_heads: int, num_kv_heads: int, head_dim: int, device, kv_fp8: bool = False) -> StepPlan:
-        """The step's work plan, built on the GPU once per `meta` object (and pool type) and reused after."""
-        if self._planned is not meta or self._planned_fp8 != kv_fp8:
-            self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), kv_fp8)
+    def plan(self, meta, num_heads: int, num_kv_heads: int, head_dim: int, device, kv_fp8: bool = False,
+             pool: int | None = None) -> StepPlan:
+        """The step's work plan, built on the GPU once per `meta` object (and pool type: `pool`, a MLLM_POOL_* code, or
+        `kv_fp8`) and reused after."""
+        if pool is None:
+            pool = _native.POOL_FP8 if kv_fp8 else _native.POOL_16BIT
+        if self._planned is not meta or self._planned_pool != pool:
+            self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), pool)
         return self._plan
 
-    def attend(self, q, k_cache, v_cache, meta, out, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    def _plan_for(self, meta, q, k_cache) -> StepPlan:
+        return self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, pool=pool_type(k_cache))
+
+    def attend(self, q, k_cache, v_cache, meta, out, k_scale=1.0, v_scale=1.0) -> None:
         """Attention of every new token over its row's context in the pool, written into `out`."""
-        plan = self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, is_fp8(k_cache))
+        if k_cache.dtype == FP4:
+            check_scales(k_cache, k_scale, v_scale)
+        plan = self._plan_for(meta, q, k_cache)
         if plan.num_decode and plan.num_prefill and self.overlap_mixed and not torch.cuda.is_current_stream_capturing():
             # decode is enqueued first; the prefill's workgroups take CUs as the decode's free up
             cur = torch.cuda.current_stream(q.device)
@@ -442,11 +580,18 @@ class HipBackend(AttentionBackend):
         if plan.num_prefill:
             self.run_prefill(q, k_cache, v_cache, meta, out, k_scale, v_scale)
 
-    def run_decode(self, q, k_cache, v_cache, meta, out, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    def run_decode(self, q, k_cache, v_cache, meta, out, k_scale=1.0, v_scale=1.0) -> None:
         """Split-KV decode of the rows with one new token (reference paged_torch_ref.py:47-59)."""
         plan = self._plan
         num_blocks, bs, hkv, dh = k_cache.shape
         ws = self._workspace_for(plan.workspace_bytes, q.device)
+        if k_cache.dtype == FP4:
+            self._lib.call("mllm_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+                           v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv,
+                           2 * dh, plan.meta_ptrs[2], _ptr(plan.decode_work), plan.num_decode, plan.num_merge,
+                           plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
+                           out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes, _native.stream_ptr(q.device))
+            return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
                 q.shape[1], hkv, dh, *plan.decode_args, dh ** -0.5, _native.dtype_code(q.dtype))
         tail = (out.data_ptr(), out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes,
@@ -466,10 +611,17 @@ class HipBackend(AttentionBackend):
                        out.stride(0), out.stride(1), _ptr(self._workspace), plan.workspace_bytes,
                        _native.stream_ptr(q.device))
 
-    def run_prefill(self, q, k_cache, v_cache, meta, out, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    def run_prefill(self, q, k_cache, v_cache, meta, out, k_scale=1.0, v_scale=1.0) -> None:
         """MFMA attention of the rows with several new tokens (reference paged_torch_ref.py:61-73)."""
         plan = self._plan
         num_blocks, bs, hkv, dh = k_cache.shape
+        if k_cache.dtype == FP4:
+            self._lib.call("mllm_paged_prefill_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+                           v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv,
+                           2 * dh, *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile,
+                           (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(), out.stride(0), out.stride(1),
+                           _native.stream_ptr(q.device))
+            return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
                 q.shape[1], hkv, dh, *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile,
                 dh ** -0.5, _native.dtype_code(q.dtype))
@@ -479,14 +631,16 @@ class HipBackend(AttentionBackend):
         else:
             self._lib.call("mllm_paged_prefill", *args, *tail)
 
-    def _make_plan(self, meta, h: int, hkv: int, dh: int, dev, stream: int, kv_fp8: bool = False) -> None:
+    def _make_plan(self, meta, h: int, hkv: int, dh: int, dev, stream: int, pool: int = _native.POOL_16BIT) -> None:
+        kv_fp8, kv_fp4 = pool == _native.POOL_FP8, pool == _native.POOL_FP4
         news, lens, bs = meta.num_new, meta.seq_lens, meta.block_size
         pages = [-(-length // bs) for length in lens]
         decode_pages = sum(p for p, nn in zip(pages, news) if nn == 1)
         # a graph-captured step (StaticDecodeMetadata) stages its split size on the device; the
         # capacities then cover the smallest split it may stage
         split_dev = getattr(meta, "split_dev", None)
-        c = meta.split_min if split_dev is not None else pages_per_split(decode_pages, hkv, h, kv_fp8, device_cus(dev))
+        c = meta.split_min if split_dev is not None \
+            else pages_per_split(decode_pages, hkv, h, kv_fp8, device_cus(dev), kv_fp4=kv_fp4)
         g = h // hkv
         q_tile = prefill_q_tile(news, g, hkv, kv_fp8, device_cus(dev))
         decode_rows = sum(1 for nn in news if nn == 1)
@@ -509,7 +663,7 @@ class HipBackend(AttentionBackend):
                      meta.seq_lens_i32.data_ptr())
         self._plan = StepPlan(c, q_tile, n_dec, n_merge, n_pf, dec, mrg, pf, ws, meta_ptrs,
                               (*meta_ptrs, _ptr(dec), n_dec, _ptr(mrg), n_merge, c))
-        self._planned, self._planned_fp8 = meta, kv_fp8
+        self._planned, self._planned_pool = meta, pool
         if self.check_plan and n_dec and not torch.cuda.is_current_stream_capturing():
             check_plan_header(dec)
 

@@ -11,6 +11,11 @@ docs/distributed_inference_plan.md:310) stores e4m3fn(x / scale) with one scale 
 and `v_scale[l]` for layer l, which the model passes to the backend with the layer's pools.  One block of
 Llama-3.1-8B is then 32 KB per layer, so the same HBM holds twice the tokens.
 
+A pool of dtype torch.float4_e2m1fn_x2 stores 4-bit codes with a power-of-two scale for 32 dims of a token and head: the
+pools are [num_blocks, block_size, Hkv, Dh / 2] (two codes to a byte), `k_scale[l]` [num_blocks, block_size, Hkv, Dh / 32]
+and `v_scale[l]` [num_blocks, Hkv, Dh / 32, block_size] torch.float8_e8m0fnu tensors (include/minillm_hip.h has the
+format).  One block of Llama-3.1-8B is 17 KB per layer, so the same HBM holds 3.76 times the tokens of 16 bits.
+
 `PagedStep` is the pool as one forward pass sees it: the pool plus that step's metadata.
 """
 
@@ -18,30 +23,79 @@ from __future__ import annotations
 
 import torch
 
+from .. import _native
+
 BLOCK_SIZE = 16
+FP4 = torch.float4_e2m1fn_x2
+FP4_BLOCK = 32  # dims per scale of a 4-bit pool
 
 
 class PagedKVCache:
     def __init__(self, config, num_blocks: int, device: torch.device | str, dtype: torch.dtype,
                  block_size: int = BLOCK_SIZE, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
-        shape = (num_blocks, block_size, config.num_key_value_heads, config.head_dim)
-        self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(config.num_hidden_layers)]
-        self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(config.num_hidden_layers)]
+        hkv, dh = config.num_key_value_heads, config.head_dim
+        self.fp4 = dtype == FP4
+        if self.fp4 and dh % (2 * FP4_BLOCK):
+            raise ValueError(f"a 4-bit pool needs a head_dim that is a multiple of {2 * FP4_BLOCK}, not {dh}")
+        self.head_dim = dh
+        shape = (num_blocks, block_size, hkv, dh // 2 if self.fp4 else dh)
+        zeros = torch.uint8 if self.fp4 else dtype  # torch fills no 4-bit tensor on a GPU
+        self.k = [torch.zeros(shape, device=device, dtype=zeros).view(dtype) for _ in range(config.num_hidden_layers)]
+        self.v = [torch.zeros(shape, device=device, dtype=zeros).view(dtype) for _ in range(config.num_hidden_layers)]
         self.num_blocks = num_blocks
         self.block_size = block_size
         self.quantized = dtype == torch.float8_e4m3fn
         if not self.quantized and (k_scale != 1.0 or v_scale != 1.0):
             raise ValueError("k_scale / v_scale apply to fp8 pools only")
-        self.k_scale = [float(k_scale)] * config.num_hidden_layers
-        self.v_scale = [float(v_scale)] * config.num_hidden_layers
+        self.k_scale: list = [float(k_scale)] * config.num_hidden_layers
+        self.v_scale: list = [float(v_scale)] * config.num_hidden_layers
+        if self.fp4:
+            blocks = dh // FP4_BLOCK
+            for scales, of in ((self.k_scale, (num_blocks, block_size, hkv, blocks)),
+                               (self.v_scale, (num_blocks, hkv, blocks, block_size))):
+                scales[:] = [torch.zeros(of, device=device, dtype=torch.uint8).view(torch.float8_e8m0fnu) for _ in scales]
 
     def scales(self, layer: int) -> dict:
-        """Keyword arguments of the backend call for `layer`: its scales for an fp8 pool, none otherwise."""
-        return {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer]} if self.quantized else {}
+        """Keyword arguments of the backend call for `layer`: its scales for an fp8 or 4-bit pool, none otherwise."""
+        return {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer]} if self.quantized or self.fp4 else {}
+
+    def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The values of K and V at `slots` [n] (int64, on the pool's device; as a step's slot_mapping names them), both
+        [n, Hkv, Dh] of `dtype`: by default the pool's own, bfloat16 for fp8 and 4-bit pools.  A 4-bit pool is read with the
+        16-bit type it was written with."""
+        k, v = self.k[layer], self.v[layer]
+        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != k.device:
+            raise ValueError("slots must be one row of int64 on the pool's device")
+        dtype = dtype or (torch.bfloat16 if self.quantized or self.fp4 else k.dtype)
+        if not self.fp4:
+            got = []
+            for pool, scale in ((k, self.k_scale[layer]), (v, self.v_scale[layer])):
+                raw = pool.view(torch.uint8) if self.quantized else pool
+                rows = raw.flatten(0, 1).index_select(0, slots)
+                got.append((rows.view(pool.dtype).float() * scale if self.quantized else rows).to(dtype))
+            return got[0], got[1]
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("a 4-bit pool is read as bfloat16 or float16")
+        if k.device.type != "cuda":
+            raise RuntimeError(f"reading a 4-bit pool needs a GPU device, got {k.device}")
+        nb, bs, hkv, half = k.shape
+        slots = slots.contiguous()
+        n = slots.numel()
+        out = torch.empty((2, n, hkv, 2 * half), dtype=dtype, device=k.device)
+        with torch.cuda.device(k.device):
+            _native.lib().call("mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
+                               self.v_scale[layer].data_ptr(), nb, bs, hkv, 2 * half, slots.data_ptr(), n,
+                               _native.dtype_code(dtype), out[0].data_ptr(), out[1].data_ptr(),
+                               _native.stream_ptr(k.device))
+        return out[0], out[1]
 
     @staticmethod
     def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE) -> int:
-        """K and V, every layer: 2 x layers x block_size x KV heads x head_dim x bytes per element."""
+        """K and V, every layer: 2 x layers x block_size x KV heads x head_dim x bytes per element (4-bit pools: half a
+        byte, and a scale byte for 32 dims)."""
+        if dtype == FP4:
+            row = config.head_dim // 2 + config.head_dim // FP4_BLOCK
+            return 2 * config.num_hidden_layers * block_size * config.num_key_value_heads * row
         elem = torch.tensor([], dtype=dtype).element_size()
         return 2 * config.num_hidden_layers * block_size * config.num_key_value_heads * config.head_dim * elem
 

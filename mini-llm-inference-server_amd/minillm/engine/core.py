@@ -103,7 +103,7 @@ class EngineCore:
         passes the oracle's).  `chunked_prefill` mixes decode rows and prompt chunks in one step under the
         token budget (see Scheduler).  `kv_cache_dtype` defaults to the model's dtype; torch.float8_e4m3fn
         gives an fp8 pool whose K and V tensors of every layer use the per-tensor scales `kv_scales`
-        (k_scale, v_scale).  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
+        (k_scale, v_scale); torch.float4_e2m1fn_x2 gives a 4-bit pool with block scales.  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
         captured HIP graphs (DecodeGraphs); prefill and mixed steps stay eager.  `sampler(requests,
         logits)` picks each row's next token from its logits [rows, vocab] (default: greedy argmax); a
         row whose prompt chunk stops short of its end ignores its pick."""

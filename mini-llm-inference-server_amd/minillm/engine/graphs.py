@@ -83,7 +83,7 @@ class DecodeGraphs:
             pages = min(bucket * self.tables.max_blocks, self.cache.num_blocks + bucket)
             cap = self._capacity[bucket] = decode_records_bound(
                 pages, bucket, self.num_kv_heads, self.num_heads, self.cache.quantized, device_cus(self.device),
-                pad_pages=bucket)
+                pad_pages=bucket, kv_fp4=self.cache.fp4)
         return cap
 
     def fits(self, seqs: list[SeqStep]) -> bool:
@@ -126,7 +126,7 @@ class DecodeGraphs:
         split, runs 4-wavefront workgroups over them (the launch shape does not change a wavefront's
         arithmetic)."""
         return pages_per_split(pages, self.num_kv_heads, self.num_heads, self.cache.quantized,
-                               device_cus(self.device))
+                               device_cus(self.device), kv_fp4=self.cache.fp4)
 
     def _stage(self, c: _Captured, keys, seqs: list[SeqStep], token_ids: list[int]) -> None:
         bs = self.block_size

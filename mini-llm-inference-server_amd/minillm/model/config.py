@@ -15,7 +15,7 @@ from typing import Any
 # keys every config.json must hold, and the optional ones with the value taken when they are absent
 _REQUIRED_KEYS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_layers", "num_attention_heads",
                   "rms_norm_eps")
-_DEFAULTS = {"tie_word_embeddings": False, "max_position_embeddings": 8192}
+_DEFAULTS = {"tie_word_embeddings": False, "max_position_embeddings": 8192, "qk_norm": False}
 
 
 def _rope_fields(d: Mapping[str, Any]) -> tuple[float, dict[str, Any] | None]:
@@ -65,6 +65,7 @@ class LlamaConfig:
     tie_word_embeddings: bool = False
     max_position_embeddings: int = 8192
     eos_token_ids: tuple[int, ...] = field(default_factory=tuple)
+    qk_norm: bool = False  # RMSNorm of every query and key head before the rotation
 
     @property
     def num_kv_groups(self) -> int:

@@ -9,6 +9,7 @@ a submodule's `__call__` does nothing but its class's `forward`, so that a fused
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -16,7 +17,7 @@ from torch.autograd import forward_ad
 from torch.nn.modules import module as _module
 
 from .. import _native
-from ..attention.hip_backend import FP8, HipBackend
+from ..attention.hip_backend import FP4, FP8, HipBackend, check_norms, check_scales, layer_pool
 from ..cache.paged import PagedKVCache, PagedStep
 
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -94,6 +95,52 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dty
     _native.lib().call("mllm_rope_table", positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half,
                        _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr(), _native.stream_ptr(positions.device))
     return cos, sin
+
+
+def head_norms_ok(q_norm, k_norm, x: torch.Tensor, head_dim: int) -> bool:
+    """Whether the head norms of q and k may run with the rotation: two norms of one class and eps that do nothing but their
+    forward, plain weights of x's type."""
+    return (bare(q_norm, type(k_norm)) and bare(k_norm, type(q_norm)) and q_norm.eps == k_norm.eps
+            and all(m.weight.shape == (head_dim,) and _plain_weight(m.weight, x) for m in (q_norm, k_norm)))
+
+
+def qk_norm_rope_ok(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> bool:
+    """Whether `qk_norm_rope` takes the model's q (already `usable`), k and tables: its head sizes and row alignment, and
+    few enough tokens for one launch."""
+    b, h, t, dh = q.shape
+    rows = b * t * (h + k.shape[1])
+    lanes = 1 << max(0, dh // 16 - 1).bit_length()
+    return (dh % 16 == 0 and dh <= 1024 and 0 < rows * lanes <= MAX_GROUPS * 256
+            and all(type(x) is torch.Tensor and x.dtype == q.dtype and x.device == q.device and x.stride(-1) == 1
+                    and x.data_ptr() % 16 == 0 and not any(s % 8 for s in x.stride()[:-1]) for x in (q, k, cos, sin))
+            and cos.shape == (b, t, dh) == sin.shape)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head of q [B, H, T, Dh] and k [B, Hkv, T, Dh], then their rotation by cos and sin [B, T, Dh], in
+    one launch: fp32 arithmetic, one rounding.  Dh a multiple of 16, at most 1024; bfloat16 or float16 throughout."""
+    b, h, t, dh = q.shape
+    if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != (t, dh):
+        raise ValueError(f"k must be [B, Hkv, T, Dh] = [{b}, Hkv, {t}, {dh}] to match q")
+    if cos.shape != (b, t, dh) or sin.shape != (b, t, dh):
+        raise ValueError(f"cos and sin must be [B, T, Dh] = [{b}, {t}, {dh}]")
+    if any(x.dtype != q.dtype or x.device != q.device for x in (k, cos, sin)):
+        raise ValueError("q, k, cos and sin must share one dtype and device")
+    if q.dtype not in _DTYPES or q.device.type != "cuda":
+        raise ValueError("q must be bfloat16 or float16 on a GPU")
+    check_norms((q_weight, k_weight, eps), q)
+    q, k, cos, sin = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, cos, sin))
+    if sin.stride() != cos.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    q_out = torch.empty((b, h, t, dh), dtype=q.dtype, device=q.device)
+    k_out = torch.empty((b, k.shape[1], t, dh), dtype=q.dtype, device=q.device)
+    with torch.cuda.device(q.device):
+        _native.lib().call("mllm_qk_norm_rope", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], cos.data_ptr(),
+                           sin.data_ptr(), *cos.stride()[:2], q_weight.data_ptr(), k_weight.data_ptr(), eps, b, t, h,
+                           k.shape[1], dh, _native.dtype_code(q.dtype), q_out.data_ptr(), k_out.data_ptr(),
+                           _native.stream_ptr(q.device))
+    return q_out, k_out
 
 
 def sum_ok(x: torch.Tensor, y: torch.Tensor) -> bool:
@@ -212,15 +259,22 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     i = attn.layer_idx
     kc, vc = cache.k[i], cache.v[i]
     if not (kc.dim() == 4 and kc.shape == vc.shape and kc.dtype == vc.dtype and kc.device == vc.device == x.device
-            and kc.shape[2] == hkv and kc.shape[3] == dh and kc.shape[1] == meta.block_size and kc.is_contiguous()
+            and kc.shape[2] == hkv and kc.shape[3] * (2 if kc.dtype == FP4 else 1) == dh and kc.shape[1] == meta.block_size and kc.is_contiguous()
             and vc.is_contiguous() and n == meta.query_start_loc[-1]):
         return None
-    ks, vs = (cache.k_scale[i], cache.v_scale[i]) if cache.quantized else (1.0, 1.0)
-    if kc.dtype == FP8:
+    ks, vs = (cache.k_scale[i], cache.v_scale[i]) if cache.quantized or cache.fp4 else (1.0, 1.0)
+    if kc.dtype == FP4:
+        check_scales(kc, ks, vs)
+    elif kc.dtype == FP8:
         if not (0 < ks < math.inf and 0 < vs < math.inf):
             return None
     elif kc.dtype != x.dtype or ks != 1.0 or vs != 1.0:
         return None
+    qk_norm = None
+    if getattr(attn, "q_norm", None) is not None:  # heads normed in the launch that rotates
+        if not head_norms_ok(attn.q_norm, attn.k_norm, x, dh):
+            return None
+        qk_norm = (attn.q_norm.weight, attn.k_norm.weight, attn.q_norm.eps)
     lib, mlp = _native.lib(), layer.mlp
     gate = mlp.gate_proj.weight
     ffn = gate.shape[0]
@@ -228,9 +282,10 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
                           device=x.device)
     step = backend.layer_step(meta, n, h, x.dtype, kc)
     out = torch.empty_like(x)
-    lib.call("mllm_decoder_layer", step, x.data_ptr(), d, norm1.weight.data_ptr(), norm1.eps, wq.data_ptr(), wk.data_ptr(),
-             wv.data_ptr(), attn.o_proj.weight.data_ptr(), norm2.weight.data_ptr(), norm2.eps, gate.data_ptr(),
-             mlp.up_proj.weight.data_ptr(), mlp.down_proj.weight.data_ptr(), ffn, cos.data_ptr(), sin.data_ptr(),
-             dh, kc.data_ptr(), vc.data_ptr(), ks, vs, scratch.data_ptr(), scratch.numel(), out.data_ptr(),
+    pool = layer_pool(kc, vc, ks, vs, qk_norm)
+    lib.call("mllm_decoder_layer_pool", step, x.data_ptr(), d, norm1.weight.data_ptr(), norm1.eps, wq.data_ptr(),
+             wk.data_ptr(), wv.data_ptr(), attn.o_proj.weight.data_ptr(), norm2.weight.data_ptr(), norm2.eps,
+             gate.data_ptr(), mlp.up_proj.weight.data_ptr(), mlp.down_proj.weight.data_ptr(), ffn, cos.data_ptr(),
+             sin.data_ptr(), dh, ctypes.addressof(pool), scratch.data_ptr(), scratch.numel(), out.data_ptr(),
              _native.stream_ptr(x.device))
     return out

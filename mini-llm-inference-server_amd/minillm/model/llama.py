@@ -81,6 +81,9 @@ class LlamaAttention(nn.Module):
         self.k_proj = nn.Linear(d, hkv * dh, bias=False)
         self.v_proj = nn.Linear(d, hkv * dh, bias=False)
         self.o_proj = nn.Linear(h * dh, d, bias=False)
+        # RMSNorm of every query and key head before the rotation (config.qk_norm)
+        self.q_norm = RMSNorm(dh, config.rms_norm_eps) if config.qk_norm else None
+        self.k_norm = RMSNorm(dh, config.rms_norm_eps) if config.qk_norm else None
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kv_cache=None,
                 key_valid: torch.Tensor | None = None) -> torch.Tensor:
@@ -98,25 +101,45 @@ class LlamaAttention(nn.Module):
         else:
             q, k, v = q_proj(x), k_proj(x), v_proj(x)
         q, k, v = (p.view(b, t, -1, dh).transpose(1, 2) for p in (q, k, v))
-        if getattr(kv_cache, "ragged", False):
-            # ragged step: one row of every sequence's new tokens -> [N, heads, Dh] views for the backend
-            layer = self.layer_idx
-            pools = (kv_cache.cache.k[layer], kv_cache.cache.v[layer], kv_cache.meta)
-            scales = kv_cache.cache.scales(layer)  # fp8 pools only
-            if getattr(self.backend, "fuse_rotary", False) and b == 1:
-                # the backend rotates q and k itself, in the launch that appends k and v
-                out = self.backend.forward_rotary(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1),
-                                                  cos[0], sin[0], *pools, **scales)
-            else:
-                q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
-                out = self.backend.forward(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), *pools,
-                                           **scales)
-            return out.reshape(b, t, -1)
+        ragged = getattr(kv_cache, "ragged", False)
+        fused_norms = {}
+        if getattr(self, "q_norm", None) is not None:
+            if kernels.usable(q) and kernels.head_norms_ok(self.q_norm, self.k_norm, q, dh):
+                norms = (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps)
+                if ragged and getattr(self.backend, "fuse_rotary", False) and b == 1:
+                    fused_norms = {"qk_norm": norms}  # in the backend's launch that rotates and appends
+                elif not ragged and kv_cache is None and kernels.qk_norm_rope_ok(q, k, cos, sin):
+                    q, k = kernels.qk_norm_rope(q, k, cos, sin, *norms)
+                    return self._contiguous(q, k, v, key_valid)
+            if not fused_norms:
+                q, k = self.q_norm(q), self.k_norm(k)
+        if ragged:
+            return self._paged(q, k, v, cos, sin, kv_cache, fused_norms)
         q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
         if kv_cache is not None:
             raise ValueError("only paged ragged caches (PagedStep) are supported")
+        return self._contiguous(q, k, v, key_valid)
+
+    def _contiguous(self, q, k, v, key_valid) -> torch.Tensor:
+        b, _, t, _ = q.shape
         out = self.backend.prefill(q, k, v, key_valid=key_valid)
         return out.transpose(1, 2).reshape(b, t, -1)
+
+    def _paged(self, q, k, v, cos, sin, kv_cache, fused_norms: dict) -> torch.Tensor:
+        """Ragged step: one row of every sequence's new tokens -> [N, heads, Dh] views for the backend."""
+        b, _, t, _ = q.shape
+        layer = self.layer_idx
+        pools = (kv_cache.cache.k[layer], kv_cache.cache.v[layer], kv_cache.meta)
+        scales = kv_cache.cache.scales(layer)  # fp8 and 4-bit pools
+        if getattr(self.backend, "fuse_rotary", False) and b == 1:
+            # the backend rotates q and k itself, in the launch that appends k and v
+            out = self.backend.forward_rotary(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1),
+                                              cos[0], sin[0], *pools, **scales, **fused_norms)
+        else:
+            q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
+            out = self.backend.forward(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), *pools,
+                                       **scales)
+        return out.reshape(b, t, -1)
 
 
 class LlamaMLP(nn.Module):
