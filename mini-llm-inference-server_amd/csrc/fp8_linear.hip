@@ -1,0 +1,397 @@
+// Linear layers of 8-bit blocks: y[M, N] = x[M, K] . w[N, K]^T with e4m3 codes and one power-of-two scale (e8m0) for
+// 128 x 128 weights and for 128 columns of a row of x, which is quantised here (no counterpart in the reference).
+//   sx = the least power of two with max|x_block| / sx <= 448, xq = e4m3(x / sx), to nearest with ties to even
+//   y[m][n] = T( sum_b sx[m][b] sw[n / 128][b] sum_{k in block b} xq[m][k] wq[n][k] )
+// Every step but the rounding to e4m3 and the fp32 sums is exact.  v_mfma_scale_f32_16x16x128_f8f6f4 takes a block per
+// instruction and applies both scales, so the accumulators run through K without a vector instruction.  An infinity or a
+// NaN in a block of x makes its scale, and the row's outputs, NaN.
+//
+// MFMA operands: lane (n, g) = (l % 16, l / 16) holds row n's bytes 16 g .. + 15 and 64 + 16 g .. + 15 of the block, of the
+// weights and of x alike (the order of k within a block does not matter: one scale covers it).  Weights are the A operand, so
+// a lane ends with four consecutive outputs of one row of y.
+#include <math.h>
+
+#include "common.h"
+
+namespace mllm {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kBlock = 128;    // K per scale, and rows of weights
+constexpr int kFewRows = 64;   // rows of x up to which the weight-streaming kernel runs
+
+__device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+template <int OPSEL_X>
+__device__ __forceinline__ f32x4 mfma_fp8(i32x8 w, i32x8 x, f32x4 c, int sw, int sx) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, sw, OPSEL_X, sx);
+}
+
+// A byte at a uniform address, as a scalar load of the dword that holds it.
+__device__ __forceinline__ int scalar_byte(const uint8_t* at) {
+  typedef const __attribute__((address_space(4))) uint32_t ConstU32;
+  const uintptr_t p = (uintptr_t)at;
+  return (int)((*(ConstU32*)(p & ~(uintptr_t)3) >> (8 * (p & 3))) & 0xffu);
+}
+
+// ---------------------------------------------------------------- quantisation of x
+
+// Largest of the 16-bit patterns without their sign (they order as the magnitudes do; infinities and NaN are on top).
+__device__ __forceinline__ uint32_t max_abs16(u32x4 x, uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+  return m;
+}
+// Scale exponent of a block whose largest 16-bit pattern is m: 448 = 1.75 2^8, so floor(log2) - 8, one more where the
+// mantissa is above 1.75.
+template <typename T>
+__device__ __forceinline__ uint32_t x_scale_exp(uint32_t m);
+template <>
+__device__ __forceinline__ uint32_t x_scale_exp<BF16>(uint32_t m) {
+  const uint32_t u = m << 16;
+  if (u >= 0x7f800000u) return 255u;
+  return (uint32_t)max((int)((u + 0x1fffffu) >> 23) - 8, 1);
+}
+template <>
+__device__ __forceinline__ uint32_t x_scale_exp<F16>(uint32_t m) {
+  const uint32_t u = __float_as_uint(f16_bits_to_f32((uint16_t)m));
+  if (u >= 0x7f800000u) return 255u;
+  return (uint32_t)max((int)((u + 0x1fffffu) >> 23) - 8, 1);
+}
+// Four 16-bit values (two dwords) -> four e4m3 codes of x / scale.
+template <typename T>
+__device__ __forceinline__ uint32_t quant4_e4m3(uint32_t a, uint32_t b, float scale);
+template <>
+__device__ __forceinline__ uint32_t quant4_e4m3<BF16>(uint32_t a, uint32_t b, float scale) {
+  i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(i16x2{0, 0}, __builtin_bit_cast(bf16x2, a), scale, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, b), scale, true));
+}
+template <>
+__device__ __forceinline__ uint32_t quant4_e4m3<F16>(uint32_t a, uint32_t b, float scale) {
+  i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(i16x2{0, 0}, __builtin_bit_cast(f16x2, a), scale, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, b), scale, true));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 quant16_e4m3(u32x4 lo, u32x4 hi, uint32_t e) {
+  const float s = __uint_as_float(e << 23);
+  return u32x4{quant4_e4m3<T>(lo[0], lo[1], s), quant4_e4m3<T>(lo[2], lo[3], s), quant4_e4m3<T>(hi[0], hi[1], s),
+               quant4_e4m3<T>(hi[2], hi[3], s)};
+}
+
+// ---------------------------------------------------------------- few rows: the weights streamed once
+
+struct RowsArgs {
+  const char* x;  // bytes
+  int64_t x_st;   // row stride, bytes
+  int M, K, N, blocks;
+  const char* w;  // [N][128 blocks]
+  const uint8_t* ws;
+  uint16_t* y;
+};
+
+constexpr int kRowsWaves = 8;
+
+// One workgroup per 16 weight rows, eight wavefronts along K.  Bound by the weights, N K bytes read once; each wavefront
+// quantises its own columns of x, so there is one launch and no exchange but the eight partial sums in LDS.
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * kRowsWaves) void fp8_rows_kernel(const RowsArgs a) {
+  __shared__ f32x4 red[kRowsWaves][MT][64];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = 16 * blockIdx.x;
+  const int first = a.blocks * wave / kRowsWaves, end = a.blocks * (wave + 1) / kRowsWaves;
+  const char* wp = a.w + (int64_t)min(n0 + n, a.N - 1) * a.blocks * kBlock + 16 * g;
+  const uint8_t* ws = a.ws + (int64_t)(n0 / kBlock) * a.blocks;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const char* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xp[m] = a.x + min(16 * m + n, a.M - 1) * a.x_st;
+  constexpr int kAhead = 4;  // blocks of weights in flight
+  u32x4 w[kAhead][2];
+  auto load_w = [&](u32x4 (&r)[2], int b) {
+    r[0] = ld16_nt(wp + (int64_t)b * kBlock);
+    r[1] = ld16_nt(wp + (int64_t)b * kBlock + 64);
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (first + u < end) load_w(w[u], first + u);
+  for (int b0 = first; b0 < end; b0 += kAhead) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int b = b0 + u;
+      if (b >= end) break;
+      const i32x8 wv = join(w[u][0], w[u][1]);
+      const int sw = scalar_byte(ws + b);
+      const int k0 = b * kBlock + 16 * g;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        u32x4 v[4] = {};
+        if (k0 < a.K) {  // K is a multiple of 16: a lane's 16 columns are all there or none
+          v[0] = ld16(xp[m] + 2 * k0);
+          v[1] = ld16(xp[m] + 2 * k0 + 16);
+        }
+        if (k0 + 64 < a.K) {
+          v[2] = ld16(xp[m] + 2 * k0 + 128);
+          v[3] = ld16(xp[m] + 2 * k0 + 144);
+        }
+        uint32_t top = max_abs16(v[3], max_abs16(v[2], max_abs16(v[1], max_abs16(v[0], 0u))));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        const uint32_t e = x_scale_exp<T>(top);
+        acc[m] = mfma_fp8<0>(wv, join(quant16_e4m3<T>(v[0], v[1], e), quant16_e4m3<T>(v[2], v[3], e)), acc[m], sw, (int)e);
+      }
+      if (b + kAhead < end) load_w(w[u], b + kAhead);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
+  __syncthreads();
+  const int i = threadIdx.x;
+  if (i >= 64 * MT) return;
+  const int m = 16 * (i >> 6) + n, col = n0 + 4 * g;  // lane (n, g): row m of y, outputs 4 g .. + 3 of the tile
+  f32x4 s = red[0][i >> 6][lane];
+#pragma unroll
+  for (int k = 1; k < kRowsWaves; ++k) s += red[k][i >> 6][lane];
+  if (m < a.M && col < a.N) st8(a.y + (int64_t)m * a.N + col, u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])});
+}
+
+// ---------------------------------------------------------------- many rows: x quantised once, then tiles
+
+// xq [M][128 blocks] codes; scales as the tile kernel's lanes read them: sx[block][row / 64][row % 16] is a dword, byte
+// (row / 16) % 4 of it the row's scale.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_quant_kernel(const char* __restrict__ x, int64_t x_st, unsigned M, int K, int blocks,
+                                                       char* __restrict__ xq, uint8_t* __restrict__ sx, unsigned groups64) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;  // 16 columns each, eight threads a block
+  const unsigned per_row = 8u * (unsigned)blocks;
+  const unsigned m = i / per_row, c = i - m * per_row;
+  if (m >= M) return;
+  const int k0 = 16 * (int)c;
+  u32x4 lo = {0, 0, 0, 0}, hi = lo;
+  if (k0 < K) {
+    lo = ld16(x + m * x_st + 2 * k0);
+    hi = ld16(x + m * x_st + 2 * k0 + 16);
+  }
+  uint32_t top = max_abs16(hi, max_abs16(lo, 0u));
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  const uint32_t e = x_scale_exp<T>(top);
+  st16(xq + 16 * (int64_t)i, quant16_e4m3<T>(lo, hi, e));
+  if ((c & 7) == 0) sx[((int64_t)(c >> 3) * groups64 + (m >> 6)) * 64 + 4 * (m & 15) + ((m >> 4) & 3)] = (uint8_t)e;
+}
+
+struct TileArgs {
+  const char* xq;
+  const uint8_t* sx;
+  const char* w;
+  const uint8_t* ws;
+  int M, N, blocks, groups64;
+  int tiles_n, tiles_m, ksplit;
+  uint16_t* y;
+  float* part;  // ksplit > 1: [ksplit][M][N]
+};
+
+// y tile of BN weight rows x BM rows of x per workgroup, WN x WM wavefronts of (BN / WN) x (BM / WM) each.  Codes go through
+// LDS by DMA, a block of K (128 bytes a row) per step, double buffered; 16-byte piece j of row r lies at j ^ (r % 8), so
+// that eight lanes of an operand read hit distinct banks.
+template <typename T, int BN, int BM, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a) {
+  constexpr int kWaves = WN * WM;
+  constexpr int kA = BN * kBlock, kB = BM * kBlock, kStage = kA + kB + 4 * 64 * (BM / 256 ? BM / 256 : 1);
+  constexpr int FN = BN / WN / 16, FM = BM / WM / 16;  // 16-row operands per wavefront
+  static_assert(BM / WM == 64, "a wavefront's rows of x share one dword of scales per lane");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave % WN, wm = wave / WN;
+
+  // workgroups are dealt round-robin to the 8 XCDs: each takes a contiguous run of the tiles, ordered in bands of four
+  // tiles of weights, so that the workgroups of one L2 share both operands
+  const int tiles = a.tiles_n * a.tiles_m;
+  const int ks = blockIdx.x / tiles, id = blockIdx.x % tiles;
+  const int per = tiles / 8, rest = tiles % 8, xcd = id % 8;
+  const int t = xcd * per + min(xcd, rest) + id / 8;
+  const int band = t / (4 * a.tiles_m), bn = min(4, a.tiles_n - 4 * band), in = t - 4 * a.tiles_m * band;
+  const int n0 = BN * (4 * band + in % bn), m0 = BM * (in / bn);
+  const int first = a.blocks * ks / a.ksplit, steps = a.blocks * (ks + 1) / a.ksplit - first;
+
+  const int64_t row_bytes = (int64_t)a.blocks * kBlock;
+  const char* wbase = a.w + n0 * row_bytes + (int64_t)first * kBlock;
+  const char* xbase = a.xq + m0 * row_bytes + (int64_t)first * kBlock;
+  // one DMA instruction fills 1 KB: 8 rows, lane l row l / 8, place l % 8
+  constexpr int kDmaA = BN / 8 / kWaves, kDmaB = BM / 8 / kWaves;
+  const int dr = lane >> 3, dc = (lane & 7) ^ dr;
+  unsigned offa[kDmaA], offb[kDmaB];
+#pragma unroll
+  for (int i = 0; i < kDmaA; ++i)
+    offa[i] = (unsigned)min(8 * (kDmaA * wave + i) + dr, a.N - 1 - n0) * (unsigned)row_bytes + 16u * dc;
+#pragma unroll
+  for (int i = 0; i < kDmaB; ++i)
+    offb[i] = (unsigned)min(8 * (kDmaB * wave + i) + dr, a.M - 1 - m0) * (unsigned)row_bytes + 16u * dc;
+  // scales of the tile's rows of x: BM bytes, 64 to a row group; groups past the last repeat it
+  const unsigned offs = 64u * (unsigned)min(m0 / 64 + lane / 16, a.groups64 - 1) + 4u * (lane & 15);
+  auto load = [&](int s) {
+    char* st = lds + (s & 1) * kStage;
+    const char* wb = wbase + (int64_t)s * kBlock;
+    const char* xb = xbase + (int64_t)s * kBlock;
+#pragma unroll
+    for (int i = 0; i < kDmaA; ++i) dma16(wb, offa[i], lds_offset(st) + 1024 * (kDmaA * wave + i));
+#pragma unroll
+    for (int i = 0; i < kDmaB; ++i) dma16(xb, offb[i], lds_offset(st + kA) + 1024 * (kDmaB * wave + i));
+    if (wave == 0) dma4(reinterpret_cast<const char*>(a.sx) + (int64_t)(first + s) * a.groups64 * 64, offs, lds_offset(st + kA + kB));
+  };
+
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nb0 = (n0 + wn * (BN / WN)) / kBlock;  // the wavefront's weights lie in one row of blocks (past N: repeated)
+  const uint8_t* wsrow = a.ws + (int64_t)min(nb0, (a.N - 1) / kBlock) * a.blocks + first;
+  const int rl = n & 7, c0 = 16 * (g ^ rl), c1 = 16 * ((4 + g) ^ rl);
+  load(0);
+  barrier_vm<0>();
+  for (int s = 0; s < steps; ++s) {
+    if (s + 1 < steps) load(s + 1);
+    const char* st = lds + (s & 1) * kStage;
+    const char* pa = st + (wn * (BN / WN) + n) * kBlock;
+    const char* pb = st + kA + (wm * 64 + n) * kBlock;
+    const int sx = *reinterpret_cast<const int*>(st + kA + kB + 64 * wm + 4 * n);
+    const int sw = scalar_byte(wsrow + s);
+    i32x8 xb[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) xb[j] = join(ld16(pb + 16 * j * kBlock + c0), ld16(pb + 16 * j * kBlock + c1));
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const i32x8 wv = join(ld16(pa + 16 * i * kBlock + c0), ld16(pa + 16 * i * kBlock + c1));
+      acc[i][0] = mfma_fp8<0>(wv, xb[0], acc[i][0], sw, sx);
+      acc[i][1] = mfma_fp8<1>(wv, xb[1], acc[i][1], sw, sx);
+      acc[i][2] = mfma_fp8<2>(wv, xb[2], acc[i][2], sw, sx);
+      acc[i][3] = mfma_fp8<3>(wv, xb[3], acc[i][3], sw, sx);
+    }
+    barrier_vm<0>();
+  }
+#pragma unroll
+  for (int i = 0; i < FN; ++i) {
+    const int col = n0 + wn * (BN / WN) + 16 * i + 4 * g;
+    if (col >= a.N) continue;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int m = m0 + wm * 64 + 16 * j + n;
+      if (m >= a.M) continue;
+      const f32x4 v = acc[i][j];
+      if (a.ksplit > 1)
+        *reinterpret_cast<f32x4*>(a.part + ((int64_t)ks * a.M + m) * a.N + col) = v;
+      else
+        st8(a.y + (int64_t)m * a.N + col, u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])});
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launch rules
+
+struct Plan {
+  bool few, large;
+  int ksplit;
+  int64_t xq_bytes, sx_bytes, part_bytes;
+};
+constexpr int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+Plan plan_linear(int64_t m, int64_t n, int64_t blocks, int cus) {
+  Plan p{};
+  p.few = m <= kFewRows;
+  if (p.few) return p;
+  const int64_t large = ((n + 255) / 256) * ((m + 255) / 256), small = ((n + 127) / 128) * ((m + 127) / 128);
+  p.large = large * 4 >= 3 * (int64_t)cus;
+  p.ksplit = 1;
+  if (!p.large && small < cus) {
+    int64_t ks = cus / small;
+    if (ks > 8) ks = 8;
+    if (ks > blocks / 4) ks = blocks / 4;
+    p.ksplit = ks < 1 ? 1 : (int)ks;
+  }
+  p.xq_bytes = align256(m * blocks * kBlock);
+  p.sx_bytes = align256(blocks * ((m + 63) / 64) * 64);
+  p.part_bytes = p.ksplit > 1 ? align256(4 * p.ksplit * m * n) : 0;
+  return p;
+}
+
+}  // namespace
+}  // namespace mllm
+
+extern "C" int64_t mllm_fp8_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t num_cus) {
+  using namespace mllm;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const Plan p = plan_linear(m, n, (k + kBlock - 1) / kBlock, num_cus > 0 ? num_cus : device_cus());
+  return p.xq_bytes + p.sx_bytes + p.part_bytes;
+}
+
+extern "C" int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64_t k, const void* weight,
+                               const void* weight_scales, int64_t n, int32_t dtype, void* workspace,
+                               int64_t workspace_bytes, void* out, void* stream) {
+  using namespace mllm;
+  const std::string fn = "mllm_fp8_linear";
+  MLLM_REQUIRE(dtype == MLLM_DTYPE_BF16 || dtype == MLLM_DTYPE_F16, MLLM_ERR_UNSUPPORTED,
+               fn + ": dtype must be bfloat16 or float16");
+  MLLM_REQUIRE(m >= 0 && n > 0 && k > 0, MLLM_ERR_INVALID, fn + ": bad sizes");
+  MLLM_REQUIRE(k % 16 == 0 && n % 16 == 0, MLLM_ERR_UNSUPPORTED, fn + ": k and n must be multiples of 16");
+  // 32-bit offsets within a tile of 256 rows; launches below 2^31 workgroups
+  MLLM_REQUIRE(k <= (1 << 23) && n < (1 << 28) && m < (1ll << 31) - 256, MLLM_ERR_UNSUPPORTED, fn + ": sizes too large");
+  if (m == 0) return MLLM_OK;
+  MLLM_REQUIRE(x && weight && weight_scales && out, MLLM_ERR_INVALID, fn + ": null pointer");
+  MLLM_REQUIRE(((uintptr_t)x | (uintptr_t)weight | (uintptr_t)out) % 16 == 0 && x_stride % 8 == 0 &&
+                   (uintptr_t)weight_scales % 4 == 0,
+               MLLM_ERR_UNSUPPORTED, fn + ": operands must be 16-byte aligned");
+  const int blocks = (int)((k + kBlock - 1) / kBlock);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const Plan p = plan_linear(m, n, blocks, device_cus());
+  if (p.few) {
+    RowsArgs a{(const char*)x, 2 * x_stride, (int)m, (int)k, (int)n, blocks, (const char*)weight, (const uint8_t*)weight_scales,
+               (uint16_t*)out};
+    auto launch = [&](auto tag) {
+      using T = decltype(tag);
+      const unsigned grid = (unsigned)(n / 16);
+      if (m <= 16)
+        fp8_rows_kernel<T, 1><<<grid, 64 * kRowsWaves, 0, st>>>(a);
+      else if (m <= 32)
+        fp8_rows_kernel<T, 2><<<grid, 64 * kRowsWaves, 0, st>>>(a);
+      else
+        fp8_rows_kernel<T, 4><<<grid, 64 * kRowsWaves, 0, st>>>(a);
+    };
+    if (dtype == MLLM_DTYPE_BF16)
+      launch(BF16{});
+    else
+      launch(F16{});
+    return check_launch(fn.c_str());
+  }
+  MLLM_REQUIRE(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= p.xq_bytes + p.sx_bytes + p.part_bytes,
+               MLLM_ERR_INVALID, fn + ": workspace too small or not 256-byte aligned");
+  const int64_t quant_groups = (m * blocks * 8 + 255) / 256;
+  const int64_t bn = p.large ? 256 : 128;
+  const int64_t tiles_n = (n + bn - 1) / bn, tiles_m = (m + bn - 1) / bn, groups = tiles_n * tiles_m * p.ksplit;
+  MLLM_REQUIRE(quant_groups <= kMaxGroups256 && groups <= kMaxGroups256 / 2, MLLM_ERR_UNSUPPORTED, fn + ": too many rows");
+  char* base = static_cast<char*>(workspace);
+  TileArgs a{base, (const uint8_t*)base + p.xq_bytes, (const char*)weight, (const uint8_t*)weight_scales, (int)m, (int)n, blocks,
+             (int)((m + 63) / 64), (int)tiles_n, (int)tiles_m, p.ksplit, (uint16_t*)out, (float*)(base + p.xq_bytes + p.sx_bytes)};
+  auto launch = [&](auto tag) {
+    using T = decltype(tag);
+    fp8_quant_kernel<T><<<(unsigned)quant_groups, 256, 0, st>>>((const char*)x, 2 * x_stride, (unsigned)m, (int)k, blocks, base,
+                                                               (uint8_t*)base + p.xq_bytes, (unsigned)a.groups64);
+    if (p.large)
+      fp8_tile_kernel<T, 256, 256, 2, 4><<<(unsigned)groups, 512, 0, st>>>(a);
+    else
+      fp8_tile_kernel<T, 128, 128, 2, 2><<<(unsigned)groups, 256, 0, st>>>(a);
+  };
+  if (dtype == MLLM_DTYPE_BF16)
+    launch(BF16{});
+  else
+    launch(F16{});
+  const int rc = check_launch(fn.c_str());
+  if (rc != MLLM_OK || p.ksplit == 1) return rc;
+  return mllm_sum_partials(a.part, p.ksplit, m, n, nullptr, dtype, out, stream);
+}

@@ -27,12 +27,13 @@ _transform = torch._C._functorch.peek_interpreter_stack  # the innermost active 
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor  # also of a wrapper that outlived its transform
 
 
-def usable(x: torch.Tensor, dtype: torch.dtype | None = None) -> bool:
-    """`dtype`: the type of the call's operands where x is not one of them.  Whether a compiler is at work is asked first:
+def usable(x: torch.Tensor, dtype: torch.dtype | None = None, grad_ok: bool = False) -> bool:
+    """`dtype`: the type of the call's operands where x is not one of them.  `grad_ok`: the caller has refused inputs that need
+    a gradient, so gradients may be on.  Whether a compiler is at work is asked first:
     dynamo knows that answer while it traces and leaves out the rest, some of which it cannot trace.  Inside a transform
     (vmap and the like) any operand may be a wrapper without storage, not only x, so none is let through."""
     return (not torch.compiler.is_compiling() and type(x) is torch.Tensor and x.is_cuda
-            and (dtype or x.dtype) in _DTYPES and not torch.is_grad_enabled() and not torch.is_autocast_enabled()
+            and (dtype or x.dtype) in _DTYPES and (grad_ok or not torch.is_grad_enabled()) and not torch.is_autocast_enabled()
             and not torch._C._len_torch_dispatch_stack() and not torch._C._len_torch_function_stack()
             and _transform() is None and not _wrapped(x) and forward_ad._current_level < 0 and not torch.jit.is_tracing()
             and x.device.index == torch.cuda.current_device() and _native.available())

@@ -1,0 +1,157 @@
+"""Linear layers of 8-bit blocks without a GPU: the torch path against the definition in float64, and refusals."""
+
+import pytest
+import torch
+
+from minillm import _native
+from minillm.model import fp8
+from minillm.model.fp8 import Fp8Linear, quantize_, quantize_blocks, quantize_rows
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    if not _native.LIB_PATH.exists():
+        import build_hip
+
+        build_hip.build()
+
+
+def values(codes, e):
+    """codes [..., B] and e8m0 scales [...] -> float64 values."""
+    return codes.double() * torch.exp2(e.view(torch.uint8).double() - 127)[..., None]
+
+
+def nearest_e4m3(y):
+    """y (float64, |y| <= 448) to the nearest of e4m3's 253 finite values, a tie to the even code."""
+    grid = torch.arange(127, dtype=torch.uint8).view(E4M3).double()
+    d = (y.abs()[..., None] - grid).abs()
+    near = d == d.amin(-1, keepdim=True)
+    even = near.clone()
+    even[..., 1::2] = False
+    pick = torch.where(even.any(-1), even.double().argmax(-1), near.double().argmax(-1))
+    return grid[pick] * torch.sign(y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_are_quantised_by_the_definition(dtype):
+    g = torch.Generator().manual_seed(0)
+    x = (torch.randn(40, 400, generator=g) * torch.exp(4 * torch.randn(40, 1, generator=g)) * 0.01).to(dtype)
+    x[0], x[1, :128], x[2, 5], x[3, 130] = 0, 448.0, 449.0, 448.0
+    codes, e = quantize_rows(x)
+    assert codes.shape == (40, 512) and e.shape == (40, 4) and codes.dtype == E4M3 and e.dtype == E8M0
+    b = torch.nn.functional.pad(x.double(), (0, 112)).view(40, 4, 128)
+    s = torch.exp2(e.view(torch.uint8).double() - 127)
+    amax = b.abs().amax(-1)
+    assert bool((amax <= 448 * s).all()) and bool((amax[amax > 0] > 224 * s[amax > 0]).all())  # the least power of two
+    assert torch.equal(values(codes.view(40, 4, 128), e), nearest_e4m3(b / s[..., None]) * s[..., None])
+
+
+def test_blocks_that_are_not_finite():
+    x = torch.ones(3, 256)
+    x[1, 3], x[2, 200] = float("inf"), float("nan")
+    codes, e = quantize_rows(x)
+    assert e.view(torch.uint8)[:, 0].tolist()[1] == 255 and e.view(torch.uint8)[2].tolist()[1] == 255
+    y = Fp8Linear.from_linear(torch.nn.Linear(256, 16, bias=False))(x)
+    assert torch.isfinite(y[0]).all() and torch.isnan(y[1:]).all()
+
+
+@pytest.mark.parametrize("n,k", [(16, 16), (272, 400), (128, 128), (48, 1040)])
+def test_layer_is_the_product_of_the_quantised_values(n, k):
+    torch.manual_seed(n)
+    lin = torch.nn.Linear(k, n, bias=False)
+    layer = Fp8Linear.from_linear(lin)
+    codes, s = quantize_blocks(lin.weight.detach())
+    w = codes.double() * torch.exp2(s.view(torch.uint8).double() - 127).repeat_interleave(128, 0)[:n] \
+        .repeat_interleave(128, 1)[:, :k]
+    assert torch.equal(layer.dequantized().double(), w)
+    assert bool(((w - lin.weight.double()).abs() <= 2.0 ** -4 * lin.weight.double().abs() + 2.0 ** -10 * lin.weight.abs().max()).all())
+    x = torch.randn(2, 3, k)
+    with torch.no_grad():
+        y = layer(x)
+    c, e = quantize_rows(x.view(6, k))
+    v = values(c.view(6, -1, 128), e).flatten(1)[:, :k]
+    # fp32 sums of k products: each addition is off by at most 2^-24 of the magnitudes' sum
+    bound = k * 2.0 ** -24 * (v.abs() @ w.abs().t()) + 2.0 ** -24 * (v @ w.t()).abs()
+    assert bool(((y.view(6, n).double() - v @ w.t()).abs() <= bound).all())
+    assert layer(x[:0]).shape == (0, 3, n)
+
+
+def test_state_round_trip_and_parts():
+    layer = Fp8Linear.from_linear(torch.nn.Linear(400, 272, bias=False))
+    assert layer.weight.shape == (272, 512) and bool((layer.weight.view(torch.uint8)[:, 400:] == 0).all())
+    other = Fp8Linear(400, 272)
+    other.load_state_dict(layer.state_dict())
+    x = torch.randn(2, 400)
+    assert torch.equal(other(x), layer(x)) and "in_features=400" in repr(layer)
+    codes = torch.zeros(32, 256).to(E4M3)
+    kept = Fp8Linear.from_parts(codes, torch.full((1, 2), 127, dtype=torch.uint8).view(E8M0))
+    assert kept.weight.data_ptr() == codes.data_ptr()  # not copied
+
+
+def test_refusals():
+    codes, s = quantize_blocks(torch.randn(32, 256))
+    for bad in ((codes.view(torch.uint8), s), (codes[0], s)):
+        with pytest.raises(ValueError, match="float8_e4m3fn"):
+            Fp8Linear.from_parts(*bad)
+    for bad in (s.view(torch.uint8), s[:, :1], s.t()):
+        with pytest.raises(ValueError, match="weight_scale"):
+            Fp8Linear.from_parts(codes, bad)
+    for n, k in ((16, 24), (8, 16), (0, 16)):
+        with pytest.raises(ValueError, match="multiples of 16"):
+            Fp8Linear(k, n)
+    with pytest.raises(ValueError, match="no bias"):
+        Fp8Linear.from_linear(torch.nn.Linear(16, 16))
+    layer = Fp8Linear.from_parts(codes, s)
+    with pytest.raises(ValueError, match="256 columns"):
+        layer(torch.randn(3, 128))
+    with pytest.raises(RuntimeError, match="inference"):
+        layer(torch.randn(3, 256, requires_grad=True))
+    with torch.no_grad():
+        layer(torch.randn(3, 256, requires_grad=True))
+
+
+def test_entry_point_checks_its_arguments():
+    lib = _native.lib()
+    a = 1 << 20  # an aligned address that nothing reads: every call below is refused before its launch
+
+    def call(x=a, stride=256, m=100, k=256, w=a, s=a, n=256, dtype=2, ws=None, size=0, out=a):
+        lib.call("mllm_fp8_linear", x, stride, m, k, w, s, n, dtype, ws, size, out, None)
+
+    for kw, match in ((dict(dtype=0), "bfloat16 or float16"), (dict(k=0), "bad sizes"), (dict(m=-1), "bad sizes"),
+                      (dict(k=264), "multiples of 16"), (dict(n=250), "multiples of 16"), (dict(k=1 << 24), "too large"),
+                      (dict(x=None), "null pointer"), (dict(s=None), "null pointer"), (dict(x=a + 2), "aligned"),
+                      (dict(stride=257), "aligned"), (dict(s=a + 1), "aligned"), (dict(), "workspace"),
+                      (dict(ws=a + 16, size=1 << 40), "workspace"), (dict(ws=a, size=1), "workspace")):
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+    call(m=0, x=None, w=None, s=None, out=None)
+    need = lib.fn("mllm_fp8_linear_workspace_bytes")
+    assert need(0, 256, 256, 256) == 0 and need(64, 4096, 4096, 256) == 0 < need(65, 4096, 4096, 256)
+    assert need(8192, 4096, 4096, 256) >= 8192 * (4096 + 32)
+    assert fp8.FEW_ROWS == 64 and need(fp8.FEW_ROWS, 16, 16, 256) == 0 < need(fp8.FEW_ROWS + 1, 16, 16, 256)
+
+
+def test_quantize_model():
+    from minillm.attention.base import AttentionBackend
+    from minillm.model.config import LlamaConfig
+    from minillm.model.llama import LlamaForCausalLM, random_init_
+
+    class Causal(AttentionBackend):
+        def prefill(self, q, k, v, key_valid=None, **kwargs):
+            g = q.shape[1] // k.shape[1]
+            return torch.nn.functional.scaled_dot_product_attention(q, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1),
+                                                                    is_causal=True)
+
+        def forward(self, *args):
+            raise NotImplementedError
+
+    cfg = LlamaConfig(vocab_size=96, hidden_size=64, intermediate_size=144, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=16, rms_norm_eps=1e-5, rope_theta=1e4, qk_norm=True)
+    model = random_init_(LlamaForCausalLM(cfg, Causal()))
+    assert quantize_(model) is model and quantize_(model) is model  # a second time changes nothing
+    kinds = [type(m).__name__ for m in model.modules()]
+    assert kinds.count("Fp8Linear") == 14 and kinds.count("Linear") == 1
+    with torch.no_grad():
+        assert torch.isfinite(model(torch.arange(20)[None])).all()
