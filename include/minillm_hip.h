@@ -425,7 +425,7 @@ int mllm_paged_prefill_fp8(const void* q, int64_t q_stride_tok, int64_t q_stride
  * in fp8 and 512 in 16 bits.  OCP microscaling: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives), two to a byte with
  * the even dim in the low half, and one e8m0 scale for 32 consecutive dims of a token and head.
  *   codes     [num_blocks, block_size, Hkv, Dh / 2] bytes
- *   k_scales  [num_blocks, block_size, Hkv, Dh / 32] bytes
+ *   k_scales  [num_blocks, block_size, Dh / 32, Hkv] bytes
  *   v_scales  [num_blocks, Hkv, Dh / 32, block_size] bytes
  *   value = e2m1(code) * 2^(scale - 127); scale 255: NaN
  * A block is stored under the least power of two below which its largest magnitude rounds to at most 6 (its magnitude is
@@ -448,13 +448,14 @@ int mllm_kv_read_fp4(const void* k_cache, const void* v_cache, const void* k_sca
                      int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
                      const int64_t* slots, int64_t num_slots, int32_t dtype, void* k_out, void* v_out, void* stream);
 
-/* mllm_paged_decode over a 4-bit pool; mllm_merge_splits combines its partials unchanged.  Codes and scales 16-byte aligned. */
+/* mllm_paged_decode over a 4-bit pool with the merge of its cut rows (mllm_merge_splits) behind it.  Codes and scales 16-byte
+ * aligned. */
 int mllm_paged_decode_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
                           const void* v_cache, const void* k_scales, const void* v_scales, int64_t num_blocks,
                           int32_t block_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                          const int32_t* kv_indices, const int32_t* decode_work, int32_t num_decode_work,
-                          int32_t num_merge_work, int32_t pages_per_split, float softmax_scale, int32_t dtype,
-                          void* out, int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                          const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* decode_work,
+                          int32_t num_decode_work, const int32_t* merge_work, int32_t num_merge_work,
+                          int32_t pages_per_split, float softmax_scale, int32_t dtype, void* out, int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
 /* mllm_paged_prefill over a 4-bit pool. */

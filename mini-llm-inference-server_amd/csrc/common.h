@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "minillm_hip.h"
 
@@ -141,22 +142,25 @@ __device__ __forceinline__ uint32_t fp4_scale_exp(float amax) {
 // The conversions' scale operand: they read bits 30:23 only, and take 255 as NaN.
 __device__ __forceinline__ float e8m0_to_f32(uint32_t e) { return __uint_as_float(e << 23); }
 
-// Eight e2m1 codes (one dword) -> eight 16-bit values, exact within Fp4Range.
+// The two e2m1 codes of byte b of a dword (b a constant) -> two 16-bit values, exact within Fp4Range.
 template <typename T>
-__device__ __forceinline__ u32x4 fp4x8_to(uint32_t w, float scale);
-template <>
-__device__ __forceinline__ u32x4 fp4x8_to<BF16>(uint32_t w, float scale) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+__device__ __forceinline__ uint32_t fp4x2_to(uint32_t w, float scale, int b) {
+  if constexpr (std::is_same<T, BF16>::value) {
+    return __builtin_bit_cast(uint32_t, b == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)
+                                        : b == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)
+                                        : b == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)
+                                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+  } else {
+    return __builtin_bit_cast(uint32_t, b == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)
+                                        : b == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)
+                                        : b == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)
+                                                 : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
+  }
 }
-template <>
-__device__ __forceinline__ u32x4 fp4x8_to<F16>(uint32_t w, float scale) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+// Eight e2m1 codes (one dword) -> eight 16-bit values.
+template <typename T>
+__device__ __forceinline__ u32x4 fp4x8_to(uint32_t w, float scale) {
+  return u32x4{fp4x2_to<T>(w, scale, 0), fp4x2_to<T>(w, scale, 1), fp4x2_to<T>(w, scale, 2), fp4x2_to<T>(w, scale, 3)};
 }
 // Eight 16-bit values -> eight codes of x / scale, to nearest with ties to even, saturated at 6.
 template <typename T>

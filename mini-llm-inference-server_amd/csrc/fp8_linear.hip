@@ -199,12 +199,13 @@ struct TileArgs {
 // y tile of BN weight rows x BM rows of x per workgroup, WN x WM wavefronts of (BN / WN) x (BM / WM) each.  Codes go through
 // LDS by DMA, a block of K (128 bytes a row) per step, double buffered; 16-byte piece j of row r lies at j ^ (r % 8), so
 // that eight lanes of an operand read hit distinct banks.
-template <typename T, int BN, int BM, int WN, int WM>
-__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a) {
+template <typename T, int BN, int BM, int WN, int WM, int OCC>
+__global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void fp8_tile_kernel(const TileArgs a) {
   constexpr int kWaves = WN * WM;
   constexpr int kA = BN * kBlock, kB = BM * kBlock, kStage = kA + kB + 4 * 64 * (BM / 256 ? BM / 256 : 1);
   constexpr int FN = BN / WN / 16, FM = BM / WM / 16;  // 16-row operands per wavefront
-  static_assert(BM / WM == 64, "a wavefront's rows of x share one dword of scales per lane");
+  constexpr int kRowsX = BM / WM;                      // rows of x per wavefront
+  static_assert(kRowsX % 64 == 0, "a dword of scales per lane serves 64 rows of x");
   __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -217,8 +218,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a
   const int per = tiles / 8, rest = tiles % 8, xcd = id % 8;
   const int t = xcd * per + min(xcd, rest) + id / 8;
   const int band = t / (4 * a.tiles_m), bn = min(4, a.tiles_n - 4 * band), in = t - 4 * a.tiles_m * band;
-  const int n0 = BN * (4 * band + in % bn), m0 = BM * (in / bn);
-  const int first = a.blocks * ks / a.ksplit, steps = a.blocks * (ks + 1) / a.ksplit - first;
+  // (divisions run on the vector unit: tell the compiler that the results are uniform)
+  const int n0 = __builtin_amdgcn_readfirstlane(BN * (4 * band + in % bn)), m0 = __builtin_amdgcn_readfirstlane(BM * (in / bn));
+  const int first = __builtin_amdgcn_readfirstlane(a.blocks * ks / a.ksplit);
+  const int steps = __builtin_amdgcn_readfirstlane(a.blocks * (ks + 1) / a.ksplit) - first;
 
   const int64_t row_bytes = (int64_t)a.blocks * kBlock;
   const char* wbase = a.w + n0 * row_bytes + (int64_t)first * kBlock;
@@ -260,8 +263,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a
     if (s + 1 < steps) load(s + 1);
     const char* st = lds + (s & 1) * kStage;
     const char* pa = st + (wn * (BN / WN) + n) * kBlock;
-    const char* pb = st + kA + (wm * 64 + n) * kBlock;
-    const int sx = *reinterpret_cast<const int*>(st + kA + kB + 64 * wm + 4 * n);
+    const char* pb = st + kA + (wm * kRowsX + n) * kBlock;
+    int sx[kRowsX / 64];
+#pragma unroll
+    for (int j = 0; j < kRowsX / 64; ++j) sx[j] = *reinterpret_cast<const int*>(st + kA + kB + kRowsX * wm + 64 * j + 4 * n);
     const int sw = scalar_byte(wsrow + s);
     i32x8 xb[FM];
 #pragma unroll
@@ -269,10 +274,13 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       const i32x8 wv = join(ld16(pa + 16 * i * kBlock + c0), ld16(pa + 16 * i * kBlock + c1));
-      acc[i][0] = mfma_fp8<0>(wv, xb[0], acc[i][0], sw, sx);
-      acc[i][1] = mfma_fp8<1>(wv, xb[1], acc[i][1], sw, sx);
-      acc[i][2] = mfma_fp8<2>(wv, xb[2], acc[i][2], sw, sx);
-      acc[i][3] = mfma_fp8<3>(wv, xb[3], acc[i][3], sw, sx);
+#pragma unroll
+      for (int j = 0; j < FM; j += 4) {
+        acc[i][j] = mfma_fp8<0>(wv, xb[j], acc[i][j], sw, sx[j / 4]);
+        acc[i][j + 1] = mfma_fp8<1>(wv, xb[j + 1], acc[i][j + 1], sw, sx[j / 4]);
+        acc[i][j + 2] = mfma_fp8<2>(wv, xb[j + 2], acc[i][j + 2], sw, sx[j / 4]);
+        acc[i][j + 3] = mfma_fp8<3>(wv, xb[j + 3], acc[i][j + 3], sw, sx[j / 4]);
+      }
     }
     barrier_vm<0>();
   }
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const TileArgs a
     if (col >= a.N) continue;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const int m = m0 + wm * 64 + 16 * j + n;
+      const int m = m0 + wm * kRowsX + 16 * j + n;
       if (m >= a.M) continue;
       const f32x4 v = acc[i][j];
       if (a.ksplit > 1)
@@ -383,9 +391,9 @@ extern "C" int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64
     fp8_quant_kernel<T><<<(unsigned)quant_groups, 256, 0, st>>>((const char*)x, 2 * x_stride, (unsigned)m, (int)k, blocks, base,
                                                                (uint8_t*)base + p.xq_bytes, (unsigned)a.groups64);
     if (p.large)
-      fp8_tile_kernel<T, 256, 256, 2, 4><<<(unsigned)groups, 512, 0, st>>>(a);
+      fp8_tile_kernel<T, 256, 256, 2, 4, 2><<<(unsigned)groups, 512, 0, st>>>(a);
     else
-      fp8_tile_kernel<T, 128, 128, 2, 2><<<(unsigned)groups, 256, 0, st>>>(a);
+      fp8_tile_kernel<T, 128, 128, 2, 2, 2><<<(unsigned)groups, 256, 0, st>>>(a);
   };
   if (dtype == MLLM_DTYPE_BF16)
     launch(BF16{});

@@ -81,7 +81,7 @@ struct Fp4Pool {
 
 // Byte of `scales` of (slot, head, dim block).
 __device__ __forceinline__ int64_t k_scale_at(int64_t slot, int h, int blk, int hkv, int nblk) {
-  return (slot * hkv + h) * nblk + blk;
+  return (slot * nblk + blk) * hkv + h;
 }
 __device__ __forceinline__ int64_t v_scale_at(int64_t slot, int h, int blk, int hkv, int nblk, int bs) {
   const int64_t page = slot / bs;

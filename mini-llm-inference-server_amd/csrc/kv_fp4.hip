@@ -1,10 +1,10 @@
 // 4-bit KV pool: append a step's K and V rows, and read rows back (no counterpart in the reference; see common.h for the
 // codes and scales).
 //
-// Layout: codes [num_blocks, block_size, Hkv, Dh / 2] bytes, as the other pools.  K scales [num_blocks, block_size, Hkv,
-// Dh / 32], a token's scales together: a decode lane multiplies with the keys of one token.  V scales [num_blocks, Hkv,
-// Dh / 32, block_size], a dim block's tokens together: a decode lane holds four consecutive tokens of one dim block and
-// gets their scales as one dword.
+// Layout: codes [num_blocks, block_size, Hkv, Dh / 2] bytes, as the other pools.  Scales lie as the decode kernel's lanes
+// read them: K scales [num_blocks, block_size, Dh / 32, Hkv], because a lane multiplies with one dim block of one token's keys
+// of adjacent heads; V scales [num_blocks, Hkv, Dh / 32, block_size], because a lane holds consecutive tokens of one dim block.
+// Either way a lane's scales are one load.
 //
 // One thread moves eight dims: 16 bytes of a 16-bit row, four bytes of codes.  A block's largest magnitude is the
 // maximum over its four threads of the 16-bit patterns without their sign, which order as the magnitudes do and put

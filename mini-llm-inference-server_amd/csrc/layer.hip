@@ -69,9 +69,9 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
   if (s->num_decode_work > 0) {
     if (fp4)
       rc = mllm_paged_decode_fp4(qa, qa_st, qa_sh, p->k_cache, p->v_cache, p->k_scales, p->v_scales, s->num_blocks,
-                                 s->block_size, s->num_heads, s->num_kv_heads, s->head_dim, s->kv_indices, s->decode_work,
-                                 s->num_decode_work, s->num_merge_work, s->pages_per_split, s->softmax_scale, s->dtype,
-                                 out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
+                                 s->block_size, s->num_heads, s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indices,
+                                 s->decode_work, s->num_decode_work, s->merge_work, s->num_merge_work,
+                                 s->pages_per_split, s->softmax_scale, s->dtype, out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
     else if (fp8)
       rc = mllm_paged_decode_fp8(qa, qa_st, qa_sh, p->k_cache, p->v_cache, s->num_blocks, s->block_size, s->num_heads,
                                  s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indptr, s->kv_indices,
@@ -85,8 +85,9 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
                              s->pages_per_split, s->softmax_scale, s->dtype, out, row, s->head_dim, s->workspace,
                              s->workspace_bytes, stream);
     if (rc != MLLM_OK) return rc;
-    rc = mllm_merge_splits(s->merge_work, s->num_merge_work, s->num_decode_work, s->num_heads, s->head_dim,
-                           s->qo_indptr, s->dtype, out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
+    if (!fp4)  // the 4-bit decode merges by itself
+      rc = mllm_merge_splits(s->merge_work, s->num_merge_work, s->num_decode_work, s->num_heads, s->head_dim,
+                             s->qo_indptr, s->dtype, out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
     if (rc != MLLM_OK) return rc;
   }
   if (s->num_prefill_work > 0) {

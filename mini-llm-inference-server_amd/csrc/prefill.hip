@@ -146,8 +146,9 @@ __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const Prefi
     constexpr int kBlocks = kHeadDim / kFp4Block;
     const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
     const uint64_t page = (uint64_t)b * (unsigned)(a.Hkv * kBlocks * a.bs);
-    const unsigned col = head_bytes / (kHeadDim / 2) * kBlocks + ((lane & 7) >> 1);  // the head's dim block
-    const uint8_t* sp = IS_V ? a.vs + page + (col * (unsigned)a.bs + tok) : a.ks + page + ((unsigned)(tok * a.Hkv * kBlocks) + col);
+    const unsigned h = head_bytes / (kHeadDim / 2), c = (lane & 7) >> 1;  // KV head, dim block
+    const uint8_t* sp = IS_V ? a.vs + page + ((h * kBlocks + c) * (unsigned)a.bs + tok)
+                             : a.ks + page + ((unsigned)(tok * kBlocks) + c) * (unsigned)a.Hkv + h;
     return {ld8(p), *sp};
   }
 }

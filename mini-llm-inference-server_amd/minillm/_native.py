@@ -110,8 +110,8 @@ SIGNATURES = {
     "mllm_kv_append_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
                                           _i64, _p]),
     "mllm_kv_read_fp4": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p]),
-    "mllm_paged_decode_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _i32,
-                                             _i32, _i32, _f32, _i32, _p, _i64, _i64, _p, _i64, _p]),
+    "mllm_paged_decode_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32,
+                                             _p, _i32, _i32, _f32, _i32, _p, _i64, _i64, _p, _i64, _p]),
     "mllm_paged_prefill_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p,
                                               _p, _i32, _i32, _f32, _i32, _p, _i64, _i64, _p]),
     "mllm_qk_norm_rope_kv_append": (ctypes.c_int, [_p, _p, _p, _f32, _p]),

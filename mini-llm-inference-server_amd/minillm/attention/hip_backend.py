@@ -84,10 +84,7 @@ MIN_SPLIT_PAGES = 2  # the smallest bin the heuristic picks (16-bit pools)
 
 def fp4_heads(num_heads: int, num_kv_heads: int) -> int:
     """KV heads a wavefront of mllm_paged_decode_fp4 takes (the library's rule)."""
-    group = num_heads // num_kv_heads
-    if num_kv_heads % 4 == 0 and 4 * group <= 16:
-        return 4
-    return 2 if num_kv_heads % 2 == 0 and 2 * group <= 16 else 1
+    return 2 if num_kv_heads % 2 == 0 and 2 * (num_heads // num_kv_heads) <= 16 else 1
 
 
 def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None = None, kv_fp8: bool = False,
@@ -119,9 +116,9 @@ def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None 
     forced = os.environ.get("MLLM_PAGES_PER_SPLIT")
     if forced:
         return max(1, min(MAX_SPLIT_PAGES, int(forced)))
-    if kv_fp4:  # one round of the resident wavefronts, 2 per SIMD
-        per_bin = num_kv_heads // fp4_heads(num_heads or 4 * num_kv_heads, num_kv_heads)
-        per_round = max(1, num_cus * 4 * 2 // per_bin)
+    if kv_fp4:  # one workgroup per CU, each on up to four groups of fp4_heads KV heads
+        per_bin = -(-(num_kv_heads // fp4_heads(num_heads or 4 * num_kv_heads, num_kv_heads)) // 4)
+        per_round = max(1, num_cus // per_bin)
         rounds = max(1, math.ceil(decode_pages / (MAX_SPLIT_PAGES * per_round)))
         return max(MIN_SPLIT_PAGES, min(MAX_SPLIT_PAGES, math.ceil(decode_pages / (rounds * per_round))))
     if whole_pages and not kv_fp8 and num_kv_heads % WHOLE_PAGE_WAVES == 0 and decode_pages > 0:
@@ -264,7 +261,7 @@ def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
     """ValueError unless k_scale and v_scale are the block scales of a 4-bit pool."""
     nb, bs, hkv, half = k_cache.shape
     blocks = 2 * half // FP4_BLOCK
-    for name, t, shape in (("k_scale", k_scale, (nb, bs, hkv, blocks)), ("v_scale", v_scale, (nb, hkv, blocks, bs))):
+    for name, t, shape in (("k_scale", k_scale, (nb, bs, blocks, hkv)), ("v_scale", v_scale, (nb, hkv, blocks, bs))):
         if not isinstance(t, torch.Tensor) or t.dtype != SCALES4:
             raise ValueError(f"with a 4-bit pool, {name} is its float8_e8m0fnu tensor of block scales")
         if t.shape != shape or not t.is_contiguous() or t.device != k_cache.device:
@@ -568,7 +565,8 @@ class HipBackend(AttentionBackend):
                 side = self._side[q.device] = torch.cuda.Stream(q.device)  # default priority
             ready = cur.record_event()  # the append (and everything before it) has landed
             self.run_decode(q, k_cache, v_cache, meta, out, k_scale, v_scale)
-            self.run_merge(q, meta, out)
+            if k_cache.dtype != FP4:  # whose decode call merges
+                self.run_merge(q, meta, out)
             side.wait_event(ready)
             with torch.cuda.stream(side):
                 self.run_prefill(q, k_cache, v_cache, meta, out, k_scale, v_scale)
@@ -576,7 +574,8 @@ class HipBackend(AttentionBackend):
             return
         if plan.num_decode:
             self.run_decode(q, k_cache, v_cache, meta, out, k_scale, v_scale)
-            self.run_merge(q, meta, out)
+            if k_cache.dtype != FP4:  # whose decode call merges
+                self.run_merge(q, meta, out)
         if plan.num_prefill:
             self.run_prefill(q, k_cache, v_cache, meta, out, k_scale, v_scale)
 
@@ -588,8 +587,8 @@ class HipBackend(AttentionBackend):
         if k_cache.dtype == FP4:
             self._lib.call("mllm_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
                            v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv,
-                           2 * dh, plan.meta_ptrs[2], _ptr(plan.decode_work), plan.num_decode, plan.num_merge,
-                           plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
+                           2 * dh, plan.meta_ptrs[0], plan.meta_ptrs[2], _ptr(plan.decode_work), plan.num_decode,
+                           _ptr(plan.merge_work), plan.num_merge, plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
                            out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes, _native.stream_ptr(q.device))
             return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,

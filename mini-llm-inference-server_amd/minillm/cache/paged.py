@@ -12,7 +12,7 @@ and `v_scale[l]` for layer l, which the model passes to the backend with the lay
 Llama-3.1-8B is then 32 KB per layer, so the same HBM holds twice the tokens.
 
 A pool of dtype torch.float4_e2m1fn_x2 stores 4-bit codes with a power-of-two scale for 32 dims of a token and head: the
-pools are [num_blocks, block_size, Hkv, Dh / 2] (two codes to a byte), `k_scale[l]` [num_blocks, block_size, Hkv, Dh / 32]
+pools are [num_blocks, block_size, Hkv, Dh / 2] (two codes to a byte), `k_scale[l]` [num_blocks, block_size, Dh / 32, Hkv]
 and `v_scale[l]` [num_blocks, Hkv, Dh / 32, block_size] torch.float8_e8m0fnu tensors (include/minillm_hip.h has the
 format).  One block of Llama-3.1-8B is 17 KB per layer, so the same HBM holds 3.76 times the tokens of 16 bits.
 
@@ -51,7 +51,7 @@ class PagedKVCache:
         self.v_scale: list = [float(v_scale)] * config.num_hidden_layers
         if self.fp4:
             blocks = dh // FP4_BLOCK
-            for scales, of in ((self.k_scale, (num_blocks, block_size, hkv, blocks)),
+            for scales, of in ((self.k_scale, (num_blocks, block_size, blocks, hkv)),
                                (self.v_scale, (num_blocks, hkv, blocks, block_size))):
                 scales[:] = [torch.zeros(of, device=device, dtype=torch.uint8).view(torch.float8_e8m0fnu) for _ in scales]
 

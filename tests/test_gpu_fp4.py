@@ -94,7 +94,7 @@ def test_append_every_16bit_pattern(hip, dtype):
     ks, vs = cache.k_scale[0].view(torch.uint8).cpu(), cache.v_scale[0].view(torch.uint8).cpu()
     for i in (0, 17, 255):
         s = int(slots[i])
-        assert torch.equal(ks.view(512, 2, 4)[s], quantised(k[i])[1])
+        assert torch.equal(ks.view(512, 4, 2)[s], quantised(k[i])[1].t())
         assert torch.equal(vs[s // 16, :, :, s % 16], quantised(v[i])[1])
 
 
@@ -244,7 +244,7 @@ def test_nan_and_inf_reach_only_their_own_head(hip):
     for rows in ([(50, 1), (20, 1)], [(10, 40), (20, 1)]):
         _, ref, bound, (backend, cache, meta, q) = step(rows, 32, 8, torch.bfloat16, seed=6)
         page = int(meta.block_tables[0, 0])
-        cache.k_scale[0].view(torch.uint8)[page, 3, 5, 2] = 255
+        cache.k_scale[0].view(torch.uint8)[page, 3, 2, 5] = 255
         cache.v_scale[0].view(torch.uint8)[page, 1, 0, 3] = 255
         out = torch.empty_like(q)
         backend.attend(q, cache.k[0], cache.v[0], meta, out, **cache.scales(0))

@@ -31,7 +31,7 @@ def test_cache_shapes_and_bytes():
     cache = PagedKVCache(config(), 3, "cpu", FP4, block_size=32)
     assert cache.fp4 and not cache.quantized
     assert [tuple(t.shape) for t in (cache.k[1], cache.v[1], cache.k_scale[1], cache.v_scale[1])] == \
-        [(3, 32, 2, 64), (3, 32, 2, 64), (3, 32, 2, 4), (3, 2, 4, 32)]
+        [(3, 32, 2, 64), (3, 32, 2, 64), (3, 32, 4, 2), (3, 2, 4, 32)]
     assert cache.k[0].dtype == FP4 and cache.v_scale[0].dtype == E8M0
     assert cache.scales(1) == {"k_scale": cache.k_scale[1], "v_scale": cache.v_scale[1]}
     assert cache.scales(0)["k_scale"].data_ptr() != cache.scales(1)["k_scale"].data_ptr()
@@ -74,8 +74,8 @@ def test_read_of_other_pools(dtype):
 
 
 def test_split_sizes_of_4bit_pools():
-    assert hb.fp4_heads(32, 8) == 4 and hb.fp4_heads(16, 2) == 2 and hb.fp4_heads(16, 1) == 1
-    assert hb.fp4_heads(40, 8) == 2 and hb.fp4_heads(12, 4) == 4 and hb.fp4_heads(15, 5) == 1 and hb.fp4_heads(96, 8) == 1
+    assert hb.fp4_heads(32, 8) == 2 and hb.fp4_heads(16, 2) == 2 and hb.fp4_heads(16, 1) == 1
+    assert hb.fp4_heads(40, 8) == 2 and hb.fp4_heads(12, 4) == 2 and hb.fp4_heads(15, 5) == 1 and hb.fp4_heads(96, 8) == 1
     for heads, kv in ((32, 8), (16, 2), (8, 8), (16, 1)):
         for pages in (1, 5, 100, 4096, 34000, 300000):
             c = hb.pages_per_split(pages, kv, heads, kv_fp4=True)
@@ -179,7 +179,7 @@ def test_entry_points_check_their_arguments():
     lib.call("mllm_kv_read_fp4", None, None, None, None, 0, 16, 2, 128, None, 0, 2, None, None, None)
 
     def decode(h=32, hkv=8, dh=128, bs=16, split=8, dtype=2, ws=0, merges=0, q=a, scales=a):
-        lib.call("mllm_paged_decode_fp4", q, 4096, 128, a, a, scales, a, 4, bs, h, hkv, dh, a, a, 10, merges, split, 0.1, dtype,
+        lib.call("mllm_paged_decode_fp4", q, 4096, 128, a, a, scales, a, 4, bs, h, hkv, dh, a, a, a, 10, a, merges, split, 0.1, dtype,
                  a, 4096, 128, None, ws, None)
 
     for kw, match in ((dict(dh=64), "head_dim"), (dict(bs=24), "block_size"), (dict(h=30), "multiple of num_kv_heads"),
