@@ -319,76 +319,93 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
   }
 }
 
-// Log-sum-exp merge of a cut row's partials, as decode.hip's merge_kernel.  A workgroup of 256 threads takes HEADS heads of a
-// row with 256 / (32 HEADS) groups of 32 threads, four dims each; a head's groups take its partials in turn and meet
-// in LDS.  Eight heads and one group where rows have few partials; one head and eight groups where they have many (three
-// rows of 85,000 tokens: 91 us with one group).
-template <typename T, int HEADS>
+// Log-sum-exp merge of a cut row's partials, as decode.hip's merge_kernel.  Eight groups of 32 threads, four dims each: of a
+// row with at most eight partials each group takes a head; of a row with more, all groups take one head, partials in
+// turn, and meet in LDS (three rows of 85,000 tokens: 91 us with one group a head, 4.6 with eight).  The number of
+// partials alone decides, so a row's result does not depend on the launch: WIDE, for steps whose rows have many, has a
+// workgroup per head, of which every eighth serves the short rows; without it a workgroup serves eight heads of either.
+constexpr int kFewPartials = 8;
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void merge_fp4_kernel(const int4* __restrict__ merge, const float* __restrict__ part_o,
                                                        const float2* __restrict__ part_ml, int H,
                                                        const int32_t* __restrict__ qo_indptr, uint16_t* __restrict__ out,
                                                        int64_t o_st, int64_t o_sh) {
-  constexpr int kGroups = 8 / HEADS;
-  __shared__ float red[kGroups][HEADS][kHeadDim + 4];
+  __shared__ float red[8][kHeadDim + 4];
   const int4 mw = merge[blockIdx.x];
   const int first = mw.y, n = mw.z;
   if (mw.x < 0) return;  // the whole workgroup
-  const int sub = threadIdx.x >> 5, hl = sub % HEADS, grp = sub / HEADS, d0 = 4 * (threadIdx.x & 31);
-  const int head = min((int)blockIdx.y * HEADS + hl, H - 1);
-  constexpr int kAtOnce = 4;  // partials in flight; places past n read the first again and weigh it 0
-  float m = -INFINITY, l = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = grp; j0 < n; j0 += kAtOnce * kGroups) {
-    float2 ml[kAtOnce];
-    f32x4 o[kAtOnce];
+  const int grp = threadIdx.x >> 5, d0 = 4 * (threadIdx.x & 31);
+  uint16_t* row_out = out + (int64_t)qo_indptr[mw.x] * o_st + d0;
+  auto store = [&](int head, f32x4 acc, float l) {
+    const float inv = 1.f / l;
+    st8(row_out + (int64_t)head * o_sh, u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)});
+  };
+  // partials j0, j0 + step, .. below n of a head, added to (m, l, acc); four in flight
+  auto add = [&](int head, int j0, int step, float& m, float& l, f32x4& acc) {
+    for (; j0 < n; j0 += 4 * step) {
+      float2 ml[4];
+      f32x4 o[4];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int j = j0 + u * kGroups;
-      const int64_t row = (int64_t)(first + (j < n ? j : j0)) * H + head;
-      ml[u] = part_ml[row];
-      o[u] = *reinterpret_cast<const f32x4*>(part_o + row * kHeadDim + d0);
-    }
-    float mc = m;
+      for (int u = 0; u < 4; ++u) {  // places past n read the first again and weigh it 0
+        const int64_t row = (int64_t)(first + (j0 + u * step < n ? j0 + u * step : j0)) * H + head;
+        ml[u] = part_ml[row];
+        o[u] = *reinterpret_cast<const f32x4*>(part_o + row * kHeadDim + d0);
+      }
+      float mc = m;
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      if (j0 + u * kGroups >= n) ml[u].x = -INFINITY;
-      mc = fmaxf(mc, ml[u].x);
-    }
-    if (mc == -INFINITY) continue;  // segments without tiles
-    const float sc = fast_exp2(m - mc);
-    l *= sc;
-    acc *= sc;
+      for (int u = 0; u < 4; ++u) {
+        if (j0 + u * step >= n) ml[u].x = -INFINITY;
+        mc = fmaxf(mc, ml[u].x);
+      }
+      if (mc == -INFINITY) continue;  // segments without tiles
+      const float sc = fast_exp2(m - mc);
+      l *= sc;
+      acc *= sc;
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const float w = fast_exp2(ml[u].x - mc);
-      l += w * ml[u].y;
-      acc += w * o[u];
+      for (int u = 0; u < 4; ++u) {
+        const float w = fast_exp2(ml[u].x - mc);
+        l += w * ml[u].y;
+        acc += w * o[u];
+      }
+      m = mc;
     }
-    m = mc;
+  };
+  const int head0 = WIDE ? blockIdx.y & ~7 : 8 * blockIdx.y;
+  if (n <= kFewPartials) {
+    const int head = head0 + grp;
+    if ((WIDE && (blockIdx.y & 7)) || head >= H) return;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    add(head, 0, 1, m, l, acc);
+    store(head, acc, l);
+    return;
   }
-  if constexpr (kGroups > 1) {
-    float* r = red[grp][hl];
+  const int from = WIDE ? (int)blockIdx.y : head0, to = WIDE ? from + 1 : min(head0 + 8, H);
+  for (int head = from; head < to; ++head) {
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    add(head, grp, 8, m, l, acc);
+    float* r = red[grp];
     *reinterpret_cast<f32x4*>(r + d0) = acc;
     if (d0 == 0) r[kHeadDim] = m, r[kHeadDim + 1] = l;
     __syncthreads();
-    if (grp) return;
-    float mc = m;
+    if (grp == 0) {
+      float mc = m;
 #pragma unroll
-    for (int s = 1; s < kGroups; ++s) mc = fmaxf(mc, red[s][hl][kHeadDim]);
-    float w = fast_exp2(m - mc);
-    l *= w;
-    acc *= w;
+      for (int s = 1; s < 8; ++s) mc = fmaxf(mc, red[s][kHeadDim]);
+      float w = fast_exp2(m - mc);
+      l *= w;
+      acc *= w;
 #pragma unroll
-    for (int s = 1; s < kGroups; ++s) {
-      w = fast_exp2(red[s][hl][kHeadDim] - mc);
-      l += w * red[s][hl][kHeadDim + 1];
-      acc += w * *reinterpret_cast<const f32x4*>(red[s][hl] + d0);
+      for (int s = 1; s < 8; ++s) {
+        w = fast_exp2(red[s][kHeadDim] - mc);
+        l += w * red[s][kHeadDim + 1];
+        acc += w * *reinterpret_cast<const f32x4*>(red[s] + d0);
+      }
+      store(head, acc, l);
     }
+    __syncthreads();
   }
-  if ((int)blockIdx.y * HEADS + hl >= H) return;
-  const float inv = 1.f / l;
-  st8(out + (int64_t)qo_indptr[mw.x] * o_st + (int64_t)head * o_sh + d0,
-      u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)});
 }
 
 // KV heads per wavefront.
@@ -398,12 +415,12 @@ template <typename T>
 int launch_merge_fp4(const DecodeFp4Args& a, const int32_t* merge_work, int num_merge, int n_work, const int32_t* qo_indptr,
                      hipStream_t st) {
   const int4* merge = reinterpret_cast<const int4*>(merge_work);
-  // bins bound a row's partials: with many rows to merge each has few
-  if (max_bins(n_work) >= 8 * num_merge)
-    merge_fp4_kernel<T, 1><<<dim3(num_merge, a.H), 256, 0, st>>>(merge, a.part_o, a.part_ml, a.H, qo_indptr, a.out, a.o_st, a.o_sh);
+  if (max_bins(n_work) >= kFewPartials * num_merge)
+    merge_fp4_kernel<T, true><<<dim3(num_merge, a.H), 256, 0, st>>>(merge, a.part_o, a.part_ml, a.H, qo_indptr, a.out, a.o_st,
+                                                                   a.o_sh);
   else
-    merge_fp4_kernel<T, 8><<<dim3(num_merge, (a.H + 7) / 8), 256, 0, st>>>(merge, a.part_o, a.part_ml, a.H, qo_indptr, a.out,
-                                                                          a.o_st, a.o_sh);
+    merge_fp4_kernel<T, false><<<dim3(num_merge, (a.H + 7) / 8), 256, 0, st>>>(merge, a.part_o, a.part_ml, a.H, qo_indptr,
+                                                                              a.out, a.o_st, a.o_sh);
   return check_launch("mllm_paged_decode_fp4");
 }
 
