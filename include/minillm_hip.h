@@ -532,9 +532,9 @@ int mllm_decoder_layer_pool(const mllm_layer_step* step, const void* x, int64_t 
  * x [m, k] of `dtype` (BF16 or F16), element stride x_stride, rows 16-byte aligned; its blocks of 128 columns are quantised under
  * the least power of two with max|x| / 2^e <= 448 (e at least -126; a block that holds an infinity or a NaN: NaN), to
  * nearest with ties to even.  out [m, n] contiguous = T(sum over blocks of both scales times the codes' products), fp32 sums.
- * k and n multiples of 16, k <= 2^23, n < 2^28.  Up to 64 rows run without a workspace, and a row's result then depends
- * neither on the other rows nor on m; more rows need mllm_fp8_linear_workspace_bytes bytes (`num_cus` 0: the current
- * device's), 256-byte aligned, not shared with a call that may run at the same time.
+ * k and n multiples of 16, k <= 2^23, n < 2^28.  Up to 64 rows a row's result depends neither on the other rows nor on m.
+ * The workspace holds mllm_fp8_linear_workspace_bytes bytes (`num_cus` 0: the current device's; 0 bytes: none is needed),
+ * 256-byte aligned, not shared with a call that may run at the same time.
  */
 int64_t mllm_fp8_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t num_cus);
 int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64_t k, const void* weight,

@@ -11,6 +11,8 @@
 // a lane ends with four consecutive outputs of one row of y.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace mllm {
@@ -18,9 +20,12 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 128;    // K per scale, and rows of weights
-constexpr int kFewRows = 64;   // rows of x up to which the weight-streaming kernel runs
+constexpr int kFewRows = 64;                    // rows of x up to which the weights are streamed,
+constexpr int kInPlaceRows = 16;                // .. and of them those fp8_rows_kernel takes,
+constexpr int64_t kSmallWeights = 1 << 24;      // with weights of up to this many bytes
 
 __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
@@ -84,80 +89,220 @@ __device__ __forceinline__ u32x4 quant16_e4m3(u32x4 lo, u32x4 hi, uint32_t e) {
 // ---------------------------------------------------------------- few rows: the weights streamed once
 
 struct RowsArgs {
-  const char* x;  // bytes
+  const char* x;  // 16-bit rows
   int64_t x_st;   // row stride, bytes
   int M, K, N, blocks;
   const char* w;  // [N][128 blocks]
   const uint8_t* ws;
   uint16_t* y;
+  int tiles, ksplit;
+  float* part;  // ksplit > 1: [ksplit][M][N]
 };
 
 constexpr int kRowsWaves = 8;
 
-// One workgroup per 16 weight rows, eight wavefronts along K.  Bound by the weights, N K bytes read once; each wavefront
-// quantises its own columns of x, so there is one launch and no exchange but the eight partial sums in LDS.
-template <typename T, int MT>
+// Largest over the lanes that hold one row's block: l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ uint32_t max_over_g(uint32_t v) {
+  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max((uint32_t)a[0], (uint32_t)a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+// The value of lane l ^ 8.
+__device__ __forceinline__ uint32_t lane_xor8(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true); }
+
+// A wavefront's operand of x for one block: rows of up to 16 quantised in place.  With at most 8 rows, lanes n and n + 8 share
+// row n: each loads and quantises half of the lane's columns and they swap codes (columns 8 .. 15 of the product are unused).
+template <typename T, bool HALF>
+struct RowsX {
+  static constexpr int kLoads = HALF ? 2 : 4;
+  u32x4 v[kLoads];
+  static __device__ __forceinline__ int column(int k0, int j, bool second) { return k0 + (HALF ? (second ? 64 : 0) : 32 * j); }
+  // columns past K (a multiple of 16: a lane's 16 are all there or none) read the last ones and are cleared before their use
+  __device__ __forceinline__ void load(const char* row, int k0, int K, bool second) {
+#pragma unroll
+    for (int j = 0; j < kLoads; j += 2) {
+      const char* at = row + 2 * min(column(k0, j, second), K - 16);
+      v[j] = ld16(at);
+      v[j + 1] = ld16(at + 16);
+    }
+  }
+  __device__ __forceinline__ void clear_past(int k0, int K, bool second) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      if (column(k0, j & ~1, second) >= K) v[j] = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ i32x8 operand(uint32_t& e) const {
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[j][i] & 0x7fff7fffu));
+    uint32_t top = max((uint32_t)m[0], (uint32_t)m[1]);
+    if (HALF) top = max(top, lane_xor8(top));
+    e = x_scale_exp<T>(max_over_g(top));
+    const u32x4 lo = quant16_e4m3<T>(v[0], v[1], e);
+    if constexpr (HALF) return join(lo, u32x4{lane_xor8(lo[0]), lane_xor8(lo[1]), lane_xor8(lo[2]), lane_xor8(lo[3])});
+    else return join(lo, quant16_e4m3<T>(v[2], v[3], e));
+  }
+};
+
+// Both kernels are bound by the weights, N K bytes read once, and at these sizes by what surrounds the reading.
+// Up to 16 rows, small weights: one workgroup per 16 weight rows, eight wavefronts along K, x quantised by the wavefronts that
+// use it.  One launch, no exchange but the eight partial sums in LDS.  4096 x 4096 (us, from a graph, weights from memory): 6.9
+// at 1 row, 7.2 at 8, 8.3 at 16; the chunk kernel below with the launch that adds its parts 8.0, 8.7, 8.9.  What it cost to
+// quantise x in every workgroup: 8.9 at 8 rows when each of the 16 operand columns loaded a row, with maxima by dword and
+// through LDS.  Loads that bypass the cache (nt) are 5 - 10% slower in both kernels.
+template <typename T, bool HALF>
 __global__ __launch_bounds__(64 * kRowsWaves) void fp8_rows_kernel(const RowsArgs a) {
-  __shared__ f32x4 red[kRowsWaves][MT][64];
+  __shared__ f32x4 red[kRowsWaves][64];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = 16 * blockIdx.x;
   const int first = a.blocks * wave / kRowsWaves, end = a.blocks * (wave + 1) / kRowsWaves;
-  const char* wp = a.w + (int64_t)min(n0 + n, a.N - 1) * a.blocks * kBlock + 16 * g;
+  const char* wp = a.w + (int64_t)(n0 + n) * a.blocks * kBlock + 16 * g;
   const uint8_t* ws = a.ws + (int64_t)(n0 / kBlock) * a.blocks;
-  f32x4 acc[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const char* xp[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = a.x + min(16 * m + n, a.M - 1) * a.x_st;
-  constexpr int kAhead = 4;  // blocks of weights in flight
-  u32x4 w[kAhead][2];
-  auto load_w = [&](u32x4 (&r)[2], int b) {
-    r[0] = ld16_nt(wp + (int64_t)b * kBlock);
-    r[1] = ld16_nt(wp + (int64_t)b * kBlock + 64);
+  const char* xp = a.x + min(HALF ? n & 7 : n, a.M - 1) * a.x_st;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int kAhead = 2;  // blocks in flight
+  struct Stage {
+    u32x4 w[2];
+    RowsX<T, HALF> x;
+    int sw;
+  } ring[kAhead];
+  auto load = [&](Stage& s, int b) {
+    s.x.load(xp, b * kBlock + 16 * g, a.K, n >= 8);
+    s.sw = ws[b];
+    s.w[0] = ld16(wp + (int64_t)b * kBlock);
+    s.w[1] = ld16(wp + (int64_t)b * kBlock + 64);
+  };
+  auto use = [&](Stage& s, int b) {
+    if ((b + 1) * kBlock > a.K) s.x.clear_past(b * kBlock + 16 * g, a.K, n >= 8);
+    uint32_t e;
+    const i32x8 xv = s.x.operand(e);
+    acc = mfma_fp8<0>(join(s.w[0], s.w[1]), xv, acc, s.sw, (int)e);
   };
 #pragma unroll
   for (int u = 0; u < kAhead; ++u)
-    if (first + u < end) load_w(w[u], first + u);
-  for (int b0 = first; b0 < end; b0 += kAhead) {
+    if (first + u < end) load(ring[u], first + u);
+  int b = first;
+  for (; b + 2 * kAhead <= end; b += kAhead) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int b = b0 + u;
-      if (b >= end) break;
-      const i32x8 wv = join(w[u][0], w[u][1]);
-      const int sw = scalar_byte(ws + b);
-      const int k0 = b * kBlock + 16 * g;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        u32x4 v[4] = {};
-        if (k0 < a.K) {  // K is a multiple of 16: a lane's 16 columns are all there or none
-          v[0] = ld16(xp[m] + 2 * k0);
-          v[1] = ld16(xp[m] + 2 * k0 + 16);
-        }
-        if (k0 + 64 < a.K) {
-          v[2] = ld16(xp[m] + 2 * k0 + 128);
-          v[3] = ld16(xp[m] + 2 * k0 + 144);
-        }
-        uint32_t top = max_abs16(v[3], max_abs16(v[2], max_abs16(v[1], max_abs16(v[0], 0u))));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const uint32_t e = x_scale_exp<T>(top);
-        acc[m] = mfma_fp8<0>(wv, join(quant16_e4m3<T>(v[0], v[1], e), quant16_e4m3<T>(v[2], v[3], e)), acc[m], sw, (int)e);
-      }
-      if (b + kAhead < end) load_w(w[u], b + kAhead);
+      use(ring[u], b + u);
+      load(ring[u], b + u + kAhead);
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
-  __syncthreads();
-  const int i = threadIdx.x;
-  if (i >= 64 * MT) return;
-  const int m = 16 * (i >> 6) + n, col = n0 + 4 * g;  // lane (n, g): row m of y, outputs 4 g .. + 3 of the tile
-  f32x4 s = red[0][i >> 6][lane];
+  for (int u = 0; u < kAhead; ++u) {
+    if (b + u < end) use(ring[u], b + u);
+    if (b + u + kAhead < end) load(ring[u], b + u + kAhead);
+  }
 #pragma unroll
-  for (int k = 1; k < kRowsWaves; ++k) s += red[k][i >> 6][lane];
-  if (m < a.M && col < a.N) st8(a.y + (int64_t)m * a.N + col, u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])});
+  for (int u = 0; u < kAhead - 1; ++u)
+    if (b + u + kAhead < end) use(ring[u], b + u + kAhead);
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave > 0) return;
+  f32x4 s = red[0][lane];  // lane (n, g): row n of y, outputs 4 g .. + 3 of the tile
+#pragma unroll
+  for (int k = 1; k < kRowsWaves; ++k) s += red[k][lane];
+  if (n < a.M && !(HALF && n >= 8)) st8(a.y + (int64_t)n * a.N + n0 + 4 * g, u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])});
+}
+
+// Up to 64 rows: a workgroup takes 128 weight rows, 16 a wavefront, and a part of K in chunks of kChunk blocks.  Its wavefronts
+// quantise the chunk of x together, a block of 16 rows each, into LDS in operand order while weights load: x is read and
+// quantised once per 128 weight rows.  Parts, one workgroup per CU, meet in fp32 (mllm_sum_partials).  Measured as above,
+// 14336 x 4096 / 4096 x 14336, 8 rows 16.9 / 17.8 us (3.5 / 3.3 TB/s with both launches), 32 rows 20.6 / -, 64 rows 25.6 /
+// 24.6.  Workgroups of 16 weight rows (fp8_rows_kernel's way) took 20.2 / 20.9 at 8 rows, 73 / 60 at 64; with x quantised
+// once by another launch 26.9 / 30.6 at 64.  Two workgroups per CU: 25.1 / 20.3 at 8 rows.
+template <typename T, int MT, bool HALF>
+__global__ __launch_bounds__(64 * kRowsWaves) void fp8_chunk_kernel(const RowsArgs a) {
+  constexpr int kChunk = MT == 1 ? 8 : 4;
+  constexpr int kTasks = MT * kChunk / kRowsWaves;  // blocks of 16 rows per wavefront
+  __shared__ u32x4 codes[2][kChunk][MT][2][64];     // lane's 16-byte halves
+  __shared__ uint8_t scales[2][kChunk][16][4];      // [row % 16][row / 16]
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % a.tiles, ks = blockIdx.x / a.tiles;
+  const int n0 = kBlock * tile + 16 * wave;
+  const int first = (int)((int64_t)a.blocks * ks / a.ksplit), end = (int)((int64_t)a.blocks * (ks + 1) / a.ksplit);
+  const char* wp = a.w + (int64_t)min(n0 + n, a.N - 1) * a.blocks * kBlock + 16 * g;
+  const uint8_t* ws = a.ws + (int64_t)tile * a.blocks;
+  const char* xp[kTasks];
+#pragma unroll
+  for (int i = 0; i < kTasks; ++i) {
+    const int m = 16 * ((wave + kRowsWaves * i) % MT) + (HALF ? n & 7 : n);
+    xp[i] = a.x + min(m, a.M - 1) * a.x_st;
+  }
+  u32x4 w[kChunk][2];
+  int sw[kChunk];
+  RowsX<T, HALF> x[kTasks];
+  auto task_block = [&](int i) { return (wave + kRowsWaves * i) / MT; };
+  auto load_x = [&](int b0) {
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i)
+      if (b0 + task_block(i) < end) x[i].load(xp[i], (b0 + task_block(i)) * kBlock + 16 * g, a.K, n >= 8);
+  };
+  auto load_w = [&](int u, int b) {
+    sw[u] = ws[b];
+    w[u][0] = ld16(wp + (int64_t)b * kBlock);
+    w[u][1] = ld16(wp + (int64_t)b * kBlock + 64);
+  };
+  auto quantise = [&](int b0, int buf) {
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      const int u = task_block(i), m = (wave + kRowsWaves * i) % MT;
+      if (b0 + u >= end) continue;
+      if ((b0 + u + 1) * kBlock > a.K) x[i].clear_past((b0 + u) * kBlock + 16 * g, a.K, n >= 8);
+      uint32_t e;
+      const i32x8 v = x[i].operand(e);
+      codes[buf][u][m][0][lane] = u32x4{(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+      codes[buf][u][m][1][lane] = u32x4{(uint32_t)v[4], (uint32_t)v[5], (uint32_t)v[6], (uint32_t)v[7]};
+      if (g == 0) scales[buf][u][n][m] = (uint8_t)e;
+    }
+  };
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int u, int buf) {
+    const i32x8 wv = join(w[u][0], w[u][1]);
+    const int sx = *reinterpret_cast<const int*>(scales[buf][u][n]);
+    acc[0] = mfma_fp8<0>(wv, join(codes[buf][u][0][0][lane], codes[buf][u][0][1][lane]), acc[0], sw[u], sx);
+    if constexpr (MT > 1) acc[1] = mfma_fp8<1>(wv, join(codes[buf][u][1][0][lane], codes[buf][u][1][1][lane]), acc[1], sw[u], sx);
+    if constexpr (MT > 2) {
+      acc[2] = mfma_fp8<2>(wv, join(codes[buf][u][2][0][lane], codes[buf][u][2][1][lane]), acc[2], sw[u], sx);
+      acc[3] = mfma_fp8<3>(wv, join(codes[buf][u][3][0][lane], codes[buf][u][3][1][lane]), acc[3], sw[u], sx);
+    }
+  };
+  load_x(first);
+#pragma unroll
+  for (int u = 0; u < kChunk; ++u)
+    if (first + u < end) load_w(u, first + u);
+  quantise(first, 0);
+  barrier_lds();
+  // a chunk: the next one's x loads, this one's products, each block's weights replaced by the next chunk's, the next one's codes
+  for (int b0 = first, buf = 0; b0 < end; b0 += kChunk, buf ^= 1) {
+    load_x(b0 + kChunk);
+#pragma unroll
+    for (int u = 0; u < kChunk; ++u) {
+      if (b0 + u < end) multiply(u, buf);
+      if (b0 + kChunk + u < end) load_w(u, b0 + kChunk + u);
+    }
+    quantise(b0 + kChunk, buf ^ 1);
+    barrier_lds();
+  }
+  const int col = n0 + 4 * g;  // lane (n, g): row 16 m + n of y, outputs 4 g .. + 3 of the wavefront's
+  if (col >= a.N) return;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = 16 * m + n;
+    if (row >= a.M || (HALF && n >= 8)) continue;
+    if (a.ksplit > 1)
+      *reinterpret_cast<f32x4*>(a.part + ((int64_t)ks * a.M + row) * a.N + col) = acc[m];
+    else
+      st8(a.y + (int64_t)row * a.N + col, u32x2{pack2<T>(acc[m][0], acc[m][1]), pack2<T>(acc[m][2], acc[m][3])});
+  }
 }
 
 // ---------------------------------------------------------------- many rows: x quantised once, then tiles
@@ -304,7 +449,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OC
 // ---------------------------------------------------------------- launch rules
 
 struct Plan {
-  bool few, large;
+  bool rows, chunk, large;
   int ksplit;
   int64_t xq_bytes, sx_bytes, part_bytes;
 };
@@ -312,19 +457,26 @@ constexpr int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 Plan plan_linear(int64_t m, int64_t n, int64_t blocks, int cus) {
   Plan p{};
-  p.few = m <= kFewRows;
-  if (p.few) return p;
-  const int64_t large = ((n + 255) / 256) * ((m + 255) / 256), small = ((n + 127) / 128) * ((m + 127) / 128);
-  p.large = large * 4 >= 3 * (int64_t)cus;
   p.ksplit = 1;
-  if (!p.large && small < cus) {
-    int64_t ks = cus / small;
-    if (ks > 8) ks = 8;
-    if (ks > blocks / 4) ks = blocks / 4;
-    p.ksplit = ks < 1 ? 1 : (int)ks;
+  p.rows = m <= kInPlaceRows && n * blocks * kBlock <= kSmallWeights;
+  p.chunk = !p.rows && m <= kFewRows;
+  if (p.rows) return p;
+  if (p.chunk) {
+    // the parts do not depend on m, and those of small weights are the wavefronts' of fp8_rows_kernel: neither does a row's result
+    const int64_t tiles = (n + kBlock - 1) / kBlock, ks = (cus + tiles / 2) / tiles;
+    p.ksplit = n * blocks * kBlock <= kSmallWeights ? kRowsWaves : (int)(ks < 1 ? 1 : ks > blocks ? blocks : ks);
+  } else {
+    const int64_t large = ((n + 255) / 256) * ((m + 255) / 256), small = ((n + 127) / 128) * ((m + 127) / 128);
+    p.large = large * 4 >= 3 * (int64_t)cus;
+    if (!p.large && small < cus) {
+      int64_t ks = cus / small;
+      if (ks > 8) ks = 8;
+      if (ks > blocks / 4) ks = blocks / 4;
+      p.ksplit = ks < 1 ? 1 : (int)ks;
+    }
+    p.xq_bytes = align256(m * blocks * kBlock);
+    p.sx_bytes = align256(blocks * ((m + 63) / 64) * 64);
   }
-  p.xq_bytes = align256(m * blocks * kBlock);
-  p.sx_bytes = align256(blocks * ((m + 63) / 64) * 64);
   p.part_bytes = p.ksplit > 1 ? align256(4 * p.ksplit * m * n) : 0;
   return p;
 }
@@ -358,38 +510,35 @@ extern "C" int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64
   const int blocks = (int)((k + kBlock - 1) / kBlock);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const Plan p = plan_linear(m, n, blocks, device_cus());
-  if (p.few) {
-    RowsArgs a{(const char*)x, 2 * x_stride, (int)m, (int)k, (int)n, blocks, (const char*)weight, (const uint8_t*)weight_scales,
-               (uint16_t*)out};
-    auto launch = [&](auto tag) {
-      using T = decltype(tag);
-      const unsigned grid = (unsigned)(n / 16);
-      if (m <= 16)
-        fp8_rows_kernel<T, 1><<<grid, 64 * kRowsWaves, 0, st>>>(a);
-      else if (m <= 32)
-        fp8_rows_kernel<T, 2><<<grid, 64 * kRowsWaves, 0, st>>>(a);
-      else
-        fp8_rows_kernel<T, 4><<<grid, 64 * kRowsWaves, 0, st>>>(a);
-    };
-    if (dtype == MLLM_DTYPE_BF16)
-      launch(BF16{});
-    else
-      launch(F16{});
-    return check_launch(fn.c_str());
-  }
-  MLLM_REQUIRE(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= p.xq_bytes + p.sx_bytes + p.part_bytes,
-               MLLM_ERR_INVALID, fn + ": workspace too small or not 256-byte aligned");
+  const int64_t need = p.xq_bytes + p.sx_bytes + p.part_bytes;
+  MLLM_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= need), MLLM_ERR_INVALID,
+               fn + ": workspace too small or not 256-byte aligned");
   const int64_t quant_groups = (m * blocks * 8 + 255) / 256;
   const int64_t bn = p.large ? 256 : 128;
   const int64_t tiles_n = (n + bn - 1) / bn, tiles_m = (m + bn - 1) / bn, groups = tiles_n * tiles_m * p.ksplit;
-  MLLM_REQUIRE(quant_groups <= kMaxGroups256 && groups <= kMaxGroups256 / 2, MLLM_ERR_UNSUPPORTED, fn + ": too many rows");
+  MLLM_REQUIRE(p.rows || p.chunk || (quant_groups <= kMaxGroups256 && groups <= kMaxGroups256 / 2), MLLM_ERR_UNSUPPORTED,
+               fn + ": too many rows");
   char* base = static_cast<char*>(workspace);
-  TileArgs a{base, (const uint8_t*)base + p.xq_bytes, (const char*)weight, (const uint8_t*)weight_scales, (int)m, (int)n, blocks,
-             (int)((m + 63) / 64), (int)tiles_n, (int)tiles_m, p.ksplit, (uint16_t*)out, (float*)(base + p.xq_bytes + p.sx_bytes)};
+  uint8_t* sx = (uint8_t*)base + p.xq_bytes;
+  RowsArgs r{(const char*)x, 2 * x_stride, (int)m, (int)k, (int)n, blocks, (const char*)weight, (const uint8_t*)weight_scales,
+             (uint16_t*)out, (int)((n + kBlock - 1) / kBlock), p.ksplit, (float*)(sx + p.sx_bytes)};
+  TileArgs a{base, sx, (const char*)weight, (const uint8_t*)weight_scales, (int)m, (int)n, blocks, (int)((m + 63) / 64),
+             (int)tiles_n, (int)tiles_m, p.ksplit, (uint16_t*)out, (float*)(sx + p.sx_bytes)};
   auto launch = [&](auto tag) {
     using T = decltype(tag);
-    fp8_quant_kernel<T><<<(unsigned)quant_groups, 256, 0, st>>>((const char*)x, 2 * x_stride, (unsigned)m, (int)k, blocks, base,
-                                                               (uint8_t*)base + p.xq_bytes, (unsigned)a.groups64);
+    if (p.rows) {
+      if (m <= 8) return fp8_rows_kernel<T, true><<<(unsigned)(n / 16), 64 * kRowsWaves, 0, st>>>(r);
+      return fp8_rows_kernel<T, false><<<(unsigned)(n / 16), 64 * kRowsWaves, 0, st>>>(r);
+    }
+    if (p.chunk) {
+      const unsigned grid = (unsigned)(r.tiles * r.ksplit);
+      if (m <= 8) return fp8_chunk_kernel<T, 1, true><<<grid, 64 * kRowsWaves, 0, st>>>(r);
+      if (m <= 16) return fp8_chunk_kernel<T, 1, false><<<grid, 64 * kRowsWaves, 0, st>>>(r);
+      if (m <= 32) return fp8_chunk_kernel<T, 2, false><<<grid, 64 * kRowsWaves, 0, st>>>(r);
+      return fp8_chunk_kernel<T, 4, false><<<grid, 64 * kRowsWaves, 0, st>>>(r);
+    }
+    fp8_quant_kernel<T><<<(unsigned)quant_groups, 256, 0, st>>>((const char*)x, 2 * x_stride, (unsigned)m, (int)k, blocks, base, sx,
+                                                               (unsigned)a.groups64);
     if (p.large)
       fp8_tile_kernel<T, 256, 256, 2, 4, 2><<<(unsigned)groups, 512, 0, st>>>(a);
     else
@@ -400,6 +549,6 @@ extern "C" int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64
   else
     launch(F16{});
   const int rc = check_launch(fn.c_str());
-  if (rc != MLLM_OK || p.ksplit == 1) return rc;
-  return mllm_sum_partials(a.part, p.ksplit, m, n, nullptr, dtype, out, stream);
+  if (rc != MLLM_OK || p.ksplit <= 1) return rc;
+  return mllm_sum_partials(r.part, p.ksplit, m, n, nullptr, dtype, out, stream);
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(os.environ.get("MLLM_HIP_LIB", Path(__file__).resolve().parent / "_lib" / "libminillm_hip.so"))
@@ -53,6 +54,19 @@ class LayerPool(ctypes.Structure):
 
     _fields_ = [("k_cache", _p), ("v_cache", _p), ("k_scales", _p), ("v_scales", _p), ("k_scale", _f32),
                 ("v_scale", _f32), ("q_norm", _p), ("k_norm", _p), ("norm_eps", _f32)]
+
+
+def packer(cls):
+    """bytes of a struct from all its fields in order, in a quarter of the time a ctypes.Structure takes; a call takes them
+    where it takes the struct's address."""
+    codes = {_p: "P", _i64: "q", _i32: "i", _f32: "f"}
+    form = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0q")
+    assert form.size == ctypes.sizeof(cls)
+    return form.pack
+
+
+pack_rope_append = packer(RopeAppend)
+pack_layer_pool = packer(LayerPool)
 
 
 # symbol -> (restype, argtypes); the exact list include/minillm_hip.h declares
@@ -165,6 +179,19 @@ class NativeLib:
 
     def call(self, name: str, *args) -> None:
         self._check(getattr(self._cdll, name)(*args))
+
+    def launch(self, device, name: str, *args) -> None:
+        """call(name, *args, stream) on the current stream of `device`, which need not be the current device."""
+        import torch
+
+        index = device.index
+        if index is None or index == torch._C._cuda_getDevice():
+            status = getattr(self._cdll, name)(*args, stream_ptr(device))
+        else:
+            with torch.cuda.device(index):
+                status = getattr(self._cdll, name)(*args, stream_ptr(device))
+        if status != OK:
+            self._check(status)
 
     def workspace_bytes(self, num_work: int, num_heads: int, head_dim: int) -> int:
         return int(self._cdll.mllm_decode_workspace_bytes(num_work, num_heads, head_dim))

@@ -104,45 +104,43 @@ class Fp8Linear(nn.Module):
             raise ValueError(f"x must have {self.in_features} columns, not {x.shape[-1]}")
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("Fp8Linear is for inference: its rounding of x has no gradient (call it under no_grad)")
-        if kernels.usable(x, grad_ok=True) and self._kernel_ok(x):
-            return self._kernel(x)
+        if kernels.usable(x, grad_ok=True):
+            y = self._kernel(x)
+            if y is not None:
+                return y
+        elif not torch.compiler.is_compiling() and x.is_cuda and not _native.available():
+            _native.lib()  # raises: a GPU without the library is an error
         codes, e = quantize_rows(x.reshape(-1, self.in_features))
         rows = (codes.float().unflatten(1, (-1, BLOCK)) * _powers(e.view(torch.uint8))[..., None]).flatten(1)
         y = rows[:, :self.in_features] @ self.dequantized().t()
         return y.to(x.dtype).view(*x.shape[:-1], self.out_features)
 
-    def _kernel_ok(self, x: torch.Tensor) -> bool:
-        w, s = self.weight, self.weight_scale
-        rows = x.numel() // self.in_features
-        return (w.device == s.device == x.device and w.is_contiguous() and s.is_contiguous() and w.data_ptr() % 16 == 0
-                and s.data_ptr() % 4 == 0 and self.in_features <= 1 << 23 and self.out_features < 1 << 28
-                and rows * w.shape[1] <= kernels.MAX_GROUPS * 4096)
-
-    def _kernel(self, x: torch.Tensor) -> torch.Tensor:
-        k, n = self.in_features, self.out_features
+    def _kernel(self, x: torch.Tensor) -> torch.Tensor | None:
+        """The library's product, or None for operands that it does not take."""
+        k, n, device = self.in_features, self.out_features, x.device
+        w, s = self._buffers["weight"], self._buffers["weight_scale"]
+        m = x.numel() // k
+        if not (w.device == device == s.device and w.is_contiguous() and s.is_contiguous() and w.data_ptr() % 16 == 0
+                and s.data_ptr() % 4 == 0 and k <= 1 << 23 and n < 1 << 28 and m * w.shape[1] <= kernels.MAX_GROUPS * 4096):
+            return None
         if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
             rows, stride = x, x.stride(0)
         else:
             rows, stride = x.contiguous(), k
             if rows.data_ptr() % 16:
                 rows = rows.clone()
-        m = x.numel() // k
-        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], n))
         if m == 0:
             return out
         lib = _native.lib()
-        size = 0 if m <= FEW_ROWS else lib.fn("mllm_fp8_linear_workspace_bytes")(m, n, k, 0)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        lib.call("mllm_fp8_linear", rows.data_ptr(), stride, m, k, self.weight.data_ptr(), self.weight_scale.data_ptr(), n,
-                 _native.dtype_code(x.dtype), None if work is None else work.data_ptr(), size, out.data_ptr(),
-                 _native.stream_ptr(x.device))
+        size = lib.fn("mllm_fp8_linear_workspace_bytes")(m, n, k, 0)
+        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        lib.launch(device, "mllm_fp8_linear", rows.data_ptr(), stride, m, k, w.data_ptr(), s.data_ptr(), n,
+                   _native.dtype_code(x.dtype), None if work is None else work.data_ptr(), size, out.data_ptr())
         return out
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}"
-
-
-FEW_ROWS = 64  # rows up to which the library streams the weights and needs no workspace
 
 
 @torch.no_grad()

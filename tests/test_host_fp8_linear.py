@@ -128,9 +128,9 @@ def test_entry_point_checks_its_arguments():
             call(**kw)
     call(m=0, x=None, w=None, s=None, out=None)
     need = lib.fn("mllm_fp8_linear_workspace_bytes")
-    assert need(0, 256, 256, 256) == 0 and need(64, 4096, 4096, 256) == 0 < need(65, 4096, 4096, 256)
+    assert need(0, 256, 256, 256) == 0 and need(16, 4096, 4096, 256) == 0 < need(17, 4096, 4096, 256) < need(65, 4096, 4096, 256)
+    assert need(1, 14336, 4096, 256) == 2 * 4 * 14336  # two parts of K, fp32
     assert need(8192, 4096, 4096, 256) >= 8192 * (4096 + 32)
-    assert fp8.FEW_ROWS == 64 and need(fp8.FEW_ROWS, 16, 16, 256) == 0 < need(fp8.FEW_ROWS + 1, 16, 16, 256)
 
 
 def test_quantize_model():
