@@ -261,10 +261,11 @@ def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
     """ValueError unless k_scale and v_scale are the block scales of a 4-bit pool."""
     nb, bs, hkv, half = k_cache.shape
     blocks = 2 * half // FP4_BLOCK
+    device = k_cache.device
     for name, t, shape in (("k_scale", k_scale, (nb, bs, blocks, hkv)), ("v_scale", v_scale, (nb, hkv, blocks, bs))):
         if not isinstance(t, torch.Tensor) or t.dtype != SCALES4:
             raise ValueError(f"with a 4-bit pool, {name} is its float8_e8m0fnu tensor of block scales")
-        if t.shape != shape or not t.is_contiguous() or t.device != k_cache.device:
+        if t.shape != shape or not t.is_contiguous() or t.device != device:
             raise ValueError(f"{name} must be contiguous {list(shape)} on the pool's device")
 
 
@@ -278,16 +279,13 @@ def check_norms(qk_norm, q: torch.Tensor) -> None:
         raise ValueError("the head norms' eps must be finite and not negative")
 
 
-def layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm) -> _native.LayerPool:
+def layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm) -> bytes:
     """The mllm_layer_pool of a layer's checked pools, scales and head norms."""
-    pool = _native.LayerPool(k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), k_scale=1.0, v_scale=1.0)
+    norms = (0, 0, 0.0) if qk_norm is None else (qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2])
     if k_cache.dtype == FP4:
-        pool.k_scales, pool.v_scales = k_scale.data_ptr(), v_scale.data_ptr()
-    else:
-        pool.k_scale, pool.v_scale = k_scale, v_scale
-    if qk_norm is not None:
-        pool.q_norm, pool.k_norm, pool.norm_eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
-    return pool
+        return _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), 1.0,
+                                       1.0, *norms)
+    return _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, k_scale, v_scale, *norms)
 
 
 class HipBackend(AttentionBackend):
@@ -308,7 +306,6 @@ class HipBackend(AttentionBackend):
     def __init__(self) -> None:
         self._lib = _native.lib()
         self._attention_forward = self._lib.fn("mllm_attention_forward")
-        self._attention_forward_pool = self._lib.fn("mllm_attention_forward_pool")
         self._planned = None  # the AttentionMetadata the plan was last built for
         self._planned_pool = _native.POOL_16BIT  # and the pool type it was built for
         self._plan: StepPlan | None = None
@@ -345,12 +342,11 @@ class HipBackend(AttentionBackend):
         step = self._layer_step(plan, meta, q.shape[0], q.shape[1], q.shape[2], q.dtype, k_cache)
         rot = cos is not None
         if k_cache.dtype == FP4 or qk_norm is not None:
-            pool = layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm)
-            self._lib.check(self._attention_forward_pool(
-                step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                v.stride(0), v.stride(1), cos.data_ptr() if rot else None, sin.data_ptr() if rot else None,
-                cos.stride(0) if rot else 0, q_rot.data_ptr() if rot else None, ctypes.addressof(pool), out.data_ptr(),
-                _native.stream_ptr(q.device)))
+            self._lib.launch(
+                q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cos.data_ptr() if rot else None,
+                sin.data_ptr() if rot else None, cos.stride(0) if rot else 0, q_rot.data_ptr() if rot else None,
+                layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm), out.data_ptr())
             return
         self._lib.check(self._attention_forward(
             step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
@@ -482,24 +478,21 @@ class HipBackend(AttentionBackend):
             raise ValueError("q, cos and sin must share one dtype")
         if cos.stride(-1) != 1 or sin.stride() != cos.stride():
             cos, sin = cos.contiguous(), sin.contiguous()
-        wq = wk = None
-        eps = 0.0
+        wq, wk, eps = None, None, 0.0
         if qk_norm is not None:
             check_norms(qk_norm, q)
-            wq, wk, eps = qk_norm
+            wq, wk, eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
         q_rot = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
-        pool, fp4 = pool_type(k_cache), k_cache.dtype == FP4
-        args = _native.RopeAppend(
-            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride_tok=q.stride(0), q_stride_head=q.stride(1),
-            k_stride_tok=k.stride(0), k_stride_head=k.stride(1), v_stride_tok=v.stride(0), v_stride_head=v.stride(1),
-            cos=cos.data_ptr(), sin=sin.data_ptr(), cs_stride_tok=cos.stride(0), q_out=q_rot.data_ptr(),
-            q_out_stride_tok=h * dh, q_out_stride_head=dh, k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
-            k_scales=k_scale.data_ptr() if fp4 else None, v_scales=v_scale.data_ptr() if fp4 else None,
-            k_scale=1.0 if fp4 else k_scale, v_scale=1.0 if fp4 else v_scale, num_blocks=num_blocks,
-            slot_mapping=meta.slot_mapping.data_ptr(), num_tokens=n, block_size=bs, num_heads=h, num_kv_heads=hkv,
-            head_dim=dh, dtype=_native.dtype_code(q.dtype), pool=pool)
-        self._lib.call("mllm_qk_norm_rope_kv_append", ctypes.addressof(args), None if wq is None else wq.data_ptr(),
-                       None if wk is None else wk.data_ptr(), eps, _native.stream_ptr(q.device))
+        pool = pool_type(k_cache)
+        if pool == _native.POOL_FP4:
+            scales = (k_scale.data_ptr(), v_scale.data_ptr(), 1.0, 1.0)
+        else:
+            scales = (0, 0, k_scale, v_scale)
+        args = _native.pack_rope_append(  # the fields of mllm_rope_append in order
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], cos.data_ptr(),
+            sin.data_ptr(), cos.stride(0), q_rot.data_ptr(), h * dh, dh, k_cache.data_ptr(), v_cache.data_ptr(), *scales,
+            num_blocks, meta.slot_mapping.data_ptr(), n, bs, h, hkv, dh, _native.dtype_code(q.dtype), pool)
+        self._lib.launch(q.device, "mllm_qk_norm_rope_kv_append", args, wq, wk, eps)
         return q_rot
 
     def append(self, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0) -> None:
@@ -512,10 +505,10 @@ class HipBackend(AttentionBackend):
                 raise ValueError("the pools must be alike and the metadata describe k's tokens")
             check_scales(k_cache, k_scale, v_scale)
             k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
-            self._lib.call("mllm_kv_append_fp4", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                           v.stride(1), _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
-                           k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh,
-                           meta.slot_mapping.data_ptr(), k.shape[0], _native.stream_ptr(k_cache.device))
+            self._lib.launch(k_cache.device, "mllm_kv_append_fp4", k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                             *v.stride()[:2], _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
+                             k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh,
+                             meta.slot_mapping.data_ptr(), k.shape[0])
             return
         if is_fp8(k_cache):
             self._lib.call("mllm_kv_append_fp8", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
@@ -585,11 +578,12 @@ class HipBackend(AttentionBackend):
         num_blocks, bs, hkv, dh = k_cache.shape
         ws = self._workspace_for(plan.workspace_bytes, q.device)
         if k_cache.dtype == FP4:
-            self._lib.call("mllm_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                           v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv,
-                           2 * dh, plan.meta_ptrs[0], plan.meta_ptrs[2], _ptr(plan.decode_work), plan.num_decode,
-                           _ptr(plan.merge_work), plan.num_merge, plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
-                           out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes, _native.stream_ptr(q.device))
+            self._lib.launch(
+                q.device, "mllm_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv, 2 * dh,
+                plan.meta_ptrs[0], plan.meta_ptrs[2], plan.decode_args[4], plan.num_decode, plan.decode_args[6],
+                plan.num_merge, plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
+                out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes)
             return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
                 q.shape[1], hkv, dh, *plan.decode_args, dh ** -0.5, _native.dtype_code(q.dtype))
@@ -615,11 +609,11 @@ class HipBackend(AttentionBackend):
         plan = self._plan
         num_blocks, bs, hkv, dh = k_cache.shape
         if k_cache.dtype == FP4:
-            self._lib.call("mllm_paged_prefill_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                           v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv,
-                           2 * dh, *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile,
-                           (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(), out.stride(0), out.stride(1),
-                           _native.stream_ptr(q.device))
+            self._lib.launch(
+                q.device, "mllm_paged_prefill_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv, 2 * dh,
+                *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile, (2 * dh) ** -0.5,
+                _native.dtype_code(q.dtype), out.data_ptr(), out.stride(0), out.stride(1))
             return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
                 q.shape[1], hkv, dh, *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile,

@@ -82,12 +82,11 @@ class PagedKVCache:
         slots = slots.contiguous()
         n = slots.numel()
         out = torch.empty((2, n, hkv, 2 * half), dtype=dtype, device=k.device)
-        with torch.cuda.device(k.device):
-            _native.lib().call("mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
-                               self.v_scale[layer].data_ptr(), nb, bs, hkv, 2 * half, slots.data_ptr(), n,
-                               _native.dtype_code(dtype), out[0].data_ptr(), out[1].data_ptr(),
-                               _native.stream_ptr(k.device))
-        return out[0], out[1]
+        to_k, to_v = out.unbind()
+        _native.lib().launch(k.device, "mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
+                             self.v_scale[layer].data_ptr(), nb, bs, hkv, 2 * half, slots.data_ptr(), n,
+                             _native.dtype_code(dtype), to_k.data_ptr(), to_v.data_ptr())
+        return to_k, to_v
 
     @staticmethod
     def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE) -> int:

@@ -9,7 +9,6 @@ a submodule's `__call__` does nothing but its class's `forward`, so that a fused
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -136,11 +135,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         cos, sin = cos.contiguous(), sin.contiguous()
     q_out = torch.empty((b, h, t, dh), dtype=q.dtype, device=q.device)
     k_out = torch.empty((b, k.shape[1], t, dh), dtype=q.dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        _native.lib().call("mllm_qk_norm_rope", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], cos.data_ptr(),
-                           sin.data_ptr(), *cos.stride()[:2], q_weight.data_ptr(), k_weight.data_ptr(), eps, b, t, h,
-                           k.shape[1], dh, _native.dtype_code(q.dtype), q_out.data_ptr(), k_out.data_ptr(),
-                           _native.stream_ptr(q.device))
+    _native.lib().launch(q.device, "mllm_qk_norm_rope", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                         cos.data_ptr(), sin.data_ptr(), *cos.stride()[:2], q_weight.data_ptr(), k_weight.data_ptr(), eps, b,
+                         t, h, k.shape[1], dh, _native.dtype_code(q.dtype), q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -283,10 +280,9 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
                           device=x.device)
     step = backend.layer_step(meta, n, h, x.dtype, kc)
     out = torch.empty_like(x)
-    pool = layer_pool(kc, vc, ks, vs, qk_norm)
     lib.call("mllm_decoder_layer_pool", step, x.data_ptr(), d, norm1.weight.data_ptr(), norm1.eps, wq.data_ptr(),
              wk.data_ptr(), wv.data_ptr(), attn.o_proj.weight.data_ptr(), norm2.weight.data_ptr(), norm2.eps,
              gate.data_ptr(), mlp.up_proj.weight.data_ptr(), mlp.down_proj.weight.data_ptr(), ffn, cos.data_ptr(),
-             sin.data_ptr(), dh, ctypes.addressof(pool), scratch.data_ptr(), scratch.numel(), out.data_ptr(),
+             sin.data_ptr(), dh, layer_pool(kc, vc, ks, vs, qk_norm), scratch.data_ptr(), scratch.numel(), out.data_ptr(),
              _native.stream_ptr(x.device))
     return out
