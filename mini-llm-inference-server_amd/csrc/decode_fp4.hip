@@ -325,6 +325,9 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
 // partials alone decides, so a row's result does not depend on the launch: WIDE, for steps whose rows have many, has a
 // workgroup per head, of which every eighth serves the short rows; without it a workgroup serves eight heads of either.
 constexpr int kFewPartials = 8;
+// Up to this many workgroups a step is WIDE whatever its rows have: 40 rows of 256-8,192 tokens beside 8 prompt chunks 114 us
+// against 120; for 256 rows of 128-4,096 tokens, where most have few partials, 8192 workgroups take 1 us more than 1024.
+constexpr int kWideGroups = 2048;
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void merge_fp4_kernel(const int4* __restrict__ merge, const float* __restrict__ part_o,
                                                        const float2* __restrict__ part_ml, int H,
@@ -415,7 +418,7 @@ template <typename T>
 int launch_merge_fp4(const DecodeFp4Args& a, const int32_t* merge_work, int num_merge, int n_work, const int32_t* qo_indptr,
                      hipStream_t st) {
   const int4* merge = reinterpret_cast<const int4*>(merge_work);
-  if (max_bins(n_work) >= kFewPartials * num_merge)
+  if (max_bins(n_work) >= kFewPartials * num_merge || (int64_t)num_merge * a.H <= kWideGroups)
     merge_fp4_kernel<T, true><<<dim3(num_merge, a.H), 256, 0, st>>>(merge, a.part_o, a.part_ml, a.H, qo_indptr, a.out, a.o_st,
                                                                    a.o_sh);
   else
