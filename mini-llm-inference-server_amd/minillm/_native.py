@@ -158,6 +158,11 @@ class NativeLib:
         version = self._cdll.mllm_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"{path} has ABI version {version}, expected {ABI_VERSION}")
+        import torch
+
+        # what `launch` asks on every call, without Python in between where torch offers it
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", stream_ptr)
 
     def last_error(self) -> str:
         return (self._cdll.mllm_last_error() or b"").decode()
@@ -182,13 +187,13 @@ class NativeLib:
 
     def launch(self, device, name: str, *args) -> None:
         """call(name, *args, stream) on the current stream of `device`, which need not be the current device."""
-        import torch
-
         index = device.index
-        if index is None or index == torch._C._cuda_getDevice():
-            status = getattr(self._cdll, name)(*args, stream_ptr(device))
+        if index == self._current_device():
+            status = getattr(self._cdll, name)(*args, self._raw_stream(index))
         else:
-            with torch.cuda.device(index):
+            import torch
+
+            with torch.cuda.device(device):
                 status = getattr(self._cdll, name)(*args, stream_ptr(device))
         if status != OK:
             self._check(status)

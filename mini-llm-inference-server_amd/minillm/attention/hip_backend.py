@@ -504,7 +504,8 @@ class HipBackend(AttentionBackend):
             if meta.slot_mapping.numel() != k.shape[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
                 raise ValueError("the pools must be alike and the metadata describe k's tokens")
             check_scales(k_cache, k_scale, v_scale)
-            k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
+            if k.stride(2) != 1 or v.stride(2) != 1:
+                k, v = k.contiguous(), v.contiguous()
             self._lib.launch(k_cache.device, "mllm_kv_append_fp4", k.data_ptr(), *k.stride()[:2], v.data_ptr(),
                              *v.stride()[:2], _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
                              k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh,
