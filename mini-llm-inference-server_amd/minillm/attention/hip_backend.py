@@ -269,6 +269,22 @@ def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
             raise ValueError(f"{name} must be contiguous {list(shape)} on the pool's device")
 
 
+def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, out: torch.Tensor) -> None:
+    """ValueError unless q and out are [N, H, Dh] rows of the step's tokens over these 4-bit pools."""
+    _, bs, hkv, half = k_cache.shape
+    n, h, dh = q.shape
+    if dh != 2 * half or h % hkv or n != meta.query_start_loc[-1] or bs != meta.block_size:
+        raise ValueError(f"q must be [N, H, Dh] = [{meta.query_start_loc[-1]}, a multiple of {hkv}, {2 * half}], and the pool's "
+                         f"blocks {meta.block_size} tokens")
+    if out.shape != q.shape or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("out must be like q, both with unit stride in their last dimension")
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+            or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache and v_cache must be alike and contiguous")
+    if not q.device == out.device == k_cache.device == v_cache.device:
+        raise ValueError("q, out and the pools must share one device")
+
+
 def check_norms(qk_norm, q: torch.Tensor) -> None:
     """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's."""
     wq, wk, eps = qk_norm
@@ -405,6 +421,8 @@ class HipBackend(AttentionBackend):
                 raise ValueError(f"with {'an fp8' if is_fp8(k_cache) else 'a 4-bit'} pool, q, k and v must share one "
                                  f"dtype, bfloat16 or float16")
         if k_cache.dtype == FP4:
+            if not q.device == k.device == v.device == k_cache.device == v_cache.device:
+                raise ValueError("q, k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
         elif is_fp8(k_cache):
             if not (0 < k_scale < math.inf and 0 < v_scale < math.inf):
@@ -499,10 +517,13 @@ class HipBackend(AttentionBackend):
         """KV append (reference write_kv, paged_torch_ref.py:23-28): one launch for K and V."""
         num_blocks, bs, hkv, dh = k_cache.shape
         if k_cache.dtype == FP4:
-            if k.shape != (k.shape[0], hkv, 2 * dh) or v.shape != k.shape or v.dtype != k.dtype:
+            if k.dim() != 3 or k.shape[1:] != (hkv, 2 * dh) or v.shape != k.shape or v.dtype != k.dtype:
                 raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {2 * dh}] of one dtype")
-            if meta.slot_mapping.numel() != k.shape[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-                raise ValueError("the pools must be alike and the metadata describe k's tokens")
+            if meta.slot_mapping.numel() != k.shape[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+                    or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+                raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
+            if not k.device == v.device == k_cache.device == v_cache.device:
+                raise ValueError("k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
             if k.stride(2) != 1 or v.stride(2) != 1:
                 k, v = k.contiguous(), v.contiguous()
@@ -549,6 +570,7 @@ class HipBackend(AttentionBackend):
     def attend(self, q, k_cache, v_cache, meta, out, k_scale=1.0, v_scale=1.0) -> None:
         """Attention of every new token over its row's context in the pool, written into `out`."""
         if k_cache.dtype == FP4:
+            check_attend(q, k_cache, v_cache, meta, out)
             check_scales(k_cache, k_scale, v_scale)
         plan = self._plan_for(meta, q, k_cache)
         if plan.num_decode and plan.num_prefill and self.overlap_mixed and not torch.cuda.is_current_stream_capturing():

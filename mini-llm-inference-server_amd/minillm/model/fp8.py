@@ -94,6 +94,12 @@ class Fp8Linear(nn.Module):
         with torch.no_grad():
             return cls.from_parts(*quantize_blocks(linear.weight.detach()))
 
+    def _apply(self, fn, recurse=True):
+        """Moves go through, casts of floating types leave codes and scales alone."""
+        for name, dtype in (("weight", E4M3), ("weight_scale", E8M0)):
+            self._buffers[name] = fn(self._buffers[name].view(torch.uint8)).view(dtype)
+        return self
+
     def dequantized(self) -> torch.Tensor:
         """The weights' values, float32 [out_features, in_features]."""
         s = _powers(self.weight_scale.view(torch.uint8)).repeat_interleave(BLOCK, 0)[:self.out_features]

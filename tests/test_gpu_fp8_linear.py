@@ -151,10 +151,11 @@ def test_nan_weights_and_scales_stay_in_their_outputs(hip):
         assert torch.equal(bits(got[:, keep]), bits(want[:, keep]))
 
 
-def test_captured_calls(hip):
+@pytest.mark.parametrize("n,k,sizes", [(1040, 1024, (8, 300)), (9232, 2048, (8, 40)), (1040, 2048, (20, 70))])
+def test_captured_calls(hip, n, k, sizes):
     # two graphs of one layer, replayed between eager calls of other sizes
-    lin, _ = layer(1040, 1024)
-    xs = [rows(m, 1024, torch.bfloat16, seed=m).to(DEV) for m in (8, 300)]
+    lin, _ = layer(n, k)
+    xs = [rows(m, k, torch.bfloat16, seed=m).to(DEV) for m in sizes]
     graphs = []
     with torch.no_grad():
         want = [lin(x) for x in xs]
@@ -173,9 +174,26 @@ def test_captured_calls(hip):
             for (g, y), w in zip(graphs, want):
                 y.zero_()
                 g.replay()
-                lin(xs[1][:200])
+                lin(xs[1][:2 * sizes[1] // 3])
                 torch.cuda.synchronize()
                 assert torch.equal(bits(y), bits(w))
+
+
+def test_two_streams_at_once(hip):
+    lin, _ = layer(9232, 2048)
+    xs = [rows(m, 2048, torch.bfloat16, seed=m).to(DEV) for m in (40, 60, 500)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    with torch.no_grad():
+        want = [lin(x) for x in xs]
+        torch.cuda.synchronize()
+        got = [[], [], []]
+        for _ in range(5):
+            for x, s, y in zip(xs, streams, got):
+                with torch.cuda.stream(s):
+                    y.append(lin(x))
+        torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(bits(y), bits(w)) for y in ys)
 
 
 def test_model_of_8bit_blocks(hip):

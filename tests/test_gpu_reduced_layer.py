@@ -289,3 +289,35 @@ def test_contiguous_model_of_the_same_weights(hip, t):
         got = attn.attend(x, cos, sin)
         want = attn._contiguous(*kernels.qk_norm_rope(q, k, cos, sin, attn.q_norm.weight, attn.k_norm.weight, 1e-5), v, None)
     assert torch.equal(bits(got), bits(want))
+
+
+def test_two_steps_on_two_streams(hip):
+    # appends and attention of two steps over two layers' pools, each on its own stream with its own backend, at once
+    from test_gpu_fp4 import append, make_cache
+
+    from minillm.attention import get_backend
+    from minillm.attention.metadata import AttentionMetadata, SeqStep
+
+    g = torch.Generator().manual_seed(9)
+    jobs = []
+    for rows in ([(3000, 1), (70, 1), (900, 1)], [(64, 200), (1500, 1), (0, 33)]):
+        need = [-(-(c + n) // 16) for c, n in rows]
+        ids = torch.randperm(sum(need), generator=g).tolist()
+        meta = AttentionMetadata.build([SeqStep(c, n, [ids.pop() for _ in range(w)]) for (c, n), w in zip(rows, need)], 16, DEV)
+        cache = make_cache(8, sum(need))
+        append(cache, *(torch.randn(16 * sum(need), 8, 128, generator=g).bfloat16().to(DEV) for _ in range(2)),
+               torch.arange(16 * sum(need), device=DEV))
+        n = sum(m for _, m in rows)
+        q, k, v = (torch.randn(n, h, 128, generator=g).bfloat16().to(DEV) for h in (32, 8, 8))
+        be = get_backend("hip")
+        jobs.append((be, (q, k, v, cache.k[0], cache.v[0], meta), cache.scales(0), be.forward(q, k, v, cache.k[0], cache.v[0], meta,
+                                                                                           **cache.scales(0))))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], [[], []]
+    for _ in range(5):
+        for (be, args, scales, _), s, out in zip(jobs, streams, got):
+            with torch.cuda.stream(s):
+                out.append(be.forward(*args, **scales))
+    torch.cuda.synchronize()
+    for (*_, want), outs in zip(jobs, got):
+        assert all(torch.equal(bits(o), bits(want)) for o in outs)

@@ -125,6 +125,17 @@ def test_backend_refusals():
         be.append(k, k, kc, vc, Meta)
     with pytest.raises(ValueError, match="block scales"):
         be.attend(q, kc, vc, Meta, q)
+    for kw, match in ((dict(q=q[:3]), "N, H, Dh"), (dict(q=q[:, :3]), "N, H, Dh"), (dict(q=q[..., :64]), "N, H, Dh"),
+                      (dict(out=q.float()), "out must be like q"), (dict(out=q[:, :2]), "out must be like q"),
+                      (dict(out=torch.zeros(5, 4, 256, dtype=q.dtype)[..., ::2]), "unit stride"), (dict(vc=vc[:2]), "alike"),
+                      (dict(out=q.to("meta")), "one device"), (dict(q=q.to("meta")), "one device")):
+        a = dict(q=q, vc=vc, out=torch.empty_like(q)) | kw
+        with pytest.raises(ValueError, match=match):
+            be.attend(a["q"], kc, a["vc"], Meta, a["out"], **scales)
+    with pytest.raises(ValueError, match="one device"):
+        be.append(k, k.to("meta"), kc, vc, Meta, **scales)
+    with pytest.raises(ValueError, match="one device"):
+        be.forward(q.to("meta"), k, k, kc, vc, Meta, **scales)
     # 16-bit pools take neither
     p16 = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="fp8 pools only"):

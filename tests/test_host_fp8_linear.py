@@ -155,3 +155,18 @@ def test_quantize_model():
     assert kinds.count("Fp8Linear") == 14 and kinds.count("Linear") == 1
     with torch.no_grad():
         assert torch.isfinite(model(torch.arange(20)[None])).all()
+
+
+def test_casts_leave_codes_and_scales_alone():
+    layer = Fp8Linear.from_linear(torch.nn.Linear(272, 48, bias=False))
+    codes, scales = layer.weight.view(torch.uint8).clone(), layer.weight_scale.view(torch.uint8).clone()
+    x = torch.randn(3, 272)
+    want = layer(x)
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu", torch.float16)):
+        stack = cast(torch.nn.Sequential(layer, torch.nn.Linear(48, 2)))
+        assert stack[1].weight.dtype != torch.float32
+        assert layer.weight.dtype == torch.float8_e4m3fn and layer.weight_scale.dtype == torch.float8_e8m0fnu
+        assert torch.equal(layer.weight.view(torch.uint8), codes) and torch.equal(layer.weight_scale.view(torch.uint8), scales)
+        assert torch.equal(layer(x), want)
+    moved = layer.to("meta")
+    assert moved.weight.device.type == "meta" and moved.weight.dtype == torch.float8_e4m3fn
