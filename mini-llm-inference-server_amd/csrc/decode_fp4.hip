@@ -214,12 +214,12 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
   // tiles of a segment: pages past the row's last token (a block table may hold pages ahead) have none
   auto tiles_of = [&](const int4& r0) { return max(min(r0.w, (r0.z + r0.y) * a.bs) - r0.z * a.bs + 15, 0) >> 4; };
 
-  // This slice's tiles in the order they are consumed, one ahead: the segment, the tile and the block it lies in.  Behind the
-  // last one the cursor stays, and loads that tile again, unused.
+  // This slice's tiles in the order they are consumed, one ahead: the segment, the tile and the block it lies in.
   typedef const __attribute__((address_space(4))) int ConstI32;
   ConstI32* indices = (ConstI32*)a.kv_indices;
   const int glast = bw.y - 1;
   int cg = bw.x, ct = slice, cblk, csub;
+  bool more;  // the cursor is on a tile; behind the last one it stays there, without
   int4 cr = plan_rec(segs, 2 * cg);
   int cn = tiles_of(cr);
   auto settle = [&]() {  // to the slice's next tile at or behind (cg, ct), and its block
@@ -229,6 +229,7 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
       cn = tiles_of(cr);
       ct = slice;
     }
+    more = ct < cn;
     const int t = min(ct, max(cn - 1, 0));
     const int page = tpp == 1 ? t : t / tpp;
     csub = t - page * tpp;
@@ -256,18 +257,23 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
     const int tok0 = cur.r0.z * a.bs, len = cur.r0.w;
     const int ntiles = tiles_of(cur.r0);
     const SegRec after = seg_rec(segs, min(gi + 2, glast));
-    load_q(nxt.r1.x, buf ^ 1);
+    if (has_next) load_q(nxt.r1.x, buf ^ 1);
     float m_run = -INFINITY, l_run = 0.f;
     f32x4 o[D];
 #pragma unroll
     for (int m = 0; m < D; ++m) o[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     const bool runs = has_heads && slice < ntiles;
     if (has_heads) {
-      for (int t = slice; t < ntiles; t += SL) {
-        issue(ahead);
+      auto consume = [&](int t) {
         consume_tile4<T, NH>(tile, &qs[buf][grp][0][lane], myhead, a.scale_log2, tok0 + t * 16, len, g, m_run, l_run, o);
+      };
+      int t = slice;
+      for (; t < ntiles && more; t += SL) {
+        issue(ahead);
+        consume(t);
         tile = ahead;
       }
+      if (t < ntiles) consume(t);  // the bin's last: a load behind it would only be waited for (0.4 us of a small step's 11)
     }
 
     // lane (c, g): o[m][i] is dim D (4 g + i) + m of the joint row; kept where that is the column's own head
