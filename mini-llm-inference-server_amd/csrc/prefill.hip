@@ -36,8 +36,9 @@
 //
 // 4-bit pools (kv_fp4.hip) go the same way: a lane loads eight bytes, 16 codes, and the byte of their block's scale, which the
 // conversion to bf16/fp16 applies (exact).  Loads of a quarter of the bytes do not pay here, where the matrix pipes bound the
-// kernel: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 404 us, 388 from an fp8 pool, 366 by DMA
-// from a 16-bit one; the two register stages and the widening are the difference.
+// kernel: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 399 us, 391 from an fp8 pool, 370 by DMA
+// from a 16-bit one.  Without its loads in the loop the 4-bit kernel took 343, with loads but no widening 378: per-lane
+// addresses cost most of the difference (408 with the scale's address made per load, and its pair's products in two parts).
 #include <math.h>
 
 #include <type_traits>
@@ -130,32 +131,39 @@ struct Staged<kPoolFp4> {
 
 // fp8 and 4-bit pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7) is one load of 16 values per
 // lane: row 8 w + l / 8, dims 16 (l % 8) .. +15.  off: the lane's offset from the group base for a full
-// tile.  Keys past `last` load the row of `last`, as in dma_tile.
+// tile, eoff: from its rows' scales (scale_offset).  Keys past `last` load the row of `last`, as in dma_tile.
 template <int POOL, bool IS_V>
 __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const PrefillArgs& a, int blk, int kv0, int last,
-                                                   int kv_end, int w, unsigned off, unsigned head_bytes, int lane) {
+                                                   int kv_end, int w, unsigned off, unsigned eoff, unsigned head_bytes, int lane) {
   constexpr unsigned kLane = POOL == kPoolFp8 ? 16 : 8;  // bytes of 16 values
   const int key0 = kv0 + 16 * (w >> 1);
-  const char* p;
-  int tok;  // the row within its block
-  if (kv0 + kBN <= kv_end) {
-    p = group_base(pool, a, blk, key0) + off;
-    tok = (key0 & (a.bs - 1)) + 8 * (w & 1) + (lane >> 3);
-  } else {
-    tok = min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);
-    p = group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
-  }
+  const bool whole = kv0 + kBN <= kv_end;
+  const int tok = whole ? 0 : min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);  // the row within its block
   if constexpr (POOL != kPoolFp4) {
+    const char* p = whole ? group_base(pool, a, blk, key0) + off
+                          : group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
     return {ld16(p)};
   } else {
+    // a load per branch: merged, the two addresses would be a pair of registers per lane instead of a scalar and an offset
     constexpr int kBlocks = kHeadDim / kFp4Block;
-    const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
-    const uint64_t page = (uint64_t)b * (unsigned)(a.Hkv * kBlocks * a.bs);
-    const unsigned h = head_bytes / (kHeadDim / 2), c = (lane & 7) >> 1;  // KV head, dim block
-    const uint8_t* sp = IS_V ? a.vs + page + ((h * kBlocks + c) * (unsigned)a.bs + tok)
-                             : a.ks + page + ((unsigned)(tok * kBlocks) + c) * (unsigned)a.Hkv + h;
-    return {ld8(p), *sp};
+    const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u, kvh = head_bytes / (kHeadDim / 2);
+    const uint8_t* sp = (IS_V ? a.vs : a.ks) + (uint64_t)b * (unsigned)(a.Hkv * kBlocks * a.bs);
+    if (whole) {
+      const unsigned row = (unsigned)(key0 & (a.bs - 1)) + 8u * (w & 1);
+      sp += IS_V ? kvh * (unsigned)(kBlocks * a.bs) + row : row * (unsigned)(kBlocks * a.Hkv) + kvh;
+      return {ld8(group_base(pool, a, blk, key0) + off), sp[eoff]};
+    }
+    const unsigned c = (lane & 7) >> 1;  // dim block
+    sp += IS_V ? (kvh * kBlocks + c) * (unsigned)a.bs + (unsigned)tok : ((unsigned)(tok * kBlocks) + c) * (unsigned)a.Hkv + kvh;
+    return {ld8(group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7))), *sp};
   }
+}
+
+// What a lane adds to its rows' uniform scale address in a full tile (4-bit pools).
+template <bool IS_V>
+__device__ __forceinline__ unsigned scale_offset(const PrefillArgs& a, int lane) {
+  const unsigned c = (lane & 7) >> 1, r = lane >> 3;
+  return IS_V ? c * (unsigned)a.bs + r : (r * (kHeadDim / kFp4Block) + c) * (unsigned)a.Hkv;
 }
 
 // Widens a lane's 16 values to two 16-byte chunks of 16-bit values (logical chunks 2 (l % 8) and
@@ -428,6 +436,7 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
   const unsigned voff0 = (unsigned)(r0 & 15) * rb + head_bytes + 16u * v_chunk(r0, lane);
   const unsigned voff1 = (unsigned)(r1 & 15) * rb + head_bytes + 16u * v_chunk(r1, lane);
   const unsigned soff = (unsigned)(8 * (wave & 1) + (lane >> 3)) * rb + head_bytes + (POOL == kPoolFp4 ? 8u : 16u) * (lane & 7);  // fp8, fp4
+  const unsigned eoff_k = scale_offset<false>(a, lane), eoff_v = scale_offset<true>(a, lane);  // 4-bit
   const unsigned kread = (unsigned)(n * kRowBytes + 16 * (h ^ (n & 1)) + 32 * ((n & 15) >> 1));
   const unsigned vread = (unsigned)(kVBase + 1024 * h + 320 * ((lane >> 2) & 3) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 
@@ -462,8 +471,8 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
     for (int t = 0; t < 4; ++t) {
       if (t < ntiles) {
         const int b = blk_direct(t);
-        kx[t] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
-        if (t < 2) vx[t] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, wu, soff, head_bytes, lane);
+        kx[t] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
+        if (t < 2) vx[t] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
       }
     }
 #pragma unroll
@@ -523,8 +532,8 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
         load_ids(wbase, wsel);
       }
       if constexpr (POOL != kPool16) {
-        if (ta + 2 < ntiles) st_a = stage_load<POOL, true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, head_bytes, lane);
-        if (ta + 3 < ntiles) st_b = stage_load<POOL, true>(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+        if (ta + 2 < ntiles) st_a = stage_load<POOL, true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
+        if (ta + 3 < ntiles) st_b = stage_load<POOL, true>(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
       } else {
         if (ta + 2 < ntiles)
           dma_tile<true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, voff0, voff1, head_bytes, lane, v_slot(ta + 2));
@@ -536,13 +545,13 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
           dma_tile<false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, koff0, koff1, head_bytes, lane, k_slot(ta + 5));
       }
     } else if constexpr (POOL != kPool16) {
-      if (ta + 4 < ntiles) st_a = stage_load<POOL, false>(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, head_bytes, lane);
-      if (ta + 5 < ntiles) st_b = stage_load<POOL, false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, head_bytes, lane);
+      if (ta + 4 < ntiles) st_a = stage_load<POOL, false>(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
+      if (ta + 5 < ntiles) st_b = stage_load<POOL, false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
     }
     if ((p & 1) == grp) {  // matrix phase of pair j
       __builtin_amdgcn_s_setprio(1);
-      // all four products of the pair (fp8 pools keep two tiles of staging registers: no single ring)
-      const bool full = POOL == kPool16 && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
+      // all four products of the pair (fp8 pools keep two tiles of staging registers, eight of them: no single ring)
+      const bool full = POOL != kPoolFp8 && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
       if (full) {
         matrix_phase_pair<T>(lds, vread + (ta & (kRingV - 1)) * kTileBytes, kread + ((ta + 2) & (kRingK - 1)) * kTileBytes,
                              vread + ((ta + 1) & (kRingV - 1)) * kTileBytes, kread + ((ta + 3) & (kRingK - 1)) * kTileBytes,
@@ -746,16 +755,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   // fp8: this wavefront's rows as two 8-row shares (those of wavefront 2 w + i of the 8-wavefront layout)
   const unsigned soff0 = (unsigned)(lane >> 3) * rb + head_bytes + (POOL == kPoolFp4 ? 8u : 16u) * (lane & 7), soff1 = soff0 + 8 * rb;
+  const unsigned eoff_k = scale_offset<false>(a, lane), eoff_v = scale_offset<true>(a, lane);  // 4-bit
   const char* kc = reinterpret_cast<const char*>(a.kc);
   const char* vc = reinterpret_cast<const char*>(a.vc);
   typedef Staged<POOL> Staged2[2];
   auto stage_k = [&](int b, int t, Staged2& x) {
-    x[0] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, head_bytes, lane);
-    x[1] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, head_bytes, lane);
+    x[0] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, eoff_k, head_bytes, lane);
+    x[1] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, eoff_k, head_bytes, lane);
   };
   auto stage_v = [&](int b, int t, Staged2& x) {
-    x[0] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, head_bytes, lane);
-    x[1] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, head_bytes, lane);
+    x[0] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, eoff_v, head_bytes, lane);
+    x[1] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, eoff_v, head_bytes, lane);
   };
   auto store_k = [&](const Staged2& x, char* slot) {
     stage_store<T, false>(x[0], 2 * wu, lane, slot);
