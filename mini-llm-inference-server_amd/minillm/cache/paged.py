@@ -62,17 +62,19 @@ class PagedKVCache:
     def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of K and V at `slots` [n] (int64, on the pool's device; as a step's slot_mapping names them), both
         [n, Hkv, Dh] of `dtype`: by default the pool's own, bfloat16 for fp8 and 4-bit pools.  A 4-bit pool is read with the
-        16-bit type it was written with."""
+        16-bit type it was written with.  A slot outside the pool reads as zeros."""
         k, v = self.k[layer], self.v[layer]
         if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != k.device:
             raise ValueError("slots must be one row of int64 on the pool's device")
         dtype = dtype or (torch.bfloat16 if self.quantized or self.fp4 else k.dtype)
         if not self.fp4:
-            got = []
+            got, outside = [], (slots < 0) | (slots >= k.shape[0] * k.shape[1])
+            slots = slots.masked_fill(outside, 0)
             for pool, scale in ((k, self.k_scale[layer]), (v, self.v_scale[layer])):
                 raw = pool.view(torch.uint8) if self.quantized else pool
                 rows = raw.flatten(0, 1).index_select(0, slots)
-                got.append((rows.view(pool.dtype).float() * scale if self.quantized else rows).to(dtype))
+                rows = rows.view(pool.dtype).float() * scale if self.quantized else rows
+                got.append(rows.masked_fill(outside[:, None, None], 0).to(dtype))
             return got[0], got[1]
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("a 4-bit pool is read as bfloat16 or float16")

@@ -59,7 +59,7 @@ class Fp8Linear(nn.Module):
     """A bias-free linear layer of 8-bit blocks.  `weight` [out_features, in_features padded with zeros to a multiple of 128]
     e4m3, `weight_scale` [ceil(out / 128), ceil(in / 128)] e8m0; both sizes multiples of 16.  On a GPU it takes bfloat16 and
     float16 rows to the kernels; elsewhere, and under a compiler or another function mode, the same result comes from torch
-    operations in float32."""
+    operations in float32.  torch.jit.trace and vmap, which have no rule for reading a number's bits, raise."""
 
     def __init__(self, in_features: int, out_features: int, device=None) -> None:
         super().__init__()

@@ -71,6 +71,9 @@ def test_read_of_other_pools(dtype):
     for got, x, s in ((got_k, k, 0.5), (got_v, v, 2.0)):
         want = x.to(dtype).float() * (s if fp8 else 1.0)
         assert torch.equal(got, want.flatten(0, 1)[slots].to(got.dtype))
+    # a step's padding rows have no slot
+    for got in cache.read(1, torch.tensor([-1, 5, 64])):
+        assert bool((got[::2] == 0).all()) and bool((got[1] != 0).any())
 
 
 def test_split_sizes_of_4bit_pools():
