@@ -512,7 +512,8 @@ typedef struct mllm_layer_pool {
   float norm_eps;
 } mllm_layer_pool;
 
-/* mllm_attention_forward and mllm_decoder_layer over any pool type, with head norms where given (mllm_qk_norm_rope_kv_append). */
+/* mllm_attention_forward and mllm_decoder_layer over any pool type, with head norms where given (mllm_qk_norm_rope_kv_append).
+ * With k, v and cos NULL nothing is appended: the attention of q alone. */
 int mllm_attention_forward_pool(const mllm_layer_step* step, const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                                 const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v,
                                 int64_t v_stride_tok, int64_t v_stride_head, const void* cos, const void* sin,

@@ -26,7 +26,9 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
   int rc;
   const void* qa = q;
   int64_t qa_st = q_stride_tok, qa_sh = q_stride_head;
-  if (cos && (fp4 || p->q_norm)) {
+  if (!k && !v && !cos) {
+    rc = MLLM_OK;
+  } else if (cos && (fp4 || p->q_norm)) {
     mllm_rope_append r = {};
     r.q = q, r.q_stride_tok = q_stride_tok, r.q_stride_head = q_stride_head;
     r.k = k, r.k_stride_tok = k_stride_tok, r.k_stride_head = k_stride_head;
@@ -117,6 +119,7 @@ extern "C" int mllm_attention_forward(const mllm_layer_step* s, const void* q, i
                                       int64_t v_stride_head, const void* cos, const void* sin, int64_t cs_stride_tok,
                                       void* q_rot, void* k_cache, void* v_cache, float k_scale, float v_scale,
                                       void* out, void* stream) {
+  MLLM_REQUIRE(!s || s->num_tokens == 0 || k || v, MLLM_ERR_INVALID, std::string("mllm_attention_forward: null pointer"));
   mllm_layer_pool p = {};
   p.k_cache = k_cache, p.v_cache = v_cache, p.k_scale = k_scale, p.v_scale = v_scale;
   return mllm_attention_forward_pool(s, q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v, v_stride_tok,

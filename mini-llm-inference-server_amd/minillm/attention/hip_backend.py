@@ -271,15 +271,14 @@ def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
 
 def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, out: torch.Tensor) -> None:
     """ValueError unless q and out are [N, H, Dh] rows of the step's tokens over these 4-bit pools."""
-    _, bs, hkv, half = k_cache.shape
-    n, h, dh = q.shape
-    if dh != 2 * half or h % hkv or n != meta.query_start_loc[-1] or bs != meta.block_size:
-        raise ValueError(f"q must be [N, H, Dh] = [{meta.query_start_loc[-1]}, a multiple of {hkv}, {2 * half}], and the pool's "
-                         f"blocks {meta.block_size} tokens")
-    if out.shape != q.shape or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
+    pool = k_cache.shape
+    shape, tokens = q.shape, meta.query_start_loc[-1]
+    if len(shape) != 3 or shape[2] != 2 * pool[3] or shape[1] % pool[2] or shape[0] != tokens or pool[1] != meta.block_size:
+        raise ValueError(f"q must be [N, H, Dh] = [{tokens}, a multiple of {pool[2]}, {2 * pool[3]}], and the pool's blocks "
+                         f"{meta.block_size} tokens")
+    if out.shape != shape or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("out must be like q, both with unit stride in their last dimension")
-    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
-            or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if v_cache.shape != pool or v_cache.dtype != FP4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be alike and contiguous")
     if not q.device == out.device == k_cache.device == v_cache.device:
         raise ValueError("q, out and the pools must share one device")
@@ -572,6 +571,15 @@ class HipBackend(AttentionBackend):
         if k_cache.dtype == FP4:
             check_attend(q, k_cache, v_cache, meta, out)
             check_scales(k_cache, k_scale, v_scale)
+            if out.is_contiguous() and not self.overlap_mixed:  # one call for the step's launches
+                n, h, dh = q.shape
+                plan = self.plan(meta, h, k_cache.shape[2], dh, q.device, pool=_native.POOL_FP4)
+                step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache)
+                pool = _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                               v_scale.data_ptr(), 1.0, 1.0, 0, 0, 0.0)
+                self._lib.launch(q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), None,
+                                 0, 0, None, 0, 0, None, None, 0, None, pool, out.data_ptr())
+                return
         plan = self._plan_for(meta, q, k_cache)
         if plan.num_decode and plan.num_prefill and self.overlap_mixed and not torch.cuda.is_current_stream_capturing():
             # decode is enqueued first; the prefill's workgroups take CUs as the decode's free up

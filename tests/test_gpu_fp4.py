@@ -267,6 +267,18 @@ def test_output_rows_of_other_sequences_stay(hip):
     assert bool((wide == 3.0).all())
 
 
+def test_attend_in_one_call_and_launch_by_launch(hip):
+    # a contiguous output goes in one host call, a strided one and a mixed step on two streams launch by launch
+    *_, (backend, cache, meta, q) = step([(300, 1), (50, 20), (2000, 1), (0, 7)], 32, 8, torch.bfloat16, seed=9)
+    out, wide = torch.empty_like(q), torch.empty(q.shape[0], 40, 128, dtype=q.dtype, device=DEV)
+    two = torch.empty_like(q)
+    backend.attend(q, cache.k[0], cache.v[0], meta, out, **cache.scales(0))
+    backend.attend(q, cache.k[0], cache.v[0], meta, wide[:, 4:36], **cache.scales(0))
+    backend.overlap_mixed = True
+    backend.attend(q, cache.k[0], cache.v[0], meta, two, **cache.scales(0))
+    assert torch.equal(bits(out), bits(wide[:, 4:36].contiguous())) and torch.equal(bits(out), bits(two))
+
+
 def test_forward_equals_append_and_attend(hip):
     # the layer's one host call, without and with the rotation: the pool's bytes and the output of the separate calls
     from minillm.model.llama import apply_rotary

@@ -249,7 +249,17 @@ def test_layer_pool_checks():
     with pytest.raises(ValueError, match="fp8 pools only"):
         call(_native.LayerPool(k_scale=0.5, v_scale=1.0))
     call(_native.LayerPool(**ones))  # no tokens and no work
-    step.kv_fp8 = 3
+    # without k, v and cos the attention alone, here of no rows; a missing k or v, or none in the older call, is refused
+    step.num_tokens = 3
+    call(_native.LayerPool(**ones))
+    some, pool = 1 << 20, _native.LayerPool(**ones)
+    for k, v in ((some, None), (None, some)):
+        with pytest.raises(ValueError, match="null pointer"):
+            lib.check(fwd(at, some, 0, 0, k, 0, 0, v, 0, 0, None, None, 0, None, ctypes.addressof(pool), some, None))
+    step.kv_fp8 = 0
+    with pytest.raises(ValueError, match="null pointer"):
+        lib.call("mllm_attention_forward", at, some, 0, 0, None, 0, 0, None, 0, 0, None, None, 0, None, some, some, 1.0, 1.0, some, None)
+    step.kv_fp8, step.num_tokens = 3, 0
     with pytest.raises(ValueError, match="unknown pool"):
         call(_native.LayerPool(**ones))
 
