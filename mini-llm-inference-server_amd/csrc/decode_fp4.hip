@@ -202,14 +202,17 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
   const Fp4Lane at{(unsigned)c * st + 16u * g, (unsigned)((c * kBlocks4 + g) * a.Hkv), (unsigned)(4 * g) * st + 4u * NH * c,
                    (unsigned)((D * c / kFp4Block) * a.bs + 4 * g)};
 
-  auto load_q = [&](int qrow, int b) {  // by the first slice
+  u32x4 qv[4];  // the first slice's waves fetch a segment's q and put it into LDS
+  auto fetch_q = [&](int qrow) {
     if (slice) return;
     const char* qp = reinterpret_cast<const char*>(a.q + (int64_t)qrow * a.q_st + (int64_t)(kvh * a.G + (qvalid ? c : 0)) * a.q_sh);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const u32x4 v = ld16(qp + 2 * (32 * g + 8 * kk));
-      qs[b][grp][kk][lane] = qvalid ? v : u32x4{0, 0, 0, 0};
-    }
+    for (int kk = 0; kk < 4; ++kk) qv[kk] = ld16(qp + 2 * (32 * g + 8 * kk));
+  };
+  auto put_q = [&](int b) {
+    if (slice) return;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qs[b][grp][kk][lane] = qvalid ? qv[kk] : u32x4{0, 0, 0, 0};
   };
   // tiles of a segment: pages past the row's last token (a block table may hold pages ahead) have none
   auto tiles_of = [&](const int4& r0) { return max(min(r0.w, (r0.z + r0.y) * a.bs) - r0.z * a.bs + 15, 0) >> 4; };
@@ -235,20 +238,24 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
     csub = t - page * tpp;
     cblk = indices[cr.x + page];
   };
-  auto issue = [&](Fp4Tile<NH>& into) {
+  auto load = [&](Fp4Tile<NH>& into) {
     const int blk = (unsigned)cblk < (unsigned)a.num_blocks ? cblk : 0;  // else-branch never taken with valid metadata
     load_tile4<NH>(a, kvh, at, blk, csub, into);
+  };
+  auto advance = [&]() {
     ct += SL;
     settle();
   };
 
   int gi = bw.x, buf = 0;
-  SegRec cur = seg_rec(segs, gi);
-  SegRec nxt = seg_rec(segs, min(gi + 1, glast));
+  SegRec cur = seg_rec(segs, gi), nxt = cur;
   Fp4Tile<NH> tile, ahead;
   settle();
-  issue(tile);
-  load_q(cur.r1.x, 0);
+  load(tile);
+  fetch_q(cur.r1.x);
+  if (gi < glast) nxt = seg_rec(segs, gi + 1);
+  advance();
+  put_q(0);
   __syncthreads();
 
   while (true) {
@@ -256,8 +263,9 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
     const bool has_next = gi < glast;
     const int tok0 = cur.r0.z * a.bs, len = cur.r0.w;
     const int ntiles = tiles_of(cur.r0);
-    const SegRec after = seg_rec(segs, min(gi + 2, glast));
-    if (has_next) load_q(nxt.r1.x, buf ^ 1);
+    SegRec after = nxt;
+    if (gi + 2 <= glast) after = seg_rec(segs, gi + 2);
+    if (has_next) fetch_q(nxt.r1.x);
     float m_run = -INFINITY, l_run = 0.f;
     f32x4 o[D];
 #pragma unroll
@@ -269,12 +277,15 @@ __global__ __launch_bounds__(64 * kWavesFp4) __attribute__((amdgpu_waves_per_eu(
       };
       int t = slice;
       for (; t < ntiles && more; t += SL) {
-        issue(ahead);
+        load(ahead);
+        advance();
         consume(t);
         tile = ahead;
       }
       if (t < ntiles) consume(t);  // the bin's last: a load behind it would only be waited for (0.4 us of a small step's 11)
     }
+
+    if (has_next) put_q(buf ^ 1);
 
     // lane (c, g): o[m][i] is dim D (4 g + i) + m of the joint row; kept where that is the column's own head
     if (qvalid && has_heads && g * NH / 4 == myhead) {
