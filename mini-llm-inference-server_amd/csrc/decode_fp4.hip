@@ -14,10 +14,11 @@
 // in two parts, 22 bits together.
 //
 // Bound by memory and the vector pipes together.  Measured on 256 rows of 128-4,096 tokens (32 heads on 8, 630 MB), the
-// pass with its merge, us: 115 at 5.5 TB/s; the same loads without arithmetic 108; the arithmetic without loads 90.  With
+// pass with its merge, us: 114 at 5.5 TB/s; the same loads without arithmetic 108; the arithmetic without loads 90.  With
 // four heads a wavefront the accumulators spill: 130; one wavefront a bin and head pair instead of workgroups that share
 // a bin: 155; 32-token tiles with one set of registers: 140; two tiles ahead 116; three wavefronts a SIMD 119; P in two parts
-// for bf16 too 119.
+// for bf16 too 118, as one product of depth 32 over V taken twice 117.  A small step is a chain of dependent reads (plan,
+// block ids, tile, partials): four rows of 100-700 tokens 10.8 us from a graph, in bins of 2 pages; of 4 pages 12.1, of 8 13.6.
 #include <math.h>
 
 #include <type_traits>

@@ -9,7 +9,7 @@
 // One thread moves eight dims: 16 bytes of a 16-bit row, four bytes of codes.  A block's largest magnitude is the
 // maximum over its four threads of the 16-bit patterns without their sign, which order as the magnitudes do and put
 // infinities and NaN on top.  Bound by the launch up to some hundred tokens (8 tokens: 2.8 us),
-// by memory above: 8191 tokens of 8 heads of 128 dims, 42 MB, appended in 10.4 us, read back in 10.3 (4.1 TB/s).
+// by memory above: 8191 tokens of 8 heads of 128 dims, 42 MB, appended in 10.1 us, read back in 10.1 (4.2 TB/s).
 #include "kv_common.h"
 
 namespace mllm {
