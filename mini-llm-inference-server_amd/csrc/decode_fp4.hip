@@ -17,7 +17,7 @@
 // pass with its merge, us: 114 at 5.5 TB/s; the same loads without arithmetic 108; the arithmetic without loads 90.  With
 // four heads a wavefront the accumulators spill: 130; one wavefront a bin and head pair instead of workgroups that share
 // a bin: 155; 32-token tiles with one set of registers: 140; two tiles ahead 116; three wavefronts a SIMD 119; P in two parts
-// for bf16 too 118, as one product of depth 32 over V taken twice 117.  A small step is a chain of dependent reads (plan,
+// for bf16 too 3 - 4% more, also as one product of depth 32 over V taken twice.  A small step is a chain of dependent reads (plan,
 // block ids, tile, partials): four rows of 100-700 tokens 10.8 us from a graph, in bins of 2 pages; of 4 pages 12.1, of 8 13.6.
 #include <math.h>
 

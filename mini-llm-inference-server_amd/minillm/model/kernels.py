@@ -97,10 +97,10 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dty
     return cos, sin
 
 
-def head_norms_ok(q_norm, k_norm, x: torch.Tensor, head_dim: int) -> bool:
-    """Whether the head norms of q and k may run with the rotation: two norms of one class and eps that do nothing but their
-    forward, plain weights of x's type."""
-    return (bare(q_norm, type(k_norm)) and bare(k_norm, type(q_norm)) and q_norm.eps == k_norm.eps
+def head_norms_ok(q_norm, k_norm, cls: type, x: torch.Tensor, head_dim: int) -> bool:
+    """Whether the head norms of q and k may run with the rotation: two norms of `cls` (the model's RMSNorm) and one eps that do
+    nothing but their forward, plain weights of x's type."""
+    return (bare(q_norm, cls) and bare(k_norm, cls) and q_norm.eps == k_norm.eps
             and all(m.weight.shape == (head_dim,) and _plain_weight(m.weight, x) for m in (q_norm, k_norm)))
 
 
@@ -270,7 +270,7 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
         return None
     qk_norm = None
     if getattr(attn, "q_norm", None) is not None:  # heads normed in the launch that rotates
-        if not head_norms_ok(attn.q_norm, attn.k_norm, x, dh):
+        if not head_norms_ok(attn.q_norm, attn.k_norm, type(norm2), x, dh):
             return None
         qk_norm = (attn.q_norm.weight, attn.k_norm.weight, attn.q_norm.eps)
     lib, mlp = _native.lib(), layer.mlp

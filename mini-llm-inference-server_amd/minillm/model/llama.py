@@ -104,7 +104,7 @@ class LlamaAttention(nn.Module):
         ragged = getattr(kv_cache, "ragged", False)
         fused_norms = {}
         if getattr(self, "q_norm", None) is not None:
-            if kernels.usable(q) and kernels.head_norms_ok(self.q_norm, self.k_norm, q, dh):
+            if kernels.usable(q) and kernels.head_norms_ok(self.q_norm, self.k_norm, RMSNorm, q, dh):
                 norms = (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps)
                 if ragged and getattr(self.backend, "fuse_rotary", False) and b == 1:
                     fused_norms = {"qk_norm": norms}  # in the backend's launch that rotates and appends

@@ -321,3 +321,38 @@ def test_two_steps_on_two_streams(hip):
     torch.cuda.synchronize()
     for (*_, want), outs in zip(jobs, got):
         assert all(torch.equal(bits(o), bits(want)) for o in outs)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_other_norms_are_called_as_they_are(hip, monkeypatch, paged):
+    # norms of another class, and hooked ones, keep their own forward; so does the whole layer around them
+    from minillm.attention import get_backend
+    from minillm.attention.metadata import AttentionMetadata, SeqStep
+    from minillm.cache.paged import PagedKVCache, PagedStep
+    from minillm.model import kernels
+
+    def layer_norms(attn):
+        for name in ("q_norm", "k_norm"):
+            setattr(attn, name, torch.nn.LayerNorm(128, eps=1e-5, bias=False).to(DEV, torch.bfloat16))
+
+    def hooked(attn):
+        attn.k_norm.register_forward_hook(lambda m, args, out: 2 * out)
+
+    n = 9
+    x = torch.randn(1, n, 512, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    for change in (layer_norms, hooked):
+        model = make_model(seed=8, layers=1)
+        model.set_backend(get_backend("hip"))
+        layer = model.model.layers[0]
+        change(layer.self_attn)
+        cos, sin = model.model.rotary_emb(torch.arange(n, device=DEV)[None], torch.bfloat16)
+        results = []
+        for fused in (True, False):
+            with monkeypatch.context() as m:
+                if not fused:
+                    m.setattr(kernels, "head_norms_ok", lambda *args: False)
+                cache = PagedKVCache(model.config, 2, DEV, FP4)
+                step = PagedStep(cache, AttentionMetadata.build([SeqStep(0, n, [1])], 16, DEV)) if paged else None
+                with torch.no_grad():
+                    results.append(layer(x, cos, sin, step))
+        assert torch.equal(bits(results[0]), bits(results[1])), change.__name__
