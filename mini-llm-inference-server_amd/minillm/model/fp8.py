@@ -153,11 +153,14 @@ class Fp8Linear(nn.Module):
 def quantize_(model: nn.Module) -> nn.Module:
     """Replaces the projections of every decoder layer of `model` (LlamaForCausalLM) by layers of 8-bit blocks, in place.  The
     embedding and lm_head keep their weights."""
-    for layer in model.model.layers:
-        for owner, names in ((layer.self_attn, ("q_proj", "k_proj", "v_proj", "o_proj")),
-                             (layer.mlp, ("gate_proj", "up_proj", "down_proj"))):
-            for name in names:
-                linear = getattr(owner, name)
-                if isinstance(linear, nn.Linear):
-                    setattr(owner, name, Fp8Linear.from_linear(linear))
+    places = [(owner, name) for layer in model.model.layers
+              for owner, names in ((layer.self_attn, ("q_proj", "k_proj", "v_proj", "o_proj")),
+                                   (layer.mlp, ("gate_proj", "up_proj", "down_proj")))
+              for name in names if isinstance(getattr(owner, name), nn.Linear)]
+    for owner, name in places:  # all or none
+        linear = getattr(owner, name)
+        if linear.bias is not None or linear.in_features % 16 or linear.out_features % 16:
+            raise ValueError(f"{name} must have no bias and sizes that are multiples of 16, not {linear}")
+    for owner, name in places:
+        setattr(owner, name, Fp8Linear.from_linear(getattr(owner, name)))
     return model

@@ -157,6 +157,21 @@ def test_quantize_model():
         assert torch.isfinite(model(torch.arange(20)[None])).all()
 
 
+def test_quantize_changes_all_or_nothing():
+    from minillm.model.config import LlamaConfig
+    from minillm.model.llama import LlamaForCausalLM
+
+    class NoBackend:
+        pass
+
+    cfg = LlamaConfig(vocab_size=32, hidden_size=64, intermediate_size=72, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=16, rms_norm_eps=1e-5, rope_theta=1e4)
+    model = LlamaForCausalLM(cfg, NoBackend())
+    with pytest.raises(ValueError, match="gate_proj must have"):
+        quantize_(model)
+    assert not any(isinstance(m, Fp8Linear) for m in model.modules())
+
+
 def test_casts_leave_codes_and_scales_alone():
     layer = Fp8Linear.from_linear(torch.nn.Linear(272, 48, bias=False))
     codes, scales = layer.weight.view(torch.uint8).clone(), layer.weight_scale.view(torch.uint8).clone()
