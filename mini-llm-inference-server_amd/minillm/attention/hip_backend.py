@@ -287,9 +287,10 @@ def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 def check_norms(qk_norm, q: torch.Tensor) -> None:
     """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's."""
     wq, wk, eps = qk_norm
+    shape, dtype, device = q.shape[-1:], q.dtype, q.device
     for w in (wq, wk):
-        if w.shape != (q.shape[-1],) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous():
-            raise ValueError(f"the head norms' weights must be contiguous [Dh] = [{q.shape[-1]}] in q's type, on its device")
+        if w.shape != shape or w.dtype != dtype or w.device != device or not w.is_contiguous():
+            raise ValueError(f"the head norms' weights must be contiguous [Dh] = [{shape[0]}] in q's type, on its device")
     if not 0 <= eps < math.inf:
         raise ValueError("the head norms' eps must be finite and not negative")
 
@@ -491,24 +492,27 @@ class HipBackend(AttentionBackend):
         num_blocks, bs, hkv, _ = k_cache.shape
         if cos.shape != (n, dh) or sin.shape != (n, dh):
             raise ValueError(f"cos and sin must be [N, Dh] = [{n}, {dh}]")
-        if cos.dtype != q.dtype or sin.dtype != q.dtype:
+        dtype = q.dtype
+        if cos.dtype != dtype or sin.dtype != dtype:
             raise ValueError("q, cos and sin must share one dtype")
-        if cos.stride(-1) != 1 or sin.stride() != cos.stride():
-            cos, sin = cos.contiguous(), sin.contiguous()
+        sc = cos.stride()
+        if sc[1] != 1 or sin.stride() != sc:
+            cos, sin, sc = cos.contiguous(), sin.contiguous(), (dh, 1)
         wq, wk, eps = None, None, 0.0
         if qk_norm is not None:
             check_norms(qk_norm, q)
             wq, wk, eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
-        q_rot = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
+        q_rot = torch.empty_like(q, memory_format=torch.contiguous_format)
         pool = pool_type(k_cache)
         if pool == _native.POOL_FP4:
             scales = (k_scale.data_ptr(), v_scale.data_ptr(), 1.0, 1.0)
         else:
             scales = (0, 0, k_scale, v_scale)
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
         args = _native.pack_rope_append(  # the fields of mllm_rope_append in order
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], cos.data_ptr(),
-            sin.data_ptr(), cos.stride(0), q_rot.data_ptr(), h * dh, dh, k_cache.data_ptr(), v_cache.data_ptr(), *scales,
-            num_blocks, meta.slot_mapping.data_ptr(), n, bs, h, hkv, dh, _native.dtype_code(q.dtype), pool)
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], cos.data_ptr(), sin.data_ptr(),
+            sc[0], q_rot.data_ptr(), h * dh, dh, k_cache.data_ptr(), v_cache.data_ptr(), *scales, num_blocks,
+            meta.slot_mapping.data_ptr(), n, bs, h, hkv, dh, _native.dtype_code(dtype), pool)
         self._lib.launch(q.device, "mllm_qk_norm_rope_kv_append", args, wq, wk, eps)
         return q_rot
 

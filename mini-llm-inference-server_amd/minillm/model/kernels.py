@@ -121,23 +121,28 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     """RMSNorm of every head of q [B, H, T, Dh] and k [B, Hkv, T, Dh], then their rotation by cos and sin [B, T, Dh], in
     one launch: fp32 arithmetic, one rounding.  Dh a multiple of 16, at most 1024; bfloat16 or float16 throughout."""
     b, h, t, dh = q.shape
-    if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != (t, dh):
+    dtype, device, of_k, table = q.dtype, q.device, k.shape, (b, t, dh)
+    if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh:
         raise ValueError(f"k must be [B, Hkv, T, Dh] = [{b}, Hkv, {t}, {dh}] to match q")
-    if cos.shape != (b, t, dh) or sin.shape != (b, t, dh):
+    if cos.shape != table or sin.shape != table:
         raise ValueError(f"cos and sin must be [B, T, Dh] = [{b}, {t}, {dh}]")
-    if any(x.dtype != q.dtype or x.device != q.device for x in (k, cos, sin)):
+    if not (dtype == k.dtype == cos.dtype == sin.dtype and device == k.device == cos.device == sin.device):
         raise ValueError("q, k, cos and sin must share one dtype and device")
-    if q.dtype not in _DTYPES or q.device.type != "cuda":
+    if dtype not in _DTYPES or device.type != "cuda":
         raise ValueError("q must be bfloat16 or float16 on a GPU")
     check_norms((q_weight, k_weight, eps), q)
-    q, k, cos, sin = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, cos, sin))
-    if sin.stride() != cos.stride():
+    sq, sk, sc = q.stride(), k.stride(), cos.stride()
+    if sq[3] != 1 or sk[3] != 1:
+        q, k = q.contiguous(), k.contiguous()
+        sq, sk = q.stride(), k.stride()
+    if sc[2] != 1 or sin.stride() != sc:
         cos, sin = cos.contiguous(), sin.contiguous()
-    q_out = torch.empty((b, h, t, dh), dtype=q.dtype, device=q.device)
-    k_out = torch.empty((b, k.shape[1], t, dh), dtype=q.dtype, device=q.device)
-    _native.lib().launch(q.device, "mllm_qk_norm_rope", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
-                         cos.data_ptr(), sin.data_ptr(), *cos.stride()[:2], q_weight.data_ptr(), k_weight.data_ptr(), eps, b,
-                         t, h, k.shape[1], dh, _native.dtype_code(q.dtype), q_out.data_ptr(), k_out.data_ptr())
+        sc = cos.stride()
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    _native.lib().launch(device, "mllm_qk_norm_rope", q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+                         cos.data_ptr(), sin.data_ptr(), sc[0], sc[1], q_weight.data_ptr(), k_weight.data_ptr(), eps, b, t, h,
+                         of_k[1], dh, _native.dtype_code(dtype), q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
