@@ -284,10 +284,14 @@ def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         raise ValueError("q, out and the pools must share one device")
 
 
-def check_norms(qk_norm, q: torch.Tensor) -> None:
-    """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's."""
+def check_norms(qk_norm, q: torch.Tensor, *others: torch.Tensor) -> None:
+    """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's, and the `others` are of q's type on its
+    device."""
     wq, wk, eps = qk_norm
     shape, dtype, device = q.shape[-1:], q.dtype, q.device
+    for x in others:
+        if x.dtype != dtype or x.device != device:
+            raise ValueError("with head norms, q, k and v must share one dtype and device")
     for w in (wq, wk):
         if w.shape != shape or w.dtype != dtype or w.device != device or not w.is_contiguous():
             raise ValueError(f"the head norms' weights must be contiguous [Dh] = [{shape[0]}] in q's type, on its device")
@@ -401,12 +405,15 @@ class HipBackend(AttentionBackend):
 
     def _check(self, q, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0):
         n, h, dh = q.shape
-        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        of_pool, pool, dtype = k_cache.shape, k_cache.dtype, q.dtype
+        if len(of_pool) != 4 or of_pool != v_cache.shape:
             raise ValueError("k_cache and v_cache must both be [num_blocks, block_size, Hkv, Dh]")
-        _, bs, hkv, dh_c = k_cache.shape
-        if k_cache.dtype == FP4:
+        _, bs, hkv, dh_c = of_pool
+        fp4, fp8 = pool == FP4, pool == FP8
+        if fp4:
             dh_c *= 2
-        if k.shape != (n, hkv, dh) or v.shape != (n, hkv, dh) or dh_c != dh:
+        rows = (n, hkv, dh)
+        if k.shape != rows or v.shape != rows or dh_c != dh:
             raise ValueError(f"k/v must be [N, Hkv, Dh] = [{n}, {hkv}, {dh}] to match q and the pool")
         if bs != meta.block_size:
             raise ValueError(f"pool block size {bs} != metadata block size {meta.block_size}")
@@ -414,27 +421,27 @@ class HipBackend(AttentionBackend):
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
             raise ValueError("the KV pools must be contiguous")
-        if v_cache.dtype != k_cache.dtype:
+        if v_cache.dtype != pool:
             raise ValueError("k_cache and v_cache must share one dtype")
-        if is_fp8(k_cache) or k_cache.dtype == FP4:
-            if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-                raise ValueError(f"with {'an fp8' if is_fp8(k_cache) else 'a 4-bit'} pool, q, k and v must share one "
-                                 f"dtype, bfloat16 or float16")
-        if k_cache.dtype == FP4:
+        if (fp8 or fp4) and (dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype):
+            raise ValueError(f"with {'an fp8' if fp8 else 'a 4-bit'} pool, q, k and v must share one dtype, bfloat16 or "
+                             f"float16")
+        if fp4:
             if not q.device == k.device == v.device == k_cache.device == v_cache.device:
                 raise ValueError("q, k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
-        elif is_fp8(k_cache):
+        elif fp8:
             if not (0 < k_scale < math.inf and 0 < v_scale < math.inf):
                 raise ValueError("k_scale and v_scale must be positive and finite")
         else:
-            if q.dtype != k_cache.dtype:
+            if dtype != pool:
                 raise ValueError("q and the pools must share one dtype")
             if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_scale != 1.0 or v_scale != 1.0:
                 raise ValueError("k_scale / v_scale apply to fp8 pools only")
         if n != meta.query_start_loc[-1]:
             raise ValueError(f"q has {n} tokens, the metadata describes {meta.query_start_loc[-1]}")
-        return tuple(t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+        return (q if q.stride(2) == 1 else q.contiguous(), k if k.stride(2) == 1 else k.contiguous(),
+                v if v.stride(2) == 1 else v.contiguous())
 
     def forward_rotary(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0, qk_norm=None):
         """`forward` with the model's RoPE folded in: q and k arrive before the rotation (reference
@@ -444,7 +451,7 @@ class HipBackend(AttentionBackend):
         every head of q and k is normed before the rotation, in fp32 with one rounding after it."""
         q, k, v = self._check(q, k, v, k_cache, v_cache, meta, k_scale, v_scale)
         if qk_norm is not None:
-            check_norms(qk_norm, q)
+            check_norms(qk_norm, q, k, v)
         if self._split_launches(q, k_cache, meta):
             q_rot = self.rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm)
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -500,7 +507,7 @@ class HipBackend(AttentionBackend):
             cos, sin, sc = cos.contiguous(), sin.contiguous(), (dh, 1)
         wq, wk, eps = None, None, 0.0
         if qk_norm is not None:
-            check_norms(qk_norm, q)
+            check_norms(qk_norm, q, k, v)
             wq, wk, eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
         q_rot = torch.empty_like(q, memory_format=torch.contiguous_format)
         pool = pool_type(k_cache)

@@ -147,6 +147,10 @@ def test_backend_refusals():
     for bad in ((w[:64], w, 1e-5), (w, w.float(), 1e-5), (w, torch.ones(256, dtype=torch.bfloat16)[::2], 1e-5)):
         with pytest.raises(ValueError, match="weights must be contiguous"):
             be.rope_append(q, k, k, cos, cos, p16, p16.clone(), Meta, qk_norm=bad)
+    for bad_k, bad_v in ((k.float(), k), (k, k.half()), (k.to("meta"), k)):
+        for call in (be.rope_append, be.forward_rotary):
+            with pytest.raises(ValueError, match="with head norms, q, k and v"):
+                call(q, bad_k, bad_v, cos, cos, p16, p16.clone(), Meta, qk_norm=(w, w, 1e-5))
     for eps in (-1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="eps"):
             be.forward_rotary(q, k, k, cos, cos, p16, p16.clone(), Meta, qk_norm=(w, w, eps))
