@@ -215,10 +215,12 @@ __global__ __launch_bounds__(64 * kRowsWaves) void fp8_rows_kernel(const RowsArg
 
 // Up to 64 rows: a workgroup takes 128 weight rows, 16 a wavefront, and a part of K in chunks of kChunk blocks.  Its wavefronts
 // quantise the chunk of x together, a block of 16 rows each, into LDS in operand order while weights load: x is read and
-// quantised once per 128 weight rows.  Parts, one workgroup per CU, meet in fp32 (mllm_sum_partials).  Measured as above,
-// 14336 x 4096 / 4096 x 14336, 8 rows 16.9 / 17.8 us (3.5 / 3.3 TB/s with both launches), 32 rows 20.6 / -, 64 rows 25.6 /
-// 24.6.  Workgroups of 16 weight rows (fp8_rows_kernel's way) took 20.2 / 20.9 at 8 rows, 73 / 60 at 64; with x quantised
-// once by another launch 26.9 / 30.6 at 64.  Two workgroups per CU: 25.1 / 20.3 at 8 rows.
+// quantised once per 128 weight rows.  Parts, as many as leave no CU two workgroups, meet in fp32
+// (mllm_sum_partials).  Measured as above, 14336 x 4096 / 4096 x 14336, 8 rows 17.6 / 17.7 us (3.3 TB/s with both launches), 32
+// rows 20.6, 64 rows 25.3 / 24.6.  Workgroups of 16 weight rows (fp8_rows_kernel's way) took 20.2 / 20.9 at 8 rows, 73 / 60 at 64; with x quantised
+// once by another launch 26.9 / 30.6 at 64.  Two workgroups per CU: 22.1 / 18.4 at 8
+// rows, but 29.8 against 32.8 for 13312 x 8192; with some CUs taking two (20480 x 4096 in two parts) 27.4 against 24.7.  Halves
+// of K within a workgroup of 64 weight rows, which need no adding launch: no faster.
 template <typename T, int MT, bool HALF>
 __global__ __launch_bounds__(64 * kRowsWaves) void fp8_chunk_kernel(const RowsArgs a) {
   constexpr int kChunk = MT == 1 ? 8 : 4;
@@ -472,7 +474,7 @@ Plan plan_linear(int64_t m, int64_t n, int64_t blocks, int cus) {
   if (p.rows) return p;
   if (p.chunk) {
     // the parts do not depend on m, and those of small weights are the wavefronts' of fp8_rows_kernel: neither does a row's result
-    const int64_t tiles = (n + kBlock - 1) / kBlock, ks = (cus + tiles / 2) / tiles;
+    const int64_t tiles = (n + kBlock - 1) / kBlock, ks = cus / tiles;
     p.ksplit = n * blocks * kBlock <= kSmallWeights ? kRowsWaves : (int)(ks < 1 ? 1 : ks > blocks ? blocks : ks);
   } else {
     const int64_t large = ((n + 255) / 256) * ((m + 255) / 256), small = ((n + 127) / 128) * ((m + 127) / 128);

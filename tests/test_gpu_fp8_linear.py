@@ -68,7 +68,8 @@ def check(got, x, w):
 
 
 SHAPES = [(1, 128, 16), (1, 4096, 4096), (3, 16, 48), (8, 4096, 1024), (16, 144, 80), (17, 1040, 272), (33, 2048, 112),
-          (64, 14336, 4096), (64, 256, 14336), (8, 14336, 4096), (9, 2064, 9216), (32, 5008, 4112)]
+          (64, 14336, 4096), (64, 256, 14336), (8, 14336, 4096), (9, 2064, 9216), (32, 5008, 4112),
+          (8, 2064, 14336), (16, 4096, 14352), (30, 1168, 16400), (3, 1296, 13200)]
 MANY = [(65, 128, 16), (65, 4096, 4096), (100, 144, 272), (129, 2048, 96), (255, 1040, 128), (300, 512, 4096),
         (777, 4096, 1040), (2048, 272, 14336), (4100, 1024, 4112)]
 
@@ -109,7 +110,7 @@ def test_quantisation_is_the_definitions(hip, m):
         assert torch.equal(v[fine], want[fine])
 
 
-@pytest.mark.parametrize("n,k", [(1040, 4096), (8272, 2320), (4096, 4224), (16, 640), (33 * 1024, 1024)])
+@pytest.mark.parametrize("n,k", [(1040, 4096), (8272, 2320), (4096, 4224), (16, 640), (33 * 1024, 1024), (14352, 2320)])
 def test_rows_do_not_depend_on_their_batch(hip, n, k):
     lin, _ = layer(n, k)
     x = rows(64, k, torch.bfloat16).to(DEV)
