@@ -347,21 +347,24 @@ struct TileArgs {
 };
 
 // y tile of BN weight rows x BM rows of x per workgroup, WN x WM wavefronts of (BN / WN) x (BM / WM) each.  Codes go through
-// LDS by DMA, a block of K (128 bytes a row) per step, double buffered; 16-byte piece j of row r lies at j ^ (r % 8), so
-// that eight lanes of an operand read hit distinct banks.
+// LDS by DMA, a block of K (128 bytes a row) per step, STAGES - 1 steps ahead; 16-byte piece j of row r lies at j ^ (r % 8),
+// so that eight lanes of an operand read hit distinct banks.
 // Bound by the matrix instructions (4.4 PFLOP/s of them alone) and the DMA into LDS between them: a step of 256 x 256 takes
 // 1.65 us, 1.35 without its DMA, 1.38 without its products.  8192 x 14336 x 4096: 366 us, 2.6 PFLOP/s (the library's product of
 // fp8 matrices without blocks 2.7), and 59 us for quantising x, bound by memory (6 TB/s).  Measured slower there: reading a
 // step's operands before a barrier, with the DMA two steps ahead, 435 us; the two wavefronts of a SIMD reading and multiplying
 // in turn, 445; four wavefronts of 128 x 128.
-template <typename T, int BN, int BM, int WN, int WM, int OCC>
+// Tiles of 128 x 128, for products of fewer, go two workgroups to a CU with two stages each, or, where no CU gets two, with
+// four: 256 rows on 14336 x 4096 32.1 us against 40.8 (all launches, from a graph), 777 on 4096 x 4096 29.0 against 39.3,
+// 65 on 4096 x 14336 23.6 against 28.3.
+template <typename T, int BN, int BM, int WN, int WM, int OCC, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void fp8_tile_kernel(const TileArgs a) {
   constexpr int kWaves = WN * WM;
   constexpr int kA = BN * kBlock, kB = BM * kBlock, kStage = kA + kB + 4 * 64 * (BM / 256 ? BM / 256 : 1);
   constexpr int FN = BN / WN / 16, FM = BM / WM / 16;  // 16-row operands per wavefront
   constexpr int kRowsX = BM / WM;                      // rows of x per wavefront
   static_assert(kRowsX % 64 == 0, "a dword of scales per lane serves 64 rows of x");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % WN, wm = wave / WN;
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OC
   // scales of the tile's rows of x: BM bytes, 64 to a row group; groups past the last repeat it
   const unsigned offs = 64u * (unsigned)min(m0 / 64 + lane / 16, a.groups64 - 1) + 4u * (lane & 15);
   auto load = [&](int s) {
-    char* st = lds + (s & 1) * kStage;
+    char* st = lds + s % STAGES * kStage;
     const char* wb = wbase + (int64_t)s * kBlock;
     const char* xb = xbase + (int64_t)s * kBlock;
 #pragma unroll
@@ -413,11 +416,23 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OC
   const int nb0 = (n0 + wn * (BN / WN)) / kBlock;  // the wavefront's weights lie in one row of blocks (past N: repeated)
   const uint8_t* wsrow = a.ws + (int64_t)min(nb0, (a.N - 1) / kBlock) * a.blocks + first;
   const int rl = n & 7, c0 = 16 * (g ^ rl), c1 = 16 * ((4 + g) ^ rl);
-  load(0);
-  barrier_vm<0>();
+  // all loads but those of the last STAGES - 2 steps have landed, in every wavefront
+  auto landed = [&](bool more) {
+    constexpr int kLoad = kDmaA + kDmaB;
+    if (STAGES == 2 || !more)
+      barrier_vm<0>();
+    else if (wave == 0)
+      barrier_vm<(STAGES - 2) * (kLoad + 1)>();
+    else
+      barrier_vm<(STAGES - 2) * kLoad>();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < steps) load(s);
+  landed(steps >= STAGES - 1);
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) load(s + 1);
-    const char* st = lds + (s & 1) * kStage;
+    if (s + STAGES - 1 < steps) load(s + STAGES - 1);
+    const char* st = lds + s % STAGES * kStage;
     const char* pa = st + (wn * (BN / WN) + n) * kBlock;
     const char* pb = st + kA + (wm * kRowsX + n) * kBlock;
     int sx[kRowsX / 64];
@@ -438,7 +453,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(OC
         acc[i][j + 3] = mfma_fp8<3>(wv, xb[j + 3], acc[i][j + 3], sw, sx[j / 4]);
       }
     }
-    barrier_vm<0>();
+    landed(s + STAGES - 1 < steps);
   }
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
@@ -551,9 +566,11 @@ extern "C" int mllm_fp8_linear(const void* x, int64_t x_stride, int64_t m, int64
     fp8_quant_kernel<T><<<(unsigned)quant_groups, 256, 0, st>>>((const char*)x, 2 * x_stride, (unsigned)m, (int)k, blocks, base, sx,
                                                                (unsigned)a.groups64);
     if (p.large)
-      fp8_tile_kernel<T, 256, 256, 2, 4, 2><<<(unsigned)groups, 512, 0, st>>>(a);
+      fp8_tile_kernel<T, 256, 256, 2, 4, 2, 2><<<(unsigned)groups, 512, 0, st>>>(a);
+    else if (groups <= device_cus())
+      fp8_tile_kernel<T, 128, 128, 2, 2, 1, 4><<<(unsigned)groups, 256, 0, st>>>(a);
     else
-      fp8_tile_kernel<T, 128, 128, 2, 2, 2><<<(unsigned)groups, 256, 0, st>>>(a);
+      fp8_tile_kernel<T, 128, 128, 2, 2, 2, 2><<<(unsigned)groups, 256, 0, st>>>(a);
   };
   if (dtype == MLLM_DTYPE_BF16)
     launch(BF16{});
