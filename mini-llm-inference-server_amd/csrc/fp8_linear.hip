@@ -350,7 +350,8 @@ struct TileArgs {
 // LDS by DMA, a block of K (128 bytes a row) per step, STAGES - 1 steps ahead; 16-byte piece j of row r lies at j ^ (r % 8),
 // so that eight lanes of an operand read hit distinct banks.
 // Bound by the matrix instructions (4.4 PFLOP/s of them alone) and the DMA into LDS between them: a step of 256 x 256 takes
-// 1.65 us, 1.35 without its DMA, 1.38 without its products.  8192 x 14336 x 4096: 366 us, 2.6 PFLOP/s (the library's product of
+// 1.65 us, 1.35 without its DMA, 1.38 without its products; either tile takes 40 - 47 bytes/ns per CU into LDS, also when all
+// read the same one.  8192 x 14336 x 4096: 366 us, 2.6 PFLOP/s (the library's product of
 // fp8 matrices without blocks 2.7), and 59 us for quantising x, bound by memory (6 TB/s).  Measured slower there: reading a
 // step's operands before a barrier, with the DMA two steps ahead, 435 us; the two wavefronts of a SIMD reading and multiplying
 // in turn, 445; four wavefronts of 128 x 128.
