@@ -527,20 +527,24 @@ class HipBackend(AttentionBackend):
         """KV append (reference write_kv, paged_torch_ref.py:23-28): one launch for K and V."""
         num_blocks, bs, hkv, dh = k_cache.shape
         if k_cache.dtype == FP4:
-            if k.dim() != 3 or k.shape[1:] != (hkv, 2 * dh) or v.shape != k.shape or v.dtype != k.dtype:
+            rows, dtype = k.shape, k.dtype
+            if len(rows) != 3 or rows[1] != hkv or rows[2] != 2 * dh or v.shape != rows or v.dtype != dtype:
                 raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {2 * dh}] of one dtype")
-            if meta.slot_mapping.numel() != k.shape[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+            slots = meta.slot_mapping
+            if slots.numel() != rows[0] or v_cache.shape != k_cache.shape or v_cache.dtype != FP4 \
                     or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
                 raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
-            if not k.device == v.device == k_cache.device == v_cache.device:
+            device = k_cache.device
+            if not k.device == v.device == device == v_cache.device:
                 raise ValueError("k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
-            if k.stride(2) != 1 or v.stride(2) != 1:
+            sk, sv = k.stride(), v.stride()
+            if sk[2] != 1 or sv[2] != 1:
                 k, v = k.contiguous(), v.contiguous()
-            self._lib.launch(k_cache.device, "mllm_kv_append_fp4", k.data_ptr(), *k.stride()[:2], v.data_ptr(),
-                             *v.stride()[:2], _native.dtype_code(k.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
-                             k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh,
-                             meta.slot_mapping.data_ptr(), k.shape[0])
+                sk, sv = k.stride(), v.stride()
+            self._lib.launch(device, "mllm_kv_append_fp4", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
+                             _native.dtype_code(dtype), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                             v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh, slots.data_ptr(), rows[0])
             return
         if is_fp8(k_cache):
             self._lib.call("mllm_kv_append_fp8", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),

@@ -64,7 +64,8 @@ class PagedKVCache:
         [n, Hkv, Dh] of `dtype`: by default the pool's own, bfloat16 for fp8 and 4-bit pools.  A 4-bit pool is read with the
         16-bit type it was written with.  A slot outside the pool reads as zeros."""
         k, v = self.k[layer], self.v[layer]
-        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != k.device:
+        device = k.device
+        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
             raise ValueError("slots must be one row of int64 on the pool's device")
         dtype = dtype or (torch.bfloat16 if self.quantized or self.fp4 else k.dtype)
         if not self.fp4:
@@ -78,14 +79,13 @@ class PagedKVCache:
             return got[0], got[1]
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("a 4-bit pool is read as bfloat16 or float16")
-        if k.device.type != "cuda":
-            raise RuntimeError(f"reading a 4-bit pool needs a GPU device, got {k.device}")
+        if device.type != "cuda":
+            raise RuntimeError(f"reading a 4-bit pool needs a GPU device, got {device}")
         nb, bs, hkv, half = k.shape
         slots = slots.contiguous()
         n = slots.numel()
-        out = torch.empty((2, n, hkv, 2 * half), dtype=dtype, device=k.device)
-        to_k, to_v = out.unbind()
-        _native.lib().launch(k.device, "mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
+        to_k, to_v = torch.empty((2, n, hkv, 2 * half), dtype=dtype, device=device).unbind()
+        _native.lib().launch(device, "mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
                              self.v_scale[layer].data_ptr(), nb, bs, hkv, 2 * half, slots.data_ptr(), n,
                              _native.dtype_code(dtype), to_k.data_ptr(), to_v.data_ptr())
         return to_k, to_v

@@ -119,7 +119,8 @@ def qk_norm_rope_ok(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: to
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: torch.Tensor,
                  k_weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """RMSNorm of every head of q [B, H, T, Dh] and k [B, Hkv, T, Dh], then their rotation by cos and sin [B, T, Dh], in
-    one launch: fp32 arithmetic, one rounding.  Dh a multiple of 16, at most 1024; bfloat16 or float16 throughout."""
+    one launch: fp32 arithmetic, one rounding.  Dh a multiple of 16, at most 1024; bfloat16 or float16 throughout.  For
+    inference: operands that need a gradient are refused."""
     b, h, t, dh = q.shape
     dtype, device, of_k, table = q.dtype, q.device, k.shape, (b, t, dh)
     if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh:
@@ -130,6 +131,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         raise ValueError("q, k, cos and sin must share one dtype and device")
     if dtype not in _DTYPES or device.type != "cuda":
         raise ValueError("q must be bfloat16 or float16 on a GPU")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        raise RuntimeError("qk_norm_rope is for inference: it has no gradient (call it under no_grad, or the modules)")
     check_norms((q_weight, k_weight, eps), q)
     sq, sk, sc = q.stride(), k.stride(), cos.stride()
     if sq[3] != 1 or sk[3] != 1:

@@ -155,3 +155,18 @@ def test_forward_rotary_with_norms_is_append_and_attention(hip):
         want = torch.empty_like(got)
         be.attend(q_rot, *pools, meta, want, **scales)
         assert torch.equal(bits(got), bits(want))
+
+
+def test_operands_that_need_a_gradient_are_refused(hip):
+    from minillm.model import kernels
+
+    q, k, _, cos, sin, wq, wk = inputs(1, 3, 4, 2, 64, torch.bfloat16)
+    for i in range(4):
+        args = [q, k, wq, wk]
+        args[i] = args[i].detach().clone().requires_grad_()
+        a, b, c, d = args
+        with pytest.raises(RuntimeError, match="for inference"):
+            kernels.qk_norm_rope(a, b, cos, sin, c, d, EPS)
+        with torch.no_grad():
+            got = kernels.qk_norm_rope(a, b, cos, sin, c, d, EPS)
+        assert all(torch.equal(bits(x), bits(y)) for x, y in zip(got, kernels.qk_norm_rope(q, k, cos, sin, wq, wk, EPS)))
