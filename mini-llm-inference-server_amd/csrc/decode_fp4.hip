@@ -378,13 +378,15 @@ __global__ __launch_bounds__(256) void merge_fp4_kernel(const int4* __restrict__
         if (j0 + u * step >= n) ml[u].x = -INFINITY;
         mc = fmaxf(mc, ml[u].x);
       }
-      if (mc == -INFINITY) continue;  // segments without tiles
-      const float sc = fast_exp2(m - mc);
+      // Maxima of -inf: segments without tiles, of l and O zero, or with a NaN among each tile's keys, whose l and O are NaN
+      // and stay so under the weight 0 that either gets.
+      const float ref = mc == -INFINITY ? 0.f : mc;
+      const float sc = fast_exp2(m - ref);
       l *= sc;
       acc *= sc;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float w = fast_exp2(ml[u].x - mc);
+        const float w = fast_exp2(ml[u].x - ref);
         l += w * ml[u].y;
         acc += w * o[u];
       }

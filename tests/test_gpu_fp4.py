@@ -319,3 +319,33 @@ def test_forward_equals_append_and_attend(hip):
         fresh()
         q_rot = backend.rope_append(q, k, v, cos, sin, *pools[:2], meta, **cache.scales(0))
         assert torch.equal(bits(q_rot), bits(rot[0].contiguous())) and all(torch.equal(a, b) for a, b in zip(state(), after))
+
+
+# partials that hold a NaN in each of their tiles, of how many: the first four of a head's eight; one that is alone in its
+# group of the merge; every one of a group; the last; all
+NAN_PARTIALS = [(6, (0, 1, 2, 3)), (8, (0, 1, 2, 3)), (9, (3,)), (12, (5,)), (15, (7,)), (20, (2, 10, 18)), (21, (20,)), (3, (0, 1, 2))]
+
+
+@pytest.mark.parametrize("parts,bad", NAN_PARTIALS)
+@pytest.mark.parametrize("others", [0, 100], ids=["alone", "among100"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_segments_of_nan_keys_reach_the_merged_row(hip, monkeypatch, parts, bad, others, dtype):
+    # bins of two pages; with 100 other cut rows a workgroup of the merge serves eight heads
+    monkeypatch.setenv("MLLM_PAGES_PER_SPLIT", "2")
+    rows = [(32 * parts - 5, 1)] + [(60, 1)] * others
+    _, ref, bound, (backend, cache, meta, q) = step(rows, 32, 8, dtype, seed=parts)
+    merges = backend.plan(meta, 32, 8, 128, q.device, pool=2).merge_work.view(-1, 4).cpu()
+    assert merges[merges[:, 0] == 0][:, 2].tolist() == [parts] and int((merges[:, 0] >= 0).sum()) == 1 + others
+    pages = meta.block_tables[0].cpu().tolist()
+    scales = cache.k_scale[0].view(torch.uint8)
+    for p in bad:
+        scales[pages[2 * p], 3, 2, 5] = 255
+        scales[pages[2 * p + 1], 1, 0, 5] = 255
+    out = torch.empty_like(q)
+    backend.attend(q, cache.k[0], cache.v[0], meta, out, **cache.scales(0))
+    out = out.cpu()
+    assert torch.isnan(out[0, 20:24]).all()  # KV head 5
+    clean = [x for x in range(32) if not 20 <= x < 24]
+    check(out[:1, clean].double(), ref[:1, clean], bound[:1, clean])
+    if others:
+        check(out[1:].double(), ref[1:], bound[1:])
