@@ -213,7 +213,7 @@ class StepPlan:
     meta_ptrs: tuple = ()
     decode_args: tuple = ()
     # the mllm_layer_step of mllm_attention_forward, built on the plan's first layer call and rebuilt when
-    # the pools' shape, the dtypes or the workspace change
+    # the pools' shape, the head counts, the dtypes or the workspace change
     layer_key: tuple | None = None
     layer_step: object = None
     layer_addr: int = 0
@@ -327,7 +327,7 @@ class HipBackend(AttentionBackend):
         self._lib = _native.lib()
         self._attention_forward = self._lib.fn("mllm_attention_forward")
         self._planned = None  # the AttentionMetadata the plan was last built for
-        self._planned_pool = _native.POOL_16BIT  # and the pool type it was built for
+        self._planned_key = None  # and the pool type, head counts and head size it was built for
         self._plan: StepPlan | None = None
         self._workspace: torch.Tensor | None = None
         self._side: dict = {}  # device -> the stream mixed steps run their prefill launch on
@@ -385,11 +385,12 @@ class HipBackend(AttentionBackend):
         """Address of the plan's mllm_layer_step for these pools and this workspace."""
         ws = self._workspace
         pool = pool_type(k_cache)
-        key = (k_cache.shape[0], k_cache.shape[1], dtype, pool, ws.data_ptr() if ws is not None else 0)
+        hkv = k_cache.shape[2]
+        key = (k_cache.shape[0], k_cache.shape[1], num_heads, hkv, dh, dtype, pool, ws.data_ptr() if ws is not None else 0)
         if plan.layer_key == key:
             return plan.layer_addr
         ws = self._workspace_for(plan.workspace_bytes, k_cache.device)
-        num_blocks, bs, hkv, _ = k_cache.shape
+        num_blocks, bs = k_cache.shape[:2]
         step = _native.LayerStep(
             num_blocks=num_blocks, num_tokens=n, slot_mapping=meta.slot_mapping.data_ptr(),
             qo_indptr=plan.meta_ptrs[0], kv_indptr=plan.meta_ptrs[1], kv_indices=plan.meta_ptrs[2],
@@ -400,7 +401,7 @@ class HipBackend(AttentionBackend):
             num_kv_heads=hkv, head_dim=dh, block_size=bs, dtype=_native.dtype_code(dtype), kv_fp8=pool,
             softmax_scale=dh ** -0.5)
         plan.layer_step, plan.layer_addr = step, ctypes.addressof(step)
-        plan.layer_key = (num_blocks, bs, dtype, pool, ws.data_ptr() if ws is not None else 0)
+        plan.layer_key = (num_blocks, bs, num_heads, hkv, dh, dtype, pool, ws.data_ptr() if ws is not None else 0)
         return plan.layer_addr
 
     def _check(self, q, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0):
@@ -570,11 +571,11 @@ class HipBackend(AttentionBackend):
 
     def plan(self, meta, num_heads: int, num_kv_heads: int, head_dim: int, device, kv_fp8: bool = False,
              pool: int | None = None) -> StepPlan:
-        """The step's work plan, built on the GPU once per `meta` object (and pool type: `pool`, a MLLM_POOL_* code, or
-        `kv_fp8`) and reused after."""
+        """The step's work plan, built on the GPU once per `meta` object, pool type (`pool`, a MLLM_POOL_* code, or `kv_fp8`),
+        head counts and head size, and reused after."""
         if pool is None:
             pool = _native.POOL_FP8 if kv_fp8 else _native.POOL_16BIT
-        if self._planned is not meta or self._planned_pool != pool:
+        if self._planned is not meta or self._planned_key != (pool, num_heads, num_kv_heads, head_dim):
             self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), pool)
         return self._plan
 
@@ -702,7 +703,7 @@ class HipBackend(AttentionBackend):
                      meta.seq_lens_i32.data_ptr())
         self._plan = StepPlan(c, q_tile, n_dec, n_merge, n_pf, dec, mrg, pf, ws, meta_ptrs,
                               (*meta_ptrs, _ptr(dec), n_dec, _ptr(mrg), n_merge, c))
-        self._planned, self._planned_pool = meta, pool
+        self._planned, self._planned_key = meta, (pool, h, hkv, dh)
         if self.check_plan and n_dec and not torch.cuda.is_current_stream_capturing():
             check_plan_header(dec)
 

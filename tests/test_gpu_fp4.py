@@ -349,3 +349,22 @@ def test_segments_of_nan_keys_reach_the_merged_row(hip, monkeypatch, parts, bad,
     check(out[:1, clean].double(), ref[:1, clean], bound[:1, clean])
     if others:
         check(out[1:].double(), ref[1:], bound[1:])
+
+
+def test_layers_of_other_head_counts_share_a_steps_metadata(hip):
+    # each call of one backend is what a backend of its own gives
+    from minillm.attention.hip_backend import HipBackend
+
+    *_, (backend, first, meta, q0) = step([(300, 1), (40, 9), (2000, 1)], 32, 8, torch.bfloat16, seed=13)
+    g = torch.Generator().manual_seed(14)
+    for h, hkv in ((8, 8), (8, 2), (32, 8), (32, 2), (4, 4)):
+        cache = make_cache(hkv, first.num_blocks)
+        n = first.num_blocks * 16
+        k, v = (torch.randn(n, hkv, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+        append(cache, k, v, torch.arange(n, device=DEV))
+        q = torch.randn(q0.shape[0], h, 128, generator=g).to(torch.bfloat16).to(DEV)
+        rows = torch.full((q0.shape[0] + 1, h, 128), 3.0, dtype=q.dtype, device=DEV)  # the last row lies behind the step
+        want = torch.empty_like(q)
+        backend.attend(q, cache.k[0], cache.v[0], meta, rows[:-1], **cache.scales(0))
+        HipBackend().attend(q, cache.k[0], cache.v[0], meta, want, **cache.scales(0))
+        assert torch.equal(bits(rows[:-1]), bits(want)) and bool((rows[-1] == 3.0).all())

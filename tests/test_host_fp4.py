@@ -290,3 +290,53 @@ def test_config_names_head_norms():
     d = {k: v for k, v in LLAMA_3_1_8B.items()}
     assert LlamaConfig.from_dict(d).qk_norm is False
     assert LlamaConfig.from_dict({**d, "qk_norm": True}).qk_norm is True
+
+
+class Recorder:
+    """A library that launches nothing and keeps what `mllm_attention_forward_pool` was asked for."""
+
+    def __init__(self):
+        self.steps, self.plans = [], 0
+
+    def call(self, name, *args):
+        self.plans += name == "mllm_plan"
+
+    def launch(self, device, name, *args):
+        assert name == "mllm_attention_forward_pool"
+        step = _native.LayerStep.from_address(args[0])
+        self.steps.append({f: getattr(step, f) for f, _ in step._fields_})
+
+    def workspace_bytes(self, num_work, num_heads, head_dim):
+        return 4 * num_work * num_heads * head_dim
+
+
+def test_head_counts_are_each_calls_own(monkeypatch):
+    # one step's metadata with layers of other head counts: the plan and the step's arguments follow the call
+    from minillm.attention.metadata import AttentionMetadata
+
+    monkeypatch.setattr(_native, "stream_ptr", lambda device: 0)
+    be = hb.HipBackend()
+    be._lib, be.check_plan = Recorder(), False
+    meta = AttentionMetadata._arenas(16, [0, 1, 2, 22], [300, 40, 20], 22, 19, 24, "cpu")
+    layouts = [(32, 8), (8, 8), (8, 2), (32, 8), (2, 2)]
+    for h, hkv in layouts:
+        cache = PagedKVCache(config(num_attention_heads=h, num_key_value_heads=hkv), 24, "cpu", FP4)
+        q = torch.zeros(22, h, 128, dtype=torch.bfloat16)
+        for _ in range(2):  # the second call finds the first one's
+            be.attend(q, cache.k[0], cache.v[0], meta, torch.empty_like(q), **cache.scales(0))
+    assert be._lib.plans == len(layouts)
+    for i, (h, hkv) in enumerate(layouts):
+        a, b = be._lib.steps[2 * i:2 * i + 2]
+        assert a == b and (a["num_heads"], a["num_kv_heads"], a["head_dim"]) == (h, hkv, 128)
+        assert a["q_tile_tokens"] == hb.prefill_q_tile([1, 1, 20], h // hkv, hkv) and a["kv_fp8"] == 2
+        assert a["pages_per_split"] == hb.pages_per_split(22, hkv, h, kv_fp4=True)
+        assert a["workspace_bytes"] == 4 * a["num_decode_work"] * h * 128 > 0
+    # the other pools' layers
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        for h, hkv, dh in ((32, 8, 128), (8, 8, 128), (8, 2, 128), (8, 2, 64)):
+            pool = torch.zeros(24, 16, hkv, dh, dtype=torch.uint8 if dtype.itemsize == 1 else dtype).view(dtype)
+            for _ in range(2):
+                step = _native.LayerStep.from_address(be.layer_step(meta, 22, h, torch.bfloat16, pool))
+                assert (step.num_heads, step.num_kv_heads, step.head_dim) == (h, hkv, dh)
+                assert step.workspace_bytes == 4 * step.num_decode_work * h * dh
+    assert be._lib.plans == len(layouts) + 8
