@@ -13,6 +13,8 @@ elsewhere.  For inference: a call whose input needs a gradient is refused.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 import torch.nn.functional as F
 from torch import nn
@@ -34,6 +36,11 @@ def _scale_exponents(amax: torch.Tensor) -> torch.Tensor:
 
 def _powers(e: torch.Tensor) -> torch.Tensor:
     return torch.where(e == 255, float("nan"), (e.int() << 23).view(torch.float32))
+
+
+def _no_autocast(device_type: str):
+    """A context in which a product keeps its operands' type, whatever autocast is on (meta tensors have none)."""
+    return nullcontext() if device_type == "meta" else torch.autocast(device_type, enabled=False)
 
 
 def quantize_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -118,7 +125,8 @@ class Fp8Linear(nn.Module):
             _native.lib()  # raises: a GPU without the library is an error
         codes, e = quantize_rows(x.reshape(-1, self.in_features))
         rows = (codes.float().unflatten(1, (-1, BLOCK)) * _powers(e.view(torch.uint8))[..., None]).flatten(1)
-        y = rows[:, :self.in_features] @ self.dequantized().t()
+        with _no_autocast(x.device.type):
+            y = rows[:, :self.in_features] @ self.dequantized().t()
         return y.to(x.dtype).view(*x.shape[:-1], self.out_features)
 
     def _kernel(self, x: torch.Tensor) -> torch.Tensor | None:

@@ -185,3 +185,19 @@ def test_casts_leave_codes_and_scales_alone():
         assert torch.equal(layer(x), want)
     moved = layer.to("meta")
     assert moved.weight.device.type == "meta" and moved.weight.dtype == torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast_does_not_reach_the_product(dtype):
+    layer = Fp8Linear.from_linear(torch.nn.Linear(400, 48, bias=False))
+    x = torch.randn(5, 400)
+    x[2] *= 1e6  # past fp16's range
+    want = layer(x)
+    assert torch.isfinite(want).all()
+    compiled = torch.compile(layer, fullgraph=True, backend="eager")
+    with torch.no_grad(), torch.autocast("cpu", dtype):
+        for call in (layer, compiled):
+            got = call(x)
+            assert got.dtype == x.dtype and torch.equal(got, want)
+        assert torch.is_autocast_enabled("cpu") and torch.equal(layer(x[:2].to(dtype)), layer(x[:2].to(dtype).float()).to(dtype))
+    assert layer.to("meta")(x.to("meta")).shape == (5, 48)  # a device that has no autocast
