@@ -35,7 +35,9 @@ def _scale_exponents(amax: torch.Tensor) -> torch.Tensor:
 
 
 def _powers(e: torch.Tensor) -> torch.Tensor:
-    return torch.where(e == 255, float("nan"), (e.int() << 23).view(torch.float32))
+    """2^(e - 127) of e8m0 codes, 255 NaN; of code 0, below float32's normal numbers, bit 22 alone."""
+    bits = torch.where(e == 0, 1 << 22, e.int() << 23)
+    return torch.where(e == 255, float("nan"), bits.view(torch.float32))
 
 
 def _no_autocast(device_type: str):

@@ -220,3 +220,27 @@ def test_model_of_8bit_blocks(hip):
             assert torch.equal(bits(got), bits(mlp.down_proj(h)))
             ids = torch.randint(0, 320, (1, t), generator=torch.Generator().manual_seed(t)).to(DEV)
             assert torch.isfinite(model(ids)).all()
+
+
+def check32(got, x, w):
+    """The product in torch operations, float32: k additions, each off by at most 2^-24 of the sum of the magnitudes."""
+    v = quantised(x)
+    want = v @ w.t()
+    bound = x.shape[1] * 2.0 ** -24 * (v.abs() @ w.abs().t()) + 2.0 ** -24 * want.abs()
+    assert bool(((got.double().cpu() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("m", [3, 20, 100, 300])
+def test_the_least_scale(hip, m):
+    # scale code 0 is 2^-127 in each product form and in torch operations on the GPU
+    lin, w = layer(4112 if m == 300 else 272, 400, seed=m)
+    scales = lin.weight_scale.view(torch.uint8)
+    before = scales[0].clone()
+    scales[0] = 0
+    w[:128] *= two_to(-before.long().cpu()).repeat_interleave(128)[:400]  # 2^(before - 127) to 2^-127
+    x = (rows(m, 400, torch.float32, seed=m) * 2.0 ** 100).bfloat16()
+    with torch.no_grad():
+        got = lin(x.to(DEV))
+        assert bool((got[:, :128] != 0).any())
+        check(got, x, w)
+        check32(lin(x.float().to(DEV)), x, w)

@@ -201,3 +201,16 @@ def test_autocast_does_not_reach_the_product(dtype):
             assert got.dtype == x.dtype and torch.equal(got, want)
         assert torch.is_autocast_enabled("cpu") and torch.equal(layer(x[:2].to(dtype)), layer(x[:2].to(dtype).float()).to(dtype))
     assert layer.to("meta")(x.to("meta")).shape == (5, 48)  # a device that has no autocast
+
+
+def test_every_scale_code_is_its_power_of_two():
+    e = torch.arange(256, dtype=torch.uint8)
+    want = torch.where(e == 255, float("nan"), torch.exp2(e.double() - 127))
+    assert torch.equal(fp8._powers(e).double().nan_to_num(-1.0), want.nan_to_num(-1.0))
+    # weights quantised elsewhere under the least scale, and rows large enough for normal sums
+    codes = torch.arange(16 * 128, dtype=torch.int32).remainder(127).to(torch.uint8).view(16, 128).view(E4M3)
+    layer = Fp8Linear.from_parts(codes, torch.zeros(1, 1, dtype=torch.uint8).view(E8M0))
+    assert torch.equal(layer.dequantized().double(), codes.double() * 2.0 ** -127)
+    x = torch.full((2, 128), 2.0 ** 90)
+    y = layer(x)
+    assert bool((y > 0).all()) and torch.equal(y.double(), (x.double() @ (codes.double() * 2.0 ** -127).t()))
