@@ -244,3 +244,13 @@ def test_the_least_scale(hip, m):
         assert bool((got[:, :128] != 0).any())
         check(got, x, w)
         check32(lin(x.float().to(DEV)), x, w)
+
+
+def test_autocast_keeps_the_definition(hip):
+    lin, w = layer(272, 400, seed=5)
+    x = rows(20, 400, torch.float32, seed=6)
+    for dtype in (torch.bfloat16, torch.float16):
+        with torch.no_grad(), torch.autocast("cuda", dtype):
+            got = lin(x.to(DEV))
+        assert got.dtype == x.dtype
+        check32(got, x, w)
