@@ -104,9 +104,11 @@ class Fp8Linear(nn.Module):
             return cls.from_parts(*quantize_blocks(linear.weight.detach()))
 
     def _apply(self, fn, recurse=True):
-        """Moves go through, casts of floating types leave codes and scales alone."""
+        """Moves go through, casts leave codes and scales alone (Module.type casts bytes too: of that the device is kept)."""
         for name, dtype in (("weight", E4M3), ("weight_scale", E8M0)):
-            self._buffers[name] = fn(self._buffers[name].view(torch.uint8)).view(dtype)
+            held = self._buffers[name].view(torch.uint8)
+            got = fn(held)
+            self._buffers[name] = (got if got.dtype == torch.uint8 else held.to(got.device)).view(dtype)
         return self
 
     def dequantized(self) -> torch.Tensor:

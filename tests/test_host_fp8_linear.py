@@ -214,3 +214,12 @@ def test_every_scale_code_is_its_power_of_two():
     x = torch.full((2, 128), 2.0 ** 90)
     y = layer(x)
     assert bool((y > 0).all()) and torch.equal(y.double(), (x.double() @ (codes.double() * 2.0 ** -127).t()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, torch.bfloat16, "torch.HalfTensor"])
+def test_type_leaves_codes_and_scales_alone(dtype):
+    layer = Fp8Linear.from_linear(torch.nn.Linear(272, 48, bias=False))
+    codes, scales = layer.weight.view(torch.uint8).clone(), layer.weight_scale.view(torch.uint8).clone()
+    torch.nn.Sequential(layer, torch.nn.Linear(48, 2)).type(dtype)
+    assert layer.weight.dtype == E4M3 and layer.weight_scale.dtype == E8M0
+    assert torch.equal(layer.weight.view(torch.uint8), codes) and torch.equal(layer.weight_scale.view(torch.uint8), scales)
