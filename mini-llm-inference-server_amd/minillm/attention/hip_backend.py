@@ -437,8 +437,9 @@ class HipBackend(AttentionBackend):
         else:
             if dtype != pool:
                 raise ValueError("q and the pools must share one dtype")
-            if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_scale != 1.0 or v_scale != 1.0:
-                raise ValueError("k_scale / v_scale apply to fp8 pools only")
+            for scale in (k_scale, v_scale):  # a number or a tensor of one; block scales are neither
+                if isinstance(scale, torch.Tensor) and (scale.numel() != 1 or scale.dtype == SCALES4) or scale != 1.0:
+                    raise ValueError("k_scale / v_scale apply to fp8 pools only")
         if n != meta.query_start_loc[-1]:
             raise ValueError(f"q has {n} tokens, the metadata describes {meta.query_start_loc[-1]}")
         return (q if q.stride(2) == 1 else q.contiguous(), k if k.stride(2) == 1 else k.contiguous(),

@@ -340,3 +340,15 @@ def test_head_counts_are_each_calls_own(monkeypatch):
                 assert (step.num_heads, step.num_kv_heads, step.head_dim) == (h, hkv, dh)
                 assert step.workspace_bytes == 4 * step.num_decode_work * h * dh
     assert be._lib.plans == len(layouts) + 8
+
+
+def test_a_16bit_pool_takes_a_scale_of_one_as_a_tensor():
+    be = hb.HipBackend()
+    p16 = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
+    q, k = torch.zeros(5, 4, 128, dtype=torch.bfloat16), torch.zeros(5, 2, 128, dtype=torch.bfloat16)
+    for one in (1.0, 1, torch.tensor(1.0), torch.ones(1, dtype=torch.float64)):
+        assert len(be._check(q, k, k, p16, p16.clone(), Meta, one, one)) == 3
+    for bad in (0.5, torch.tensor(0.5), torch.ones(2), torch.tensor([127], dtype=torch.uint8).view(E8M0)):
+        for scales in ((1.0, bad), (bad, 1.0)):
+            with pytest.raises(ValueError, match="fp8 pools only"):
+                be._check(q, k, k, p16, p16.clone(), Meta, *scales)
