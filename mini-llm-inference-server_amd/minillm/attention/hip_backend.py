@@ -299,6 +299,14 @@ def check_norms(qk_norm, q: torch.Tensor, *others: torch.Tensor) -> None:
         raise ValueError("the head norms' eps must be finite and not negative")
 
 
+def check_device(q: torch.Tensor, *others: torch.Tensor) -> None:
+    """ValueError unless the tables and pools of a call lie where q does."""
+    device = q.device
+    for x in others:
+        if x.device != device:
+            raise ValueError(f"q, cos, sin and the pools must share one device, not {device} and {x.device}")
+
+
 def layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm) -> bytes:
     """The mllm_layer_pool of a layer's checked pools, scales and head norms."""
     norms = (0, 0, 0.0) if qk_norm is None else (qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2])
@@ -464,6 +472,8 @@ class HipBackend(AttentionBackend):
             raise ValueError(f"cos and sin must be [N, Dh] = [{n}, {dh}]")
         if cos.dtype != q.dtype or sin.dtype != q.dtype:
             raise ValueError("q, cos, sin and the pools must share one dtype (or the pools be fp8)")
+        if qk_norm is not None or k_cache.dtype == FP4:
+            check_device(q, cos, sin, k_cache, v_cache)
         if cos.stride(-1) != 1 or sin.stride() != cos.stride():
             cos, sin = cos.contiguous(), sin.contiguous()
         q_rot = torch.empty((n, h, dh), dtype=q.dtype, device=q.device)
@@ -504,6 +514,7 @@ class HipBackend(AttentionBackend):
         dtype = q.dtype
         if cos.dtype != dtype or sin.dtype != dtype:
             raise ValueError("q, cos and sin must share one dtype")
+        check_device(q, cos, sin, k_cache, v_cache)
         sc = cos.stride()
         if sc[1] != 1 or sin.stride() != sc:
             cos, sin, sc = cos.contiguous(), sin.contiguous(), (dh, 1)

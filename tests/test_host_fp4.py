@@ -352,3 +352,21 @@ def test_a_16bit_pool_takes_a_scale_of_one_as_a_tensor():
         for scales in ((1.0, bad), (bad, 1.0)):
             with pytest.raises(ValueError, match="fp8 pools only"):
                 be._check(q, k, k, p16, p16.clone(), Meta, *scales)
+
+
+def test_tables_and_pools_of_another_device_are_refused():
+    be = hb.HipBackend()
+    w = torch.ones(128, dtype=torch.bfloat16)
+    q, k = torch.zeros(5, 4, 128, dtype=torch.bfloat16), torch.zeros(5, 2, 128, dtype=torch.bfloat16)
+    cos = torch.zeros(5, 128, dtype=torch.bfloat16)
+    cache, p16 = PagedKVCache(config(), 3, "cpu", FP4), torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
+    pools = {"norms": (p16, p16.clone(), dict(qk_norm=(w, w, 1e-5))), "fp4": (cache.k[0], cache.v[0], cache.scales(0)),
+             "both": (cache.k[0], cache.v[0], dict(qk_norm=(w, w, 1e-5), **cache.scales(0)))}
+    for kc, vc, kw in pools.values():
+        for call in (be.rope_append, be.forward_rotary):
+            for c, s in ((cos.to("meta"), cos), (cos, cos.to("meta"))):
+                with pytest.raises(ValueError, match="one device"):
+                    call(q, k, k, c, s, kc, vc, Meta, **kw)
+            for a, b in ((kc.to("meta"), vc), (kc, vc.to("meta"))):
+                with pytest.raises(ValueError, match="one device|pool's device"):
+                    call(q, k, k, cos, cos, a, b, Meta, **kw)
