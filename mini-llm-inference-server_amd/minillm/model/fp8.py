@@ -164,7 +164,8 @@ class Fp8Linear(nn.Module):
 @torch.no_grad()
 def quantize_(model: nn.Module) -> nn.Module:
     """Replaces the projections of every decoder layer of `model` (LlamaForCausalLM) by layers of 8-bit blocks, in place.  The
-    embedding and lm_head keep their weights."""
+    embedding and lm_head keep their weights.  A projection that does more than nn.Linear (a forward of its own, hooks) is
+    refused: the layer in its place would not do it."""
     places = [(owner, name) for layer in model.model.layers
               for owner, names in ((layer.self_attn, ("q_proj", "k_proj", "v_proj", "o_proj")),
                                    (layer.mlp, ("gate_proj", "up_proj", "down_proj")))
@@ -173,6 +174,10 @@ def quantize_(model: nn.Module) -> nn.Module:
         linear = getattr(owner, name)
         if linear.bias is not None or linear.in_features % 16 or linear.out_features % 16:
             raise ValueError(f"{name} must have no bias and sizes that are multiples of 16, not {linear}")
+        held = linear.__dict__
+        if type(linear).forward is not nn.Linear.forward or "forward" in held or any(
+                held[hooks] for hooks in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")):
+            raise ValueError(f"{name} must be a linear layer without a forward or hooks of its own, not {linear}")
     for owner, name in places:
         setattr(owner, name, Fp8Linear.from_linear(getattr(owner, name)))
     return model

@@ -223,3 +223,43 @@ def test_type_leaves_codes_and_scales_alone(dtype):
     torch.nn.Sequential(layer, torch.nn.Linear(48, 2)).type(dtype)
     assert layer.weight.dtype == E4M3 and layer.weight_scale.dtype == E8M0
     assert torch.equal(layer.weight.view(torch.uint8), codes) and torch.equal(layer.weight_scale.view(torch.uint8), scales)
+
+
+def test_quantize_refuses_projections_that_do_more():
+    from minillm.model.config import LlamaConfig
+    from minillm.model.llama import LlamaForCausalLM
+
+    class NoBackend:
+        pass
+
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Named(torch.nn.Linear):
+        pass
+
+    def model():
+        cfg = LlamaConfig(vocab_size=32, hidden_size=64, intermediate_size=80, num_hidden_layers=2, num_attention_heads=4,
+                          num_key_value_heads=2, head_dim=16, rms_norm_eps=1e-5, rope_theta=1e4)
+        return LlamaForCausalLM(cfg, NoBackend())
+
+    def own_forward(mlp):
+        mlp.up_proj.forward = lambda x: x
+
+    for change in (lambda mlp: setattr(mlp, "up_proj", Scaled(64, 80, bias=False)), own_forward,
+                   lambda mlp: mlp.up_proj.register_forward_hook(lambda m, a, y: 2 * y),
+                   lambda mlp: mlp.up_proj.register_forward_pre_hook(lambda m, a: a)):
+        m = model()
+        change(m.model.layers[1].mlp)
+        with pytest.raises(ValueError, match="up_proj must be a linear layer without"):
+            quantize_(m)
+        assert not any(isinstance(x, Fp8Linear) for x in m.modules())
+    m = model()  # a subclass that computes the same, and a weight that is computed
+    m.model.layers[1].mlp.up_proj = Named(64, 80, bias=False)
+    q_proj = m.model.layers[0].self_attn.q_proj
+    torch.nn.utils.parametrizations.weight_norm(q_proj)
+    want = quantize_blocks(q_proj.weight.detach())[0]
+    quantize_(m)
+    assert sum(isinstance(x, Fp8Linear) for x in m.modules()) == 14
+    assert torch.equal(m.model.layers[0].self_attn.q_proj.weight[:, :64].view(torch.uint8), want.view(torch.uint8))
