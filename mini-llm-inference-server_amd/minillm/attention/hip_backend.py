@@ -30,6 +30,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -588,7 +589,10 @@ class HipBackend(AttentionBackend):
         if pool is None:
             pool = _native.POOL_FP8 if kv_fp8 else _native.POOL_16BIT
         if self._planned is not meta or self._planned_key != (pool, num_heads, num_kv_heads, head_dim):
-            self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), pool)
+            device = torch.device(device)
+            away = device.type == "cuda" and device.index not in (None, torch.cuda.current_device())
+            with torch.cuda.device(device) if away else nullcontext():  # a launch needs its stream's device current
+                self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), pool)
         return self._plan
 
     def _plan_for(self, meta, q, k_cache) -> StepPlan:

@@ -370,3 +370,26 @@ def test_tables_and_pools_of_another_device_are_refused():
             for a, b in ((kc.to("meta"), vc), (kc, vc.to("meta"))):
                 with pytest.raises(ValueError, match="one device|pool's device"):
                     call(q, k, k, cos, cos, a, b, Meta, **kw)
+
+
+def test_a_plan_is_launched_with_its_device_current(monkeypatch):
+    # as the launches behind it are (NativeLib.launch); two devices that are only named
+    be, current, seen = hb.HipBackend(), [0], []
+
+    class On:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(_native, "stream_ptr", lambda device: 100 + device.index)
+    monkeypatch.setattr(be, "_make_plan", lambda meta, h, hkv, dh, device, stream, pool: seen.append((current[0], stream)))
+    be.plan(Meta, 32, 8, 128, torch.device("cuda:0"), pool=2)
+    be.plan(Meta, 32, 8, 128, torch.device("cuda:1"), pool=2)
+    assert seen == [(0, 100), (1, 101)] and current == [0]
