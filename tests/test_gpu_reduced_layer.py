@@ -356,3 +356,50 @@ def test_other_norms_are_called_as_they_are(hip, monkeypatch, paged):
                 with torch.no_grad():
                     results.append(layer(x, cos, sin, step))
         assert torch.equal(bits(results[0]), bits(results[1])), change.__name__
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t", [1, 40, 300])
+def test_contiguous_norms_and_rotation_against_the_modules(hip, monkeypatch, t, dtype):
+    # What the attention of a model without a cache is given, against the formula and against the layer's own norm modules and
+    # apply_rotary.  The fused launch rounds once: eps / 2 of the result, 2^-18 of the magnitudes it sums (test_gpu_qk_norm).  The
+    # modules round the normed row, its product with the weight, the two products with cos and sin and their sum: with M
+    # those magnitudes, at most 3 eps / 2 of M and eps / 2 of the result; 1% covers a rounding of a rounded value, and tiny
+    # eps each rounding below the type's normal numbers.
+    from test_gpu_qk_norm import formula
+
+    from minillm.model import kernels
+    from minillm.model.fp8 import quantize_
+    from minillm.model.llama import apply_rotary
+
+    model = quantize_(make_model(seed=8, layers=1, dtype=dtype))
+    attn = model.model.layers[0].self_attn
+    x = torch.randn(2, t, 512, generator=torch.Generator().manual_seed(t)) * torch.logspace(-3, 0, t)[:, None]  # eps counts
+    x = x.to(dtype).to(DEV)
+    cos, sin = model.model.rotary_emb(torch.arange(t, device=DEV).expand(2, t), dtype)
+    given, fused, prefill, rotate = [], [], attn.backend.prefill, kernels.qk_norm_rope
+    monkeypatch.setattr(attn.backend, "prefill", lambda *a, **kw: (given.append(a), prefill(*a, **kw))[1])
+    monkeypatch.setattr(kernels, "qk_norm_rope", lambda *a: (fused.append(1), rotate(*a))[1])
+    with torch.no_grad():
+        out = attn.attend(x, cos, sin)
+        q, k, v = (p(x).view(2, t, -1, 128).transpose(1, 2) for p in (attn.q_proj, attn.k_proj, attn.v_proj))
+        own = [apply_rotary(norm(y), cos, sin) for norm, y in ((attn.q_norm, q), (attn.k_norm, k))]
+    (got_q, got_k, got_v), = given
+    assert fused == [1] and torch.equal(bits(got_v.contiguous()), bits(v.contiguous()))
+    eps, tiny = torch.finfo(dtype).eps, torch.finfo(dtype).tiny
+    for got, y, norm, other in ((got_q, q, attn.q_norm, own[0]), (got_k, k, attn.k_norm, own[1])):
+        ref, mag = formula(y, norm.weight, cos, sin, 1e-5)
+        once = eps / 2 * ref.abs() + 2.0 ** -18 * mag + tiny * eps
+        assert bool(((got.double() - ref).abs() <= once).all())
+        modules = 1.01 * (1.5 * eps * mag + eps / 2 * ref.abs()) + 2.0 ** -18 * mag + 8 * tiny * eps
+        assert bool(((got.double() - other.double()).abs() <= once + modules).all())
+    # and its result, against attention of them in float64: P and the output rounded, scores in fp32
+    blocked = ~causal_allowed(t, t).to(DEV)
+    for b in range(2):
+        for head in range(4):
+            qq, kk, vv = got_q[b, head].double(), got_k[b, head // 2].double().contiguous(), v[b, head // 2].double().contiguous()
+            p = torch.softmax((qq @ kk.t().contiguous() / math.sqrt(128)).masked_fill(blocked, -math.inf), -1)
+            o, a = p @ vv, p @ vv.abs()
+            size = (qq.abs() @ kk.abs().t().contiguous() / math.sqrt(128)).masked_fill(blocked, 0).amax(-1, keepdim=True)
+            bound = eps / 2 * o.abs() + (eps / 2 + 2 * 140 * 2.0 ** -24 * size + 2.0 ** -20) * a + tiny * eps
+            assert bool(((out.view(2, t, 4, 128)[b, :, head].double() - o).abs() <= bound).all())
