@@ -28,7 +28,12 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 constexpr int kBlock = 128;    // K per scale, and rows of weights
 constexpr int kFewRows = 64;                    // rows of x up to which the weights are streamed,
 constexpr int kInPlaceRows = 16;                // .. and of them those fp8_rows_kernel takes,
-constexpr int64_t kSmallWeights = 1 << 24;      // with weights of up to this many bytes
+// with weights of up to this many bytes.  Measured with either kernel for every size (us from a graph at 1 / 8 / 16 rows,
+// fp8_rows_kernel against fp8_chunk_kernel): 4096 x 4096, 16 MiB, 6.9 / 7.5 / 8.8 against 8.1 / 9.1 / 9.6; 4096 x 6144 8.9 / 9.7 /
+// 11.6 against 10.0 / 10.9 / 11.5; 6144 x 4096 8.6 / 11.0 / 14.0 against 11.5 / 12.3 / 13.0; 5120 x 5120 9.9 / 13.1 / 16.8 against
+// 11.5 / 12.4 / 13.0; 14336 x 4096 15.3 / 20.0 / 25.0 against 17.2 / 17.7 / 18.6.  From 24 MiB up the
+// first falls behind at 8 or 16 rows; up to 16 MiB it is ahead at all of them.
+constexpr int64_t kSmallWeights = 1 << 24;
 
 __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
@@ -215,8 +220,9 @@ __global__ __launch_bounds__(64 * kRowsWaves) void fp8_rows_kernel(const RowsArg
 
 // Up to 64 rows: a workgroup takes 128 weight rows, 16 a wavefront, and a part of K in chunks of kChunk blocks.  Its wavefronts
 // quantise the chunk of x together, a block of 16 rows each, into LDS in operand order while weights load: x is read and
-// quantised once per 128 weight rows.  Parts, as many as leave no CU two workgroups, meet in fp32
-// (mllm_sum_partials).  Measured as above, 14336 x 4096 / 4096 x 14336, 8 rows 17.6 / 17.7 us (3.3 TB/s with both launches), 32
+// quantised once per 128 weight rows.  Parts meet in fp32 (mllm_sum_partials): as many as leave no CU two workgroups, but
+// of small weights always eight, the wavefronts' parts of fp8_rows_kernel, whose bits a row then keeps at any number of
+// rows (a K of fewer than eight blocks leaves some of them empty: sums of zero that are written and added all the same).  Measured as above, 14336 x 4096 / 4096 x 14336, 8 rows 17.6 / 17.7 us (3.3 TB/s with both launches), 32
 // rows 20.6, 64 rows 25.3 / 24.6.  Workgroups of 16 weight rows (fp8_rows_kernel's way) took 20.2 / 20.9 at 8 rows, 73 / 60 at 64; with x quantised
 // once by another launch 26.9 / 30.6 at 64.  Two workgroups per CU: 22.1 / 18.4 at 8
 // rows, but 29.8 against 32.8 for 13312 x 8192; with some CUs taking two (20480 x 4096 in two parts) 27.4 against 24.7.  Halves

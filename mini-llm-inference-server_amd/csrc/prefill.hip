@@ -36,9 +36,11 @@
 //
 // 4-bit pools (kv_fp4.hip) go the same way: a lane loads eight bytes, 16 codes, and the byte of their block's scale, which the
 // conversion to bf16/fp16 applies (exact).  Loads of a quarter of the bytes do not pay here, where the matrix pipes bound the
-// kernel: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 399 us, 391 from an fp8 pool, 370 by DMA
+// kernel: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 396 us, 391 from an fp8 pool, 370 by DMA
 // from a 16-bit one.  Without its loads in the loop the 4-bit kernel took 343, with loads but no widening 378: per-lane
 // addresses cost most of the difference (408 with the scale's address made per load, and its pair's products in two parts).
+// P is one 16-bit value in either type, as from the other pools: relative to float64 the output is off by 2.3e-3 in bf16 and
+// 2.9e-4 in fp16, where an output that is rounded alone is off by 1.7e-3 and 2.1e-4; a second part would double the P V products.
 #include <math.h>
 
 #include <type_traits>
