@@ -249,13 +249,12 @@ def is_fp8(pool: torch.Tensor) -> bool:
 FP4 = torch.float4_e2m1fn_x2  # two e2m1 codes to an element
 SCALES4 = torch.float8_e8m0fnu  # their block scales
 FP4_BLOCK = 32  # dims per scale
+_POOLS = {FP8: _native.POOL_FP8, FP4: _native.POOL_FP4}  # of the other types: POOL_16BIT
 
 
 def pool_type(pool: torch.Tensor) -> int:
     """The library's MLLM_POOL_* of a pool."""
-    if pool.dtype == FP4:
-        return _native.POOL_FP4
-    return _native.POOL_FP8 if pool.dtype == FP8 else _native.POOL_16BIT
+    return _POOLS.get(pool.dtype, _native.POOL_16BIT)
 
 
 def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
@@ -367,10 +366,13 @@ class HipBackend(AttentionBackend):
         RoPE of q and k fused into it and the rotated q written to q_rot), decode + merge, prefill, on the
         current stream.  The arguments are the checked ones of `forward` / `forward_rotary`; q_rot and out
         are contiguous [N, H, Dh]."""
-        plan = self._plan_for(meta, q, k_cache)
-        step = self._layer_step(plan, meta, q.shape[0], q.shape[1], q.shape[2], q.dtype, k_cache)
+        n, h, dh = q.shape
+        shape, dtype = k_cache.shape, k_cache.dtype
+        pool = _POOLS.get(dtype, _native.POOL_16BIT)
+        plan = self.plan(meta, h, shape[2], dh, q.device, pool=pool)
+        step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache, shape, pool)
         rot = cos is not None
-        if k_cache.dtype == FP4 or qk_norm is not None:
+        if dtype == FP4 or qk_norm is not None:
             self._lib.launch(
                 q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cos.data_ptr() if rot else None,
@@ -386,20 +388,20 @@ class HipBackend(AttentionBackend):
     def layer_step(self, meta, n: int, num_heads: int, dtype, k_cache) -> int:
         """Address of the step's mllm_layer_step for rows of `num_heads` query heads in `dtype` and these pools (the
         plan is built on the first call with `meta`)."""
-        dh = k_cache.shape[3] * (2 if k_cache.dtype == FP4 else 1)
-        plan = self.plan(meta, num_heads, k_cache.shape[2], dh, k_cache.device, pool=pool_type(k_cache))
-        return self._layer_step(plan, meta, n, num_heads, dh, dtype, k_cache)
+        pool, shape = pool_type(k_cache), k_cache.shape
+        dh = shape[3] * (2 if pool == _native.POOL_FP4 else 1)
+        plan = self.plan(meta, num_heads, shape[2], dh, k_cache.device, pool=pool)
+        return self._layer_step(plan, meta, n, num_heads, dh, dtype, k_cache, shape, pool)
 
-    def _layer_step(self, plan: StepPlan, meta, n: int, num_heads: int, dh: int, dtype, k_cache) -> int:
-        """Address of the plan's mllm_layer_step for these pools and this workspace."""
+    def _layer_step(self, plan: StepPlan, meta, n: int, num_heads: int, dh: int, dtype, k_cache, shape, pool: int) -> int:
+        """Address of the plan's mllm_layer_step for pools of this shape and type (k_cache's, which names the head count and
+        head size of the pool) and this workspace."""
         ws = self._workspace
-        pool = pool_type(k_cache)
-        hkv = k_cache.shape[2]
-        key = (k_cache.shape[0], k_cache.shape[1], num_heads, hkv, dh, dtype, pool, ws.data_ptr() if ws is not None else 0)
+        key = (shape, num_heads, dtype, pool, ws.data_ptr() if ws is not None else 0)
         if plan.layer_key == key:
             return plan.layer_addr
         ws = self._workspace_for(plan.workspace_bytes, k_cache.device)
-        num_blocks, bs = k_cache.shape[:2]
+        num_blocks, bs, hkv, _ = shape
         step = _native.LayerStep(
             num_blocks=num_blocks, num_tokens=n, slot_mapping=meta.slot_mapping.data_ptr(),
             qo_indptr=plan.meta_ptrs[0], kv_indptr=plan.meta_ptrs[1], kv_indices=plan.meta_ptrs[2],
@@ -410,7 +412,7 @@ class HipBackend(AttentionBackend):
             num_kv_heads=hkv, head_dim=dh, block_size=bs, dtype=_native.dtype_code(dtype), kv_fp8=pool,
             softmax_scale=dh ** -0.5)
         plan.layer_step, plan.layer_addr = step, ctypes.addressof(step)
-        plan.layer_key = (num_blocks, bs, num_heads, hkv, dh, dtype, pool, ws.data_ptr() if ws is not None else 0)
+        plan.layer_key = (shape, num_heads, dtype, pool, ws.data_ptr() if ws is not None else 0)
         return plan.layer_addr
 
     def _check(self, q, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0):
@@ -606,7 +608,7 @@ class HipBackend(AttentionBackend):
             if out.is_contiguous() and not self.overlap_mixed:  # one call for the step's launches
                 n, h, dh = q.shape
                 plan = self.plan(meta, h, k_cache.shape[2], dh, q.device, pool=_native.POOL_FP4)
-                step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache)
+                step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache, k_cache.shape, _native.POOL_FP4)
                 pool = _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                                                v_scale.data_ptr(), 1.0, 1.0, 0, 0, 0.0)
                 self._lib.launch(q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), None,
