@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define MLLM_ABI_VERSION 6
+#define MLLM_ABI_VERSION 7
 
 #define MLLM_OK 0
 #define MLLM_ERR_INVALID (-1)
@@ -38,10 +38,12 @@ extern "C" {
 #define MLLM_DTYPE_F16 1
 #define MLLM_DTYPE_BF16 2
 
-/* pool types: elements of `dtype`, fp8 e4m3fn with one scale per tensor, 4 bits with block scales */
+/* pool types: elements of `dtype`, fp8 e4m3fn with one scale per tensor, 4 bits with block scales, fp8 e4m3fn with a scale
+ * for each block of tokens (page) and head */
 #define MLLM_POOL_16BIT 0
 #define MLLM_POOL_FP8 1
 #define MLLM_POOL_FP4 2
+#define MLLM_POOL_FP8_BLOCKS 4
 
 /* ABI version of the loaded library (MLLM_ABI_VERSION at build time). */
 int mllm_abi_version(void);
@@ -467,6 +469,54 @@ int mllm_paged_prefill_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride
                            int32_t q_tile_tokens, float softmax_scale, int32_t dtype, void* out,
                            int64_t out_stride_tok, int64_t out_stride_head, void* stream);
 
+/*
+ * 8-bit KV pool with a scale for each block of tokens and head.  No counterpart in the reference, whose planned fp8 cache has
+ * one scale per tensor (docs/distributed_inference_plan.md:310): nothing to calibrate, nothing that saturates.
+ *   codes               [num_blocks, block_size, Hkv, 128] e4m3fn bytes
+ *   k_scales, v_scales  [num_blocks, Hkv] e8m0 bytes, 4-byte aligned, readable up to the next multiple of 4 bytes
+ *   value = e4m3fn(code) * 2^(scale - 127); scale 255: NaN
+ * A run is a step's consecutive tokens at consecutive slots of one page.  Its exponent is the least e for which the largest
+ * finite magnitude of its tokens (of a head's K or V) is at most 448 * 2^(e - 127), kept within the exponents whose values
+ * the 16-bit type holds (bf16: 10 .. 246, fp16: 112 .. 134; magnitudes above saturate).  A run at a page's first slot begins
+ * the page's block anew under e; a run behind earlier tokens of the page takes max(e, scale), and where that grows, the codes
+ * of the slots before the run are rounded again to it.  Roundings go to nearest with ties to even; an infinity or a NaN becomes
+ * the code of NaN.  A pool is written and read with one 16-bit type.  head_dim 128, block_size 16, 32 or 64.
+ */
+
+/* KV append into such a pool: rows and slots as mllm_kv_append_fp8.  A step's tokens of a page have to be one run, as
+ * mllm_build_metadata lays them out; several runs of a page, or tokens that share a slot, leave that page undefined. */
+int mllm_kv_append_fp8_blocks(const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                              int64_t v_stride_tok, int64_t v_stride_head, int32_t src_dtype, void* k_cache, void* v_cache,
+                              void* k_scales, void* v_scales, int64_t num_blocks, int32_t block_size,
+                              int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping, int64_t num_tokens,
+                              void* stream);
+
+/* Rows slots[num_slots] of such a pool as values of `dtype`: k_out, v_out [num_slots, Hkv, 128], contiguous.  A slot outside the
+ * pool reads as zeros. */
+int mllm_kv_read_fp8_blocks(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+                            int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                            const int64_t* slots, int64_t num_slots, int32_t dtype, void* k_out, void* v_out,
+                            void* stream);
+
+/* mllm_paged_decode over such a pool with the merge of its cut rows behind it.  Codes 16-byte aligned. */
+int mllm_paged_decode_fp8_blocks(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                 const void* v_cache, const void* k_scales, const void* v_scales, int64_t num_blocks,
+                                 int32_t block_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* decode_work,
+                                 int32_t num_decode_work, const int32_t* merge_work, int32_t num_merge_work,
+                                 int32_t pages_per_split, float softmax_scale, int32_t dtype, void* out,
+                                 int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/* mllm_paged_prefill over such a pool. */
+int mllm_paged_prefill_fp8_blocks(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                  const void* v_cache, const void* k_scales, const void* v_scales, int64_t num_blocks,
+                                  int32_t block_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                  const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                  const int32_t* seq_lens, const int32_t* prefill_work, int32_t num_prefill_work,
+                                  int32_t q_tile_tokens, float softmax_scale, int32_t dtype, void* out,
+                                  int64_t out_stride_tok, int64_t out_stride_head, void* stream);
+
 /* The arguments of mllm_qk_norm_rope_kv_append: those of mllm_rope_kv_append / _fp8, the pool's type and block scales. */
 typedef struct mllm_rope_append {
   const void *q, *k, *v;       /* [N, heads, Dh], element strides (tok, head), rows 16-byte aligned */
@@ -476,7 +526,7 @@ typedef struct mllm_rope_append {
   void* q_out;
   int64_t q_out_stride_tok, q_out_stride_head;
   void *k_cache, *v_cache;
-  void *k_scales, *v_scales;   /* MLLM_POOL_FP4 */
+  void *k_scales, *v_scales;   /* MLLM_POOL_FP4, MLLM_POOL_FP8_BLOCKS */
   float k_scale, v_scale;      /* MLLM_POOL_FP8 */
   int64_t num_blocks;
   const int64_t* slot_mapping; /* [N]; slots outside the pool are not written */
@@ -490,8 +540,8 @@ typedef struct mllm_rope_append {
  * RMSNorm of each query and key head (weights q_norm, k_norm [Dh]) with the model's RoPE and the append in one launch; no
  * counterpart in the reference, whose q and k are not normed:
  *   y = x * rsqrt(mean(x^2) + eps) * w,  q_out / pool row = y * cos + rotate_half(y) * sin,  v copied (or quantized)
- * in fp32 with one rounding to `dtype`; fp8 and 4-bit pools quantize the rounded k and v as their appends do.  Without norms
- * (both NULL, 4-bit pools only): mllm_rope_kv_append's rotation.  head_dim a multiple of 16 (4-bit pools: 64), at most 1024.
+ * in fp32 with one rounding to `dtype`; the other pools quantize the rounded k and v as their appends do.  Without norms
+ * (both NULL, pools with block scales only): mllm_rope_kv_append's rotation.  head_dim a multiple of 16 (4-bit pools: 64), at most 1024.
  */
 int mllm_qk_norm_rope_kv_append(const mllm_rope_append* args, const void* q_norm, const void* k_norm, float eps,
                                 void* stream);
@@ -506,7 +556,7 @@ int mllm_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, c
 /* A layer's pools and head norms, for the entry points below. */
 typedef struct mllm_layer_pool {
   void *k_cache, *v_cache;
-  void *k_scales, *v_scales;      /* 4-bit pools */
+  void *k_scales, *v_scales;      /* pools with block scales */
   float k_scale, v_scale;         /* fp8 pools; 1 otherwise */
   const void *q_norm, *k_norm;    /* head norm weights [Dh], or both NULL; they need cos and sin */
   float norm_eps;

@@ -27,6 +27,11 @@ int device_cus();
     if (!(cond)) return ::mllm::fail((code), (msg)); \
   } while (0)
 
+// Whether `pool` is a MLLM_POOL_* code.
+constexpr bool known_pool(int pool) {
+  return pool == MLLM_POOL_16BIT || pool == MLLM_POOL_FP8 || pool == MLLM_POOL_FP4 || pool == MLLM_POOL_FP8_BLOCKS;
+}
+
 // HIP takes fewer than 2^32 work-items along x: workgroups of 256 threads a launch may have.
 constexpr int64_t kMaxGroups256 = (1ll << 24) - 1;
 
@@ -88,24 +93,24 @@ __device__ __forceinline__ uint32_t f32_to_e4m3fn_bits(float f) {
   return sign | ((r - (120u << 23)) >> 20);            // exponent bias 127 -> 7
 }
 
-// Four e4m3fn values (bytes 0-3 of w) -> four bf16 / fp16 values, two per dword, in byte order.  Exact:
-// every e4m3fn value, subnormals and NaN included, is representable in both 16-bit formats.
+// Four e4m3fn values (bytes 0-3 of w) times a power of two -> four bf16 / fp16 values, two per dword, in byte order.  Exact
+// where the 16-bit format holds the products, as with scale 1: it holds every e4m3fn value, subnormals and NaN included.
 template <typename T>
-__device__ __forceinline__ u32x2 fp8x4_to(uint32_t w);
+__device__ __forceinline__ u32x2 fp8x4_to(uint32_t w, float scale = 1.f);
 template <>
-__device__ __forceinline__ u32x2 fp8x4_to<BF16>(uint32_t w) {
-  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))};
+__device__ __forceinline__ u32x2 fp8x4_to<BF16>(uint32_t w, float scale) {
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
 }
 template <>
-__device__ __forceinline__ u32x2 fp8x4_to<F16>(uint32_t w) {
-  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true))};
+__device__ __forceinline__ u32x2 fp8x4_to<F16>(uint32_t w, float scale) {
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))};
 }
 // Eight e4m3fn values (two dwords) -> eight 16-bit values (16 bytes).
 template <typename T>
-__device__ __forceinline__ u32x4 fp8x8_to(uint32_t w0, uint32_t w1) {
-  const u32x2 lo = fp8x4_to<T>(w0), hi = fp8x4_to<T>(w1);
+__device__ __forceinline__ u32x4 fp8x8_to(uint32_t w0, uint32_t w1, float scale = 1.f) {
+  const u32x2 lo = fp8x4_to<T>(w0, scale), hi = fp8x4_to<T>(w1, scale);
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 

@@ -7,6 +7,11 @@
 #include "common.h"
 
 namespace mllm {
+
+// mllm_qk_norm_rope_kv_append into an 8-bit pool with block scales (kv_fp8_blocks.hip): arguments that entry point has checked.
+int rope_append_fp8_blocks(const std::string& fn, const mllm_rope_append& r, const void* q_norm, const void* k_norm, float eps,
+                           void* stream);
+
 namespace {
 
 template <typename T>

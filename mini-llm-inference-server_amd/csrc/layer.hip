@@ -14,13 +14,13 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
   const std::string fn = "mllm_attention_forward";
   MLLM_REQUIRE(s, MLLM_ERR_INVALID, fn + ": null step");
   MLLM_REQUIRE(p, MLLM_ERR_INVALID, fn + ": null pool");
-  MLLM_REQUIRE(s->kv_fp8 >= MLLM_POOL_16BIT && s->kv_fp8 <= MLLM_POOL_FP4, MLLM_ERR_INVALID, fn + ": unknown pool type");
+  MLLM_REQUIRE(known_pool(s->kv_fp8), MLLM_ERR_INVALID, fn + ": unknown pool type");
   MLLM_REQUIRE(s->kv_fp8 == MLLM_POOL_FP8 || (p->k_scale == 1.f && p->v_scale == 1.f), MLLM_ERR_INVALID,
                fn + ": k_scale / v_scale apply to fp8 pools only");
   MLLM_REQUIRE(!cos == !sin && (!cos || q_rot), MLLM_ERR_INVALID, fn + ": cos, sin and q_rot go together");
   MLLM_REQUIRE(!p->q_norm == !p->k_norm && (!p->q_norm || cos), MLLM_ERR_INVALID,
                fn + ": q_norm and k_norm go together, with cos and sin");
-  const bool fp8 = s->kv_fp8 == MLLM_POOL_FP8, fp4 = s->kv_fp8 == MLLM_POOL_FP4;
+  const bool fp8 = s->kv_fp8 == MLLM_POOL_FP8, fp4 = s->kv_fp8 == MLLM_POOL_FP4, blocks8 = s->kv_fp8 == MLLM_POOL_FP8_BLOCKS;
   const int64_t slots = s->num_blocks * s->block_size;
   const int64_t row = (int64_t)s->num_heads * s->head_dim;  // q_rot and out: contiguous [N, H, Dh]
   int rc;
@@ -28,7 +28,7 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
   int64_t qa_st = q_stride_tok, qa_sh = q_stride_head;
   if (!k && !v && !cos) {
     rc = MLLM_OK;
-  } else if (cos && (fp4 || p->q_norm)) {
+  } else if (cos && (fp4 || blocks8 || p->q_norm)) {
     mllm_rope_append r = {};
     r.q = q, r.q_stride_tok = q_stride_tok, r.q_stride_head = q_stride_head;
     r.k = k, r.k_stride_tok = k_stride_tok, r.k_stride_head = k_stride_head;
@@ -50,10 +50,11 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
                                    v_stride_head, cos, sin, cs_stride_tok, s->num_heads, s->num_kv_heads, s->head_dim,
                                    s->dtype, q_rot, row, s->head_dim, p->k_cache, p->v_cache, slots, s->slot_mapping,
                                    s->num_tokens, stream);
-  } else if (fp4) {
-    rc = mllm_kv_append_fp4(k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head, s->dtype, p->k_cache,
-                            p->v_cache, p->k_scales, p->v_scales, s->num_blocks, s->block_size, s->num_kv_heads,
-                            s->head_dim, s->slot_mapping, s->num_tokens, stream);
+  } else if (fp4 || blocks8) {
+    const auto append = fp4 ? mllm_kv_append_fp4 : mllm_kv_append_fp8_blocks;
+    rc = append(k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head, s->dtype, p->k_cache, p->v_cache,
+                p->k_scales, p->v_scales, s->num_blocks, s->block_size, s->num_kv_heads, s->head_dim, s->slot_mapping,
+                s->num_tokens, stream);
   } else {
     rc = fp8 ? mllm_kv_append_fp8(k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head, s->dtype, p->k_cache,
                                   p->v_cache, slots, s->num_kv_heads, s->head_dim, s->slot_mapping, s->num_tokens,
@@ -69,11 +70,12 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
     qa_sh = s->head_dim;
   }
   if (s->num_decode_work > 0) {
-    if (fp4)
-      rc = mllm_paged_decode_fp4(qa, qa_st, qa_sh, p->k_cache, p->v_cache, p->k_scales, p->v_scales, s->num_blocks,
-                                 s->block_size, s->num_heads, s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indices,
-                                 s->decode_work, s->num_decode_work, s->merge_work, s->num_merge_work,
-                                 s->pages_per_split, s->softmax_scale, s->dtype, out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
+    if (fp4 || blocks8)
+      rc = (fp4 ? mllm_paged_decode_fp4 : mllm_paged_decode_fp8_blocks)(
+          qa, qa_st, qa_sh, p->k_cache, p->v_cache, p->k_scales, p->v_scales, s->num_blocks, s->block_size, s->num_heads,
+          s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indices, s->decode_work, s->num_decode_work, s->merge_work,
+          s->num_merge_work, s->pages_per_split, s->softmax_scale, s->dtype, out, row, s->head_dim, s->workspace,
+          s->workspace_bytes, stream);
     else if (fp8)
       rc = mllm_paged_decode_fp8(qa, qa_st, qa_sh, p->k_cache, p->v_cache, s->num_blocks, s->block_size, s->num_heads,
                                  s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indptr, s->kv_indices,
@@ -87,17 +89,17 @@ extern "C" int mllm_attention_forward_pool(const mllm_layer_step* s, const void*
                              s->pages_per_split, s->softmax_scale, s->dtype, out, row, s->head_dim, s->workspace,
                              s->workspace_bytes, stream);
     if (rc != MLLM_OK) return rc;
-    if (!fp4)  // the 4-bit decode merges by itself
+    if (!fp4 && !blocks8)  // whose decode calls merge by themselves
       rc = mllm_merge_splits(s->merge_work, s->num_merge_work, s->num_decode_work, s->num_heads, s->head_dim,
                              s->qo_indptr, s->dtype, out, row, s->head_dim, s->workspace, s->workspace_bytes, stream);
     if (rc != MLLM_OK) return rc;
   }
   if (s->num_prefill_work > 0) {
-    if (fp4)
-      rc = mllm_paged_prefill_fp4(qa, qa_st, qa_sh, p->k_cache, p->v_cache, p->k_scales, p->v_scales, s->num_blocks,
-                                  s->block_size, s->num_heads, s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indptr,
-                                  s->kv_indices, s->seq_lens, s->prefill_work, s->num_prefill_work, s->q_tile_tokens,
-                                  s->softmax_scale, s->dtype, out, row, s->head_dim, stream);
+    if (fp4 || blocks8)
+      rc = (fp4 ? mllm_paged_prefill_fp4 : mllm_paged_prefill_fp8_blocks)(
+          qa, qa_st, qa_sh, p->k_cache, p->v_cache, p->k_scales, p->v_scales, s->num_blocks, s->block_size, s->num_heads,
+          s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indptr, s->kv_indices, s->seq_lens, s->prefill_work,
+          s->num_prefill_work, s->q_tile_tokens, s->softmax_scale, s->dtype, out, row, s->head_dim, stream);
     else if (fp8)
       rc = mllm_paged_prefill_fp8(qa, qa_st, qa_sh, p->k_cache, p->v_cache, s->num_blocks, s->block_size,
                                   s->num_heads, s->num_kv_heads, s->head_dim, s->qo_indptr, s->kv_indptr,

@@ -69,7 +69,7 @@ struct PrefillArgs {
   const int4* work;  // the plan's prefill records, two int4 each (see the kernel)
   float scale_log2;  // softmax scale x k_scale x log2(e)
   float v_scale;     // output scale of an fp8 pool
-  const uint8_t *ks, *vs;  // block scales of a 4-bit pool (kv_fp4.hip)
+  const uint8_t *ks, *vs;  // block scales of a 4-bit pool (kv_fp4.hip) or of an 8-bit one (kv_fp8_blocks.hip)
   uint16_t* out;
   int64_t o_st, o_sh;
 };
@@ -116,9 +116,11 @@ __device__ __forceinline__ void dma_tile(const char* pool, const PrefillArgs& a,
   }
 }
 
+typedef const __attribute__((address_space(4))) uint32_t ConstU32;
+
 // What the pool holds, and with it the way of a tile into LDS: DMA, or through registers to be widened.
-enum Pool { kPool16 = 0, kPoolFp8 = 1, kPoolFp4 = 2 };
-constexpr int head_row_bytes(int pool) { return pool == kPool16 ? 2 * kHeadDim : (pool == kPoolFp8 ? kHeadDim : kHeadDim / 2); }
+enum Pool { kPool16 = 0, kPoolFp8 = 1, kPoolFp4 = 2, kPoolFp8Blocks = 3 };
+constexpr int head_row_bytes(int pool) { return pool == kPool16 ? 2 * kHeadDim : (pool == kPoolFp4 ? kHeadDim / 2 : kHeadDim); }
 
 // One lane's 16 values of a tile on their way through registers.
 template <int POOL>
@@ -130,6 +132,11 @@ struct Staged<kPoolFp4> {
   u32x2 x;
   uint32_t e;  // their block's scale
 };
+template <>
+struct Staged<kPoolFp8Blocks> {
+  u32x4 x;
+  uint32_t e;  // their page's scale (uniform: a wavefront's rows lie in one page)
+};
 
 // fp8 and 4-bit pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7) is one load of 16 values per
 // lane: row 8 w + l / 8, dims 16 (l % 8) .. +15.  off: the lane's offset from the group base for a full
@@ -137,14 +144,21 @@ struct Staged<kPoolFp4> {
 template <int POOL, bool IS_V>
 __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const PrefillArgs& a, int blk, int kv0, int last,
                                                    int kv_end, int w, unsigned off, unsigned eoff, unsigned head_bytes, int lane) {
-  constexpr unsigned kLane = POOL == kPoolFp8 ? 16 : 8;  // bytes of 16 values
+  constexpr unsigned kLane = POOL == kPoolFp4 ? 8 : 16;  // bytes of 16 values
   const int key0 = kv0 + 16 * (w >> 1);
   const bool whole = kv0 + kBN <= kv_end;
   const int tok = whole ? 0 : min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);  // the row within its block
   if constexpr (POOL != kPoolFp4) {
     const char* p = whole ? group_base(pool, a, blk, key0) + off
                           : group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
-    return {ld16(p)};
+    if constexpr (POOL != kPoolFp8Blocks) {
+      return {ld16(p)};
+    } else {
+      const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
+      const uint64_t at = (uint64_t)b * (unsigned)a.Hkv + head_bytes / kHeadDim;
+      ConstU32* words = (ConstU32*)(IS_V ? a.vs : a.ks);
+      return {ld16(p), words[at >> 2] >> (8 * (unsigned)(at & 3))};
+    }
   } else {
     // a load per branch: merged, the two addresses would be a pair of registers per lane instead of a scalar and an offset
     constexpr int kBlocks = kHeadDim / kFp4Block;
@@ -177,9 +191,12 @@ __device__ __forceinline__ void stage_store(const Staged<POOL>& s, int w, int la
   const int sw = IS_V ? 4 * (r & 3) : (r & 15);
   char* row = slot + r * kRowBytes;
   u32x4 lo, hi;
-  if constexpr (POOL != kPoolFp4) {
+  if constexpr (POOL != kPoolFp4 && POOL != kPoolFp8Blocks) {
     lo = fp8x8_to<T>(s.x[0], s.x[1]);
     hi = fp8x8_to<T>(s.x[2], s.x[3]);
+  } else if constexpr (POOL == kPoolFp8Blocks) {  // the conversions read bits 30:23 of their scale alone
+    lo = fp8x8_to<T>(s.x[0], s.x[1], e8m0_to_f32(s.e));
+    hi = fp8x8_to<T>(s.x[2], s.x[3], e8m0_to_f32(s.e));
   } else {
     lo = fp4x8_to<T>(s.x[0], e8m0_to_f32(s.e));
     hi = fp4x8_to<T>(s.x[1], e8m0_to_f32(s.e));
@@ -553,7 +570,7 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
     if ((p & 1) == grp) {  // matrix phase of pair j
       __builtin_amdgcn_s_setprio(1);
       // all four products of the pair (fp8 pools keep two tiles of staging registers, eight of them: no single ring)
-      const bool full = POOL != kPoolFp8 && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
+      const bool full = POOL != kPoolFp8 && POOL != kPoolFp8Blocks && ta + 3 < ntiles && (ta + 3) * kBN <= wave_qp_hi;
       if (full) {
         matrix_phase_pair<T>(lds, vread + (ta & (kRingV - 1)) * kTileBytes, kread + ((ta + 2) & (kRingK - 1)) * kTileBytes,
                              vread + ((ta + 1) & (kRingV - 1)) * kTileBytes, kread + ((ta + 3) & (kRingK - 1)) * kTileBytes,
@@ -910,7 +927,10 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
                                   int64_t out_stride_head, int pool, float k_scale, float v_scale, const void* k_scales,
                   const void* v_scales, void* stream) {
   using namespace mllm;
-  const std::string fn = pool == kPoolFp4 ? "mllm_paged_prefill_fp4" : (pool == kPoolFp8 ? "mllm_paged_prefill_fp8" : "mllm_paged_prefill");
+  static const char* const kNames[] = {"mllm_paged_prefill", "mllm_paged_prefill_fp8", "mllm_paged_prefill_fp4",
+                                       "mllm_paged_prefill_fp8_blocks"};
+  const std::string fn = kNames[pool];
+  const bool scaled = pool == kPoolFp4 || pool == kPoolFp8Blocks;
   MLLM_REQUIRE(dtype == MLLM_DTYPE_BF16 || dtype == MLLM_DTYPE_F16, MLLM_ERR_UNSUPPORTED,
                fn + ": dtype must be bfloat16 or float16");
   MLLM_REQUIRE(head_dim == kHeadDim, MLLM_ERR_UNSUPPORTED, fn + ": head_dim must be 128");
@@ -928,8 +948,10 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
   MLLM_REQUIRE(num_prefill_work >= 0, MLLM_ERR_INVALID, fn + ": negative count");
   if (num_prefill_work == 0) return MLLM_OK;
   MLLM_REQUIRE(q && k_cache && v_cache && out && qo_indptr && kv_indptr && kv_indices && seq_lens && prefill_work &&
-                   (pool != kPoolFp4 || (k_scales && v_scales)),
+                   (!scaled || (k_scales && v_scales)),
                MLLM_ERR_INVALID, fn + ": null pointer");
+  MLLM_REQUIRE(pool != kPoolFp8Blocks || ((uintptr_t)k_scales | (uintptr_t)v_scales) % 4 == 0, MLLM_ERR_UNSUPPORTED,
+               fn + ": scales must be 4-byte aligned");
   const bool aligned = ((uintptr_t)q % 16 == 0) && ((uintptr_t)out % 16 == 0) && ((uintptr_t)k_cache % 16 == 0) &&
                        ((uintptr_t)v_cache % 16 == 0) && (q_stride_tok * 2) % 16 == 0 &&
                        (q_stride_head * 2) % 16 == 0 && (out_stride_tok * 2) % 16 == 0 && (out_stride_head * 2) % 16 == 0;
@@ -978,6 +1000,8 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
   };
   if (pool == kPoolFp4)
     of_type(std::integral_constant<int, kPoolFp4>{});
+  else if (pool == kPoolFp8Blocks)
+    of_type(std::integral_constant<int, kPoolFp8Blocks>{});
   else if (pool == kPoolFp8)
     of_type(std::integral_constant<int, kPoolFp8>{});
   else
@@ -1025,4 +1049,18 @@ extern "C" int mllm_paged_prefill_fp4(const void* q, int64_t q_stride_tok, int64
                        num_kv_heads, head_dim, qo_indptr, kv_indptr, kv_indices, seq_lens, prefill_work,
                        num_prefill_work, q_tile_tokens, softmax_scale, dtype, out, out_stride_tok, out_stride_head,
                        mllm::kPoolFp4, 1.f, 1.f, k_scales, v_scales, stream);
+}
+
+extern "C" int mllm_paged_prefill_fp8_blocks(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                                      const void* v_cache, const void* k_scales, const void* v_scales,
+                                      int64_t num_blocks, int32_t block_size, int32_t num_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                      const int32_t* kv_indices, const int32_t* seq_lens, const int32_t* prefill_work,
+                                      int32_t num_prefill_work, int32_t q_tile_tokens, float softmax_scale,
+                                      int32_t dtype, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                                      void* stream) {
+  return paged_prefill(q, q_stride_tok, q_stride_head, k_cache, v_cache, num_blocks, block_size, num_heads,
+                       num_kv_heads, head_dim, qo_indptr, kv_indptr, kv_indices, seq_lens, prefill_work,
+                       num_prefill_work, q_tile_tokens, softmax_scale, dtype, out, out_stride_tok, out_stride_head,
+                       mllm::kPoolFp8Blocks, 1.f, 1.f, k_scales, v_scales, stream);
 }

@@ -196,24 +196,24 @@ extern "C" int mllm_qk_norm_rope_kv_append(const mllm_rope_append* r, const void
   MLLM_REQUIRE(r, MLLM_ERR_INVALID, fn + ": null arguments");
   const int rc = check_qk(fn, r->dtype, r->num_tokens, r->num_heads, r->num_kv_heads, r->head_dim, eps);
   if (rc != MLLM_OK) return rc;
-  MLLM_REQUIRE(r->pool == MLLM_POOL_16BIT || r->pool == MLLM_POOL_FP8 || r->pool == MLLM_POOL_FP4, MLLM_ERR_INVALID,
-               fn + ": unknown pool type");
-  const bool fp4 = r->pool == MLLM_POOL_FP4;
+  MLLM_REQUIRE(known_pool(r->pool), MLLM_ERR_INVALID, fn + ": unknown pool type");
+  const bool fp4 = r->pool == MLLM_POOL_FP4, scaled = fp4 || r->pool == MLLM_POOL_FP8_BLOCKS;
   MLLM_REQUIRE(!fp4 || r->head_dim % 64 == 0, MLLM_ERR_UNSUPPORTED, fn + ": head_dim must be a multiple of 64 for a 4-bit pool");
-  MLLM_REQUIRE(!q_norm == !k_norm && (q_norm || fp4), MLLM_ERR_INVALID,
-               fn + ": q_norm and k_norm go together (without them, 4-bit pools only)");
+  MLLM_REQUIRE(!q_norm == !k_norm && (q_norm || scaled), MLLM_ERR_INVALID,
+               fn + ": q_norm and k_norm go together (without them, 8-bit pools with block scales and 4-bit pools only)");
   MLLM_REQUIRE(r->num_blocks >= 0 && r->block_size > 0, MLLM_ERR_INVALID, fn + ": bad pool sizes");
   MLLM_REQUIRE(r->pool != MLLM_POOL_FP8 || (r->k_scale > 0.f && r->v_scale > 0.f && r->k_scale < INFINITY && r->v_scale < INFINITY),
                MLLM_ERR_INVALID, fn + ": scales must be positive and finite");
   if (r->num_tokens == 0) return MLLM_OK;
   MLLM_REQUIRE(r->q && r->k && r->v && r->cos && r->sin && r->q_out && r->k_cache && r->v_cache && r->slot_mapping &&
-                   (!fp4 || (r->k_scales && r->v_scales)),
+                   (!scaled || (r->k_scales && r->v_scales)),
                MLLM_ERR_INVALID, fn + ": null pointer");
   const uintptr_t ptrs = (uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->cos | (uintptr_t)r->sin |
                          (uintptr_t)r->q_out | (uintptr_t)r->k_cache | (uintptr_t)r->v_cache | (uintptr_t)q_norm | (uintptr_t)k_norm;
   const int64_t strides = r->q_stride_tok | r->q_stride_head | r->k_stride_tok | r->k_stride_head | r->v_stride_tok |
                           r->v_stride_head | r->cs_stride_tok | r->q_out_stride_tok | r->q_out_stride_head;
   MLLM_REQUIRE(ptrs % 16 == 0 && strides % 8 == 0, MLLM_ERR_UNSUPPORTED, fn + ": rows must be 16-byte aligned");
+  if (r->pool == MLLM_POOL_FP8_BLOCKS) return rope_append_fp8_blocks(fn, *r, q_norm, k_norm, eps, stream);
   QkArgs a{};
   a.q = (const char*)r->q, a.q_st = 2 * r->q_stride_tok, a.q_sh = 2 * r->q_stride_head;
   a.k = (const char*)r->k, a.k_st = 2 * r->k_stride_tok, a.k_sh = 2 * r->k_stride_head;

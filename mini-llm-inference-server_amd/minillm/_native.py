@@ -17,8 +17,8 @@ LIB_PATH = Path(os.environ.get("MLLM_HIP_LIB", Path(__file__).resolve().parent /
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, -1, -2, -3
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-ABI_VERSION = 6
-POOL_16BIT, POOL_FP8, POOL_FP4 = 0, 1, 2
+ABI_VERSION = 7
+POOL_16BIT, POOL_FP8, POOL_FP4, POOL_FP8_BLOCKS = 0, 1, 2, 4
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -120,6 +120,14 @@ SIGNATURES = {
     "mllm_paged_decode_fp8": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                              _i32, _p, _i32, _i32, _f32, _i32, _f32, _f32, _p, _i64, _i64, _p, _i64,
                                              _p]),
+    # 8-bit pools with a scale for each block of tokens and head
+    "mllm_kv_append_fp8_blocks": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
+                                          _i64, _p]),
+    "mllm_kv_read_fp8_blocks": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p]),
+    "mllm_paged_decode_fp8_blocks": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32,
+                                             _p, _i32, _i32, _f32, _i32, _p, _i64, _i64, _p, _i64, _p]),
+    "mllm_paged_prefill_fp8_blocks": (ctypes.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p,
+                                              _p, _i32, _i32, _f32, _i32, _p, _i64, _i64, _p]),
     # 4-bit pools (e2m1 codes, e8m0 block scales), head norms
     "mllm_kv_append_fp4": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
                                           _i64, _p]),

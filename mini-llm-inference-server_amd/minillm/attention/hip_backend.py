@@ -21,6 +21,11 @@ A pool of dtype torch.float4_e2m1fn_x2 ([num_blocks, block_size, Hkv, Dh / 2], t
 entry points; `k_scale` and `v_scale` are then the pool's block scales, torch.float8_e8m0fnu tensors (PagedKVCache keeps
 them; include/minillm_hip.h has the format).
 
+A pool of dtype torch.float8_e4m3fn whose `k_scale` and `v_scale` are torch.float8_e8m0fnu tensors [num_blocks, Hkv] holds a
+scale for each block of tokens (page) and head instead of one per tensor, and selects the `_fp8_blocks` entry points:
+nothing to calibrate.  A step's tokens of a page have to be consecutive rows at consecutive slots, as
+`AttentionMetadata.build` lays them out.
+
 `forward_rotary` and `rope_append` take `qk_norm=(q weight, k weight, eps)`: RMSNorm of every query and key head in the
 launch that rotates and appends (`mllm_qk_norm_rope_kv_append`), into any of the pools.
 """
@@ -84,7 +89,7 @@ MIN_SPLIT_PAGES = 2  # the smallest bin the heuristic picks (16-bit pools)
 
 
 def fp4_heads(num_heads: int, num_kv_heads: int) -> int:
-    """KV heads a wavefront of mllm_paged_decode_fp4 takes (the library's rule)."""
+    """KV heads a wavefront of mllm_paged_decode_fp4 and of mllm_paged_decode_fp8_blocks takes (the library's rule)."""
     return 2 if num_kv_heads % 2 == 0 and 2 * (num_heads // num_kv_heads) <= 16 else 1
 
 
@@ -117,7 +122,7 @@ def pages_per_split(decode_pages: int, num_kv_heads: int, num_heads: int | None 
     forced = os.environ.get("MLLM_PAGES_PER_SPLIT")
     if forced:
         return max(1, min(MAX_SPLIT_PAGES, int(forced)))
-    if kv_fp4:  # one workgroup per CU, each on up to four groups of fp4_heads KV heads
+    if kv_fp4:  # pools with block scales: one workgroup per CU, each on up to four groups of fp4_heads KV heads
         per_bin = -(-(num_kv_heads // fp4_heads(num_heads or 4 * num_kv_heads, num_kv_heads)) // 4)
         per_round = max(1, num_cus // per_bin)
         rounds = max(1, math.ceil(decode_pages / (MAX_SPLIT_PAGES * per_round)))
@@ -250,35 +255,46 @@ FP4 = torch.float4_e2m1fn_x2  # two e2m1 codes to an element
 SCALES4 = torch.float8_e8m0fnu  # their block scales
 FP4_BLOCK = 32  # dims per scale
 _POOLS = {FP8: _native.POOL_FP8, FP4: _native.POOL_FP4}  # of the other types: POOL_16BIT
+# pools with block scales: one decode kernel, which merges its cut rows by itself
+SCALED = frozenset((_native.POOL_FP4, _native.POOL_FP8_BLOCKS))
 
 
-def pool_type(pool: torch.Tensor) -> int:
-    """The library's MLLM_POOL_* of a pool."""
-    return _POOLS.get(pool.dtype, _native.POOL_16BIT)
+def pool_type(pool: torch.Tensor, k_scale=None) -> int:
+    """The library's MLLM_POOL_* of a pool: an fp8 one with a tensor of e8m0 scales has a scale for each page and head."""
+    dtype = pool.dtype
+    if dtype == FP8 and isinstance(k_scale, torch.Tensor) and k_scale.dtype == SCALES4:
+        return _native.POOL_FP8_BLOCKS
+    return _POOLS.get(dtype, _native.POOL_16BIT)
 
 
 def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
-    """ValueError unless k_scale and v_scale are the block scales of a 4-bit pool."""
-    nb, bs, hkv, half = k_cache.shape
-    blocks = 2 * half // FP4_BLOCK
+    """ValueError unless k_scale and v_scale are the block scales of a 4-bit or (with a scale for each page and head) an 8-bit
+    pool."""
+    nb, bs, hkv, width = k_cache.shape
+    if k_cache.dtype == FP4:
+        blocks = 2 * width // FP4_BLOCK
+        k_shape, v_shape, kind = (nb, bs, blocks, hkv), (nb, hkv, blocks, bs), "a 4-bit pool"
+    else:
+        k_shape, v_shape, kind = (nb, hkv), (nb, hkv), "block scales"
     device = k_cache.device
-    for name, t, shape in (("k_scale", k_scale, (nb, bs, blocks, hkv)), ("v_scale", v_scale, (nb, hkv, blocks, bs))):
+    for name, t, shape in (("k_scale", k_scale, k_shape), ("v_scale", v_scale, v_shape)):
         if not isinstance(t, torch.Tensor) or t.dtype != SCALES4:
-            raise ValueError(f"with a 4-bit pool, {name} is its float8_e8m0fnu tensor of block scales")
+            raise ValueError(f"with {kind}, {name} is a float8_e8m0fnu tensor of block scales")
         if t.shape != shape or not t.is_contiguous() or t.device != device:
             raise ValueError(f"{name} must be contiguous {list(shape)} on the pool's device")
 
 
 def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, out: torch.Tensor) -> None:
-    """ValueError unless q and out are [N, H, Dh] rows of the step's tokens over these 4-bit pools."""
-    pool = k_cache.shape
+    """ValueError unless q and out are [N, H, Dh] rows of the step's tokens over these pools with block scales."""
+    pool, dtype = k_cache.shape, k_cache.dtype
+    dh = pool[3] * (2 if dtype == FP4 else 1)
     shape, tokens = q.shape, meta.query_start_loc[-1]
-    if len(shape) != 3 or shape[2] != 2 * pool[3] or shape[1] % pool[2] or shape[0] != tokens or pool[1] != meta.block_size:
-        raise ValueError(f"q must be [N, H, Dh] = [{tokens}, a multiple of {pool[2]}, {2 * pool[3]}], and the pool's blocks "
+    if len(shape) != 3 or shape[2] != dh or shape[1] % pool[2] or shape[0] != tokens or pool[1] != meta.block_size:
+        raise ValueError(f"q must be [N, H, Dh] = [{tokens}, a multiple of {pool[2]}, {dh}], and the pool's blocks "
                          f"{meta.block_size} tokens")
     if out.shape != shape or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("out must be like q, both with unit stride in their last dimension")
-    if v_cache.shape != pool or v_cache.dtype != FP4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if v_cache.shape != pool or v_cache.dtype != dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be alike and contiguous")
     if not q.device == out.device == k_cache.device == v_cache.device:
         raise ValueError("q, out and the pools must share one device")
@@ -310,7 +326,7 @@ def check_device(q: torch.Tensor, *others: torch.Tensor) -> None:
 def layer_pool(k_cache, v_cache, k_scale, v_scale, qk_norm) -> bytes:
     """The mllm_layer_pool of a layer's checked pools, scales and head norms."""
     norms = (0, 0, 0.0) if qk_norm is None else (qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2])
-    if k_cache.dtype == FP4:
+    if pool_type(k_cache, k_scale) in SCALED:
         return _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), 1.0,
                                        1.0, *norms)
     return _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, k_scale, v_scale, *norms)
@@ -345,19 +361,19 @@ class HipBackend(AttentionBackend):
     def forward(self, q, k, v, k_cache, v_cache, meta, k_scale: float = 1.0, v_scale: float = 1.0):
         q, k, v = self._check(q, k, v, k_cache, v_cache, meta, k_scale, v_scale)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if self._split_launches(q, k_cache, meta):
+        if self._split_launches(q, k_cache, meta, k_scale):
             self.append(k, v, k_cache, v_cache, meta, k_scale, v_scale)
             self.attend(q, k_cache, v_cache, meta, out, k_scale, v_scale)
         else:
             self.run_layer(q, k, v, k_cache, v_cache, meta, out, k_scale=k_scale, v_scale=v_scale)
         return out
 
-    def _split_launches(self, q, k_cache, meta) -> bool:
+    def _split_launches(self, q, k_cache, meta, k_scale=None) -> bool:
         """Whether this layer runs as separate calls: only a mixed step with `overlap_mixed` set, whose
         prefill goes to a second stream."""
         if not self.overlap_mixed:
             return False
-        plan = self._plan_for(meta, q, k_cache)
+        plan = self._plan_for(meta, q, k_cache, k_scale)
         return bool(plan.num_decode and plan.num_prefill) and not torch.cuda.is_current_stream_capturing()
 
     def run_layer(self, q, k, v, k_cache, v_cache, meta, out, cos=None, sin=None, q_rot=None,
@@ -367,12 +383,11 @@ class HipBackend(AttentionBackend):
         current stream.  The arguments are the checked ones of `forward` / `forward_rotary`; q_rot and out
         are contiguous [N, H, Dh]."""
         n, h, dh = q.shape
-        shape, dtype = k_cache.shape, k_cache.dtype
-        pool = _POOLS.get(dtype, _native.POOL_16BIT)
+        shape, pool = k_cache.shape, pool_type(k_cache, k_scale)
         plan = self.plan(meta, h, shape[2], dh, q.device, pool=pool)
         step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache, shape, pool)
         rot = cos is not None
-        if dtype == FP4 or qk_norm is not None:
+        if pool in SCALED or qk_norm is not None:
             self._lib.launch(
                 q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cos.data_ptr() if rot else None,
@@ -385,10 +400,10 @@ class HipBackend(AttentionBackend):
             cos.stride(0) if rot else 0, q_rot.data_ptr() if rot else None, k_cache.data_ptr(), v_cache.data_ptr(),
             k_scale, v_scale, out.data_ptr(), _native.stream_ptr(q.device)))
 
-    def layer_step(self, meta, n: int, num_heads: int, dtype, k_cache) -> int:
+    def layer_step(self, meta, n: int, num_heads: int, dtype, k_cache, k_scale=None) -> int:
         """Address of the step's mllm_layer_step for rows of `num_heads` query heads in `dtype` and these pools (the
         plan is built on the first call with `meta`)."""
-        pool, shape = pool_type(k_cache), k_cache.shape
+        pool, shape = pool_type(k_cache, k_scale), k_cache.shape
         dh = shape[3] * (2 if pool == _native.POOL_FP4 else 1)
         plan = self.plan(meta, num_heads, shape[2], dh, k_cache.device, pool=pool)
         return self._layer_step(plan, meta, n, num_heads, dh, dtype, k_cache, shape, pool)
@@ -422,6 +437,7 @@ class HipBackend(AttentionBackend):
             raise ValueError("k_cache and v_cache must both be [num_blocks, block_size, Hkv, Dh]")
         _, bs, hkv, dh_c = of_pool
         fp4, fp8 = pool == FP4, pool == FP8
+        scaled = fp4 or fp8 and pool_type(k_cache, k_scale) in SCALED
         if fp4:
             dh_c *= 2
         rows = (n, hkv, dh)
@@ -438,7 +454,7 @@ class HipBackend(AttentionBackend):
         if (fp8 or fp4) and (dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype):
             raise ValueError(f"with {'an fp8' if fp8 else 'a 4-bit'} pool, q, k and v must share one dtype, bfloat16 or "
                              f"float16")
-        if fp4:
+        if scaled:
             if not q.device == k.device == v.device == k_cache.device == v_cache.device:
                 raise ValueError("q, k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
@@ -465,7 +481,7 @@ class HipBackend(AttentionBackend):
         q, k, v = self._check(q, k, v, k_cache, v_cache, meta, k_scale, v_scale)
         if qk_norm is not None:
             check_norms(qk_norm, q, k, v)
-        if self._split_launches(q, k_cache, meta):
+        if self._split_launches(q, k_cache, meta, k_scale):
             q_rot = self.rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm)
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             self.attend(q_rot, k_cache, v_cache, meta, out, k_scale, v_scale)
@@ -475,7 +491,7 @@ class HipBackend(AttentionBackend):
             raise ValueError(f"cos and sin must be [N, Dh] = [{n}, {dh}]")
         if cos.dtype != q.dtype or sin.dtype != q.dtype:
             raise ValueError("q, cos, sin and the pools must share one dtype (or the pools be fp8)")
-        if qk_norm is not None or k_cache.dtype == FP4:
+        if qk_norm is not None or pool_type(k_cache, k_scale) in SCALED:
             check_device(q, cos, sin, k_cache, v_cache)
         if cos.stride(-1) != 1 or sin.stride() != cos.stride():
             cos, sin = cos.contiguous(), sin.contiguous()
@@ -487,7 +503,7 @@ class HipBackend(AttentionBackend):
     def rope_append(self, q, k, v, cos, sin, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0, qk_norm=None):
         """Rotary embedding of q and k plus the KV append (`mllm_rope_kv_append`); returns the rotated q.  With
         `qk_norm` the heads of q and k are normed first (`mllm_qk_norm_rope_kv_append`)."""
-        if k_cache.dtype == FP4 or qk_norm is not None:
+        if qk_norm is not None or pool_type(k_cache, k_scale) in SCALED:
             return self._norm_rope_append(q, k, v, cos, sin, k_cache, v_cache, meta, k_scale, v_scale, qk_norm)
         n, h, dh = q.shape
         num_blocks, bs, hkv, _ = k_cache.shape
@@ -526,8 +542,8 @@ class HipBackend(AttentionBackend):
             check_norms(qk_norm, q, k, v)
             wq, wk, eps = qk_norm[0].data_ptr(), qk_norm[1].data_ptr(), qk_norm[2]
         q_rot = torch.empty_like(q, memory_format=torch.contiguous_format)
-        pool = pool_type(k_cache)
-        if pool == _native.POOL_FP4:
+        pool = pool_type(k_cache, k_scale)
+        if pool in SCALED:
             scales = (k_scale.data_ptr(), v_scale.data_ptr(), 1.0, 1.0)
         else:
             scales = (0, 0, k_scale, v_scale)
@@ -542,12 +558,15 @@ class HipBackend(AttentionBackend):
     def append(self, k, v, k_cache, v_cache, meta, k_scale=1.0, v_scale=1.0) -> None:
         """KV append (reference write_kv, paged_torch_ref.py:23-28): one launch for K and V."""
         num_blocks, bs, hkv, dh = k_cache.shape
-        if k_cache.dtype == FP4:
+        pool = pool_type(k_cache, k_scale)
+        if pool in SCALED:
             rows, dtype = k.shape, k.dtype
-            if len(rows) != 3 or rows[1] != hkv or rows[2] != 2 * dh or v.shape != rows or v.dtype != dtype:
-                raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {2 * dh}] of one dtype")
+            if pool == _native.POOL_FP4:
+                dh *= 2
+            if len(rows) != 3 or rows[1] != hkv or rows[2] != dh or v.shape != rows or v.dtype != dtype:
+                raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {dh}] of one dtype")
             slots = meta.slot_mapping
-            if slots.numel() != rows[0] or v_cache.shape != k_cache.shape or v_cache.dtype != FP4 \
+            if slots.numel() != rows[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
                     or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
                 raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
             device = k_cache.device
@@ -558,9 +577,10 @@ class HipBackend(AttentionBackend):
             if sk[2] != 1 or sv[2] != 1:
                 k, v = k.contiguous(), v.contiguous()
                 sk, sv = k.stride(), v.stride()
-            self._lib.launch(device, "mllm_kv_append_fp4", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
-                             _native.dtype_code(dtype), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                             v_scale.data_ptr(), num_blocks, bs, hkv, 2 * dh, slots.data_ptr(), rows[0])
+            self._lib.launch(device, "mllm_kv_append_fp4" if pool == _native.POOL_FP4 else "mllm_kv_append_fp8_blocks",
+                             k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], _native.dtype_code(dtype),
+                             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs,
+                             hkv, dh, slots.data_ptr(), rows[0])
             return
         if is_fp8(k_cache):
             self._lib.call("mllm_kv_append_fp8", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
@@ -597,24 +617,26 @@ class HipBackend(AttentionBackend):
                 self._make_plan(meta, num_heads, num_kv_heads, head_dim, device, _native.stream_ptr(device), pool)
         return self._plan
 
-    def _plan_for(self, meta, q, k_cache) -> StepPlan:
-        return self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, pool=pool_type(k_cache))
+    def _plan_for(self, meta, q, k_cache, k_scale=None) -> StepPlan:
+        return self.plan(meta, q.shape[1], k_cache.shape[2], q.shape[2], q.device, pool=pool_type(k_cache, k_scale))
 
     def attend(self, q, k_cache, v_cache, meta, out, k_scale=1.0, v_scale=1.0) -> None:
         """Attention of every new token over its row's context in the pool, written into `out`."""
-        if k_cache.dtype == FP4:
+        kind = pool_type(k_cache, k_scale)
+        merges = kind in SCALED  # the decode call merges by itself
+        if merges:
             check_attend(q, k_cache, v_cache, meta, out)
             check_scales(k_cache, k_scale, v_scale)
             if out.is_contiguous() and not self.overlap_mixed:  # one call for the step's launches
                 n, h, dh = q.shape
-                plan = self.plan(meta, h, k_cache.shape[2], dh, q.device, pool=_native.POOL_FP4)
-                step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache, k_cache.shape, _native.POOL_FP4)
+                plan = self.plan(meta, h, k_cache.shape[2], dh, q.device, pool=kind)
+                step = self._layer_step(plan, meta, n, h, dh, q.dtype, k_cache, k_cache.shape, kind)
                 pool = _native.pack_layer_pool(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                                                v_scale.data_ptr(), 1.0, 1.0, 0, 0, 0.0)
                 self._lib.launch(q.device, "mllm_attention_forward_pool", step, q.data_ptr(), q.stride(0), q.stride(1), None,
                                  0, 0, None, 0, 0, None, None, 0, None, pool, out.data_ptr())
                 return
-        plan = self._plan_for(meta, q, k_cache)
+        plan = self._plan_for(meta, q, k_cache, k_scale)
         if plan.num_decode and plan.num_prefill and self.overlap_mixed and not torch.cuda.is_current_stream_capturing():
             # decode is enqueued first; the prefill's workgroups take CUs as the decode's free up
             cur = torch.cuda.current_stream(q.device)
@@ -623,7 +645,7 @@ class HipBackend(AttentionBackend):
                 side = self._side[q.device] = torch.cuda.Stream(q.device)  # default priority
             ready = cur.record_event()  # the append (and everything before it) has landed
             self.run_decode(q, k_cache, v_cache, meta, out, k_scale, v_scale)
-            if k_cache.dtype != FP4:  # whose decode call merges
+            if not merges:
                 self.run_merge(q, meta, out)
             side.wait_event(ready)
             with torch.cuda.stream(side):
@@ -632,7 +654,7 @@ class HipBackend(AttentionBackend):
             return
         if plan.num_decode:
             self.run_decode(q, k_cache, v_cache, meta, out, k_scale, v_scale)
-            if k_cache.dtype != FP4:  # whose decode call merges
+            if not merges:
                 self.run_merge(q, meta, out)
         if plan.num_prefill:
             self.run_prefill(q, k_cache, v_cache, meta, out, k_scale, v_scale)
@@ -642,12 +664,15 @@ class HipBackend(AttentionBackend):
         plan = self._plan
         num_blocks, bs, hkv, dh = k_cache.shape
         ws = self._workspace_for(plan.workspace_bytes, q.device)
-        if k_cache.dtype == FP4:
+        pool = pool_type(k_cache, k_scale)
+        if pool in SCALED:
+            fp4 = pool == _native.POOL_FP4
+            dh = 2 * dh if fp4 else dh
             self._lib.launch(
-                q.device, "mllm_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv, 2 * dh,
-                plan.meta_ptrs[0], plan.meta_ptrs[2], plan.decode_args[4], plan.num_decode, plan.decode_args[6],
-                plan.num_merge, plan.pages_per_split, (2 * dh) ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
+                q.device, "mllm_paged_decode_fp4" if fp4 else "mllm_paged_decode_fp8_blocks", q.data_ptr(), q.stride(0),
+                q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs,
+                q.shape[1], hkv, dh, plan.meta_ptrs[0], plan.meta_ptrs[2], plan.decode_args[4], plan.num_decode,
+                plan.decode_args[6], plan.num_merge, plan.pages_per_split, dh ** -0.5, _native.dtype_code(q.dtype), out.data_ptr(),
                 out.stride(0), out.stride(1), _ptr(ws), plan.workspace_bytes)
             return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
@@ -673,11 +698,14 @@ class HipBackend(AttentionBackend):
         """MFMA attention of the rows with several new tokens (reference paged_torch_ref.py:61-73)."""
         plan = self._plan
         num_blocks, bs, hkv, dh = k_cache.shape
-        if k_cache.dtype == FP4:
+        pool = pool_type(k_cache, k_scale)
+        if pool in SCALED:
+            fp4 = pool == _native.POOL_FP4
+            dh = 2 * dh if fp4 else dh
             self._lib.launch(
-                q.device, "mllm_paged_prefill_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs, q.shape[1], hkv, 2 * dh,
-                *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile, (2 * dh) ** -0.5,
+                q.device, "mllm_paged_prefill_fp4" if fp4 else "mllm_paged_prefill_fp8_blocks", q.data_ptr(), q.stride(0),
+                q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, bs,
+                q.shape[1], hkv, dh, *plan.meta_ptrs, _ptr(plan.prefill_work), plan.num_prefill, plan.q_tile, dh ** -0.5,
                 _native.dtype_code(q.dtype), out.data_ptr(), out.stride(0), out.stride(1))
             return
         args = (q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, bs,
@@ -690,7 +718,7 @@ class HipBackend(AttentionBackend):
             self._lib.call("mllm_paged_prefill", *args, *tail)
 
     def _make_plan(self, meta, h: int, hkv: int, dh: int, dev, stream: int, pool: int = _native.POOL_16BIT) -> None:
-        kv_fp8, kv_fp4 = pool == _native.POOL_FP8, pool == _native.POOL_FP4
+        kv_fp8, scaled = pool == _native.POOL_FP8, pool in SCALED
         news, lens, bs = meta.num_new, meta.seq_lens, meta.block_size
         pages = [-(-length // bs) for length in lens]
         decode_pages = sum(p for p, nn in zip(pages, news) if nn == 1)
@@ -698,7 +726,7 @@ class HipBackend(AttentionBackend):
         # capacities then cover the smallest split it may stage
         split_dev = getattr(meta, "split_dev", None)
         c = meta.split_min if split_dev is not None \
-            else pages_per_split(decode_pages, hkv, h, kv_fp8, device_cus(dev), kv_fp4=kv_fp4)
+            else pages_per_split(decode_pages, hkv, h, kv_fp8, device_cus(dev), kv_fp4=scaled)
         g = h // hkv
         q_tile = prefill_q_tile(news, g, hkv, kv_fp8, device_cus(dev))
         decode_rows = sum(1 for nn in news if nn == 1)

@@ -16,6 +16,11 @@ pools are [num_blocks, block_size, Hkv, Dh / 2] (two codes to a byte), `k_scale[
 and `v_scale[l]` [num_blocks, Hkv, Dh / 32, block_size] torch.float8_e8m0fnu tensors (include/minillm_hip.h has the
 format).  One block of Llama-3.1-8B is 17 KB per layer, so the same HBM holds 3.76 times the tokens of 16 bits.
 
+With `block_scales`, a pool of dtype torch.float8_e4m3fn has a power-of-two scale for each page and head instead of one per
+tensor: `k_scale[l]` and `v_scale[l]` are torch.float8_e8m0fnu tensors [num_blocks, Hkv].  They follow the tokens that come
+into a page (include/minillm_hip.h has the rule), so there is nothing to calibrate and nothing saturates; one byte for 16
+tokens of a head.
+
 `PagedStep` is the pool as one forward pass sees it: the pool plus that step's metadata.
 """
 
@@ -28,15 +33,24 @@ from .. import _native
 BLOCK_SIZE = 16
 FP4 = torch.float4_e2m1fn_x2
 FP4_BLOCK = 32  # dims per scale of a 4-bit pool
+FP8 = torch.float8_e4m3fn
 
 
 class PagedKVCache:
     def __init__(self, config, num_blocks: int, device: torch.device | str, dtype: torch.dtype,
-                 block_size: int = BLOCK_SIZE, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+                 block_size: int = BLOCK_SIZE, k_scale: float = 1.0, v_scale: float = 1.0,
+                 block_scales: bool = False) -> None:
         hkv, dh = config.num_key_value_heads, config.head_dim
         self.fp4 = dtype == FP4
         if self.fp4 and dh % (2 * FP4_BLOCK):
             raise ValueError(f"a 4-bit pool needs a head_dim that is a multiple of {2 * FP4_BLOCK}, not {dh}")
+        self.block_scales = bool(block_scales)
+        if self.block_scales:
+            if dtype != FP8:
+                raise ValueError("block_scales is for pools of float8_e4m3fn (a 4-bit pool always has them)")
+            if dh != 128 or block_size not in (16, 32, 64):
+                raise ValueError(f"a pool with block scales needs a head_dim of 128 and blocks of 16, 32 or 64 tokens, not "
+                                 f"{dh} and {block_size}")
         self.head_dim = dh
         shape = (num_blocks, block_size, hkv, dh // 2 if self.fp4 else dh)
         zeros = torch.uint8 if self.fp4 else dtype  # torch fills no 4-bit tensor on a GPU
@@ -44,9 +58,9 @@ class PagedKVCache:
         self.v = [torch.zeros(shape, device=device, dtype=zeros).view(dtype) for _ in range(config.num_hidden_layers)]
         self.num_blocks = num_blocks
         self.block_size = block_size
-        self.quantized = dtype == torch.float8_e4m3fn
-        if not self.quantized and (k_scale != 1.0 or v_scale != 1.0):
-            raise ValueError("k_scale / v_scale apply to fp8 pools only")
+        self.quantized = dtype == FP8
+        if (not self.quantized or self.block_scales) and (k_scale != 1.0 or v_scale != 1.0):
+            raise ValueError("k_scale / v_scale apply to fp8 pools only, and not with block_scales")
         self.k_scale: list = [float(k_scale)] * config.num_hidden_layers
         self.v_scale: list = [float(v_scale)] * config.num_hidden_layers
         if self.fp4:
@@ -54,6 +68,9 @@ class PagedKVCache:
             for scales, of in ((self.k_scale, (num_blocks, block_size, blocks, hkv)),
                                (self.v_scale, (num_blocks, hkv, blocks, block_size))):
                 scales[:] = [torch.zeros(of, device=device, dtype=torch.uint8).view(torch.float8_e8m0fnu) for _ in scales]
+        elif self.block_scales:
+            for scales in (self.k_scale, self.v_scale):
+                scales[:] = [_page_scales(num_blocks, hkv, device) for _ in scales]
 
     def scales(self, layer: int) -> dict:
         """Keyword arguments of the backend call for `layer`: its scales for an fp8 or 4-bit pool, none otherwise."""
@@ -61,14 +78,14 @@ class PagedKVCache:
 
     def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of K and V at `slots` [n] (int64, on the pool's device; as a step's slot_mapping names them), both
-        [n, Hkv, Dh] of `dtype`: by default the pool's own, bfloat16 for fp8 and 4-bit pools.  A 4-bit pool is read with the
-        16-bit type it was written with.  A slot outside the pool reads as zeros."""
+        [n, Hkv, Dh] of `dtype`: by default the pool's own, bfloat16 for fp8 and 4-bit pools.  A pool with block scales is read
+        with the 16-bit type it was written with.  A slot outside the pool reads as zeros."""
         k, v = self.k[layer], self.v[layer]
         device = k.device
         if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
             raise ValueError("slots must be one row of int64 on the pool's device")
         dtype = dtype or (torch.bfloat16 if self.quantized or self.fp4 else k.dtype)
-        if not self.fp4:
+        if not (self.fp4 or self.block_scales):
             got, outside = [], (slots < 0) | (slots >= k.shape[0] * k.shape[1])
             slots = slots.masked_fill(outside, 0)
             for pool, scale in ((k, self.k_scale[layer]), (v, self.v_scale[layer])):
@@ -78,34 +95,44 @@ class PagedKVCache:
                 got.append(rows.masked_fill(outside[:, None, None], 0).to(dtype))
             return got[0], got[1]
         if dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError("a 4-bit pool is read as bfloat16 or float16")
+            raise ValueError(f"{'a 4-bit pool' if self.fp4 else 'a pool with block scales'} is read as bfloat16 or float16")
         if device.type != "cuda":
-            raise RuntimeError(f"reading a 4-bit pool needs a GPU device, got {device}")
-        nb, bs, hkv, half = k.shape
+            raise RuntimeError(f"reading {'a 4-bit pool' if self.fp4 else 'a pool with block scales'} needs a GPU device, got {device}")
+        nb, bs, hkv, _ = k.shape
+        dh = self.head_dim
         slots = slots.contiguous()
         n = slots.numel()
-        to_k, to_v = torch.empty((2, n, hkv, 2 * half), dtype=dtype, device=device).unbind()
-        _native.lib().launch(device, "mllm_kv_read_fp4", k.data_ptr(), v.data_ptr(), self.k_scale[layer].data_ptr(),
-                             self.v_scale[layer].data_ptr(), nb, bs, hkv, 2 * half, slots.data_ptr(), n,
-                             _native.dtype_code(dtype), to_k.data_ptr(), to_v.data_ptr())
+        to_k, to_v = torch.empty((2, n, hkv, dh), dtype=dtype, device=device).unbind()
+        _native.lib().launch(device, "mllm_kv_read_fp4" if self.fp4 else "mllm_kv_read_fp8_blocks", k.data_ptr(),
+                             v.data_ptr(), self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr(), nb, bs, hkv, dh,
+                             slots.data_ptr(), n, _native.dtype_code(dtype), to_k.data_ptr(), to_v.data_ptr())
         return to_k, to_v
 
     @staticmethod
-    def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE) -> int:
+    def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE, block_scales: bool = False) -> int:
         """K and V, every layer: 2 x layers x block_size x KV heads x head_dim x bytes per element (4-bit pools: half a
-        byte, and a scale byte for 32 dims)."""
+        byte, and a scale byte for 32 dims), with `block_scales` a byte more per KV head."""
         if dtype == FP4:
             row = config.head_dim // 2 + config.head_dim // FP4_BLOCK
             return 2 * config.num_hidden_layers * block_size * config.num_key_value_heads * row
         elem = torch.tensor([], dtype=dtype).element_size()
-        return 2 * config.num_hidden_layers * block_size * config.num_key_value_heads * config.head_dim * elem
+        row = block_size * config.head_dim * elem + bool(block_scales)
+        return 2 * config.num_hidden_layers * config.num_key_value_heads * row
 
     @classmethod
-    def blocks_for_bytes(cls, config, dtype: torch.dtype, num_bytes: int, block_size: int = BLOCK_SIZE) -> int:
-        return num_bytes // cls.bytes_per_block(config, dtype, block_size)
+    def blocks_for_bytes(cls, config, dtype: torch.dtype, num_bytes: int, block_size: int = BLOCK_SIZE,
+                         block_scales: bool = False) -> int:
+        return num_bytes // cls.bytes_per_block(config, dtype, block_size, block_scales)
 
     def step(self, meta) -> PagedStep:
         return PagedStep(self, meta)
+
+
+def _page_scales(num_blocks: int, hkv: int, device) -> torch.Tensor:
+    """e8m0 scales [num_blocks, Hkv] of zeros, in memory that is readable up to the next multiple of four bytes."""
+    n = num_blocks * hkv
+    whole = torch.zeros(-(-n // 4) * 4, device=device, dtype=torch.uint8)
+    return whole[:n].view(torch.float8_e8m0fnu).view(num_blocks, hkv)
 
 
 class PagedStep:

@@ -96,14 +96,14 @@ class EngineCore:
                  max_num_batched_tokens: int | None = None, num_kv_blocks: int | None = None,
                  enable_prefix_caching: bool = True, model_id: str = "unknown", metadata_builder=None,
                  chunked_prefill: bool = False, kv_cache_dtype: torch.dtype | None = None,
-                 kv_scales: tuple[float, float] = (1.0, 1.0), decode_graphs=None, sampler=None) -> None:
+                 kv_scales: tuple[float, float] | str = (1.0, 1.0), decode_graphs=None, sampler=None) -> None:
         """The step's metadata comes from a device-resident mirror of the block tables (DeviceBlockTables:
         only new block ids travel each step); `metadata_builder(seqs, block_size, device)` replaces that with
         another implementation of the same contract (AttentionMetadata.build uploads every table; a test
         passes the oracle's).  `chunked_prefill` mixes decode rows and prompt chunks in one step under the
         token budget (see Scheduler).  `kv_cache_dtype` defaults to the model's dtype; torch.float8_e4m3fn
         gives an fp8 pool whose K and V tensors of every layer use the per-tensor scales `kv_scales`
-        (k_scale, v_scale); torch.float4_e2m1fn_x2 gives a 4-bit pool with block scales.  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
+        (k_scale, v_scale), or, with `kv_scales="blocks"`, a scale for each page and head; torch.float4_e2m1fn_x2 gives a 4-bit pool with block scales.  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
         captured HIP graphs (DecodeGraphs); prefill and mixed steps stay eager.  `sampler(requests,
         logits)` picks each row's next token from its logits [rows, vocab] (default: greedy argmax); a
         row whose prompt chunk stops short of its end ignores its pick."""
@@ -118,8 +118,12 @@ class EngineCore:
         if num_kv_blocks is None:  # room for every sequence at full length
             num_kv_blocks = max_batch_size * blocks_per_seq
         self.kv_dtype = kv_cache_dtype or self.dtype
-        self.cache = PagedKVCache(model.config, num_kv_blocks, self.device, self.kv_dtype, k_scale=kv_scales[0],
-                                  v_scale=kv_scales[1])
+        block_scales = kv_scales == "blocks"
+        if isinstance(kv_scales, str) and not block_scales:
+            raise ValueError(f'kv_scales is (k_scale, v_scale) or "blocks", not {kv_scales!r}')
+        k_scale, v_scale = (1.0, 1.0) if block_scales else kv_scales
+        self.cache = PagedKVCache(model.config, num_kv_blocks, self.device, self.kv_dtype, k_scale=k_scale,
+                                  v_scale=v_scale, block_scales=block_scales)
         self.prefix = PrefixCache() if enable_prefix_caching else None
         self.blocks = BlockManager(num_kv_blocks, BLOCK_SIZE, self.prefix)
         self.scheduler = Scheduler(max_batch_size, max_num_batched_tokens or DEFAULT_MAX_NUM_BATCHED_TOKENS,
@@ -128,7 +132,7 @@ class EngineCore:
         self._salt_keys = {"block_size": BLOCK_SIZE, "kv_dtype": str(self.kv_dtype).removeprefix("torch."),
                            "layout": "NHD", "model": model_id}
         if self.cache.quantized:  # the stored bytes depend on the scales too
-            self._salt_keys["kv_scales"] = [kv_scales[0], kv_scales[1]]
+            self._salt_keys["kv_scales"] = "blocks" if block_scales else [k_scale, v_scale]
         self.tables = DeviceBlockTables(max_batch_size, blocks_per_seq, self.device) if metadata_builder is None \
             else None
         self.graphs = None

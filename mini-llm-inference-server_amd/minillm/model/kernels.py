@@ -16,7 +16,7 @@ from torch.autograd import forward_ad
 from torch.nn.modules import module as _module
 
 from .. import _native
-from ..attention.hip_backend import FP4, FP8, HipBackend, check_norms, check_scales, layer_pool
+from ..attention.hip_backend import FP4, FP8, SCALED, HipBackend, check_norms, check_scales, layer_pool, pool_type
 from ..cache.paged import PagedKVCache, PagedStep
 
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -269,7 +269,7 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
             and vc.is_contiguous() and n == meta.query_start_loc[-1]):
         return None
     ks, vs = (cache.k_scale[i], cache.v_scale[i]) if cache.quantized or cache.fp4 else (1.0, 1.0)
-    if kc.dtype == FP4:
+    if pool_type(kc, ks) in SCALED:
         check_scales(kc, ks, vs)
     elif kc.dtype == FP8:
         if not (0 < ks < math.inf and 0 < vs < math.inf):
@@ -286,7 +286,7 @@ def decoder_layer(layer, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     ffn = gate.shape[0]
     scratch = torch.empty(lib.fn("mllm_decoder_layer_scratch_bytes")(n, d, ffn, h, hkv, dh), dtype=torch.uint8,
                           device=x.device)
-    step = backend.layer_step(meta, n, h, x.dtype, kc)
+    step = backend.layer_step(meta, n, h, x.dtype, kc, ks)
     out = torch.empty_like(x)
     lib.call("mllm_decoder_layer_pool", step, x.data_ptr(), d, norm1.weight.data_ptr(), norm1.eps, wq.data_ptr(),
              wk.data_ptr(), wv.data_ptr(), attn.o_proj.weight.data_ptr(), norm2.weight.data_ptr(), norm2.eps,
