@@ -553,6 +553,30 @@ int mllm_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, c
                       const void* k_norm, float eps, int32_t batch, int32_t seq, int32_t num_heads,
                       int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void* q_out, void* k_out, void* stream);
 
+/*
+ * Rotation of queries and keys by their positions.  The reference rotates half-split pairs of whole heads, by tables in the
+ * model's type (src/minillm/model/llama.py:58-72); here also adjacent pairs, the first dims of a head alone, and angles that
+ * hold at far positions.
+ *   t = position * inv_freq[i] in 64 bits,  out[a] = factor * (x[a] cos t - x[b] sin t),  out[b] = factor * (x[b] cos t + x[a] sin t)
+ * for i < pairs, with (a, b) = (i, i + pairs), or (2 i, 2 i + 1) when `interleaved`; dims from 2 * pairs on are copied.  fp32
+ * arithmetic, one rounding to `dtype`.
+ * q [B, H, T, Dh], k [B, Hkv, T, Dh] with element strides (batch, head, token), unit stride in Dh; positions [B, T] with strides
+ * (batch, token); inv_freq [pairs] fp32 -> q_out, k_out: contiguous [B, T, heads, Dh].  pairs <= Dh / 2, at most 512.
+ */
+int mllm_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
+                int64_t k_st, const int64_t* positions, int64_t p_sb, int64_t p_st, const float* inv_freq, int32_t pairs,
+                int32_t interleaved, float factor, int32_t batch, int32_t seq, int32_t num_heads, int32_t num_kv_heads,
+                int32_t head_dim, int32_t dtype, void* q_out, void* k_out, void* stream);
+
+/*
+ * Copies of pages within pools (a fork's copy of a last page that is not full, a compaction): page dst[i] of every tensor becomes
+ * its page src[i].  No counterpart in the reference.  tensors, page_bytes, src and dst are host arrays, read before the call
+ * returns: `num_tensors` device pointers of pools (or their scales) of num_pages pages of page_bytes[t] bytes each, and
+ * num_pairs pages.  A page written twice, or read and written, is refused.
+ */
+int mllm_copy_pages(const uint64_t* tensors, const int64_t* page_bytes, int32_t num_tensors, int64_t num_pages,
+                    const int64_t* src, const int64_t* dst, int64_t num_pairs, void* stream);
+
 /* A layer's pools and head norms, for the entry points below. */
 typedef struct mllm_layer_pool {
   void *k_cache, *v_cache;

@@ -139,6 +139,9 @@ SIGNATURES = {
     "mllm_qk_norm_rope_kv_append": (ctypes.c_int, [_p, _p, _p, _f32, _p]),
     "mllm_qk_norm_rope": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _f32, _i32,
                                          _i32, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "mllm_rotary": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i32, _f32, _i32, _i32,
+                                   _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "mllm_copy_pages": (ctypes.c_int, [_p, _p, _i32, _i64, _p, _p, _i64, _p]),
     "mllm_fp8_linear_workspace_bytes": (ctypes.c_int64, [_i64, _i64, _i64, _i32]),
     "mllm_fp8_linear": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _i64, _p, _p]),
     "mllm_attention_forward_pool": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p,

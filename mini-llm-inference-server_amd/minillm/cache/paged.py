@@ -26,6 +26,11 @@ tokens of a head.
 
 from __future__ import annotations
 
+import struct
+from itertools import chain
+from operator import is_
+
+import numpy as np
 import torch
 
 from .. import _native
@@ -58,6 +63,7 @@ class PagedKVCache:
         self.v = [torch.zeros(shape, device=device, dtype=zeros).view(dtype) for _ in range(config.num_hidden_layers)]
         self.num_blocks = num_blocks
         self.block_size = block_size
+        self._pages: tuple | None = None  # _page_tensors
         self.quantized = dtype == FP8
         if (not self.quantized or self.block_scales) and (k_scale != 1.0 or v_scale != 1.0):
             raise ValueError("k_scale / v_scale apply to fp8 pools only, and not with block_scales")
@@ -108,6 +114,53 @@ class PagedKVCache:
                              slots.data_ptr(), n, _native.dtype_code(dtype), to_k.data_ptr(), to_v.data_ptr())
         return to_k, to_v
 
+    def copy_blocks(self, src, dst) -> None:
+        """Block dst[i] becomes a copy of block src[i], in every layer's K, V and scales: one call on the current stream of the
+        pool's device.  `src` and `dst` are sequences of block ids on the host, of one length.  A block written twice, or read
+        and written, is refused (ValueError), as is one outside the pool; nothing is copied then."""
+        src, dst = _block_ids(src), _block_ids(dst)
+        if src.shape != dst.shape:
+            raise ValueError(f"{src.size} blocks to copy from and {dst.size} to copy to")
+        if not src.size:
+            return
+        device = self.k[0].device
+        if device.type != "cuda":
+            self._copy_on_host(src, dst)
+            return
+        tensors, pointers, nbytes = self._page_tensors()
+        _native.lib().launch(device, "mllm_copy_pages", pointers, nbytes, len(tensors), self.num_blocks, src.ctypes.data,
+                             dst.ctypes.data, src.size)
+
+    def _copy_on_host(self, src: np.ndarray, dst: np.ndarray) -> None:
+        """`copy_blocks` of a pool that is not on a GPU, in torch operations, under the same rules."""
+        for b in np.concatenate([src, dst]):
+            if not 0 <= b < self.num_blocks:
+                raise ValueError(f"block {b} is outside the pool")
+        if np.unique(dst).size != dst.size:
+            raise ValueError("a block is written twice")
+        if np.intersect1d(src, dst).size:
+            raise ValueError("a block is read and written")
+        src, dst = torch.from_numpy(src), torch.from_numpy(dst)
+        for t in self._page_tensors()[0]:
+            raw = t.view(torch.uint8)
+            raw[dst] = raw[src]
+
+    def _page_tensors(self):
+        """Every tensor that holds pages, their addresses and their bytes per page, as arrays mllm_copy_pages reads: made
+        once, and again when an entry of the lists has been replaced."""
+        lists = (self.k, self.v, self.k_scale, self.v_scale) if self.fp4 or self.block_scales else (self.k, self.v)
+        held = self._pages
+        if held is not None and len(held[0]) == sum(map(len, lists)) and all(map(is_, chain(*lists), held[0])):
+            return held
+        tensors = tuple(chain(*lists))
+        for t in tensors:
+            if t.shape[0] != self.num_blocks or not t.is_contiguous() or t.device != self.k[0].device:
+                raise ValueError(f"the pools and their scales must be contiguous, of {self.num_blocks} blocks, on one device")
+        nbytes = [t.numel() * t.element_size() // max(1, self.num_blocks) for t in tensors]
+        self._pages = (tensors, struct.pack(f"{len(tensors)}Q", *(t.data_ptr() for t in tensors)),
+                       struct.pack(f"{len(tensors)}q", *nbytes))
+        return self._pages
+
     @staticmethod
     def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE, block_scales: bool = False) -> int:
         """K and V, every layer: 2 x layers x block_size x KV heads x head_dim x bytes per element (4-bit pools: half a
@@ -126,6 +179,16 @@ class PagedKVCache:
 
     def step(self, meta) -> PagedStep:
         return PagedStep(self, meta)
+
+
+def _block_ids(ids) -> np.ndarray:
+    """A sequence of block ids as one row of int64."""
+    if isinstance(ids, torch.Tensor) and ids.is_cuda:
+        raise ValueError("block ids are taken from the host")
+    ids = np.asarray(ids)
+    if ids.ndim != 1 or ids.size and ids.dtype.kind not in "iu":
+        raise ValueError("block ids must be one row of whole numbers")
+    return np.ascontiguousarray(ids, dtype=np.int64)
 
 
 def _page_scales(num_blocks: int, hkv: int, device) -> torch.Tensor:

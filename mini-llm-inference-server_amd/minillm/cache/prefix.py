@@ -79,6 +79,17 @@ class PrefixCache:
             del self._block_by_name[self._name_by_block[block]]
             self._name_by_block[block] = None
 
+    def move(self, src: int, dst: int) -> None:
+        """The name of block `src`, if it has one, is that of `dst` from now on (its contents have moved)."""
+        if not self.is_cached(src):
+            return
+        name = self._name_by_block[src]
+        self._name_by_block[src] = None
+        if dst >= len(self._name_by_block):
+            self._name_by_block.extend([None] * (dst + 1 - len(self._name_by_block)))
+        self._name_by_block[dst] = name
+        self._block_by_name[name] = dst
+
     def clear(self) -> None:
         """Drops every name.  Only for a cache no block manager is using: a manager keeps counts of the idle
         blocks it parked as named (an engine clears through BlockManager.clear_cache, which drops the names

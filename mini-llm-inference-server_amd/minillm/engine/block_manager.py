@@ -97,6 +97,50 @@ class BlockManager:
             if self._holders[b] == 0:
                 self._park(b, NAMED if self._named(b) else BLANK)
 
+    def fork(self, table: list[int], num_tokens: int, reserve_tokens: int = 0) -> tuple[list[int], list[tuple[int, int]]]:
+        """A second table over the first `num_tokens` tokens of `table`: it shares the full blocks and gets a block of its own
+        for a last one that is not full, with room for `reserve_tokens` in all.  Returns it and the (from, to) blocks to copy
+        (PagedKVCache.copy_blocks) before either table grows."""
+        full = int(num_tokens) // self.block_size
+        used = self.blocks_for(num_tokens)
+        if used > len(table):
+            raise ValueError(f"a table of {len(table)} blocks does not hold {num_tokens} tokens")
+        fresh = self.allocate(max(used, self.blocks_for(reserve_tokens)) - full)  # first: it raises where none are left
+        self.acquire(table[:full])
+        return table[:full] + fresh, [(table[full], fresh[0])] if used > full else []
+
+    def trim(self, table: list[int], num_tokens: int) -> None:
+        """Releases the blocks of `table` behind its first `num_tokens` tokens, in place."""
+        keep = self.blocks_for(num_tokens)
+        if keep < len(table):
+            tail = table[keep:]
+            del table[keep:]
+            self.free(tail)
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Moves every block that holds K/V (held, or named by the prefix cache) into the lowest ids.  Returns the (from, to)
+        blocks to copy (PagedKVCache.copy_blocks): no block is in both roles.  Names, holders and the order of eviction follow;
+        tables that list a moved block are the caller's to rewrite."""
+        live = {b: (tier, t) for t, (tier, b) in self._live()}
+        keeps = [b for b in range(self.num_blocks) if self._holders[b] or live[b][0] == NAMED]
+        gaps = [b for b in range(len(keeps)) if not self._holders[b] and live[b][0] == BLANK]
+        moves = list(zip((b for b in keeps if b >= len(keeps)), gaps))
+        for src, dst in moves:
+            self._holders[dst], self._holders[src] = self._holders[src], 0
+            if self.prefix is not None:
+                self.prefix.move(src, dst)
+            blank, (tier, ticket) = live[dst][1], live.get(src, (BLANK, -1))
+            # an idle named block keeps its place in the order (a held one has none), the gap passes its own on
+            self._ticket[dst], self._ticket[src] = ticket, blank
+            live[src] = (BLANK, blank)
+            if ticket >= 0:
+                live[dst] = (tier, ticket)
+            else:
+                del live[dst]
+        self._heap = [(tier, t, b) for b, (tier, t) in live.items()]
+        heapq.heapify(self._heap)
+        return moves
+
     def clear_cache(self) -> None:
         """Every idle-named block becomes blank (its name dropped), in eviction order."""
         named = sorted((t, b) for t, (tier, b) in self._live() if tier == NAMED)

@@ -180,6 +180,39 @@ class EngineCore:
         if req is not None:
             self._aborted.append(self._final_output(req, [], "abort"))
 
+    def fork(self, req_id: str, new_req_id: str, max_tokens: int | None = None) -> None:
+        """A running request goes on twice from where it stands: a second one, `new_req_id`, with the same prompt and output so
+        far, on the same blocks but for a copy of a last one that is not full.  Its outputs are the tokens after the fork, and
+        num_output_tokens counts those before it too.  `max_tokens` (default: the request's own) counts all of its output.
+        ValueError for a request that does not run or a name that is taken, RuntimeError where no row or block is free."""
+        sched = self.scheduler
+        req = next((r for r in sched.running if r.req_id == req_id), None)
+        if req is None:
+            raise ValueError(f"no running request {req_id!r}")
+        if any(r.req_id == new_req_id for r in (*sched.running, *sched.waiting)):
+            raise ValueError(f"a request {new_req_id!r} is there already")
+        most = req.max_tokens if max_tokens is None else int(max_tokens)
+        if most <= len(req.output):
+            raise ValueError(f"max_tokens {most} leaves none after the {len(req.output)} of the output so far")
+        longest = len(req.prompt) + most
+        if longest > self.max_model_len or self.blocks.blocks_for(longest) > self.blocks.num_blocks:
+            raise ValueError(f"a request of {longest} tokens does not fit max_model_len {self.max_model_len} or the pool of "
+                             f"{self.blocks.num_blocks} KV blocks")
+        _, copies = sched.fork(req, new_req_id, most, {**req.timeline, "forked": now_ns()})
+        self._copy(copies)
+
+    def compact(self) -> int:
+        """Moves every block that holds K/V to the front of the pool and returns their number n: `cache.k[layer][:n]` and the like
+        are then all that the pool holds."""
+        moves = self.blocks.compact()
+        self._copy(moves)
+        self.scheduler.moved(moves)
+        return self.blocks.num_blocks - self.blocks.num_free + self.blocks.num_cached
+
+    def _copy(self, moves: list[tuple[int, int]]) -> None:
+        if moves:
+            self.cache.copy_blocks([a for a, _ in moves], [b for _, b in moves])
+
     # ------------------------------------------------------------------ state
 
     def has_work(self) -> bool:

@@ -239,6 +239,29 @@ class Scheduler:
         self.waiting.appendleft(victim)
         return victim
 
+    # ------------------------------------------------------------------ forks and moved blocks
+
+    def fork(self, req: Request, req_id: str, max_tokens: int, timeline: dict) -> tuple[Request, list[tuple[int, int]]]:
+        """A running request's continuation under a name of its own, on the same blocks but for a last one that is not full,
+        and the (from, to) blocks to copy."""
+        if len(self.running) >= self.max_num_seqs:
+            raise RuntimeError(f"{len(self.running)} requests run already, and at most {self.max_num_seqs} may")
+        waits = req.num_tokens - req.num_cached > 1  # within its prompt: blocks for all of it
+        table, copies = self.blocks.fork(req.block_ids, req.num_cached, req.num_tokens if waits else 0)
+        full = req.num_cached // self.blocks.block_size
+        child = Request(req_id, list(req.prompt), max_tokens, req.stop_ids, timeline, output=list(req.output), block_ids=table,
+                        num_cached=req.num_cached, root=req.root, block_hashes=list(req.block_hashes),
+                        num_named=min(req.num_named, full), num_cached_tokens=req.num_cached_tokens)
+        self.running.append(child)
+        return child, copies
+
+    def moved(self, moves: list[tuple[int, int]]) -> None:
+        """Rewrites the running requests' tables after blocks have moved (as new lists, which are uploaded whole)."""
+        to = dict(moves)
+        for req in self.running:
+            if not to.keys().isdisjoint(req.block_ids):
+                req.block_ids = [to.get(b, b) for b in req.block_ids]
+
     # ------------------------------------------------------------------ leaving
 
     def finish(self, reqs: list[Request]) -> None:

@@ -17,6 +17,9 @@ _REQUIRED_KEYS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_
                   "rms_norm_eps")
 _DEFAULTS = {"tie_word_embeddings": False, "max_position_embeddings": 8192, "qk_norm": False}
 
+# scaling types whose angles the model takes as the reference does; the others go with the positions' kernel
+REFERENCE_SCALING = (None, "llama3")
+
 
 def _rope_fields(d: Mapping[str, Any]) -> tuple[float, dict[str, Any] | None]:
     """(rope_theta, rope_scaling) of a config dictionary.
@@ -61,16 +64,33 @@ class LlamaConfig:
     head_dim: int
     rms_norm_eps: float
     rope_theta: float
-    rope_scaling: dict[str, Any] | None = None  # llama3 frequency scaling, or None for plain RoPE
+    rope_scaling: dict[str, Any] | None = None  # llama3, linear or yarn frequency scaling, or None for plain RoPE
     tie_word_embeddings: bool = False
     max_position_embeddings: int = 8192
     eos_token_ids: tuple[int, ...] = field(default_factory=tuple)
     qk_norm: bool = False  # RMSNorm of every query and key head before the rotation
+    rope_interleaved: bool = False  # pairs (2 i, 2 i + 1) instead of (i, i + half)
+    partial_rotary_factor: float = 1.0  # the part of each head, from its front, that is rotated
 
     @property
     def num_kv_groups(self) -> int:
         """Query heads per KV head."""
         return self.num_attention_heads // self.num_key_value_heads
+
+    @property
+    def rotary_dim(self) -> int:
+        """Dims of a head that are rotated, an even number."""
+        dim = int(self.head_dim * self.partial_rotary_factor)
+        if not 0 < dim <= self.head_dim or dim % 2:
+            raise ValueError(f"partial_rotary_factor {self.partial_rotary_factor} of head_dim {self.head_dim} is {dim} dims: need "
+                             f"an even number of them")
+        return dim
+
+    @property
+    def reference_rope(self) -> bool:
+        """Whether the rotation is the reference's: half-split pairs of whole heads, plain or llama3 frequencies."""
+        return not self.rope_interleaved and self.rotary_dim == self.head_dim \
+            and (self.rope_scaling or {}).get("rope_type") in REFERENCE_SCALING
 
     @classmethod
     def from_dict(cls, d: Mapping[str, Any]) -> LlamaConfig:
@@ -84,6 +104,9 @@ class LlamaConfig:
         kw["num_key_value_heads"] = d.get("num_key_value_heads", heads)  # absent: one KV head per query head
         kw["head_dim"] = d.get("head_dim") or kw["hidden_size"] // heads
         kw["rope_theta"], kw["rope_scaling"] = _rope_fields(d)
+        nested = d.get("rope_parameters") or {}
+        kw["partial_rotary_factor"] = float(nested.get("partial_rotary_factor", d.get("partial_rotary_factor", 1.0)))
+        kw["rope_interleaved"] = bool(d.get("rope_interleaved", d.get("rope_interleave", False)))
         kw["eos_token_ids"] = _eos_ids(d.get("eos_token_id"))
         return cls(**kw)
 

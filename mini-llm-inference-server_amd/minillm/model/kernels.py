@@ -149,6 +149,48 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     return q_out, k_out
 
 
+def rotary_ok(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> bool:
+    """Whether `rotary` takes the model's q (already `usable`), k, positions and frequencies: few enough tokens for one launch."""
+    return (0 < positions.numel() <= MAX_GROUPS and inv_freq.numel() <= 512 and positions.dtype == torch.int64
+            and all(type(x) is torch.Tensor and not _wrapped(x) and x.device == q.device for x in (k, positions, inv_freq)))
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
+           factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """q [B, H, T, Dh] and k [B, Hkv, T, Dh] turned by positions [B, T] (int64) times inv_freq [R / 2] (float32), angles in 64
+    bits: the first R dims of each head in pairs (i, i + R / 2), or (2 i, 2 i + 1) when `interleaved`, scaled by `factor`;
+    dims behind them are copied.  bfloat16 or float16; fp32 arithmetic, one rounding.  Returns [B, H, T, Dh] and
+    [B, Hkv, T, Dh], token by token in memory.  For inference: operands that need a gradient are refused."""
+    b, h, t, dh = q.shape
+    dtype, device, of_k = q.dtype, q.device, k.shape
+    if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh or of_k[1] < 1:
+        raise ValueError(f"k must be [B, Hkv, T, Dh] = [{b}, Hkv, {t}, {dh}] to match q")
+    if positions.shape != (b, t) or positions.dtype != torch.int64:
+        raise ValueError(f"positions must be [B, T] = [{b}, {t}] of int64")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not 0 < 2 * inv_freq.shape[0] <= dh:
+        raise ValueError(f"inv_freq must be one row of float32, one to Dh / 2 = {dh // 2} of them")
+    if not (dtype == k.dtype and device == k.device == positions.device == inv_freq.device):
+        raise ValueError("q and k must share one dtype, and all operands one device")
+    if dtype not in _DTYPES or device.type != "cuda":
+        raise ValueError("q must be bfloat16 or float16 on a GPU")
+    if not math.isfinite(factor):
+        raise ValueError("factor must be finite")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or inv_freq.requires_grad):
+        raise RuntimeError("rotary is for inference: it has no gradient (call it under no_grad)")
+    sq, sk, sp = q.stride(), k.stride(), positions.stride()
+    if sq[3] != 1 or sk[3] != 1:
+        q, k = q.contiguous(), k.contiguous()
+        sq, sk = q.stride(), k.stride()
+    hkv = of_k[1]
+    q_out = torch.empty((b, t, h, dh), dtype=dtype, device=device)
+    k_out = torch.empty((b, t, hkv, dh), dtype=dtype, device=device)
+    _native.lib().launch(device, "mllm_rotary", q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+                         positions.data_ptr(), sp[0], sp[1], inv_freq.contiguous().data_ptr(), inv_freq.shape[0],
+                         bool(interleaved), factor, b, t, h, hkv, dh, _native.dtype_code(dtype), q_out.data_ptr(),
+                         k_out.data_ptr())
+    return q_out.transpose(1, 2), k_out.transpose(1, 2)
+
+
 def sum_ok(x: torch.Tensor, y: torch.Tensor) -> bool:
     return type(y) is torch.Tensor and y.shape == x.shape and _rows_ok(y, x)
 

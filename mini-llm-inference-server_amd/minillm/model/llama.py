@@ -19,7 +19,7 @@ from torch import nn
 from ..attention import AttentionBackend, get_backend
 from . import kernels
 from .config import LlamaConfig
-from .rope import compute_inv_freq
+from .rope import attention_factor, compute_inv_freq, rotate
 
 
 class RMSNorm(nn.Module):
@@ -81,6 +81,9 @@ class LlamaAttention(nn.Module):
         self.k_proj = nn.Linear(d, hkv * dh, bias=False)
         self.v_proj = nn.Linear(d, hkv * dh, bias=False)
         self.o_proj = nn.Linear(h * dh, d, bias=False)
+        # another rotation than the reference's goes by the positions instead of tables (`_turn`)
+        self.by_position = not config.reference_rope
+        self.rope_factor = attention_factor(config)
         # RMSNorm of every query and key head before the rotation (config.qk_norm)
         self.q_norm = RMSNorm(dh, config.rms_norm_eps) if config.qk_norm else None
         self.k_norm = RMSNorm(dh, config.rms_norm_eps) if config.qk_norm else None
@@ -91,7 +94,8 @@ class LlamaAttention(nn.Module):
 
     def attend(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kv_cache=None,
                key_valid: torch.Tensor | None = None) -> torch.Tensor:
-        """The attention output before o_proj, [B, T, H Dh]."""
+        """The attention output before o_proj, [B, T, H Dh].  Where the rotation goes by the positions, cos and sin are the
+        positions [B, T] and the frequencies."""
         b, t, _ = x.shape
         dh = self.config.head_dim
         q_proj, k_proj, v_proj = self.q_proj, self.k_proj, self.v_proj
@@ -104,7 +108,7 @@ class LlamaAttention(nn.Module):
         ragged = getattr(kv_cache, "ragged", False)
         fused_norms = {}
         if getattr(self, "q_norm", None) is not None:
-            if kernels.usable(q) and kernels.head_norms_ok(self.q_norm, self.k_norm, RMSNorm, q, dh):
+            if not self.by_position and kernels.usable(q) and kernels.head_norms_ok(self.q_norm, self.k_norm, RMSNorm, q, dh):
                 norms = (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps)
                 if ragged and getattr(self.backend, "fuse_rotary", False) and b == 1:
                     fused_norms = {"qk_norm": norms}  # in the backend's launch that rotates and appends
@@ -115,10 +119,18 @@ class LlamaAttention(nn.Module):
                 q, k = self.q_norm(q), self.k_norm(k)
         if ragged:
             return self._paged(q, k, v, cos, sin, kv_cache, fused_norms)
-        q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
+        q, k = self._turn(q, k, cos, sin)
         if kv_cache is not None:
             raise ValueError("only paged ragged caches (PagedStep) are supported")
         return self._contiguous(q, k, v, key_valid)
+
+    def _turn(self, q, k, cos, sin):
+        if not self.by_position:
+            return apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
+        form = (self.config.rope_interleaved, self.rope_factor)
+        if kernels.usable(q) and kernels.rotary_ok(q, k, cos, sin):
+            return kernels.rotary(q, k, cos, sin, *form)
+        return rotate(q, cos, sin, *form), rotate(k, cos, sin, *form)
 
     def _contiguous(self, q, k, v, key_valid) -> torch.Tensor:
         b, _, t, _ = q.shape
@@ -131,12 +143,12 @@ class LlamaAttention(nn.Module):
         layer = self.layer_idx
         pools = (kv_cache.cache.k[layer], kv_cache.cache.v[layer], kv_cache.meta)
         scales = kv_cache.cache.scales(layer)  # fp8 and 4-bit pools
-        if getattr(self.backend, "fuse_rotary", False) and b == 1:
+        if getattr(self.backend, "fuse_rotary", False) and b == 1 and not self.by_position:
             # the backend rotates q and k itself, in the launch that appends k and v
             out = self.backend.forward_rotary(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1),
                                               cos[0], sin[0], *pools, **scales, **fused_norms)
         else:
-            q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
+            q, k = self._turn(q, k, cos, sin)
             out = self.backend.forward(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), *pools,
                                        **scales)
         return out.reshape(b, t, -1)
@@ -209,6 +221,7 @@ class LlamaModel(nn.Module):
         self.layers = nn.ModuleList(LlamaDecoderLayer(config, backend, i) for i in range(config.num_hidden_layers))
         self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps)
         self.rotary_emb = RotaryEmbedding(config)
+        self.by_position = not config.reference_rope
 
     def forward(self, input_ids, positions, kv_cache=None, attention_mask=None):
         if kv_cache is not None:
@@ -217,7 +230,10 @@ class LlamaModel(nn.Module):
         else:
             key_valid = None if attention_mask is None else attention_mask.to(torch.bool)
         x = self.embed_tokens(input_ids)
-        cos, sin = self.rotary_emb(positions, x.dtype)  # shared by every layer
+        if self.by_position:
+            cos, sin = positions, self.rotary_emb.inv_freq(x.device)
+        else:
+            cos, sin = self.rotary_emb(positions, x.dtype)  # shared by every layer
         for layer in self.layers:
             x = layer(x, cos, sin, kv_cache, key_valid)
         if kv_cache is not None:
