@@ -560,13 +560,20 @@ int mllm_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, c
  *   t = position * inv_freq[i] in 64 bits,  out[a] = factor * (x[a] cos t - x[b] sin t),  out[b] = factor * (x[b] cos t + x[a] sin t)
  * for i < pairs, with (a, b) = (i, i + pairs), or (2 i, 2 i + 1) when `interleaved`; dims from 2 * pairs on are copied.  fp32
  * arithmetic, one rounding to `dtype`.
- * q [B, H, T, Dh], k [B, Hkv, T, Dh] with element strides (batch, head, token), unit stride in Dh; positions [B, T] with strides
- * (batch, token); inv_freq [pairs] fp32 -> q_out, k_out: contiguous [B, T, heads, Dh].  pairs <= Dh / 2, at most 512.
+ * All rows have unit stride in Dh; other strides are in elements.  pairs <= Dh / 2, at most 512; Dh at most 4096.
  */
-int mllm_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
-                int64_t k_st, const int64_t* positions, int64_t p_sb, int64_t p_st, const float* inv_freq, int32_t pairs,
-                int32_t interleaved, float factor, int32_t batch, int32_t seq, int32_t num_heads, int32_t num_kv_heads,
-                int32_t head_dim, int32_t dtype, void* q_out, void* k_out, void* stream);
+typedef struct mllm_rotary_args {
+  const void *q, *k;                               /* [B, H, T, Dh], [B, Hkv, T, Dh] */
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st;      /* strides: batch, head, token */
+  const int64_t* positions;                        /* [B, T] */
+  int64_t p_sb, p_st;
+  const float* inv_freq;                           /* [pairs] */
+  void *q_out, *k_out;                             /* as q and k, over neither of them */
+  int64_t qo_sb, qo_sh, qo_st, ko_sb, ko_sh, ko_st;
+  float factor;
+  int32_t pairs, interleaved, batch, seq, num_heads, num_kv_heads, head_dim, dtype;
+} mllm_rotary_args;
+int mllm_rotary(const mllm_rotary_args* args, void* stream);
 
 /*
  * Copies of pages within pools (a fork's copy of a last page that is not full, a compaction): page dst[i] of every tensor becomes

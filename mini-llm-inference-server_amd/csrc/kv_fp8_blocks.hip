@@ -12,11 +12,12 @@
 // the same values however its tokens came in, but for those below 2^-6 of the scale, which round twice.  An infinity or a
 // NaN becomes the code of NaN in its own place and takes no part in amax.
 //
-// A wavefront takes a window of 4 W tokens of one head's K or V: 16 lanes hold a token's 128 dims, 16 bytes each, four tokens
-// side by side, W times.  Each token's amax comes from its 16 lanes; runs are merged over the window's tokens in scalar
-// registers.  Tokens of a run outside the window are read for their amax alone, so no wavefront waits for another.  The
-// wavefront of a run's first token writes the scale and rounds the codes before it; the others read the old scale or the new
-// one and get the same maximum from either.
+// A wavefront takes up to 4 W tokens of one head's K or V together: 16 lanes hold a token's 128 dims, 16 bytes each, four tokens
+// side by side, W times.  Each token's amax comes from its 16 lanes; runs are merged over the tokens in scalar registers.
+// Tokens of a run outside these are read for their amax alone, so no wavefront waits for another.  The wavefront of a run's
+// first token writes the scale and rounds the codes before it; the others read the old scale or the new one and get the
+// same maximum from either.  In steps of many tokens and pages of 16, a wavefront takes the runs that begin in its window of 16
+// tokens, whole, so that every row is read once.
 #include "kv_common.h"
 
 namespace mllm {
@@ -64,14 +65,17 @@ __device__ __forceinline__ float sum16(float x) {
   return x + __uint_as_float(dpp<kMirror>(__float_as_uint(x)));
 }
 
-// The largest finite magnitude (pattern) of eight values; `bad`: whether one is not finite.
-template <typename T>
-__device__ __forceinline__ uint32_t finite_max8(u32x4 x, bool& bad) {
+// The largest magnitude (pattern) of eight values, past infinity's for a NaN.
+__device__ __forceinline__ uint32_t max8(u32x4 x) {
   constexpr uint32_t kSign = 0x7fff7fffu;
   const uint32_t m = max_u16x2(max_u16x2(x[0] & kSign, x[1] & kSign), max_u16x2(x[2] & kSign, x[3] & kSign));
-  uint32_t a = max(m & 0xffffu, m >> 16);
-  bad = a >= Fp8Range<T>::inf;
-  if (bad) {
+  return max(m & 0xffffu, m >> 16);
+}
+// The largest finite one.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_max8(u32x4 x) {
+  uint32_t a = max8(x);
+  if (a >= Fp8Range<T>::inf) {
     a = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -103,7 +107,8 @@ __device__ __forceinline__ uint32_t pk4(uint32_t a, uint32_t b, float scale) {
   }
 }
 
-// Eight values -> eight codes of x / 2^(e - 127), to nearest with ties to even, at most 448; not finite: NaN.
+// Eight values -> eight codes of x / 2^(e - 127), to nearest with ties to even, at most 448; not finite (where `bad` says that
+// there may be some): NaN.
 template <typename T>
 __device__ __forceinline__ u32x2 codes8(u32x4 x, int e, bool bad) {
   constexpr uint32_t kTop = Fp8Range<T>::top * 0x10001u;
@@ -199,8 +204,8 @@ __global__ __launch_bounds__(256) void append_fp8_blocks_kernel(const BlocksArgs
   const unsigned per_window = 2u * (unsigned)a.hkv, window = wave / per_window;
   const int hv = (int)(wave - window * per_window), h = hv >> 1;
   const bool is_v = hv & 1;
-  const int64_t t0 = (int64_t)window * (4 * W);
-  if (t0 >= a.n) return;
+  const int64_t t_window = (int64_t)window * (4 * W);
+  if (t_window >= a.n) return;
   const char* src = is_v ? a.v + h * a.v_sh : a.k + h * a.k_sh;
   const int64_t st = is_v ? a.v_st : a.k_st;
   char* codes = (is_v ? a.vc : a.kc) + (int64_t)h * kDh;
@@ -218,94 +223,160 @@ __global__ __launch_bounds__(256) void append_fp8_blocks_kernel(const BlocksArgs
     }
   };
 
-  // the window's tokens: 4 p + j of lanes 16 j ..
-  u32x4 x[W];
-  int64_t slot[W];
-  bool first[W];  // begins a run, or has no slot
-  uint32_t top[W];
-  bool bad[W];
-#pragma unroll
-  for (int p = 0; p < W; ++p) {
-    const int64_t t = t0 + 4 * p + j, at = min(t, (int64_t)a.n - 1);
-    const int64_t s = a.slots[at], before = at > 0 ? a.slots[at - 1] : -1;
-    slot[p] = t < a.n && s >= 0 && s < a.num_slots ? s : -1;
-    first[p] = slot[p] < 0 || before != s - 1 || (s & (a.bs - 1)) == 0;
-    x[p] = row(at);
-  }
-  // tokens before and behind the window on a chain of slots of one page
-  const int64_t last = min(t0 + 4 * W, (int64_t)a.n) - 1;
-  const int64_t s0 = a.slots[t0], sl = a.slots[last];
   const int mask = a.bs - 1;
-  const int64_t tb = t0 - 1 - lane, ta = last + 1 + lane;
-  const bool chain_b = s0 >= 0 && s0 < a.num_slots && lane < (int)(s0 & mask) && tb >= 0 && a.slots[max(tb, (int64_t)0)] == s0 - 1 - lane;
-  const bool chain_a = sl >= 0 && sl < a.num_slots && (int)(sl & mask) + 1 + lane < a.bs && ta < a.n &&
-                       a.slots[min(ta, (int64_t)a.n - 1)] == sl + 1 + lane;
-  const int nb = __builtin_ctzll(~__ballot(chain_b)), na = __builtin_ctzll(~__ballot(chain_a));  // at most bs - 1 of 64 lanes
+  // the first `rows` codes of a page, to a scale 2^d times smaller than theirs
+  auto round_again = [&](int64_t page, int rows, int d) {
+    const float two_d = e8m0_to_f32((uint32_t)max(127 + d, 1));  // what 2^-126 leaves rounds to zero as well
+    for (int r = lane >> 3; r < rows; r += 8) {
+      char* c = codes + ((page << a.bs_shift) + r) * row_bytes + 16 * (lane & 7);
+      u32x4 w = ld16(c);
 #pragma unroll
-  for (int p = 0; p < W; ++p) top[p] = max16(finite_max8<T>(x[p], bad[p]));
-  auto beyond = [&](int64_t from, int count) {
-    uint32_t m = 0;
-    for (int i = 0; i < count; i += 4) {
-      bool b;
-      const uint32_t f = finite_max8<T>(row(from + min(i + j, count - 1)), b);
-      m = max(m, f);
+      for (int i = 0; i < 4; ++i) w[i] = again4(w[i], two_d);
+      st16(c, w);
     }
-    m = max16(m);
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-    return (uint32_t)__builtin_amdgcn_readfirstlane(max(m, (uint32_t)__shfl_xor((int)m, 32, 64)));
   };
-  const uint32_t top_b = nb ? beyond(t0 - nb, nb) : 0u, top_a = na ? beyond(last + 1, na) : 0u;
-
-  // each token's run: its largest magnitude and where it began (relative to t0), over the window's tokens in order
-  uint32_t run[4 * W];
-  int start[4 * W];
-  bool begins[4 * W];
-  uint32_t cur = top_b;
-  int at = -nb;
-#pragma unroll
-  for (int i = 0; i < 4 * W; ++i) {
-    begins[i] = (__ballot(first[i >> 2]) >> (16 * (i & 3))) & 1;
-    const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)top[i >> 2], 16 * (i & 3));
-    at = begins[i] ? i : at;
-    cur = begins[i] ? m : max(cur, m);
-    run[i] = cur;
-    start[i] = at;
+  // The runs that begin in the window: tokens [from, to) of it.  Of 16 tokens on a chain one lies at a page's first slot, so
+  // the next run begins within 16 tokens of the window's end.
+  constexpr bool kWhole = W > 1;
+  const bool whole = kWhole && a.bs == 16;
+  int from = 0, to = 4 * W;
+  uint64_t starts = 0;
+  int64_t its_slot = -1;  // of token t_window + lane
+  if (whole) {
+    const int64_t t = t_window + lane, at = min(t, (int64_t)a.n - 1), s = a.slots[at], s1 = a.slots[max(at - 1, (int64_t)0)];
+    if (t < a.n && s >= 0 && s < a.num_slots) its_slot = s;
+    starts = __ballot(its_slot < 0 || (s & mask) == 0 || t == 0 || s1 != s - 1);
+    if (!(starts & 0xffff)) return;
+    from = __builtin_ctzll(starts);
+    to = 16 + __builtin_ctzll(starts >> 16);
   }
+  while (true) {
+    // up to 16 tokens of whole runs
+    const int count = whole && to - from > 16 ? 63 - __builtin_clzll((starts >> from) & 0x1fffe) : to - from;
+    const int64_t t0 = t_window + from, last = min(t0 + count, (int64_t)a.n) - 1;
+    if (t0 >= a.n) return;
+    if (whole && __builtin_popcountll((starts >> from) & (~0ull >> (64 - count))) == 1) {  // one run: what prompts are made of
+      const int64_t s0 = ((int64_t)__builtin_amdgcn_readlane((int)(its_slot >> 32), from) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)its_slot, from);
+      if (s0 >= 0) {
+        u32x4 x[W];
+        const int64_t page = s0 >> a.bs_shift;
+        const int before = (int)(s0 & mask);
+        int old = 0;
+        if (before) old = scales[page * a.hkv];
 #pragma unroll
-  for (int i = 4 * W - 1; i >= 0; --i) {
-    if (t0 + i == last) run[i] = max(run[i], top_a);  // (tokens past the last have no slot)
-    if (i + 1 < 4 * W && !begins[i + 1]) run[i] = run[i + 1];
-  }
-
+        for (int p = 0; p < W; ++p) {
+          const int i = 4 * p + j;
+          x[p] = u32x4{0, 0, 0, 0};
+          if (4 * p < count) x[p] = row(t0 + min(i, count - 1));
+        }
+        uint32_t m = 0;
 #pragma unroll
-  for (int p = 0; p < W; ++p) {
-    const uint32_t m = j == 0 ? run[4 * p] : (j == 1 ? run[4 * p + 1] : (j == 2 ? run[4 * p + 2] : run[4 * p + 3]));
-    const int s = j == 0 ? start[4 * p] : (j == 1 ? start[4 * p + 1] : (j == 2 ? start[4 * p + 2] : start[4 * p + 3]));
-    const bool in = slot[p] >= 0;
-    const int64_t at_slot = in ? slot[p] : 0, page = at_slot >> a.bs_shift;
-    const int before = (int)(at_slot & mask) - (4 * p + j - s);  // slots of the page before the run
-    int e = block_exp8<T>(m), old = e;
-    if (in && before > 0) {
-      old = scales[page * a.hkv];
-      e = max(e, old);
+        for (int p = 0; p < W; ++p) m = max(m, max8(x[p]));
+        const bool bad = __any(m >= Fp8Range<T>::inf);
+        if (bad) {
+          m = 0;
+#pragma unroll
+          for (int p = 0; p < W; ++p) m = max(m, finite_max8<T>(x[p]));
+        }
+        m = max16(m);
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        const int e = before ? max(block_exp8<T>(m), __builtin_amdgcn_readfirstlane(old)) : block_exp8<T>(m);
+        char* to_codes = codes + (s0 + j) * row_bytes + 8 * ln;
+#pragma unroll
+        for (int p = 0; p < W; ++p)
+          if (4 * p + j < count) st8(to_codes + 4 * p * row_bytes, codes8<T>(x[p], e, bad));
+        if (lane == 0) scales[page * a.hkv] = (uint8_t)e;
+        if (before && e > old) round_again(page, before, old - e);
+      }
+      from += count;
+      if (from >= to) return;
+      continue;
     }
-    const bool owner = in && first[p];
-    if (in) st8(codes + at_slot * row_bytes + 8 * ln, codes8<T>(x[p], e, bad[p]));
-    if (owner && ln == 0 && (before == 0 || e != old)) scales[page * a.hkv] = (uint8_t)e;
-    for (uint64_t grow = __ballot(owner && ln == 0 && e > old); grow; grow &= grow - 1) {
-      const int from = __builtin_ctzll(grow);
-      const int64_t pg = (int64_t)__builtin_amdgcn_readlane((int)page, from);
-      const int rows = __builtin_amdgcn_readlane(before, from);
-      const int d = 127 + __builtin_amdgcn_readlane(old - e, from);
-      const float two_d = e8m0_to_f32((uint32_t)max(d, 1));  // what 2^-126 leaves rounds to zero as well
-      for (int r = lane >> 3; r < rows; r += 8) {
-        char* c = codes + ((pg << a.bs_shift) + r) * row_bytes + 16 * (lane & 7);
-        u32x4 w = ld16(c);
+    // the tokens: t0 + 4 p + j of lanes 16 j ..
+    u32x4 x[W];
+    int64_t slot[W];
+    bool first[W];  // begins a run, or has no slot
+    uint32_t top[W];
+    bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = again4(w[i], two_d);
-        st16(c, w);
+    for (int p = 0; p < W; ++p) {
+      const int64_t t = t0 + 4 * p + j, at = min(t, last);
+      const int64_t s = a.slots[at], before = at > 0 ? a.slots[at - 1] : -1;
+      slot[p] = t <= last && s >= 0 && s < a.num_slots ? s : -1;
+      first[p] = slot[p] < 0 || before != s - 1 || (s & (a.bs - 1)) == 0;
+      x[p] = row(at);
+    }
+    // tokens before and behind these on a chain of slots of one page
+    const int64_t s0 = a.slots[t0], sl = a.slots[last];
+    const int64_t tb = t0 - 1 - lane, ta = last + 1 + lane;
+    const bool chain_b = s0 >= 0 && s0 < a.num_slots && lane < (int)(s0 & mask) && tb >= 0 && a.slots[max(tb, (int64_t)0)] == s0 - 1 - lane;
+    const bool chain_a = sl >= 0 && sl < a.num_slots && (int)(sl & mask) + 1 + lane < a.bs && ta < a.n &&
+                         a.slots[min(ta, (int64_t)a.n - 1)] == sl + 1 + lane;
+    const int nb = __builtin_ctzll(~__ballot(chain_b)), na = __builtin_ctzll(~__ballot(chain_a));  // at most bs - 1 of 64 lanes
+#pragma unroll
+    for (int p = 0; p < W; ++p) {
+      const uint32_t f = finite_max8<T>(x[p]);
+      bad |= f != max8(x[p]);
+      top[p] = max16(f);
+    }
+    bad = __any(bad);
+    auto beyond = [&](int64_t at, int n) {
+      uint32_t m = 0;
+      for (int i = 0; i < n; i += 4) {
+        m = max(m, finite_max8<T>(row(at + min(i + j, n - 1))));
+      }
+      m = max16(m);
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+      return (uint32_t)__builtin_amdgcn_readfirstlane(max(m, (uint32_t)__shfl_xor((int)m, 32, 64)));
+    };
+    const uint32_t top_b = nb ? beyond(t0 - nb, nb) : 0u, top_a = na ? beyond(last + 1, na) : 0u;
+
+    // each token's run: its largest magnitude and where it began (relative to t0), over the tokens in order
+    uint32_t run[4 * W];
+    int start[4 * W];
+    bool begins[4 * W];
+    uint32_t cur = top_b;
+    int at = -nb;
+#pragma unroll
+    for (int i = 0; i < 4 * W; ++i) {
+      begins[i] = (__ballot(first[i >> 2]) >> (16 * (i & 3))) & 1;
+      const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)top[i >> 2], 16 * (i & 3));
+      at = begins[i] ? i : at;
+      cur = begins[i] ? m : max(cur, m);
+      run[i] = cur;
+      start[i] = at;
+    }
+#pragma unroll
+    for (int i = 4 * W - 1; i >= 0; --i) {
+      if (t0 + i == last) run[i] = max(run[i], top_a);  // (tokens past the last have no slot)
+      if (i + 1 < 4 * W && !begins[i + 1]) run[i] = run[i + 1];
+    }
+
+#pragma unroll
+    for (int p = 0; p < W; ++p) {
+      const uint32_t m = j == 0 ? run[4 * p] : (j == 1 ? run[4 * p + 1] : (j == 2 ? run[4 * p + 2] : run[4 * p + 3]));
+      const int s = j == 0 ? start[4 * p] : (j == 1 ? start[4 * p + 1] : (j == 2 ? start[4 * p + 2] : start[4 * p + 3]));
+      const bool in = slot[p] >= 0;
+      const int64_t at_slot = in ? slot[p] : 0, page = at_slot >> a.bs_shift;
+      const int before = (int)(at_slot & mask) - (4 * p + j - s);  // slots of the page before the run
+      int e = block_exp8<T>(m), old = e;
+      if (in && before > 0) {
+        old = scales[page * a.hkv];
+        e = max(e, old);
+      }
+      const bool owner = in && first[p];
+      if (in) st8(codes + at_slot * row_bytes + 8 * ln, codes8<T>(x[p], e, bad));
+      if (owner && ln == 0 && (before == 0 || e != old)) scales[page * a.hkv] = (uint8_t)e;
+      for (uint64_t grow = __ballot(owner && ln == 0 && e > old); grow; grow &= grow - 1) {
+        const int of = __builtin_ctzll(grow);
+        round_again(__builtin_amdgcn_readlane((int)page, of), __builtin_amdgcn_readlane(before, of),
+                    __builtin_amdgcn_readlane(old - e, of));
       }
     }
+    from += count;
+    if (!whole || from >= to) return;
   }
 }
 

@@ -5,8 +5,8 @@
 // are copied.  Angles are products in 64 bits, reduced to a part of a turn there: in 32 bits a position of 10^6 is off by
 // up to 0.06 rad.  The rest is fp32 with one rounding at the end.
 //
-// A workgroup takes a few tokens: it computes their cosines and sines once, into LDS, and turns all heads' rows with them.  Bound
-// by memory: each row is read once and written once.
+// Each thread takes one piece of a row, its workgroup the cosines and sines of the tokens that its pieces lie in, once, through
+// LDS, while the rows are on their way.  Bound by memory: each row is read once and written once.
 #include "kv_common.h"
 
 namespace mllm {
@@ -19,12 +19,16 @@ struct RotaryArgs {
   int64_t p_sb, p_st;
   const float* inv_freq;
   float factor;
-  char *q_out, *k_out;  // [B, T, heads, Dh], contiguous
+  char *q_out, *k_out;
+  int64_t qo_sb, qo_st, qo_sh, ko_sb, ko_st, ko_sh;
   unsigned tokens, T;
-  int H, Hkv, dh, half, per_group;  // half: pairs; per_group: tokens of a workgroup
+  int H, Hkv, dh, half;  // half: pairs
 };
 
-constexpr int kMaxPairs = 512;  // of a workgroup's tokens together
+constexpr int kMaxPairs = 512;
+// Cosines a workgroup may need: those of the tokens that 256 pieces lie in.  Two heads at least, a piece turns eight pairs at most:
+// whole tokens take 4 pairs a piece, and the first and the last may be cut.
+constexpr int kTable = 4 * 256 + 2 * kMaxPairs;
 
 template <typename T, int VEC>
 struct Vals {
@@ -50,71 +54,75 @@ struct Vals {
 // VEC 8: 16-byte pieces; 1: element by element, for other alignments and dims.
 template <typename T, bool INTER, int VEC>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
-  __shared__ __attribute__((aligned(16))) float cs[kMaxPairs], sn[kMaxPairs];
-  const unsigned t0 = blockIdx.x * (unsigned)a.per_group;
-  const unsigned n = min((unsigned)a.per_group, a.tokens - t0);
-  for (unsigned i = threadIdx.x; i < n * (unsigned)a.half; i += 256) {
-    const unsigned u = i / (unsigned)a.half, d = i - u * (unsigned)a.half, t = t0 + u, b = t / a.T;
-    const double turns = (double)a.positions[b * a.p_sb + (t - b * a.T) * a.p_st] * (double)a.inv_freq[d] * 0.15915494309189535;
-    const float part = (float)(turns - __builtin_rint(turns));  // of a turn, as v_sin and v_cos take it
-    cs[i] = a.factor * __builtin_amdgcn_cosf(part);
-    sn[i] = a.factor * __builtin_amdgcn_sinf(part);
-  }
-  __syncthreads();
-  // items of a head: the turned pieces (with their partners, where those lie apart), then the copied ones
+  __shared__ __attribute__((aligned(16))) float cs[kTable], sn[kTable];
+  // pieces of a head: the turned ones (with their partners, where those lie apart), then the copied ones
   const unsigned turned = (unsigned)(INTER ? 2 * a.half / (VEC == 1 ? 2 : VEC) : a.half / VEC);
-  const unsigned per_head = turned + (unsigned)(a.dh - 2 * a.half) / VEC, heads = (unsigned)(a.H + a.Hkv);
-  const unsigned per_token = per_head * heads;
-  for (unsigned i = threadIdx.x; i < n * per_token; i += 256) {
-    const unsigned u = i / per_token, r = i - u * per_token, head = r / per_head, it = r - head * per_head;
-    const unsigned t = t0 + u, b = t / a.T;
+  const unsigned per_head = turned + (unsigned)(a.dh - 2 * a.half) / VEC, per_token = per_head * (unsigned)(a.H + a.Hkv);
+  const uint64_t first = (uint64_t)blockIdx.x * 256u;
+  const unsigned t0 = (unsigned)(first / per_token), r0 = (unsigned)(first - (uint64_t)t0 * per_token);  // its first token and piece of it
+  const unsigned i = r0 + threadIdx.x, u = i / per_token, r = i - u * per_token, head = r / per_head, it = r - head * per_head;
+  const unsigned t = t0 + u;
+  const bool in = t < a.tokens, copied = it >= turned;
+  constexpr bool kTwo = !(INTER && VEC == 8);  // a piece's partner is a piece of its own
+  Vals<T, VEC> x, y;
+  char* dst = nullptr;
+  if (in) {
+    const unsigned b = t / a.T;
     const int64_t tt = t - b * a.T;
     const bool is_q = head < (unsigned)a.H;
     const int64_t h = is_q ? head : head - (unsigned)a.H;
-    const char* src = is_q ? a.q + b * a.q_sb + tt * a.q_st + h * a.q_sh : a.k + b * a.k_sb + tt * a.k_st + h * a.k_sh;
-    char* dst = (is_q ? a.q_out + ((int64_t)t * a.H + h) * a.dh * 2 : a.k_out + ((int64_t)t * a.Hkv + h) * a.dh * 2);
-    Vals<T, VEC> x, y;
-    if (it >= turned) {
-      const unsigned at = 2 * (2 * a.half + (it - turned) * VEC);
-      x.load(src + at);
-      x.store(dst + at);
-      continue;
-    }
-    const float *c = cs + u * a.half, *s = sn + u * a.half;
-    if constexpr (INTER && VEC == 8) {
-      x.load(src + 16 * it);
+    const unsigned lo = 2 * (copied ? 2 * a.half + (it - turned) * VEC : (INTER && VEC == 1 ? 2 * it : it * VEC));
+    const char* src = (is_q ? a.q + b * a.q_sb + tt * a.q_st + h * a.q_sh : a.k + b * a.k_sb + tt * a.k_st + h * a.k_sh) + lo;
+    dst = (is_q ? a.q_out + b * a.qo_sb + tt * a.qo_st + h * a.qo_sh : a.k_out + b * a.ko_sb + tt * a.ko_st + h * a.ko_sh) + lo;
+    x.load(src);
+    if (kTwo && !copied) y.load(src + 2 * (INTER ? 1 : a.half));
+  }
+  const unsigned n = min((r0 + 255) / per_token + 1, a.tokens - t0);  // tokens of this workgroup
+  for (unsigned c = threadIdx.x; c < n * (unsigned)a.half; c += 256) {
+    const unsigned w = c / (unsigned)a.half, d = c - w * (unsigned)a.half, tok = t0 + w, b = tok / a.T;
+    const double turns = (double)a.positions[b * a.p_sb + (tok - b * a.T) * a.p_st] * (double)a.inv_freq[d] * 0.15915494309189535;
+    const float part = (float)(turns - __builtin_rint(turns));  // of a turn, as v_sin and v_cos take it
+    cs[c] = a.factor * __builtin_amdgcn_cosf(part);
+    sn[c] = a.factor * __builtin_amdgcn_sinf(part);
+  }
+  __syncthreads();
+  if (!in) return;
+  if (copied) {
+    x.store(dst);
+    return;
+  }
+  const unsigned at = u * (unsigned)a.half + it * (INTER && VEC == 8 ? 4 : VEC);
+  const float *c = cs + at, *s = sn + at;
+  if constexpr (!kTwo) {
+    Vals<T, VEC> z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float cc = c[4 * it + e], ss = s[4 * it + e];
-        y.f[2 * e] = x.f[2 * e] * cc - x.f[2 * e + 1] * ss;
-        y.f[2 * e + 1] = x.f[2 * e + 1] * cc + x.f[2 * e] * ss;
-      }
-      y.store(dst + 16 * it);
-    } else {
-      const unsigned lo = 2 * (INTER ? 2 * it : it * VEC), hi = lo + 2 * (unsigned)(INTER ? 1 : a.half);
-      x.load(src + lo);
-      y.load(src + hi);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float cc = c[it * VEC + e], ss = s[it * VEC + e], p = x.f[e], q = y.f[e];
-        x.f[e] = p * cc - q * ss;
-        y.f[e] = q * cc + p * ss;
-      }
-      x.store(dst + lo);
-      y.store(dst + hi);
+    for (int e = 0; e < 4; ++e) {
+      z.f[2 * e] = x.f[2 * e] * c[e] - x.f[2 * e + 1] * s[e];
+      z.f[2 * e + 1] = x.f[2 * e + 1] * c[e] + x.f[2 * e] * s[e];
     }
+    z.store(dst);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float p = x.f[e], q = y.f[e];
+      x.f[e] = p * c[e] - q * s[e];
+      y.f[e] = q * c[e] + p * s[e];
+    }
+    x.store(dst);
+    y.store(dst + 2 * (INTER ? 1 : a.half));
   }
 }
 
 }  // namespace
 }  // namespace mllm
 
-extern "C" int mllm_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
-                           int64_t k_st, const int64_t* positions, int64_t p_sb, int64_t p_st, const float* inv_freq,
-                           int32_t pairs, int32_t interleaved, float factor, int32_t batch, int32_t seq, int32_t num_heads,
-                           int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void* q_out, void* k_out, void* stream) {
+extern "C" int mllm_rotary(const mllm_rotary_args* args, void* stream) {
   using namespace mllm;
   const std::string fn = "mllm_rotary";
+  MLLM_REQUIRE(args, MLLM_ERR_INVALID, fn + ": null arguments");
+  const mllm_rotary_args& r = *args;
+  const int32_t batch = r.batch, seq = r.seq, num_heads = r.num_heads, num_kv_heads = r.num_kv_heads, head_dim = r.head_dim;
+  const int32_t pairs = r.pairs, dtype = r.dtype;
   MLLM_REQUIRE(dtype == MLLM_DTYPE_BF16 || dtype == MLLM_DTYPE_F16, MLLM_ERR_UNSUPPORTED,
                fn + ": dtype must be bfloat16 or float16");
   const int64_t tokens = (int64_t)batch * seq;
@@ -124,26 +132,25 @@ extern "C" int mllm_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_
   MLLM_REQUIRE(pairs > 0 && 2 * (int64_t)pairs <= head_dim, MLLM_ERR_INVALID, fn + ": at most head_dim / 2 pairs, and one at least");
   MLLM_REQUIRE(pairs <= kMaxPairs && head_dim <= 4096, MLLM_ERR_UNSUPPORTED, fn + ": head too long");
   if (tokens == 0) return MLLM_OK;
-  MLLM_REQUIRE(q && k && positions && inv_freq && q_out && k_out, MLLM_ERR_INVALID, fn + ": null pointer");
-  MLLM_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out) % 2 == 0, MLLM_ERR_UNSUPPORTED,
-               fn + ": misaligned");
+  MLLM_REQUIRE(r.q && r.k && r.positions && r.inv_freq && r.q_out && r.k_out, MLLM_ERR_INVALID, fn + ": null pointer");
+  const uintptr_t ptrs = (uintptr_t)r.q | (uintptr_t)r.k | (uintptr_t)r.q_out | (uintptr_t)r.k_out;
+  MLLM_REQUIRE(ptrs % 2 == 0, MLLM_ERR_UNSUPPORTED, fn + ": misaligned");
   RotaryArgs a{};
-  a.q = (const char*)q, a.q_sb = 2 * q_sb, a.q_st = 2 * q_st, a.q_sh = 2 * q_sh;
-  a.k = (const char*)k, a.k_sb = 2 * k_sb, a.k_st = 2 * k_st, a.k_sh = 2 * k_sh;
-  a.positions = positions, a.p_sb = p_sb, a.p_st = p_st;
-  a.inv_freq = inv_freq, a.factor = factor;
-  a.q_out = (char*)q_out, a.k_out = (char*)k_out;
+  a.q = (const char*)r.q, a.q_sb = 2 * r.q_sb, a.q_st = 2 * r.q_st, a.q_sh = 2 * r.q_sh;
+  a.k = (const char*)r.k, a.k_sb = 2 * r.k_sb, a.k_st = 2 * r.k_st, a.k_sh = 2 * r.k_sh;
+  a.positions = r.positions, a.p_sb = r.p_sb, a.p_st = r.p_st;
+  a.inv_freq = r.inv_freq, a.factor = r.factor;
+  a.q_out = (char*)r.q_out, a.qo_sb = 2 * r.qo_sb, a.qo_st = 2 * r.qo_st, a.qo_sh = 2 * r.qo_sh;
+  a.k_out = (char*)r.k_out, a.ko_sb = 2 * r.ko_sb, a.ko_st = 2 * r.ko_st, a.ko_sh = 2 * r.ko_sh;
   a.tokens = (unsigned)tokens, a.T = (unsigned)seq;
   a.H = num_heads, a.Hkv = num_kv_heads, a.dh = head_dim, a.half = pairs;
-  // several tokens to a workgroup once that leaves each CU workgroups to overlap
-  int per = 1;
-  while (per < 4 && 2 * per * pairs <= kMaxPairs && tokens >= 8ll * device_cus() * 2 * per) per *= 2;
-  a.per_group = per;
-  const int64_t groups = (tokens + per - 1) / per;
+  const int64_t strides = r.q_sb | r.q_sh | r.q_st | r.k_sb | r.k_sh | r.k_st | r.qo_sb | r.qo_sh | r.qo_st | r.ko_sb | r.ko_sh | r.ko_st;
+  const bool whole = (r.interleaved ? 2 * pairs : pairs) % 8 == 0 && (head_dim - 2 * pairs) % 8 == 0 && ptrs % 16 == 0 &&
+                     strides % 8 == 0;
+  const int vec = whole ? 8 : 1, turned = r.interleaved ? 2 * pairs / (vec == 1 ? 2 : vec) : pairs / vec;
+  const int64_t per_token = (int64_t)(turned + (head_dim - 2 * pairs) / vec) * (num_heads + num_kv_heads);
+  const int64_t groups = (tokens * per_token + 255) / 256;
   MLLM_REQUIRE(groups <= kMaxGroups256, MLLM_ERR_UNSUPPORTED, fn + ": too many tokens");
-  const bool whole = (interleaved ? 2 * pairs : pairs) % 8 == 0 && (head_dim - 2 * pairs) % 8 == 0 &&
-                     ((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out) % 16 == 0 &&
-                     (q_sb | q_sh | q_st | k_sb | k_sh | k_st) % 8 == 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   auto launch = [&](auto tag, auto inter) {
     using T = decltype(tag);
@@ -154,7 +161,7 @@ extern "C" int mllm_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_
       rotary_kernel<T, INTER, 1><<<(unsigned)groups, 256, 0, st>>>(a);
   };
   auto of_type = [&](auto tag) {
-    if (interleaved)
+    if (r.interleaved)
       launch(tag, std::true_type{});
     else
       launch(tag, std::false_type{});

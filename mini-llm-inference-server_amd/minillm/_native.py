@@ -56,6 +56,16 @@ class LayerPool(ctypes.Structure):
                 ("v_scale", _f32), ("q_norm", _p), ("k_norm", _p), ("norm_eps", _f32)]
 
 
+class RotaryArgs(ctypes.Structure):
+    """mllm_rotary_args: the arguments of mllm_rotary."""
+
+    _fields_ = [("q", _p), ("k", _p), ("q_sb", _i64), ("q_sh", _i64), ("q_st", _i64), ("k_sb", _i64), ("k_sh", _i64),
+                ("k_st", _i64), ("positions", _p), ("p_sb", _i64), ("p_st", _i64), ("inv_freq", _p), ("q_out", _p),
+                ("k_out", _p), ("qo_sb", _i64), ("qo_sh", _i64), ("qo_st", _i64), ("ko_sb", _i64), ("ko_sh", _i64),
+                ("ko_st", _i64), ("factor", _f32), ("pairs", _i32), ("interleaved", _i32), ("batch", _i32), ("seq", _i32),
+                ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
+
+
 def packer(cls):
     """bytes of a struct from all its fields in order, in a quarter of the time a ctypes.Structure takes; a call takes them
     where it takes the struct's address."""
@@ -67,6 +77,7 @@ def packer(cls):
 
 pack_rope_append = packer(RopeAppend)
 pack_layer_pool = packer(LayerPool)
+pack_rotary = packer(RotaryArgs)
 
 
 # symbol -> (restype, argtypes); the exact list include/minillm_hip.h declares
@@ -139,8 +150,7 @@ SIGNATURES = {
     "mllm_qk_norm_rope_kv_append": (ctypes.c_int, [_p, _p, _p, _f32, _p]),
     "mllm_qk_norm_rope": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _f32, _i32,
                                          _i32, _i32, _i32, _i32, _i32, _p, _p, _p]),
-    "mllm_rotary": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i32, _f32, _i32, _i32,
-                                   _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "mllm_rotary": (ctypes.c_int, [_p, _p]),
     "mllm_copy_pages": (ctypes.c_int, [_p, _p, _i32, _i64, _p, _p, _i64, _p]),
     "mllm_fp8_linear_workspace_bytes": (ctypes.c_int64, [_i64, _i64, _i64, _i32]),
     "mllm_fp8_linear": (ctypes.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _i64, _p, _p]),

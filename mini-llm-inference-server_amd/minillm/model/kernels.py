@@ -159,8 +159,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
            factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """q [B, H, T, Dh] and k [B, Hkv, T, Dh] turned by positions [B, T] (int64) times inv_freq [R / 2] (float32), angles in 64
     bits: the first R dims of each head in pairs (i, i + R / 2), or (2 i, 2 i + 1) when `interleaved`, scaled by `factor`;
-    dims behind them are copied.  bfloat16 or float16; fp32 arithmetic, one rounding.  Returns [B, H, T, Dh] and
-    [B, Hkv, T, Dh], token by token in memory.  For inference: operands that need a gradient are refused."""
+    dims behind them are copied.  bfloat16 or float16; fp32 arithmetic, one rounding.  The results have the operands' shapes
+    and their order in memory, densely.  For inference: operands that need a gradient are refused."""
     b, h, t, dh = q.shape
     dtype, device, of_k = q.dtype, q.device, k.shape
     if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh or of_k[1] < 1:
@@ -181,14 +181,20 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     if sq[3] != 1 or sk[3] != 1:
         q, k = q.contiguous(), k.contiguous()
         sq, sk = q.stride(), k.stride()
-    hkv = of_k[1]
-    q_out = torch.empty((b, t, h, dh), dtype=dtype, device=device)
-    k_out = torch.empty((b, t, hkv, dh), dtype=dtype, device=device)
-    _native.lib().launch(device, "mllm_rotary", q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
-                         positions.data_ptr(), sp[0], sp[1], inv_freq.contiguous().data_ptr(), inv_freq.shape[0],
-                         bool(interleaved), factor, b, t, h, hkv, dh, _native.dtype_code(dtype), q_out.data_ptr(),
-                         k_out.data_ptr())
-    return q_out.transpose(1, 2), k_out.transpose(1, 2)
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    so, sko = q_out.stride(), k_out.stride()
+    if so[3] != 1 or sko[3] != 1:  # of expanded operands
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        so, sko = q_out.stride(), k_out.stride()
+    args = _native.pack_rotary(  # the fields of mllm_rotary_args in order
+        q.data_ptr(), k.data_ptr(), *sq[:3], *sk[:3], positions.data_ptr(), *sp, inv_freq.data_ptr(), q_out.data_ptr(),
+        k_out.data_ptr(), *so[:3], *sko[:3], factor, inv_freq.shape[0], interleaved, b, t, h, of_k[1], dh,
+        _native.dtype_code(dtype))
+    _native.lib().launch(device, "mllm_rotary", args)
+    return q_out, k_out
 
 
 def sum_ok(x: torch.Tensor, y: torch.Tensor) -> bool:

@@ -1,8 +1,10 @@
 """What long-lived sequences need, without a GPU: 8-bit pools with block scales, copies of pages, forks and compactions, the
 rotary forms.  Sizes, host rules and refusals."""
 
+import ctypes
 import math
 import random
+from pathlib import Path
 
 import pytest
 import torch
@@ -373,7 +375,11 @@ def test_rotary_refusals():
     lib, a = _native.lib(), 1 << 20
 
     def call(q=a, pairs=64, b=1, t=1, h=4, dh=128, dtype=2, pos=a):
-        lib.call("mllm_rotary", q, 512, 128, 512, a, 256, 128, 256, pos, 1, 1, a, pairs, 0, 1.0, b, t, h, 2, dh, dtype, a, a, None)
+        args = _native.RotaryArgs(q=q, k=a, q_sb=512, q_sh=128, q_st=512, k_sb=256, k_sh=128, k_st=256, positions=pos, p_sb=1, p_st=1,
+                                  inv_freq=a, q_out=a, k_out=a, qo_sb=512, qo_sh=128, qo_st=512, ko_sb=256, ko_sh=128, ko_st=256,
+                                  factor=1.0, pairs=pairs, interleaved=0, batch=b, seq=t, num_heads=h, num_kv_heads=2, head_dim=dh,
+                                  dtype=dtype)
+        lib.call("mllm_rotary", ctypes.addressof(args), None)
 
     for kw, match in ((dict(dtype=0), "dtype"), (dict(t=-1), "sizes"), (dict(h=0), "sizes"), (dict(pairs=65), "pairs"),
                       (dict(pairs=0), "pairs"), (dict(pairs=513, dh=2048), "too long"), (dict(dh=8192), "too long"),
@@ -382,6 +388,22 @@ def test_rotary_refusals():
         with pytest.raises(ValueError, match=match):
             call(**kw)
     call(t=0, q=None)
+    with pytest.raises(ValueError, match="null arguments"):
+        lib.call("mllm_rotary", None, None)
+
+
+def test_rotary_args_match_the_header(tmp_path):
+    import subprocess
+
+    fields = [name for name, _ in _native.RotaryArgs._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "minillm_hip.h"\nint main(void) {\n'
+                   + 'printf("%zu\\n", sizeof(mllm_rotary_args));\n'
+                   + "".join(f'printf("%zu\\n", offsetof(mllm_rotary_args, {f}));\n' for f in fields) + "return 0;\n}\n")
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", "-std=c99", f"-I{include}", str(src), "-o", str(tmp_path / "layout")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(_native.RotaryArgs)] + [getattr(_native.RotaryArgs, f).offset for f in fields]
 
 
 @pytest.mark.parametrize("kw", [dict(rope_interleaved=True), dict(partial_rotary_factor=0.5),
