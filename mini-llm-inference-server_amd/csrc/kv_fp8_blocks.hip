@@ -12,12 +12,11 @@
 // the same values however its tokens came in, but for those below 2^-6 of the scale, which round twice.  An infinity or a
 // NaN becomes the code of NaN in its own place and takes no part in amax.
 //
-// A wavefront takes up to 4 W tokens of one head's K or V together: 16 lanes hold a token's 128 dims, 16 bytes each, four tokens
-// side by side, W times.  Each token's amax comes from its 16 lanes; runs are merged over the tokens in scalar registers.
-// Tokens of a run outside these are read for their amax alone, so no wavefront waits for another.  The wavefront of a run's
-// first token writes the scale and rounds the codes before it; the others read the old scale or the new one and get the
-// same maximum from either.  In steps of many tokens and pages of 16, a wavefront takes the runs that begin in its window of 16
-// tokens, whole, so that every row is read once.
+// A wavefront takes a few tokens of one head's K or V: 16 lanes hold a token's 128 dims, 16 bytes each, four tokens side by
+// side.  In steps of many tokens it takes the runs that begin in its window of 16 tokens, whole: a page's 16 tokens stay in
+// registers between their amax and their codes.  In small steps it takes four tokens (four decode rows at once) and reads what
+// else their runs hold for its amax alone, so no wavefront waits for another.  The wavefront of a run's first token writes
+// the scale and rounds the codes before it; the others read the old scale or the new one and get the same maximum from either.
 #include "kv_common.h"
 
 namespace mllm {
@@ -188,7 +187,147 @@ __device__ __forceinline__ u32x4 turned(u32x4 x, const char* cr, const char* sr,
   return o.v;
 }
 
-template <typename T, int FORM, int W>
+// One head's K or V of a pool, and its rows of the step, as a wavefront (lanes 16 j + ln) goes through them.
+template <typename T, int FORM>
+struct Appender {
+  const BlocksArgs& a;
+  const char* src;
+  int64_t st;
+  char* codes;
+  uint8_t* scales;
+  int64_t row_bytes;
+  int lane, ln, j, mask;
+  bool is_v;
+
+  __device__ __forceinline__ Appender(const BlocksArgs& args, int h, bool v, int l)
+      : a(args), src(v ? args.v + h * args.v_sh : args.k + h * args.k_sh), st(v ? args.v_st : args.k_st),
+        codes((v ? args.vc : args.kc) + (int64_t)h * kDh), scales((v ? args.vs : args.ks) + h), row_bytes((int64_t)args.hkv * kDh),
+        lane(l), ln(l & 15), j(l >> 4), mask(args.bs - 1), is_v(v) {}
+
+  // lane ln's part of token t's row, as it goes into the pool
+  __device__ __forceinline__ u32x4 row(int64_t t) const {
+    const u32x4 x = ld16(src + t * st + 16 * ln);
+    if constexpr (FORM == kPlain) {
+      return x;
+    } else {
+      if (is_v) return x;
+      return turned<T, FORM == kPlain ? kRope : FORM>(x, a.cos + t * a.cs_st, a.sin + t * a.cs_st, a.wk, a.eps, ln);
+    }
+  }
+
+  // the largest finite magnitude of a wavefront's lanes
+  static __device__ __forceinline__ uint32_t max64(uint32_t m) {
+    m = max16(m);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+    return (uint32_t)__builtin_amdgcn_readfirstlane(max(m, (uint32_t)__shfl_xor((int)m, 32, 64)));
+  }
+
+  // of n tokens from t on
+  __device__ __forceinline__ uint32_t top_of(int64_t t, int n) const {
+    uint32_t m = 0;
+    for (int i = 0; i < n; i += 4) m = max(m, finite_max8<T>(row(t + min(i + j, n - 1))));
+    return max64(m);
+  }
+
+  // the first `rows` codes of a page, to a scale 2^-d times theirs
+  __device__ __forceinline__ void round_again(int64_t page, int rows, int d) const {
+    const float two_d = e8m0_to_f32((uint32_t)max(127 + d, 1));  // what 2^-126 leaves rounds to zero as well
+    for (int r = lane >> 3; r < rows; r += 8) {
+      char* c = codes + ((page << a.bs_shift) + r) * row_bytes + 16 * (lane & 7);
+      u32x4 w = ld16(c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = again4(w[i], two_d);
+      st16(c, w);
+    }
+  }
+
+  // One whole run of n tokens from t on, at slot s0: up to 16 rows stay in registers, longer runs are read twice.
+  __device__ __forceinline__ void one_run(int64_t t, int n, int64_t s0) const {
+    constexpr int W = 4;
+    const int64_t page = s0 >> a.bs_shift;
+    const int before = (int)(s0 & mask);
+    int old = 0;
+    if (before) old = scales[page * a.hkv];
+    u32x4 x[W];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int p = 0; p < W; ++p) {
+        x[p] = u32x4{0, 0, 0, 0};
+        if (i0 + 4 * p < n) x[p] = row(t + min(i0 + 4 * p + j, n - 1));
+      }
+    };
+    load(0);
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < W; ++p) m = max(m, max8(x[p]));
+    bool bad = __any(m >= Fp8Range<T>::inf);
+    if (bad) {
+      m = 0;
+#pragma unroll
+      for (int p = 0; p < W; ++p) m = max(m, finite_max8<T>(x[p]));
+    }
+    m = max64(m);
+    if (n > 4 * W) m = max(m, top_of(t + 4 * W, n - 4 * W)), bad = true;  // (codes8 then looks for itself)
+    const int e = before ? max(block_exp8<T>(m), __builtin_amdgcn_readfirstlane(old)) : block_exp8<T>(m);
+    char* to = codes + (s0 + j) * row_bytes + 8 * ln;
+    for (int i0 = 0; i0 < n; i0 += 4 * W) {
+      if (i0) load(i0);
+#pragma unroll
+      for (int p = 0; p < W; ++p)
+        if (i0 + 4 * p + j < n) st8(to + (i0 + 4 * p) * row_bytes, codes8<T>(x[p], e, bad));
+    }
+    if (lane == 0) scales[page * a.hkv] = (uint8_t)e;
+    if (before && e > old) round_again(page, before, old - e);
+  }
+
+  // Up to four tokens from t0 on, of any runs: token t0 + j is lanes 16 j ..
+  __device__ __forceinline__ void four_tokens(int64_t t0, int count) const {
+    const int64_t last = t0 + count - 1, t = t0 + j, at = min(t, last);
+    const int64_t s = a.slots[at], s_before = at > 0 ? a.slots[at - 1] : -1, s0 = a.slots[t0], sl = a.slots[last];
+    const u32x4 x = row(at);
+    const bool in = t <= last && s >= 0 && s < a.num_slots;
+    const bool first = !in || s_before != s - 1 || (s & mask) == 0;  // begins a run, or has no slot
+    // tokens before and behind these on a chain of slots of one page
+    const int64_t tb = t0 - 1 - lane, ta = last + 1 + lane;
+    const bool chain_b = s0 >= 0 && s0 < a.num_slots && lane < (int)(s0 & mask) && tb >= 0 &&
+                         a.slots[max(tb, (int64_t)0)] == s0 - 1 - lane;
+    const bool chain_a = sl >= 0 && sl < a.num_slots && (int)(sl & mask) + 1 + lane < a.bs && ta < a.n &&
+                         a.slots[min(ta, (int64_t)a.n - 1)] == sl + 1 + lane;
+    const int nb = __builtin_ctzll(~__ballot(chain_b)), na = __builtin_ctzll(~__ballot(chain_a));  // at most bs - 1 of 64 lanes
+    const uint32_t own = finite_max8<T>(x), top = max16(own);
+    const bool bad = __any(own != max8(x));
+    const uint32_t top_b = nb ? top_of(t0 - nb, nb) : 0u, top_a = na ? top_of(last + 1, na) : 0u;
+
+    // each token's run, [from u to v) of these tokens: its largest magnitude over them and what lies beyond
+    const uint64_t f = __ballot(first);
+    const uint32_t begins = (uint32_t)((f & 1) | (f >> 15 & 2) | (f >> 30 & 4) | (f >> 45 & 8));
+    const uint32_t below = begins & ((2u << j) - 1), above = begins >> (j + 1);
+    const int u = below ? 31 - __builtin_clz(below) : -nb, v = above ? j + 1 + __builtin_ctz(above) : 4;
+    uint32_t m = max(below ? 0u : top_b, t0 + v > last ? top_a : 0u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = max(m, k >= u && k < v ? (uint32_t)__builtin_amdgcn_readlane((int)top, 16 * k) : 0u);
+
+    const int64_t slot = in ? s : 0, page = slot >> a.bs_shift;
+    const int before = (int)(slot & mask) - (j - u);  // slots of the page before the run
+    int e = block_exp8<T>(m), old = e;
+    if (in && before > 0) {
+      old = scales[page * a.hkv];
+      e = max(e, old);
+    }
+    const bool owner = in && first;
+    if (in) st8(codes + slot * row_bytes + 8 * ln, codes8<T>(x, e, bad));
+    if (owner && ln == 0 && (before == 0 || e != old)) scales[page * a.hkv] = (uint8_t)e;
+    for (uint64_t grow = __ballot(owner && ln == 0 && e > old); grow; grow &= grow - 1) {
+      const int of = __builtin_ctzll(grow);
+      round_again(__builtin_amdgcn_readlane((int)page, of), __builtin_amdgcn_readlane(before, of), __builtin_amdgcn_readlane(old - e, of));
+    }
+  }
+};
+
+constexpr int kWindow = 16;  // tokens in whose window a wavefront's runs begin (WHOLE)
+
+// WHOLE: the runs that begin in 16 tokens, each of them whole; without, four tokens and what their runs take.
+template <typename T, int FORM, bool WHOLE>
 __global__ __launch_bounds__(256) void append_fp8_blocks_kernel(const BlocksArgs a) {
   const int lane = threadIdx.x & 63, ln = lane & 15, j = lane >> 4;
   const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
@@ -202,181 +341,44 @@ __global__ __launch_bounds__(256) void append_fp8_blocks_kernel(const BlocksArgs
     return;
   }
   const unsigned per_window = 2u * (unsigned)a.hkv, window = wave / per_window;
-  const int hv = (int)(wave - window * per_window), h = hv >> 1;
-  const bool is_v = hv & 1;
-  const int64_t t_window = (int64_t)window * (4 * W);
-  if (t_window >= a.n) return;
-  const char* src = is_v ? a.v + h * a.v_sh : a.k + h * a.k_sh;
-  const int64_t st = is_v ? a.v_st : a.k_st;
-  char* codes = (is_v ? a.vc : a.kc) + (int64_t)h * kDh;
-  uint8_t* scales = (is_v ? a.vs : a.ks) + h;
-  const int64_t row_bytes = (int64_t)a.hkv * kDh;
-
-  // lane ln's part of token t's row, as it goes into the pool
-  auto row = [&](int64_t t) {
-    const u32x4 x = ld16(src + t * st + 16 * ln);
-    if constexpr (FORM == kPlain) {
-      return x;
-    } else {
-      if (is_v) return x;
-      return turned<T, FORM == kPlain ? kRope : FORM>(x, a.cos + t * a.cs_st, a.sin + t * a.cs_st, a.wk, a.eps, ln);
-    }
-  };
-
-  const int mask = a.bs - 1;
-  // the first `rows` codes of a page, to a scale 2^d times smaller than theirs
-  auto round_again = [&](int64_t page, int rows, int d) {
-    const float two_d = e8m0_to_f32((uint32_t)max(127 + d, 1));  // what 2^-126 leaves rounds to zero as well
-    for (int r = lane >> 3; r < rows; r += 8) {
-      char* c = codes + ((page << a.bs_shift) + r) * row_bytes + 16 * (lane & 7);
-      u32x4 w = ld16(c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = again4(w[i], two_d);
-      st16(c, w);
-    }
-  };
-  // The runs that begin in the window: tokens [from, to) of it.  Of 16 tokens on a chain one lies at a page's first slot, so
-  // the next run begins within 16 tokens of the window's end.
-  constexpr bool kWhole = W > 1;
-  const bool whole = kWhole && a.bs == 16;
-  int from = 0, to = 4 * W;
-  uint64_t starts = 0;
-  int64_t its_slot = -1;  // of token t_window + lane
-  if (whole) {
-    const int64_t t = t_window + lane, at = min(t, (int64_t)a.n - 1), s = a.slots[at], s1 = a.slots[max(at - 1, (int64_t)0)];
-    if (t < a.n && s >= 0 && s < a.num_slots) its_slot = s;
-    starts = __ballot(its_slot < 0 || (s & mask) == 0 || t == 0 || s1 != s - 1);
-    if (!(starts & 0xffff)) return;
-    from = __builtin_ctzll(starts);
-    to = 16 + __builtin_ctzll(starts >> 16);
-  }
-  while (true) {
-    // up to 16 tokens of whole runs
-    const int count = whole && to - from > 16 ? 63 - __builtin_clzll((starts >> from) & 0x1fffe) : to - from;
-    const int64_t t0 = t_window + from, last = min(t0 + count, (int64_t)a.n) - 1;
-    if (t0 >= a.n) return;
-    if (whole && __builtin_popcountll((starts >> from) & (~0ull >> (64 - count))) == 1) {  // one run: what prompts are made of
-      const int64_t s0 = ((int64_t)__builtin_amdgcn_readlane((int)(its_slot >> 32), from) << 32) |
-                         (uint32_t)__builtin_amdgcn_readlane((int)its_slot, from);
-      if (s0 >= 0) {
-        u32x4 x[W];
-        const int64_t page = s0 >> a.bs_shift;
-        const int before = (int)(s0 & mask);
-        int old = 0;
-        if (before) old = scales[page * a.hkv];
-#pragma unroll
-        for (int p = 0; p < W; ++p) {
-          const int i = 4 * p + j;
-          x[p] = u32x4{0, 0, 0, 0};
-          if (4 * p < count) x[p] = row(t0 + min(i, count - 1));
-        }
-        uint32_t m = 0;
-#pragma unroll
-        for (int p = 0; p < W; ++p) m = max(m, max8(x[p]));
-        const bool bad = __any(m >= Fp8Range<T>::inf);
-        if (bad) {
-          m = 0;
-#pragma unroll
-          for (int p = 0; p < W; ++p) m = max(m, finite_max8<T>(x[p]));
-        }
-        m = max16(m);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-        const int e = before ? max(block_exp8<T>(m), __builtin_amdgcn_readfirstlane(old)) : block_exp8<T>(m);
-        char* to_codes = codes + (s0 + j) * row_bytes + 8 * ln;
-#pragma unroll
-        for (int p = 0; p < W; ++p)
-          if (4 * p + j < count) st8(to_codes + 4 * p * row_bytes, codes8<T>(x[p], e, bad));
-        if (lane == 0) scales[page * a.hkv] = (uint8_t)e;
-        if (before && e > old) round_again(page, before, old - e);
-      }
-      from += count;
-      if (from >= to) return;
-      continue;
-    }
-    // the tokens: t0 + 4 p + j of lanes 16 j ..
-    u32x4 x[W];
-    int64_t slot[W];
-    bool first[W];  // begins a run, or has no slot
-    uint32_t top[W];
-    bool bad = false;
-#pragma unroll
-    for (int p = 0; p < W; ++p) {
-      const int64_t t = t0 + 4 * p + j, at = min(t, last);
-      const int64_t s = a.slots[at], before = at > 0 ? a.slots[at - 1] : -1;
-      slot[p] = t <= last && s >= 0 && s < a.num_slots ? s : -1;
-      first[p] = slot[p] < 0 || before != s - 1 || (s & (a.bs - 1)) == 0;
-      x[p] = row(at);
-    }
-    // tokens before and behind these on a chain of slots of one page
-    const int64_t s0 = a.slots[t0], sl = a.slots[last];
-    const int64_t tb = t0 - 1 - lane, ta = last + 1 + lane;
-    const bool chain_b = s0 >= 0 && s0 < a.num_slots && lane < (int)(s0 & mask) && tb >= 0 && a.slots[max(tb, (int64_t)0)] == s0 - 1 - lane;
-    const bool chain_a = sl >= 0 && sl < a.num_slots && (int)(sl & mask) + 1 + lane < a.bs && ta < a.n &&
-                         a.slots[min(ta, (int64_t)a.n - 1)] == sl + 1 + lane;
-    const int nb = __builtin_ctzll(~__ballot(chain_b)), na = __builtin_ctzll(~__ballot(chain_a));  // at most bs - 1 of 64 lanes
-#pragma unroll
-    for (int p = 0; p < W; ++p) {
-      const uint32_t f = finite_max8<T>(x[p]);
-      bad |= f != max8(x[p]);
-      top[p] = max16(f);
-    }
-    bad = __any(bad);
-    auto beyond = [&](int64_t at, int n) {
-      uint32_t m = 0;
-      for (int i = 0; i < n; i += 4) {
-        m = max(m, finite_max8<T>(row(at + min(i + j, n - 1))));
-      }
-      m = max16(m);
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-      return (uint32_t)__builtin_amdgcn_readfirstlane(max(m, (uint32_t)__shfl_xor((int)m, 32, 64)));
+  const int hv = (int)(wave - window * per_window);
+  const Appender<T, FORM> to(a, hv >> 1, hv & 1, lane);
+  if constexpr (!WHOLE) {
+    const int64_t t0 = (int64_t)window * 4;
+    if (t0 < a.n) to.four_tokens(t0, (int)min((int64_t)4, a.n - t0));
+  } else {
+    const int64_t t_window = (int64_t)window * kWindow;
+    if (t_window >= a.n) return;
+    // where runs begin (or tokens have no slot) among 64 tokens from `t` on; those past the last count too
+    int64_t slot = -1;
+    auto starts_from = [&](int64_t t) {
+      const int64_t at = min(t, (int64_t)a.n - 1), s = a.slots[at], s_before = a.slots[max(at - 1, (int64_t)0)];
+      const bool in = t < a.n && s >= 0 && s < a.num_slots;
+      slot = in ? s : -1;
+      return __ballot(!in || (s & to.mask) == 0 || t == 0 || s_before != s - 1);
     };
-    const uint32_t top_b = nb ? beyond(t0 - nb, nb) : 0u, top_a = na ? beyond(last + 1, na) : 0u;
-
-    // each token's run: its largest magnitude and where it began (relative to t0), over the tokens in order
-    uint32_t run[4 * W];
-    int start[4 * W];
-    bool begins[4 * W];
-    uint32_t cur = top_b;
-    int at = -nb;
-#pragma unroll
-    for (int i = 0; i < 4 * W; ++i) {
-      begins[i] = (__ballot(first[i >> 2]) >> (16 * (i & 3))) & 1;
-      const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)top[i >> 2], 16 * (i & 3));
-      at = begins[i] ? i : at;
-      cur = begins[i] ? m : max(cur, m);
-      run[i] = cur;
-      start[i] = at;
-    }
-#pragma unroll
-    for (int i = 4 * W - 1; i >= 0; --i) {
-      if (t0 + i == last) run[i] = max(run[i], top_a);  // (tokens past the last have no slot)
-      if (i + 1 < 4 * W && !begins[i + 1]) run[i] = run[i + 1];
-    }
-
-#pragma unroll
-    for (int p = 0; p < W; ++p) {
-      const uint32_t m = j == 0 ? run[4 * p] : (j == 1 ? run[4 * p + 1] : (j == 2 ? run[4 * p + 2] : run[4 * p + 3]));
-      const int s = j == 0 ? start[4 * p] : (j == 1 ? start[4 * p + 1] : (j == 2 ? start[4 * p + 2] : start[4 * p + 3]));
-      const bool in = slot[p] >= 0;
-      const int64_t at_slot = in ? slot[p] : 0, page = at_slot >> a.bs_shift;
-      const int before = (int)(at_slot & mask) - (4 * p + j - s);  // slots of the page before the run
-      int e = block_exp8<T>(m), old = e;
-      if (in && before > 0) {
-        old = scales[page * a.hkv];
-        e = max(e, old);
+    const uint64_t starts = starts_from(t_window + lane);
+    const int64_t slots16 = slot;
+    for (int at = starts ? __builtin_ctzll(starts) : 64; at < kWindow;) {
+      const uint64_t behind = starts >> (at + 1);
+      // the next run begins at most bs tokens on: of as many on a chain one lies at a page's first slot
+      int next = behind ? at + 1 + __builtin_ctzll(behind) : 64 + __builtin_ctzll(starts_from(t_window + 64 + lane));
+      const int64_t t0 = t_window + at;
+      if (t0 >= a.n) return;
+      const int64_t s0 = ((int64_t)__builtin_amdgcn_readlane((int)(slots16 >> 32), at) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)slots16, at);
+      if (next - at > 4) {
+        if (s0 >= 0) to.one_run(t0, next - at, s0);
+      } else {  // with the short ones behind it that fit and begin in the window
+        while (next < kWindow) {
+          const int end = next + 1 + __builtin_ctzll(starts >> (next + 1) | 1ull << 62);
+          if (end - at > 4) break;
+          next = end;
+        }
+        to.four_tokens(t0, (int)min((int64_t)(next - at), a.n - t0));
       }
-      const bool owner = in && first[p];
-      if (in) st8(codes + at_slot * row_bytes + 8 * ln, codes8<T>(x[p], e, bad));
-      if (owner && ln == 0 && (before == 0 || e != old)) scales[page * a.hkv] = (uint8_t)e;
-      for (uint64_t grow = __ballot(owner && ln == 0 && e > old); grow; grow &= grow - 1) {
-        const int of = __builtin_ctzll(grow);
-        round_again(__builtin_amdgcn_readlane((int)page, of), __builtin_amdgcn_readlane(before, of),
-                    __builtin_amdgcn_readlane(old - e, of));
-      }
+      at = next;
     }
-    from += count;
-    if (!whole || from >= to) return;
   }
 }
 
@@ -406,8 +408,8 @@ __global__ __launch_bounds__(256) void read_fp8_blocks_kernel(const char* __rest
   st16(out + 16, hi);
 }
 
-// Windows of four tokens up to this many, of sixteen above: few tokens are bound by the latency of a wavefront's chain, many by
-// the lanes' work, and a page's tokens in one window are read once.
+// Up to so many tokens a wavefront takes four: few tokens are bound by the latency of a wavefront's chain, many by its
+// instructions and by what is read again.
 constexpr int64_t kSmallStep = 1024;
 
 int check_blocks(const std::string& fn, int32_t dtype, int64_t num_tokens, int64_t num_blocks, int32_t block_size,
@@ -425,7 +427,7 @@ int check_blocks(const std::string& fn, int32_t dtype, int64_t num_tokens, int64
 
 int launch_append(const std::string& fn, BlocksArgs a, int form, int dtype, hipStream_t st) {
   const bool small = a.n <= kSmallStep;
-  const int64_t window = small ? 4 : 16;
+  const int64_t window = small ? 4 : kWindow;
   const int64_t pool = (a.n + window - 1) / window * 2 * a.hkv;
   const int64_t waves = pool + (form == kPlain ? 0 : ((int64_t)a.n * a.H + 3) / 4);
   MLLM_REQUIRE((waves + 3) / 4 <= kMaxGroups256, MLLM_ERR_UNSUPPORTED, fn + ": too many tokens");
@@ -435,9 +437,9 @@ int launch_append(const std::string& fn, BlocksArgs a, int form, int dtype, hipS
     using T = decltype(tag);
     constexpr int FORM = decltype(kind)::value;
     if (small)
-      append_fp8_blocks_kernel<T, FORM, 1><<<grid, 256, 0, st>>>(a);
+      append_fp8_blocks_kernel<T, FORM, false><<<grid, 256, 0, st>>>(a);
     else
-      append_fp8_blocks_kernel<T, FORM, 4><<<grid, 256, 0, st>>>(a);
+      append_fp8_blocks_kernel<T, FORM, true><<<grid, 256, 0, st>>>(a);
   };
   auto of_form = [&](auto tag) {
     if (form == kPlain)
