@@ -148,17 +148,17 @@ __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const Prefi
   const int key0 = kv0 + 16 * (w >> 1);
   const bool whole = kv0 + kBN <= kv_end;
   const int tok = whole ? 0 : min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);  // the row within its block
-  if constexpr (POOL != kPoolFp4) {
+  if constexpr (POOL == kPoolFp8Blocks) {
+    const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
+    const uint64_t at = (uint64_t)b * (unsigned)a.Hkv + head_bytes / kHeadDim;
+    ConstU32* words = (ConstU32*)(IS_V ? a.vs : a.ks);
+    const uint32_t e = words[at >> 2] >> (8 * (unsigned)(at & 3));
+    if (whole) return {ld16(group_base(pool, a, blk, key0) + off), e};  // a load per branch, as below
+    return {ld16(group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7))), e};
+  } else if constexpr (POOL != kPoolFp4) {
     const char* p = whole ? group_base(pool, a, blk, key0) + off
                           : group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
-    if constexpr (POOL != kPoolFp8Blocks) {
-      return {ld16(p)};
-    } else {
-      const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
-      const uint64_t at = (uint64_t)b * (unsigned)a.Hkv + head_bytes / kHeadDim;
-      ConstU32* words = (ConstU32*)(IS_V ? a.vs : a.ks);
-      return {ld16(p), words[at >> 2] >> (8 * (unsigned)(at & 3))};
-    }
+    return {ld16(p)};
   } else {
     // a load per branch: merged, the two addresses would be a pair of registers per lane instead of a scalar and an offset
     constexpr int kBlocks = kHeadDim / kFp4Block;

@@ -277,6 +277,10 @@ def check_scales(k_cache: torch.Tensor, k_scale, v_scale) -> None:
     else:
         k_shape, v_shape, kind = (nb, hkv), (nb, hkv), "block scales"
     device = k_cache.device
+    if isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor) and k_scale.dtype == v_scale.dtype == SCALES4 \
+            and k_scale.shape == k_shape and v_scale.shape == v_shape and k_scale.is_contiguous() and v_scale.is_contiguous() \
+            and k_scale.device == device == v_scale.device:
+        return
     for name, t, shape in (("k_scale", k_scale, k_shape), ("v_scale", v_scale, v_shape)):
         if not isinstance(t, torch.Tensor) or t.dtype != SCALES4:
             raise ValueError(f"with {kind}, {name} is a float8_e8m0fnu tensor of block scales")
@@ -566,7 +570,7 @@ class HipBackend(AttentionBackend):
             if len(rows) != 3 or rows[1] != hkv or rows[2] != dh or v.shape != rows or v.dtype != dtype:
                 raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {dh}] of one dtype")
             slots = meta.slot_mapping
-            if slots.numel() != rows[0] or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+            if slots.numel() != rows[0] or slots.device != k_cache.device or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
                     or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
                 raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
             device = k_cache.device

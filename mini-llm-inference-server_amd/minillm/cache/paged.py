@@ -128,8 +128,8 @@ class PagedKVCache:
             self._copy_on_host(src, dst)
             return
         tensors, pointers, nbytes = self._page_tensors()
-        _native.lib().launch(device, "mllm_copy_pages", pointers, nbytes, len(tensors), self.num_blocks, src.ctypes.data,
-                             dst.ctypes.data, src.size)
+        _native.lib().launch(device, "mllm_copy_pages", pointers, nbytes, len(tensors), self.num_blocks, src.tobytes(),
+                             dst.tobytes(), src.size)
 
     def _copy_on_host(self, src: np.ndarray, dst: np.ndarray) -> None:
         """`copy_blocks` of a pool that is not on a GPU, in torch operations, under the same rules."""
@@ -188,7 +188,7 @@ def _block_ids(ids) -> np.ndarray:
     ids = np.asarray(ids)
     if ids.ndim != 1 or ids.size and ids.dtype.kind not in "iu":
         raise ValueError("block ids must be one row of whole numbers")
-    return np.ascontiguousarray(ids, dtype=np.int64)
+    return ids.astype(np.int64, copy=False)
 
 
 def _page_scales(num_blocks: int, hkv: int, device) -> torch.Tensor:

@@ -151,7 +151,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
 
 def rotary_ok(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> bool:
     """Whether `rotary` takes the model's q (already `usable`), k, positions and frequencies: few enough tokens for one launch."""
-    return (0 < positions.numel() <= MAX_GROUPS and inv_freq.numel() <= 512 and positions.dtype == torch.int64
+    b, h, t, dh = q.shape
+    return (0 < b * t * (h + k.shape[1]) * dh <= MAX_GROUPS * 256 and dh <= 4096 and inv_freq.numel() <= 512
+            and positions.shape == (b, t) and positions.dtype == torch.int64 and k.dtype == q.dtype
             and all(type(x) is torch.Tensor and not _wrapped(x) and x.device == q.device for x in (k, positions, inv_freq)))
 
 

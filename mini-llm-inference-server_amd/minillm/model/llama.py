@@ -71,6 +71,8 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
 
 
 class LlamaAttention(nn.Module):
+    by_position = False  # see __init__
+
     def __init__(self, config: LlamaConfig, backend: AttentionBackend, layer_idx: int) -> None:
         super().__init__()
         self.config = config
@@ -215,6 +217,8 @@ class LlamaDecoderLayer(nn.Module):
 
 
 class LlamaModel(nn.Module):
+    by_position = False  # the layers take positions and frequencies instead of tables
+
     def __init__(self, config: LlamaConfig, backend: AttentionBackend) -> None:
         super().__init__()
         self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size)
