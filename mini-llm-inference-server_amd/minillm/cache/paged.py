@@ -27,6 +27,7 @@ tokens of a head.
 from __future__ import annotations
 
 import struct
+from array import array
 from itertools import chain
 from operator import is_
 
@@ -119,17 +120,18 @@ class PagedKVCache:
         pool's device.  `src` and `dst` are sequences of block ids on the host, of one length.  A block written twice, or read
         and written, is refused (ValueError), as is one outside the pool; nothing is copied then."""
         src, dst = _block_ids(src), _block_ids(dst)
-        if src.shape != dst.shape:
-            raise ValueError(f"{src.size} blocks to copy from and {dst.size} to copy to")
-        if not src.size:
+        n = len(src)
+        if n != len(dst):
+            raise ValueError(f"{n} blocks to copy from and {len(dst)} to copy to")
+        if not n:
             return
         device = self.k[0].device
         if device.type != "cuda":
-            self._copy_on_host(src, dst)
+            self._copy_on_host(np.asarray(src), np.asarray(dst))
             return
         tensors, pointers, nbytes = self._page_tensors()
         _native.lib().launch(device, "mllm_copy_pages", pointers, nbytes, len(tensors), self.num_blocks, src.tobytes(),
-                             dst.tobytes(), src.size)
+                             dst.tobytes(), n)
 
     def _copy_on_host(self, src: np.ndarray, dst: np.ndarray) -> None:
         """`copy_blocks` of a pool that is not on a GPU, in torch operations, under the same rules."""
@@ -181,8 +183,13 @@ class PagedKVCache:
         return PagedStep(self, meta)
 
 
-def _block_ids(ids) -> np.ndarray:
-    """A sequence of block ids as one row of int64."""
+def _block_ids(ids):
+    """A sequence of block ids as one row of int64 (an array of either kind: a list becomes one in half of numpy's time)."""
+    if type(ids) in (list, tuple, range):
+        try:
+            return array("q", ids)
+        except (TypeError, OverflowError):
+            raise ValueError("block ids must be one row of whole numbers") from None
     if isinstance(ids, torch.Tensor) and ids.is_cuda:
         raise ValueError("block ids are taken from the host")
     ids = np.asarray(ids)

@@ -182,7 +182,8 @@ def test_copy_blocks_refusals():
     cache = PagedKVCache(config(), 9, "cpu", torch.bfloat16)
     for src, dst, match in (([1], [9], "outside"), ([-1], [2], "outside"), ([1, 2], [3, 3], "written twice"),
                             ([1, 2], [2, 3], "read and written"), ([4], [4], "read and written"), ([1, 2], [3], "2 blocks"),
-                            ([1.0], [2], "whole numbers"), ([[1]], [[2]], "one row"), ([True], [2], "whole numbers")):
+                            ([1.0], [2], "whole numbers"), ([[1]], [[2]], "one row"), ([1 << 63], [2], "whole numbers"),
+                            (torch.tensor([1.0]), [2], "whole numbers"), (torch.tensor([[1]]), [2], "one row")):
         with pytest.raises(ValueError, match=match):
             cache.copy_blocks(src, dst)
     cache.k[0] = torch.zeros(8, 16, 2, 128, dtype=torch.bfloat16)
