@@ -333,6 +333,9 @@ int mllm_silu_mul(const void* gate, const void* up, int64_t n, int32_t dtype, vo
  * inv_freq[d % half])), fp32 angles, T the 16-bit `dtype`. */
 int mllm_rope_table(const int64_t* positions, int64_t n, const float* inv_freq, int32_t half, int32_t dtype, void* cos,
                     void* sin, void* stream);
+/* The same for frequencies scaled to long contexts: angles in 64 bits, cos and sin times `factor`. */
+int mllm_rope_table_scaled(const int64_t* positions, int64_t n, const float* inv_freq, int32_t half, float factor,
+                           int32_t dtype, void* cos, void* sin, void* stream);
 
 /*
  * Linear layers of few rows (reference src/minillm/model/llama.py:75-120): x [m, k] contiguous, weights [n, k] contiguous

@@ -164,6 +164,25 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const int64_t* __restri
   sin_out[o] = sin_out[o + half] = s;
 }
 
+// The same for frequencies scaled to long contexts: the angle in 64 bits, reduced to a part of a turn there (in 32 bits it is off
+// by up to 2^-24 of the position), and cos and sin times `factor`.
+template <typename T>
+__global__ __launch_bounds__(256) void rope_table_scaled_kernel(const int64_t* __restrict__ pos, int64_t n,
+                                                                const float* __restrict__ inv_freq, int half, float factor,
+                                                                uint16_t* __restrict__ cos_out,
+                                                                uint16_t* __restrict__ sin_out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * half) return;
+  const int64_t t = i / half;
+  const int d = (int)(i - t * half);
+  const double turns = (double)pos[t] * (double)inv_freq[d] * 0.15915494309189535;
+  const float part = (float)(turns - __builtin_rint(turns));
+  const uint16_t c = cvt1<T>(factor * __builtin_amdgcn_cosf(part)), s = cvt1<T>(factor * __builtin_amdgcn_sinf(part));
+  const int64_t o = 2 * t * half + d;
+  cos_out[o] = cos_out[o + half] = c;
+  sin_out[o] = sin_out[o + half] = s;
+}
+
 }  // namespace
 }  // namespace mllm
 
@@ -278,4 +297,27 @@ extern "C" int mllm_rope_table(const int64_t* positions, int64_t n, const float*
   else
     rope_table_kernel<F16><<<(unsigned)groups, 256, 0, st>>>(positions, n, inv_freq, half, (uint16_t*)cos, (uint16_t*)sin);
   return check_launch("mllm_rope_table");
+}
+
+extern "C" int mllm_rope_table_scaled(const int64_t* positions, int64_t n, const float* inv_freq, int32_t half, float factor,
+                                      int32_t dtype, void* cos, void* sin, void* stream) {
+  using namespace mllm;
+  const std::string fn = "mllm_rope_table_scaled";
+  MLLM_REQUIRE(dtype == MLLM_DTYPE_BF16 || dtype == MLLM_DTYPE_F16, MLLM_ERR_UNSUPPORTED,
+               fn + ": dtype must be bfloat16 or float16");
+  MLLM_REQUIRE(n >= 0 && half > 0 && n < (1ll << 31), MLLM_ERR_INVALID, fn + ": bad sizes");
+  if (n == 0) return MLLM_OK;
+  MLLM_REQUIRE(positions && inv_freq && cos && sin, MLLM_ERR_INVALID, fn + ": null pointer");
+  const int64_t groups = (n * half + 255) / 256;
+  MLLM_REQUIRE(groups <= kMaxGroups256, MLLM_ERR_UNSUPPORTED, fn + ": too many positions");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto launch = [&](auto tag) {
+    rope_table_scaled_kernel<decltype(tag)><<<(unsigned)groups, 256, 0, st>>>(positions, n, inv_freq, half, factor, (uint16_t*)cos,
+                                                                             (uint16_t*)sin);
+  };
+  if (dtype == MLLM_DTYPE_BF16)
+    launch(BF16{});
+  else
+    launch(F16{});
+  return check_launch(fn.c_str());
 }

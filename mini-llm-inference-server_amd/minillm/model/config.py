@@ -17,9 +17,6 @@ _REQUIRED_KEYS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_
                   "rms_norm_eps")
 _DEFAULTS = {"tie_word_embeddings": False, "max_position_embeddings": 8192, "qk_norm": False}
 
-# scaling types whose angles the model takes as the reference does; the others go with the positions' kernel
-REFERENCE_SCALING = (None, "llama3")
-
 
 def _rope_fields(d: Mapping[str, Any]) -> tuple[float, dict[str, Any] | None]:
     """(rope_theta, rope_scaling) of a config dictionary.
@@ -87,10 +84,9 @@ class LlamaConfig:
         return dim
 
     @property
-    def reference_rope(self) -> bool:
-        """Whether the rotation is the reference's: half-split pairs of whole heads, plain or llama3 frequencies."""
-        return not self.rope_interleaved and self.rotary_dim == self.head_dim \
-            and (self.rope_scaling or {}).get("rope_type") in REFERENCE_SCALING
+    def rope_by_table(self) -> bool:
+        """Whether the rotation is of half-split pairs of whole heads, by tables (as the reference's); else it goes by positions."""
+        return not self.rope_interleaved and self.rotary_dim == self.head_dim
 
     @classmethod
     def from_dict(cls, d: Mapping[str, Any]) -> LlamaConfig:

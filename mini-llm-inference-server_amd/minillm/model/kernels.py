@@ -87,11 +87,16 @@ def rope_ok(positions: torch.Tensor, dtype: torch.dtype, half: int) -> bool:
             and 0 < positions.numel() * half <= MAX_GROUPS * 256)
 
 
-def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dtype):
-    """cos, sin [..., 2 len(inv_freq)] of int64 positions."""
+def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dtype, factor: float | None = None):
+    """cos, sin [..., 2 len(inv_freq)] of int64 positions.  With a `factor` (frequencies scaled to long contexts) they are scaled
+    by it, and the angles are products in 64 bits."""
     half = inv_freq.shape[0]
     cos = torch.empty((*positions.shape, 2 * half), dtype=dtype, device=positions.device)
     sin = torch.empty_like(cos)
+    if factor is not None:
+        _native.lib().call("mllm_rope_table_scaled", positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half, factor,
+                           _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr(), _native.stream_ptr(positions.device))
+        return cos, sin
     _native.lib().call("mllm_rope_table", positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half,
                        _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr(), _native.stream_ptr(positions.device))
     return cos, sin

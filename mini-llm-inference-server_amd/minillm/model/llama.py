@@ -45,6 +45,9 @@ class RotaryEmbedding(nn.Module):
     def __init__(self, config: LlamaConfig) -> None:
         super().__init__()
         self._inv_freq = compute_inv_freq(config)
+        # linear and yarn: angles in 64 bits, cos and sin scaled; None: as the reference takes them
+        scaled = config.rope_scaling is not None and config.rope_scaling["rope_type"] != "llama3"
+        self._factor = attention_factor(config) if scaled else None
         self._on_device: dict[torch.device, torch.Tensor] = {}
 
     def inv_freq(self, device: torch.device) -> torch.Tensor:
@@ -54,9 +57,14 @@ class RotaryEmbedding(nn.Module):
         return t
 
     def forward(self, positions: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-        """positions [B, T] -> cos, sin [B, T, Dh]: float32 angles, the half-size table repeated."""
+        """positions [B, T] -> cos, sin [B, T, Dh]: float32 angles, the half-size table repeated (frequencies scaled to long
+        contexts: float64 angles, cos and sin scaled)."""
         if kernels.rope_ok(positions, dtype, self._inv_freq.shape[0]):
-            return kernels.rope_table(positions, self.inv_freq(positions.device), dtype)
+            return kernels.rope_table(positions, self.inv_freq(positions.device), dtype, self._factor)
+        if self._factor is not None:
+            ang = positions[..., None].double() * self.inv_freq(positions.device).double()
+            ang = torch.cat([ang, ang], dim=-1)
+            return (ang.cos() * self._factor).to(dtype), (ang.sin() * self._factor).to(dtype)
         ang = positions[..., None].float() * self.inv_freq(positions.device)
         ang = torch.cat([ang, ang], dim=-1)
         return ang.cos().to(dtype), ang.sin().to(dtype)
@@ -83,8 +91,8 @@ class LlamaAttention(nn.Module):
         self.k_proj = nn.Linear(d, hkv * dh, bias=False)
         self.v_proj = nn.Linear(d, hkv * dh, bias=False)
         self.o_proj = nn.Linear(h * dh, d, bias=False)
-        # another rotation than the reference's goes by the positions instead of tables (`_turn`)
-        self.by_position = not config.reference_rope
+        # adjacent pairs, or a part of the head: by the positions instead of tables (`_turn`)
+        self.by_position = not config.rope_by_table
         self.rope_factor = attention_factor(config)
         # RMSNorm of every query and key head before the rotation (config.qk_norm)
         self.q_norm = RMSNorm(dh, config.rms_norm_eps) if config.qk_norm else None
@@ -225,7 +233,7 @@ class LlamaModel(nn.Module):
         self.layers = nn.ModuleList(LlamaDecoderLayer(config, backend, i) for i in range(config.num_hidden_layers))
         self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps)
         self.rotary_emb = RotaryEmbedding(config)
-        self.by_position = not config.reference_rope
+        self.by_position = not config.rope_by_table
 
     def forward(self, input_ids, positions, kv_cache=None, attention_mask=None):
         if kv_cache is not None:

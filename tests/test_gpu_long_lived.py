@@ -35,7 +35,7 @@ def make_model(seed, layers=2, heads=4, kv_heads=2, dtype=torch.bfloat16, **kw):
 
 
 KW = dict(max_batch_size=8, num_kv_blocks=300, max_model_len=2048, kv_cache_dtype=FP8, kv_scales="blocks")
-FORMS = [{}, dict(rope_interleaved=True, rope_scaling=YARN, partial_rotary_factor=0.5), dict(qk_norm=True)]
+FORMS = [{}, dict(rope_interleaved=True, rope_scaling=YARN, partial_rotary_factor=0.5), dict(qk_norm=True, rope_scaling=YARN)]
 
 
 @pytest.mark.parametrize("steps", [
@@ -100,7 +100,7 @@ def test_one_call_layer_equals_the_kernels_one_by_one(hip, monkeypatch, form):
 
     monkeypatch.setattr(kernels, "decoder_layer", counted)
     one_call, _ = run_engine(model, get_backend("hip"), None, ps, 12, **KW)
-    assert any(calls) == ("rope_scaling" not in form)  # a rotation by position goes layer by layer
+    assert any(calls) == ("rope_interleaved" not in form)  # a rotation by position goes layer by layer
     monkeypatch.setattr(kernels, "decoder_layer", lambda *args: None)
     separate, _ = run_engine(model, get_backend("hip"), None, ps, 12, **KW)
     assert one_call == separate  # tokens and the margins of the logits

@@ -125,6 +125,21 @@ def test_other_stream_and_captured(hip):
         assert all(torch.equal(a, b) for a, b in zip(out, kernels.rotary(q, k, pos, inv, True)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scaled_tables(hip, dtype):
+    # half a step of the type, and 2^-18 before it: the part of a turn in fp32 and the hardware's cos and sin
+    from minillm.model import kernels
+
+    g = torch.Generator(device=DEV).manual_seed(4)
+    pos = torch.randint(-(1 << 22), 1 << 22, (3, 700), generator=g, device=DEV)
+    inv = (500000.0 ** -(torch.arange(0, 128, 2) / 128)).to(DEV)
+    for got, f in zip(kernels.rope_table(pos, inv, dtype, 1.3), (torch.cos, torch.sin)):
+        ang = pos[..., None].double() * inv.double()
+        want = 1.3 * f(torch.cat([ang, ang], -1))
+        fi = torch.finfo(dtype)
+        assert ((got.double() - want).abs() <= fi.eps / 2 * want.abs() + 2.0 ** -18).all()
+
+
 def test_gradients_are_refused(hip):
     from minillm.model import kernels
 

@@ -300,9 +300,10 @@ def test_compact_moves_everything_to_the_front(seed):
 
 def test_reference_rope_stays():
     cfg = LlamaConfig.from_dict(LLAMA_3_1_8B)
-    assert cfg.reference_rope and cfg.rotary_dim == 128 and attention_factor(cfg) == 1.0
-    for kw in (dict(rope_interleaved=True), dict(partial_rotary_factor=0.5), dict(rope_scaling={"rope_type": "linear", "factor": 2.0})):
-        assert not config(**kw).reference_rope
+    assert cfg.rope_by_table and cfg.rotary_dim == 128 and attention_factor(cfg) == 1.0
+    assert config(rope_scaling={"rope_type": "linear", "factor": 2.0}).rope_by_table
+    for kw in (dict(rope_interleaved=True), dict(partial_rotary_factor=0.5)):
+        assert not config(**kw).rope_by_table
     with pytest.raises(ValueError, match="even number"):
         config(head_dim=64, partial_rotary_factor=0.36).rotary_dim
     with pytest.raises(ValueError, match="even number"):
@@ -407,8 +408,28 @@ def test_rotary_args_match_the_header(tmp_path):
     assert got == [ctypes.sizeof(_native.RotaryArgs)] + [getattr(_native.RotaryArgs, f).offset for f in fields]
 
 
+@pytest.mark.parametrize("rope", [{"rope_type": "linear", "factor": 4.0},
+                                  {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}])
+def test_scaled_tables_on_the_host(rope):
+    # angles of far positions in float64, whatever the table's type; the plain and the llama3 tables as they were
+    from minillm.model.llama import RotaryEmbedding
+
+    cfg = config(rope_scaling=rope)
+    pos = torch.tensor([[0, 5, 999983, 123456789]])
+    for dtype in (torch.float64, torch.float32, torch.bfloat16):
+        cos, sin = RotaryEmbedding(cfg)(pos, dtype)
+        ang = pos[..., None].double() * compute_inv_freq(cfg).double()
+        for got, f in ((cos, torch.cos), (sin, torch.sin)):
+            assert got.dtype == dtype and torch.equal(got, (f(torch.cat([ang, ang], -1)) * attention_factor(cfg)).to(dtype))
+    plain = RotaryEmbedding(config())
+    cos, _ = plain(pos, torch.float32)
+    ang = pos[..., None].float() * compute_inv_freq(config())
+    assert torch.equal(cos, torch.cat([ang, ang], -1).cos())
+
+
 @pytest.mark.parametrize("kw", [dict(rope_interleaved=True), dict(partial_rotary_factor=0.5),
-                                dict(rope_scaling={"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64})])
+                                dict(rope_interleaved=True, partial_rotary_factor=0.5, rope_scaling={
+                                    "rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64})])
 def test_model_on_the_host_rotates_by_position(kw):
     # a contiguous forward pass on the CPU through a backend in torch operations: equal to the attention by hand
     from minillm.attention.base import AttentionBackend
