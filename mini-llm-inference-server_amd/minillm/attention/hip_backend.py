@@ -463,6 +463,8 @@ class HipBackend(AttentionBackend):
                 raise ValueError("q, k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
         elif fp8:
+            if isinstance(v_scale, torch.Tensor) and v_scale.dtype == SCALES4:
+                raise ValueError("block scales are for K and V alike")
             if not (0 < k_scale < math.inf and 0 < v_scale < math.inf):
                 raise ValueError("k_scale and v_scale must be positive and finite")
         else:
@@ -570,7 +572,8 @@ class HipBackend(AttentionBackend):
             if len(rows) != 3 or rows[1] != hkv or rows[2] != dh or v.shape != rows or v.dtype != dtype:
                 raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {dh}] of one dtype")
             slots = meta.slot_mapping
-            if slots.numel() != rows[0] or slots.device != k_cache.device or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+            if slots.numel() != rows[0] or slots.device != k_cache.device or slots.dtype != torch.int64 \
+                    or not slots.is_contiguous() or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
                     or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
                 raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
             device = k_cache.device

@@ -28,8 +28,6 @@ from __future__ import annotations
 
 import struct
 from array import array
-from itertools import chain
-from operator import is_
 
 import numpy as np
 import torch
@@ -40,6 +38,7 @@ BLOCK_SIZE = 16
 FP4 = torch.float4_e2m1fn_x2
 FP4_BLOCK = 32  # dims per scale of a 4-bit pool
 FP8 = torch.float8_e4m3fn
+_data_ptr = torch.Tensor.data_ptr
 
 
 class PagedKVCache:
@@ -104,7 +103,8 @@ class PagedKVCache:
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"{'a 4-bit pool' if self.fp4 else 'a pool with block scales'} is read as bfloat16 or float16")
         if device.type != "cuda":
-            raise RuntimeError(f"reading {'a 4-bit pool' if self.fp4 else 'a pool with block scales'} needs a GPU device, got {device}")
+            raise RuntimeError(f"reading {'a 4-bit pool' if self.fp4 else 'a pool with block scales'} needs a GPU device, got "
+                               f"{device}")
         nb, bs, hkv, _ = k.shape
         dh = self.head_dim
         slots = slots.contiguous()
@@ -129,9 +129,11 @@ class PagedKVCache:
         if device.type != "cuda":
             self._copy_on_host(np.asarray(src), np.asarray(dst))
             return
-        tensors, pointers, nbytes = self._page_tensors()
-        _native.lib().launch(device, "mllm_copy_pages", pointers, nbytes, len(tensors), self.num_blocks, src.tobytes(),
-                             dst.tobytes(), n)
+        _native.lib().launch(device, "mllm_copy_pages", *self._page_tensors(), self.num_blocks, src.tobytes(), dst.tobytes(), n)
+
+    def check_pages(self) -> None:
+        """ValueError unless `copy_blocks` can take the pools and their scales as they are."""
+        self._page_tensors()
 
     def _copy_on_host(self, src: np.ndarray, dst: np.ndarray) -> None:
         """`copy_blocks` of a pool that is not on a GPU, in torch operations, under the same rules."""
@@ -143,25 +145,29 @@ class PagedKVCache:
         if np.intersect1d(src, dst).size:
             raise ValueError("a block is read and written")
         src, dst = torch.from_numpy(src), torch.from_numpy(dst)
-        for t in self._page_tensors()[0]:
+        self._page_tensors()  # its checks
+        for t in (*self.k, *self.v, *((*self.k_scale, *self.v_scale) if self.fp4 or self.block_scales else ())):
             raw = t.view(torch.uint8)
             raw[dst] = raw[src]
 
     def _page_tensors(self):
-        """Every tensor that holds pages, their addresses and their bytes per page, as arrays mllm_copy_pages reads: made
-        once, and again when an entry of the lists has been replaced."""
-        lists = (self.k, self.v, self.k_scale, self.v_scale) if self.fp4 or self.block_scales else (self.k, self.v)
+        """The addresses of every tensor that holds pages, and their bytes per page, as arrays mllm_copy_pages reads, and their
+        number: checked and packed once, and again when one of them lies elsewhere (an entry replaced, storage swapped)."""
+        tensors = [*self.k, *self.v]
+        if self.fp4 or self.block_scales:
+            tensors += self.k_scale
+            tensors += self.v_scale
+        addresses = list(map(_data_ptr, tensors))
         held = self._pages
-        if held is not None and len(held[0]) == sum(map(len, lists)) and all(map(is_, chain(*lists), held[0])):
-            return held
-        tensors = tuple(chain(*lists))
+        if held is not None and addresses == held[0]:
+            return held[1:]
         for t in tensors:
             if t.shape[0] != self.num_blocks or not t.is_contiguous() or t.device != self.k[0].device:
                 raise ValueError(f"the pools and their scales must be contiguous, of {self.num_blocks} blocks, on one device")
         nbytes = [t.numel() * t.element_size() // max(1, self.num_blocks) for t in tensors]
-        self._pages = (tensors, struct.pack(f"{len(tensors)}Q", *(t.data_ptr() for t in tensors)),
-                       struct.pack(f"{len(tensors)}q", *nbytes))
-        return self._pages
+        self._pages = (addresses, struct.pack(f"{len(tensors)}Q", *addresses), struct.pack(f"{len(tensors)}q", *nbytes),
+                       len(tensors))
+        return self._pages[1:]
 
     @staticmethod
     def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE, block_scales: bool = False) -> int:

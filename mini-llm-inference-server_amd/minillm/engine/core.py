@@ -103,7 +103,8 @@ class EngineCore:
         passes the oracle's).  `chunked_prefill` mixes decode rows and prompt chunks in one step under the
         token budget (see Scheduler).  `kv_cache_dtype` defaults to the model's dtype; torch.float8_e4m3fn
         gives an fp8 pool whose K and V tensors of every layer use the per-tensor scales `kv_scales`
-        (k_scale, v_scale), or, with `kv_scales="blocks"`, a scale for each page and head; torch.float4_e2m1fn_x2 gives a 4-bit pool with block scales.  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
+        (k_scale, v_scale), or, with `kv_scales="blocks"`, a scale for each page and head; torch.float4_e2m1fn_x2 gives a
+        4-bit pool with block scales.  `decode_graphs` (True, or a tuple of batch buckets) runs pure decode steps as
         captured HIP graphs (DecodeGraphs); prefill and mixed steps stay eager.  `sampler(requests,
         logits)` picks each row's next token from its logits [rows, vocab] (default: greedy argmax); a
         row whose prompt chunk stops short of its end ignores its pick."""
@@ -198,12 +199,14 @@ class EngineCore:
         if longest > self.max_model_len or self.blocks.blocks_for(longest) > self.blocks.num_blocks:
             raise ValueError(f"a request of {longest} tokens does not fit max_model_len {self.max_model_len} or the pool of "
                              f"{self.blocks.num_blocks} KV blocks")
+        self.cache.check_pages()  # before anything is taken
         _, copies = sched.fork(req, new_req_id, most, {**req.timeline, "forked": now_ns()})
         self._copy(copies)
 
     def compact(self) -> int:
         """Moves every block that holds K/V to the front of the pool and returns their number n: `cache.k[layer][:n]` and the like
         are then all that the pool holds."""
+        self.cache.check_pages()  # before anything moves
         moves = self.blocks.compact()
         self._copy(moves)
         self.scheduler.moved(moves)

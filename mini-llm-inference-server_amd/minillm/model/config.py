@@ -101,7 +101,9 @@ class LlamaConfig:
         kw["head_dim"] = d.get("head_dim") or kw["hidden_size"] // heads
         kw["rope_theta"], kw["rope_scaling"] = _rope_fields(d)
         nested = d.get("rope_parameters") or {}
-        kw["partial_rotary_factor"] = float(nested.get("partial_rotary_factor", d.get("partial_rotary_factor", 1.0)))
+        part = nested.get("partial_rotary_factor")
+        part = d.get("partial_rotary_factor") if part is None else part
+        kw["partial_rotary_factor"] = 1.0 if part is None else float(part)
         kw["rope_interleaved"] = bool(d.get("rope_interleaved", d.get("rope_interleave", False)))
         kw["eos_token_ids"] = _eos_ids(d.get("eos_token_id"))
         return cls(**kw)

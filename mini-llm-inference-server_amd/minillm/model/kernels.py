@@ -94,8 +94,8 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, dtype: torch.dty
     cos = torch.empty((*positions.shape, 2 * half), dtype=dtype, device=positions.device)
     sin = torch.empty_like(cos)
     if factor is not None:
-        _native.lib().call("mllm_rope_table_scaled", positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half, factor,
-                           _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr(), _native.stream_ptr(positions.device))
+        _native.lib().launch(positions.device, "mllm_rope_table_scaled", positions.data_ptr(), positions.numel(),
+                             inv_freq.data_ptr(), half, factor, _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr())
         return cos, sin
     _native.lib().call("mllm_rope_table", positions.data_ptr(), positions.numel(), inv_freq.data_ptr(), half,
                        _native.dtype_code(dtype), cos.data_ptr(), sin.data_ptr(), _native.stream_ptr(positions.device))

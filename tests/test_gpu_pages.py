@@ -55,6 +55,20 @@ def test_copies(hip, kind, hkv, blocks, layers, bs, dh, n):
     assert all(torch.equal(t.view(torch.uint8), w) for t, w in zip(tensors(cache), want))
 
 
+def test_copies_go_where_the_pools_are(hip):
+    # storage swapped under the same tensor objects between two calls
+    cache = make_cache("fp8_blocks", 3, 30, 2)
+    cache.copy_blocks([1, 2], [3, 4])
+    old = [cache.k[1].data, cache.v_scale[0].data]
+    for t in (cache.k[1], cache.v_scale[0]):
+        t.data = t.view(torch.uint8).clone().view(t.dtype)
+    was = [t.view(torch.uint8).clone() for t in old]
+    want = expected(cache, [5, 6], [7, 8])
+    cache.copy_blocks([5, 6], [7, 8])
+    assert all(torch.equal(t.view(torch.uint8), w) for t, w in zip(tensors(cache), want))
+    assert all(torch.equal(t.view(torch.uint8), w) for t, w in zip(old, was))
+
+
 def test_refused_copies_change_nothing(hip):
     cache = make_cache("fp8_blocks", 2, 9, 2)
     was = [t.view(torch.uint8).clone() for t in tensors(cache)]

@@ -4,6 +4,7 @@ rotary forms.  Sizes, host rules and refusals."""
 import ctypes
 import math
 import random
+import struct
 from pathlib import Path
 
 import pytest
@@ -106,6 +107,12 @@ def test_backend_refusals():
         be.append(k[..., :64], k[..., :64], kc, vc, Meta, **scales)
     with pytest.raises(ValueError, match="describe k's tokens"):
         be.append(k[:3], k[:3], kc, vc, Meta, **scales)
+    for slots in (Meta.slot_mapping.int(), torch.zeros(10, dtype=torch.int64)[::2], Meta.slot_mapping.to("meta")):
+        bad = type("Bad", (Meta,), {"slot_mapping": slots})
+        with pytest.raises(ValueError, match="describe k's tokens"):
+            be.append(k, k, kc, vc, bad, **scales)
+    with pytest.raises(ValueError, match="K and V alike"):
+        be.forward(q, k, k, kc, vc, Meta, v_scale=scales["v_scale"])
     with pytest.raises(ValueError, match="alike"):
         be.append(k, k, kc, vc[:2], Meta, **scales)
     for kw, match in ((dict(q=q[:3]), "N, H, Dh"), (dict(q=q[:, :3]), "N, H, Dh"), (dict(q=q[..., :64]), "N, H, Dh"),
@@ -192,8 +199,6 @@ def test_copy_blocks_refusals():
 
 
 def test_copy_pages_checks_its_arguments():
-    import struct
-
     lib, q = _native.lib(), struct.pack
 
     def call(tensors=q("2Q", 1 << 20, 1 << 21), nbytes=q("2q", 4096, 8), n=2, pages=9, src=q("2q", 1, 2), dst=q("2q", 3, 4), pairs=2):
@@ -208,6 +213,36 @@ def test_copy_pages_checks_its_arguments():
             call(**kw)
     call(pairs=0, src=None)
     call(n=0, tensors=None)
+
+
+def test_copies_follow_pools_that_moved():
+    cache = PagedKVCache(config(head_dim=128), 6, "cpu", FP8, block_scales=True)
+    before = cache._page_tensors()
+    assert cache._page_tensors() is not None and cache._page_tensors() == before
+    kept = cache.v[1].data
+    cache.v[1].data = kept.clone()  # the same tensor object over other memory
+    cache.k_scale[0] = cache.k_scale[0].view(torch.uint8).clone().view(torch.float8_e8m0fnu)
+    after = cache._page_tensors()
+    pointers = struct.unpack(f"{after[2]}Q", after[0])
+    assert pointers == tuple(t.data_ptr() for t in (*cache.k, *cache.v, *cache.k_scale, *cache.v_scale))
+    assert pointers != struct.unpack(f"{before[2]}Q", before[0])
+    cache.k[0] = cache.k[0][1:]
+    with pytest.raises(ValueError, match="of 6 blocks"):
+        cache.check_pages()
+
+
+def test_nothing_is_taken_where_pages_cannot_be_copied():
+    from minillm.engine.core import AddRequest
+
+    core = engine()
+    core.add_request(AddRequest("a", list(range(3, 23)), 8))
+    core.step()
+    core.cache.v[0] = core.cache.v[0].transpose(0, 1)
+    free, running = core.blocks.num_free, list(core.scheduler.running)
+    for call in (lambda: core.fork("a", "b"), core.compact):
+        with pytest.raises(ValueError, match="contiguous"):
+            call()
+    assert core.blocks.num_free == free and core.scheduler.running == running
 
 
 # ------------------------------------------------------------------ forks, trims, compactions
@@ -320,6 +355,8 @@ def test_config_keys_of_the_forms():
     assert cfg.rope_interleaved and cfg.rotary_dim == 8
     cfg = LlamaConfig.from_dict({**base, "rope_interleave": True, "rope_parameters": {"rope_theta": 1e4, "partial_rotary_factor": 0.25}})
     assert cfg.rope_interleaved and cfg.rotary_dim == 4
+    for none in ({"partial_rotary_factor": None}, {"rope_parameters": {"rope_theta": 1e4, "partial_rotary_factor": None}}):
+        assert LlamaConfig.from_dict({**base, **none}).partial_rotary_factor == 1.0
 
 
 @pytest.mark.parametrize("rope", [
