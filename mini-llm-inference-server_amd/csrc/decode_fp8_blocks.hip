@@ -10,6 +10,10 @@
 //     Product m is element m of those: row r of it is dim D r + m of the joint row, and a column keeps the rows of its own head.
 // A tile lies in one page, so its scales are one byte for each of the heads: read through the scalar cache and applied by the
 // conversions.  Every code times its scale is exact in the 16-bit type.  P as in decode_fp4.hip.
+//
+// Bound by HBM reads on large steps: 256 rows of 128-4,096 tokens, 1.18 GB, 185-190 us (6.3 TB/s).  Three rows of 50,000-120,000
+// tokens over 2 KV heads in fp16, 126 MB: 24.4 us (5.2 TB/s).  Small steps are a chain of dependent reads (plan, page ids, tile):
+// 4 rows of 100-700 tokens 8.3 us, the merge 2.6.
 #include "decode_slices.h"
 
 namespace mllm {

@@ -2,7 +2,10 @@
 // which shares whole blocks alone): what a fork of a sequence or a compaction of a pool moves.
 //
 // Bound by memory: a page is read once and written once.  A wavefront moves rows of 1 KB, 16 bytes a lane, kRows of them in
-// flight; pages that are no whole number of such rows (scales) go word by word, one a thread.
+// flight: 2,999 pages of 16 KB in 16 tensors, 1.57 GB, 325 us (4.8 TB/s, what a large copy reaches); with four rows 334, with
+// plain loads and stores 385, with plain stores alone 360.  Eight pages of 32 KB in 64 tensors: 5.5 us.  Pages that are no whole
+// number of such rows (scales) go word by word, one a thread; the eight pages would take 9.4 us that way, and 256 of 16 KB in 16
+// tensors 26.3 instead of 23.2.
 #include <vector>
 
 #include "common.h"

@@ -37,7 +37,8 @@ def check(got, x, *args):
 @pytest.mark.parametrize("interleaved", [True, False])
 @pytest.mark.parametrize("b,t,h,hkv,dh,rot", [
     (1, 1, 32, 8, 128, 128), (1, 33, 8, 1, 128, 64), (4, 257, 12, 4, 64, 64), (2, 5, 3, 3, 96, 24), (3, 700, 8, 8, 256, 64),
-    (1, 9000, 4, 2, 128, 128), (2, 4, 2, 1, 40, 6), (1, 3, 1, 1, 2, 2), (1, 7, 2, 2, 1024, 1024), (1, 11, 5, 1, 80, 80)])
+    (1, 9000, 4, 2, 128, 128), (2, 4, 2, 1, 40, 6), (1, 3, 1, 1, 2, 2), (1, 7, 2, 2, 1024, 1024), (1, 11, 5, 1, 80, 80),
+    (2, 300, 4, 1, 80, 20)])
 def test_forms(hip, dtype, interleaved, b, t, h, hkv, dh, rot):
     from minillm.model import kernels
 
