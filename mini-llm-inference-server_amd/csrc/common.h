@@ -72,6 +72,13 @@ __device__ __forceinline__ uint16_t f32_to_f16_bits(float f) {
 }
 
 __device__ __forceinline__ float f16_bits_to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+template <typename T>
+__device__ __forceinline__ float to_f32(uint16_t b) {
+  if constexpr (std::is_same<T, BF16>::value)
+    return bf16_bits_to_f32(b);
+  else
+    return f16_bits_to_f32(b);
+}
 
 // ---------------------------------------------------------------- fp8 KV pool (OCP e4m3fn)
 // 1 sign, 4 exponent (bias 7) and 3 mantissa bits; no infinities, S.1111.111 is NaN; the largest finite

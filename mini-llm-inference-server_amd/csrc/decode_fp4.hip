@@ -119,7 +119,7 @@ struct Fp4Pages {
         }
       }
     }
-    const TileP<T> pt = softmax_tile<T>(s, m_run, l_run, o);
+    const auto pt = softmax_tile<T, std::is_same<T, F16>::value>(s, m_run, l_run, o);
 #pragma unroll
     for (int j = 0; j < NH; ++j)  // dword j of the four V rows, widened just in time
 #pragma unroll
@@ -131,7 +131,7 @@ struct Fp4Pages {
         for (int hf = 0; hf < 2; ++hf) {
           const u32x2 vf = u32x2{pick_halves(w[0], hf, w[1], hf), pick_halves(w[2], hf, w[3], hf)};
           const int m = 8 * j + 2 * e + hf;
-          add_pv<T>(vf, pt, o[m]);
+          add_pv(vf, pt, o[m]);
         }
       }
   }

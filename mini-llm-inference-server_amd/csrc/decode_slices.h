@@ -30,22 +30,22 @@ struct SlicesArgs {
   float2* part_ml;
 };
 
-// What two fp16 values (`hi`) leave of the floats they were rounded from, as fp16.
-__device__ __forceinline__ uint32_t f16_rest(float a, float b, uint32_t hi) {
-  return pack2<F16>(a - f16_bits_to_f32((uint16_t)hi), b - f16_bits_to_f32((uint16_t)(hi >> 16)));
+// What two 16-bit values (`hi`) leave of the floats they were rounded from, as such values.
+template <typename T>
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t hi) {
+  return pack2<T>(a - to_f32<T>((uint16_t)hi), b - to_f32<T>((uint16_t)(hi >> 16)));
 }
 
-// P of a tile for its products with V: one 16-bit value, in fp16 two.
-template <typename T>
+// P of a tile for its products with V: one 16-bit value, or (SPLIT) two.
+template <typename T, bool SPLIT>
 struct TileP {
-  static constexpr bool kSplit = std::is_same<T, F16>::value;
   u32x2 hi, lo;
 };
 
 // The online softmax over a tile's scores s (exp2 domain, masked): the running maximum, sum and accumulators brought up to
 // it, and P.
-template <typename T, int D>
-__device__ __forceinline__ TileP<T> softmax_tile(float (&s)[4], float& m_run, float& l_run, f32x4 (&o)[D]) {
+template <typename T, bool SPLIT, int D>
+__device__ __forceinline__ TileP<T, SPLIT> softmax_tile(float (&s)[4], float& m_run, float& l_run, f32x4 (&o)[D]) {
   const float mx = maximum_xor32(maximum_xor16(maximum(maximum(s[0], s[1]), maximum(s[2], s[3]))));
   if (__any(mx > m_run + 8.f)) {  // lazy rescale, as in decode.hip
     const float m_new = fmaxf(m_run, mx);
@@ -58,16 +58,16 @@ __device__ __forceinline__ TileP<T> softmax_tile(float (&s)[4], float& m_run, fl
 #pragma unroll
   for (int i = 0; i < 4; ++i) s[i] = fast_exp2(s[i] - m_run);
   l_run += sum_xor32(sum_xor16((s[0] + s[1]) + (s[2] + s[3])));
-  TileP<T> p{u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])}, {0, 0}};
-  if constexpr (TileP<T>::kSplit) p.lo = u32x2{f16_rest(s[0], s[1], p.hi[0]), f16_rest(s[2], s[3], p.hi[1])};
+  TileP<T, SPLIT> p{u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])}, {0, 0}};
+  if constexpr (SPLIT) p.lo = u32x2{rest_of<T>(s[0], s[1], p.hi[0]), rest_of<T>(s[2], s[3], p.hi[1])};
   return p;
 }
 
 // O += V P for one row m of products.
-template <typename T>
-__device__ __forceinline__ void add_pv(u32x2 v, const TileP<T>& p, f32x4& o) {
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void add_pv(u32x2 v, const TileP<T, SPLIT>& p, f32x4& o) {
   o = Mfma<T>::m16x16x16(v, p.hi, o);
-  if constexpr (TileP<T>::kSplit) o = Mfma<T>::m16x16x16(v, p.lo, o);
+  if constexpr (SPLIT) o = Mfma<T>::m16x16x16(v, p.lo, o);
 }
 
 // A workgroup of eight wavefronts takes one bin and HGW groups of NH heads: wavefront w group w % HGW and the tiles w / HGW,

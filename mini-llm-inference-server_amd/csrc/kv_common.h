@@ -15,13 +15,6 @@ int rope_append_fp8_blocks(const std::string& fn, const mllm_rope_append& r, con
 namespace {
 
 template <typename T>
-__device__ __forceinline__ float to_f32(uint16_t b) {
-  if constexpr (std::is_same<T, BF16>::value)
-    return bf16_bits_to_f32(b);
-  else
-    return f16_bits_to_f32(b);
-}
-template <typename T>
 __device__ __forceinline__ uint16_t from_f32(float f) {
   if constexpr (std::is_same<T, BF16>::value)
     return f32_to_bf16_bits(f);
