@@ -9,6 +9,8 @@ The attention's tolerance counts its roundings.  P is rounded to the 16-bit type
 most eps / 2 of sum_j p_j |v_j|; the output by eps / 2 of itself.  Scores and sums are fp32: a score s is off by at most
 (Dh + 4) 2^-24 of sum_d |q_d k_d| / sqrt(Dh), and the weights by that and 2^-21 (exp2 of an argument up to 2^8 and the
 sums).  With A = sum_j p_j |v_j| the bound is eps/2 |out| + (eps/2 + 2 D + 2^-20) A, D the largest score error of the row.
+In rows of one new token P is the sum of two 16-bit values, the second the first one's rounding error (exact in fp32) rounded
+again: (eps/2)^2 A there.
 In fp16 a P below 2^-14 is subnormal, where half a step is 2^-25 whatever p is.  P is taken relative to a maximum that some key
 of the row has reached, so its sum, by which the output is divided, is at least 1: 2^-25 sum_j |v_j| more.
 """
@@ -335,7 +337,8 @@ def step(rows, h, hkv, dtype, bs=16, seed=0, kv=None, spare=1, scale_q=1.0):
                 ds = (132 * 2.0 ** -24 * (qq.abs() @ kk.abs().t().contiguous()) / math.sqrt(128)).masked_fill(~allowed, 0).amax(-1)
                 ref[q0:q0 + n, x * per + y] = o.cpu()
                 low = 2.0 ** -25 * (allowed.double() @ vv.abs()) if dtype == torch.float16 else 0.0
-                bound[q0:q0 + n, x * per + y] = (eps / 2 * o.abs() + (eps / 2 + 2 * ds[:, None] + 2.0 ** -20) * a + tiny + low).cpu()
+                of_p = eps / 2 if n > 1 else (eps / 2) ** 2
+                bound[q0:q0 + n, x * per + y] = (eps / 2 * o.abs() + (of_p + 2 * ds[:, None] + 2.0 ** -20) * a + tiny + low).cpu()
         at, q0 = at + c + n, q0 + n
     return out.double().cpu(), ref, bound, (backend, cache, meta, q)
 
