@@ -137,8 +137,9 @@ struct Staged<kPoolFp8Blocks> {
   u32x4 x;
   uint32_t e;  // their page's scale (uniform: a wavefront's rows lie in one page)
 };
-// 8-bit blocks cost 24 prompt chunks of some 700 tokens over 2,048 405 us where a 16-bit pool takes 370: the way through registers.
-// The codes by DMA into LDS and widened from there took 0.5% less for a ring more, the full operand ring spilled (404.7).
+// 24 prompt chunks of up to 700 tokens over up to 2,048, 32 heads on 8, take 408 us from 8-bit blocks, 401 from an fp8 pool and 369
+// from a 16-bit one with the same values: the way through registers.  The codes by DMA into LDS and widened from there took 0.5%
+// less for a ring more; the full operand ring spilled and gave 0.3%.
 
 // fp8 and 4-bit pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7) is one load of 16 values per
 // lane: row 8 w + l / 8, dims 16 (l % 8) .. +15.  off: the lane's offset from the group base for a full
@@ -151,12 +152,8 @@ __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const Prefi
   const bool whole = kv0 + kBN <= kv_end;
   const int tok = whole ? 0 : min(kv0 + 8 * w + (lane >> 3), last) & (a.bs - 1);  // the row within its block
   if constexpr (POOL == kPoolFp8Blocks) {
-    const unsigned b = ((unsigned)blk < (unsigned)a.num_blocks) ? (unsigned)blk : 0u;
-    const uint64_t at = (uint64_t)b * (unsigned)a.Hkv + head_bytes / kHeadDim;
-    ConstU32* words = (ConstU32*)(IS_V ? a.vs : a.ks);
-    const uint32_t e = words[at >> 2] >> (8 * (unsigned)(at & 3));
-    if (whole) return {ld16(group_base(pool, a, blk, key0) + off), e};  // a load per branch, as below
-    return {ld16(group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7))), e};
+    if (whole) return {ld16(group_base(pool, a, blk, key0) + off), eoff};  // a load per branch, as below
+    return {ld16(group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7))), eoff};
   } else if constexpr (POOL != kPoolFp4) {
     const char* p = whole ? group_base(pool, a, blk, key0) + off
                           : group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7));
@@ -175,6 +172,16 @@ __device__ __forceinline__ Staged<POOL> stage_load(const char* pool, const Prefi
     sp += IS_V ? (kvh * kBlocks + c) * (unsigned)a.bs + (unsigned)tok : ((unsigned)(tok * kBlocks) + c) * (unsigned)a.Hkv + kvh;
     return {ld8(group_base(pool, a, blk, 0) + ((unsigned)tok * (unsigned)a.row_bytes + head_bytes + kLane * (lane & 7))), *sp};
   }
+}
+
+// Pools of 8-bit blocks: where a page's and head's scale byte lies, and that byte (bits 7:0).
+__device__ __forceinline__ unsigned page_scale_at(const PrefillArgs& a, int blk, int kvh) {
+  return ((unsigned)blk < (unsigned)a.num_blocks ? (unsigned)blk : 0u) * (unsigned)a.Hkv + (unsigned)kvh;
+}
+template <bool IS_V>
+__device__ __forceinline__ uint32_t page_scale(const PrefillArgs& a, int blk, int kvh) {
+  const unsigned at = page_scale_at(a, blk, kvh);
+  return ((ConstU32*)(IS_V ? a.vs : a.ks))[at >> 2] >> (8 * (at & 3));
 }
 
 // What a lane adds to its rows' uniform scale address in a full tile (4-bit pools).
@@ -351,6 +358,7 @@ constexpr int kRingK = 4, kRingV = 4;  // K and V tiles in LDS
 constexpr int kVBase = kRingK * kTileBytes;
 constexpr int kIdBase = (kRingK + kRingV) * kTileBytes;
 constexpr int kLdsBytes = kIdBase + 8 * 2 * 64 * 4;
+constexpr int kScaleBytes = 8 * 2 * 2 * 64 * 4;  // 8-bit blocks: the same tiles' scales of K and V
 
 // Online softmax (exp2 domain) of a pair of score tiles (keys kv0 .. kv0 + 127) -> the bf16/fp16 P^T
 // operands of both PV products.  Masks keys past each row's position when the pair reaches past the
@@ -422,7 +430,8 @@ __device__ __forceinline__ void softmax_two(STile& s0, STile& s1, u32x4 (&pf0)[2
 
 template <typename T, int POOL>
 __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
+  constexpr bool kBlocks8 = POOL == kPoolFp8Blocks;
+  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes + (kBlocks8 ? kScaleBytes : 0)];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
@@ -475,6 +484,20 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
   int wbase = 0, wsel = 0;
   auto blk_of = [&](int t) { return __builtin_amdgcn_readfirstlane(idwin[64 * wsel + t - wbase]); };
   load_ids(0, 0);
+  // 8-bit blocks: for each id of a window the dword with its page's scale, of K and of V, a phase behind the ids.  Scalar loads at
+  // each tile held up the matrix phase's first LDS operands, which wait for both at once (417.0 against 412.8 us).
+  const uint32_t* scwin = reinterpret_cast<const uint32_t*>(lds + kLdsBytes) + wu * 256;
+  auto load_scales = [&](int id, int sel) {
+    const unsigned at = page_scale_at(a, id, kvh) & ~3u;
+    dma4(reinterpret_cast<const char*>(a.ks), at, lds_offset(scwin + 128 * sel));
+    dma4(reinterpret_cast<const char*>(a.vs), at, lds_offset(scwin + 128 * sel + 64));
+  };
+  auto scale_of = [&](int t, int blk, bool v) {  // the scale byte of tile t in bits 7:0
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)scwin[128 * wsel + (v ? 64 : 0) + t - wbase]);
+    return w >> (8 * (page_scale_at(a, blk, kvh) & 3));
+  };
+  int first_id = 0;
+  if constexpr (kBlocks8) first_id = pages[min(lane * kBN + g16, last) >> a.bs_shift];
   auto blk_direct = [&](int t) { return pages[min(t * kBN + g16, last) >> a.bs_shift]; };
 
   f32x16 oacc[4];
@@ -492,10 +515,15 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
     for (int t = 0; t < 4; ++t) {
       if (t < ntiles) {
         const int b = blk_direct(t);
-        kx[t] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
-        if (t < 2) vx[t] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
+        const unsigned ek = kBlocks8 ? page_scale<false>(a, b, kvh) : eoff_k;
+        kx[t] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, wu, soff, ek, head_bytes, lane);
+        if (t < 2) {
+          const unsigned ev = kBlocks8 ? page_scale<true>(a, b, kvh) : eoff_v;
+          vx[t] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, wu, soff, ev, head_bytes, lane);
+        }
       }
     }
+    if constexpr (kBlocks8) load_scales(first_id, 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t < ntiles) {
@@ -540,6 +568,8 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
   // the odd one, each widened into LDS at the end of its phase
   Staged<POOL> st_a = {}, st_b = {};
   int k0b = 0, k1b = 0;
+  unsigned k0e = 0, k1e = 0;
+  bool fresh = false;  // a window of ids without its scales
   for (int p = 0; p < 2 * npairs; ++p) {
     const int j = p >> 1;
     const int ta = 2 * j;  // the pair's first tile
@@ -547,14 +577,20 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
       const int v0b = blk_of(ta + 2), v1b = blk_of(ta + 3);
       k0b = blk_of(ta + 4);
       k1b = blk_of(ta + 5);
+      unsigned v0e = eoff_v, v1e = eoff_v;
+      if constexpr (kBlocks8) {
+        v0e = scale_of(ta + 2, v0b, true), v1e = scale_of(ta + 3, v1b, true);
+        k0e = scale_of(ta + 4, k0b, false), k1e = scale_of(ta + 5, k1b, false);
+      }
       if (ta + 7 >= wbase + 64) {  // the next even phase reads ids of tiles ta + 4 .. ta + 7
         wsel ^= 1;
         wbase = ta + 4;
         load_ids(wbase, wsel);
+        fresh = true;
       }
       if constexpr (POOL != kPool16) {
-        if (ta + 2 < ntiles) st_a = stage_load<POOL, true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
-        if (ta + 3 < ntiles) st_b = stage_load<POOL, true>(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, eoff_v, head_bytes, lane);
+        if (ta + 2 < ntiles) st_a = stage_load<POOL, true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, soff, v0e, head_bytes, lane);
+        if (ta + 3 < ntiles) st_b = stage_load<POOL, true>(vc, a, v1b, (ta + 3) * kBN, last, kv_end, wu, soff, v1e, head_bytes, lane);
       } else {
         if (ta + 2 < ntiles)
           dma_tile<true>(vc, a, v0b, (ta + 2) * kBN, last, kv_end, wu, voff0, voff1, head_bytes, lane, v_slot(ta + 2));
@@ -566,8 +602,15 @@ __global__ __launch_bounds__(512) void prefill128_kernel(const PrefillArgs a) {
           dma_tile<false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, koff0, koff1, head_bytes, lane, k_slot(ta + 5));
       }
     } else if constexpr (POOL != kPool16) {
-      if (ta + 4 < ntiles) st_a = stage_load<POOL, false>(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
-      if (ta + 5 < ntiles) st_b = stage_load<POOL, false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, eoff_k, head_bytes, lane);
+      if constexpr (kBlocks8) {
+        // the ids have landed: the even phase waited for the V tiles it loaded behind them (without such tiles nothing will be
+        // read, and page_scale_at stays in the pool whatever it is given)
+        if (fresh) load_scales(idwin[64 * wsel + lane], wsel);
+        fresh = false;
+      }
+      const unsigned ek0 = kBlocks8 ? k0e : eoff_k, ek1 = kBlocks8 ? k1e : eoff_k;
+      if (ta + 4 < ntiles) st_a = stage_load<POOL, false>(kc, a, k0b, (ta + 4) * kBN, last, kv_end, wu, soff, ek0, head_bytes, lane);
+      if (ta + 5 < ntiles) st_b = stage_load<POOL, false>(kc, a, k1b, (ta + 5) * kBN, last, kv_end, wu, soff, ek1, head_bytes, lane);
     }
     if ((p & 1) == grp) {  // matrix phase of pair j
       __builtin_amdgcn_s_setprio(1);
@@ -781,12 +824,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const char* vc = reinterpret_cast<const char*>(a.vc);
   typedef Staged<POOL> Staged2[2];
   auto stage_k = [&](int b, int t, Staged2& x) {
-    x[0] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, eoff_k, head_bytes, lane);
-    x[1] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, eoff_k, head_bytes, lane);
+    const unsigned e = POOL == kPoolFp8Blocks ? page_scale<false>(a, b, kvh) : eoff_k;
+    x[0] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, e, head_bytes, lane);
+    x[1] = stage_load<POOL, false>(kc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, e, head_bytes, lane);
   };
   auto stage_v = [&](int b, int t, Staged2& x) {
-    x[0] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, eoff_v, head_bytes, lane);
-    x[1] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, eoff_v, head_bytes, lane);
+    const unsigned e = POOL == kPoolFp8Blocks ? page_scale<true>(a, b, kvh) : eoff_v;
+    x[0] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu, soff0, e, head_bytes, lane);
+    x[1] = stage_load<POOL, true>(vc, a, b, t * kBN, last, kv_end, 2 * wu + 1, soff1, e, head_bytes, lane);
   };
   auto store_k = [&](const Staged2& x, char* slot) {
     stage_store<T, false>(x[0], 2 * wu, lane, slot);
@@ -954,6 +999,7 @@ int paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head, co
                MLLM_ERR_INVALID, fn + ": null pointer");
   MLLM_REQUIRE(pool != kPoolFp8Blocks || ((uintptr_t)k_scales | (uintptr_t)v_scales) % 4 == 0, MLLM_ERR_UNSUPPORTED,
                fn + ": scales must be 4-byte aligned");
+  MLLM_REQUIRE(pool != kPoolFp8Blocks || num_blocks * num_kv_heads < (1ll << 32), MLLM_ERR_UNSUPPORTED, fn + ": pool too large");
   const bool aligned = ((uintptr_t)q % 16 == 0) && ((uintptr_t)out % 16 == 0) && ((uintptr_t)k_cache % 16 == 0) &&
                        ((uintptr_t)v_cache % 16 == 0) && (q_stride_tok * 2) % 16 == 0 &&
                        (q_stride_head * 2) % 16 == 0 && (out_stride_tok * 2) % 16 == 0 && (out_stride_head * 2) % 16 == 0;

@@ -386,6 +386,13 @@ def test_prefill_block_sizes(hip, bs, prefill_rows):
     check(*step([(0, 100), (77, 33), (31, 64), (250, 300)], 32, 8, torch.bfloat16, bs=bs, seed=bs)[:3])
 
 
+@pytest.mark.parametrize("h,hkv,bs", [(8, 2, 16), (6, 3, 16), (8, 1, 64), (10, 5, 32)])
+def test_prefill_behind_long_contexts(hip, h, hkv, bs, prefill_rows):
+    # ids and scales are taken 64 tiles (4,096 tokens) at a time: contexts that end around and behind such windows
+    rows = [(3839, 2), (3900, 130), (4090, 300), (8100, 64), (9000, 40), (12345, 70)]
+    check(*step(rows, h, hkv, torch.bfloat16, bs=bs, seed=hkv)[:3])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sharp_softmax(hip, dtype):
     # scores over hundreds: rows that one key wins, and the running maximum moves
