@@ -20,7 +20,7 @@
 //
 // Bound by launch latency for few tokens (32 rows of 8 heads: 3.6 us, their read back 2.9) and by memory for many: 8,200 tokens
 // of 8 heads, 50 MB, are appended in 12.1 us (4.2 TB/s; 20.9 with windows of 16 tokens that read what else their runs hold again,
-// 14.4 with one routine for all runs, whose registers halve the wavefronts on a CU) and read back in 10.4-11.0 (4.7 TB/s).
+// 14.4 with one routine for all runs, whose registers halve the wavefronts on a CU) and read back in 9.5 (5.3 TB/s).
 #include "kv_common.h"
 
 namespace mllm {
