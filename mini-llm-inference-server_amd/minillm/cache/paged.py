@@ -38,7 +38,7 @@ BLOCK_SIZE = 16
 FP4 = torch.float4_e2m1fn_x2
 FP4_BLOCK = 32  # dims per scale of a 4-bit pool
 FP8 = torch.float8_e4m3fn
-_data_ptr = torch.Tensor.data_ptr
+_data_ptr, _nbytes, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.nbytes.__get__, torch.Tensor.is_contiguous
 
 
 class PagedKVCache:
@@ -152,22 +152,24 @@ class PagedKVCache:
 
     def _page_tensors(self):
         """The addresses of every tensor that holds pages, and their bytes per page, as arrays mllm_copy_pages reads, and their
-        number: checked and packed once, and again when one of them lies elsewhere (an entry replaced, storage swapped)."""
+        number: checked and packed once, and again when one of them lies elsewhere or spans other bytes (an entry replaced, storage
+        swapped, a view of the same memory).  Pages are bytes here, so these say all that the copies go by."""
         tensors = [*self.k, *self.v]
         if self.fp4 or self.block_scales:
             tensors += self.k_scale
             tensors += self.v_scale
         addresses = list(map(_data_ptr, tensors))
+        span = (self.num_blocks, list(map(_nbytes, tensors)))
         held = self._pages
-        if held is not None and addresses == held[0]:
-            return held[1:]
+        if held is not None and addresses == held[0] and span == held[1] and all(map(_is_contiguous, tensors)):
+            return held[2:]
         for t in tensors:
             if t.shape[0] != self.num_blocks or not t.is_contiguous() or t.device != self.k[0].device:
                 raise ValueError(f"the pools and their scales must be contiguous, of {self.num_blocks} blocks, on one device")
-        nbytes = [t.numel() * t.element_size() // max(1, self.num_blocks) for t in tensors]
-        self._pages = (addresses, struct.pack(f"{len(tensors)}Q", *addresses), struct.pack(f"{len(tensors)}q", *nbytes),
+        nbytes = [n // max(1, self.num_blocks) for n in span[1]]
+        self._pages = (addresses, span, struct.pack(f"{len(tensors)}Q", *addresses), struct.pack(f"{len(tensors)}q", *nbytes),
                        len(tensors))
-        return self._pages[1:]
+        return self._pages[2:]
 
     @staticmethod
     def bytes_per_block(config, dtype: torch.dtype, block_size: int = BLOCK_SIZE, block_scales: bool = False) -> int:
