@@ -152,9 +152,17 @@ class DeviceBlockTables:
     """A device-resident mirror of the block manager's tables: one row of `max_blocks` int32 block ids per
     request (keyed by any hashable, the engine's Request objects), so a step uploads only the ids each
     request gained since its last step instead of every table (the reference's build flattens and uploads
-    all of them, metadata.py:82-83,101).  A request's list of block ids only grows while it runs; a new
-    list object (re-admission after preemption) is uploaded whole.  Row `max_rows` is reserved for
-    padding rows: its only block id is -1."""
+    all of them, metadata.py:82-83,101).  A request's list of block ids grows while it runs; a new
+    list object (re-admission after preemption) is uploaded whole.  A list that is shortened in place has to be told
+    (`shortened`, which BlockManager.trim calls): it may be as long as before at the next step and hold other blocks.
+    Row `max_rows` is reserved for padding rows: its only block id is -1."""
+
+    _cuts = 0  # lists shortened so far, whoever holds them
+
+    @staticmethod
+    def shortened() -> None:
+        """A list of block ids has lost entries in place: every mirror compares its rows with what it has uploaded, once."""
+        DeviceBlockTables._cuts += 1
 
     def __init__(self, max_rows: int, max_blocks: int, device) -> None:
         self.max_rows, self.max_blocks = int(max_rows), int(max_blocks)
@@ -164,7 +172,7 @@ class DeviceBlockTables:
         self.tables[self.pad_row * self.max_blocks] = -1
         self._free = list(range(self.max_rows - 1, -1, -1))
         self._row: dict = {}
-        self._synced: dict = {}  # key -> (the block-id list object, entries already on the device)
+        self._synced: dict = {}  # key -> (the block-id list object, its entries on the device, the cuts they have seen)
 
     def release(self, key) -> None:
         row = self._row.pop(key, None)
@@ -174,7 +182,7 @@ class DeviceBlockTables:
 
     def sync(self, keys, seqs: list[SeqStep]) -> tuple[list[int], list[int]]:
         """Rows of the step's sequences and the flat (index, id) updates that bring them up to date."""
-        rows, updates = [], []
+        rows, updates, cuts = [], [], DeviceBlockTables._cuts
         for key, s in zip(keys, seqs):
             ids = s.block_ids
             if len(ids) > self.max_blocks:
@@ -185,11 +193,17 @@ class DeviceBlockTables:
                     raise ValueError(f"more than {self.max_rows} requests hold resident table rows")
                 row = self._row[key] = self._free.pop()
             prev = self._synced.get(key)
-            start = prev[1] if prev is not None and prev[0] is ids and prev[1] <= len(ids) else 0
+            sent = prev[1] if prev is not None and prev[0] is ids else []
+            start = len(sent)
+            if start and prev[2] != cuts or start > len(ids):
+                start = next((j for j, (a, b) in enumerate(zip(sent, ids)) if a != b), min(start, len(ids)))
+                del sent[start:]
             base = row * self.max_blocks
-            for j in range(start, len(ids)):
-                updates += (base + j, ids[j])
-            self._synced[key] = (ids, len(ids))
+            if start < len(ids):
+                for j in range(start, len(ids)):
+                    updates += (base + j, ids[j])
+                sent += ids[start:]
+            self._synced[key] = (ids, sent, cuts)
             rows.append(row)
         return rows, updates
 

@@ -22,6 +22,8 @@ from collections import Counter
 
 import numpy as np
 
+from ..attention.metadata import DeviceBlockTables
+
 BLANK, NAMED = 0, 1
 
 
@@ -110,12 +112,16 @@ class BlockManager:
         return table[:full] + fresh, [(table[full], fresh[0])] if used > full else []
 
     def trim(self, table: list[int], num_tokens: int) -> None:
-        """Releases the blocks of `table` behind its first `num_tokens` tokens, in place."""
+        """Releases the blocks of `table` behind its first `num_tokens` tokens, in place; resident block tables that mirror the list
+        (DeviceBlockTables) follow it.  The owner's own counts are its own to cut: a request's num_cached, and of its names
+        (num_named, block_hashes) those of blocks that are no longer full.  A page that the cut goes through keeps the scales of
+        a pool that has them (include/minillm_hip.h)."""
         keep = self.blocks_for(num_tokens)
         if keep < len(table):
             tail = table[keep:]
             del table[keep:]
             self.free(tail)
+            DeviceBlockTables.shortened()
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves every block that holds K/V (held, or named by the prefix cache) into the lowest ids.  Returns the (from, to)
