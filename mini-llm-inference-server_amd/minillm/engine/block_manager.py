@@ -114,9 +114,16 @@ class BlockManager:
     def trim(self, table: list[int], num_tokens: int) -> None:
         """Releases the blocks of `table` behind its first `num_tokens` tokens, in place; resident block tables that mirror the list
         (DeviceBlockTables) follow it.  The owner's own counts are its own to cut: a request's num_cached, and of its names
-        (num_named, block_hashes) those of blocks that are no longer full.  A page that the cut goes through keeps the scales of
-        a pool that has them (include/minillm_hip.h)."""
+        (num_named, block_hashes) those of blocks that are no longer full.  A page that the cut goes through will take other tokens:
+        it loses its name, and ValueError if another table lists it too (`fork` then gives a table with a copy of it).  It keeps
+        the scales of a pool that has them (include/minillm_hip.h)."""
         keep = self.blocks_for(num_tokens)
+        if keep <= len(table) and int(num_tokens) % self.block_size:
+            cut = table[keep - 1]
+            if self._holders[cut] > 1:
+                raise ValueError(f"block {cut} is shared: cut a fork of the table instead")
+            if self._named(cut):
+                self.prefix.forget(cut)
         if keep < len(table):
             tail = table[keep:]
             del table[keep:]

@@ -90,3 +90,42 @@ def test_lists_that_change_at_random(seed):
         if lists and rng.random() < 0.6:
             mirror.step({k: lists[k] for k in rng.sample(list(lists), rng.randint(1, len(lists)))})
         blocks.check(list(lists.values()))
+
+
+def test_a_cut_through_a_shared_block_is_refused():
+    # its next tokens would go into the other table's block; at a block's end, or behind a copy, nothing is shared
+    blocks = BlockManager(10, 16)
+    table = blocks.allocate(4)
+    child, copies = blocks.fork(table, 64)
+    assert child == table and copies == []
+    for t in (table, child):
+        with pytest.raises(ValueError, match="shared"):
+            blocks.trim(t, 40)
+        assert len(t) == 4
+    blocks.check([table, child])
+    blocks.trim(child, 32)
+    own, copies = blocks.fork(table, 40)
+    blocks.trim(own, 33)
+    blocks.check([table, child, own])
+    blocks.free(child), blocks.free(own)
+    blocks.trim(table, 40)
+    blocks.check([table])
+    with pytest.raises(ValueError, match="shared"):
+        other, _ = blocks.fork(table, 48)
+        blocks.trim(other, 47)  # within its last block, with none to release
+
+
+def test_a_block_that_is_cut_loses_its_name():
+    from minillm.cache.prefix import PrefixCache
+
+    prefix = PrefixCache()
+    blocks = BlockManager(6, 16, prefix)
+    table = blocks.allocate(3)
+    for i, b in enumerate(table):
+        prefix.insert(b"%d" % i, b)
+    blocks.trim(table, 20)
+    assert prefix.lookup([b"0", b"1"]) == table[:1] and blocks.num_cached == 1  # the third, whole and idle
+    blocks.check([table])
+    blocks.trim(table, 16)
+    assert prefix.lookup([b"0"]) == table
+    blocks.check([table])
