@@ -131,13 +131,24 @@ class BlockManager:
             DeviceBlockTables.shortened()
 
     def compact(self) -> list[tuple[int, int]]:
-        """Moves every block that holds K/V (held, or named by the prefix cache) into the lowest ids.  Returns the (from, to)
-        blocks to copy (PagedKVCache.copy_blocks): no block is in both roles.  Names, holders and the order of eviction follow;
-        tables that list a moved block are the caller's to rewrite."""
+        """Moves every block that holds K/V (held, or named by the prefix cache) into the lowest ids: `gaps` and `move` in one.
+        Returns the (from, to) blocks to copy (PagedKVCache.copy_blocks); tables that list a moved block are the caller's to
+        rewrite."""
+        moves = self.gaps()
+        self.move(moves)
+        return moves
+
+    def gaps(self) -> list[tuple[int, int]]:
+        """The (from, to) blocks that bring every block with K/V into the lowest ids: no block is in both roles, and those to copy
+        to hold nothing.  Changes nothing itself."""
+        tier = {b: tier for _, (tier, b) in self._live()}
+        keeps = [b for b in range(self.num_blocks) if self._holders[b] or tier[b] == NAMED]
+        gaps = [b for b in range(len(keeps)) if not self._holders[b] and tier[b] == BLANK]
+        return list(zip((b for b in keeps if b >= len(keeps)), gaps))
+
+    def move(self, moves: list[tuple[int, int]]) -> None:
+        """The blocks `gaps` gave have been copied: names, holders and the order of eviction follow."""
         live = {b: (tier, t) for t, (tier, b) in self._live()}
-        keeps = [b for b in range(self.num_blocks) if self._holders[b] or live[b][0] == NAMED]
-        gaps = [b for b in range(len(keeps)) if not self._holders[b] and live[b][0] == BLANK]
-        moves = list(zip((b for b in keeps if b >= len(keeps)), gaps))
         for src, dst in moves:
             self._holders[dst], self._holders[src] = self._holders[src], 0
             if self.prefix is not None:
@@ -152,7 +163,6 @@ class BlockManager:
                 del live[dst]
         self._heap = [(tier, t, b) for b, (tier, t) in live.items()]
         heapq.heapify(self._heap)
-        return moves
 
     def clear_cache(self) -> None:
         """Every idle-named block becomes blank (its name dropped), in eviction order."""

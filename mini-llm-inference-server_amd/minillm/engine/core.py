@@ -200,15 +200,21 @@ class EngineCore:
             raise ValueError(f"a request of {longest} tokens does not fit max_model_len {self.max_model_len} or the pool of "
                              f"{self.blocks.num_blocks} KV blocks")
         self.cache.check_pages()  # before anything is taken
-        _, copies = sched.fork(req, new_req_id, most, {**req.timeline, "forked": now_ns()})
-        self._copy(copies)
+        child, copies = sched.fork(req, new_req_id, most, {**req.timeline, "forked": now_ns()})
+        try:
+            self._copy(copies)
+        except BaseException:  # it has not run: its blocks are free again
+            self.blocks.free(child.block_ids)
+            raise
+        sched.join(child)
 
     def compact(self) -> int:
         """Moves every block that holds K/V to the front of the pool and returns their number n: `cache.k[layer][:n]` and the like
         are then all that the pool holds."""
-        self.cache.check_pages()  # before anything moves
-        moves = self.blocks.compact()
-        self._copy(moves)
+        self.cache.check_pages()
+        moves = self.blocks.gaps()
+        self._copy(moves)  # to blocks that hold nothing: where it raises, all is as it was
+        self.blocks.move(moves)
         self.scheduler.moved(moves)
         return self.blocks.num_blocks - self.blocks.num_free + self.blocks.num_cached
 

@@ -243,7 +243,7 @@ class Scheduler:
 
     def fork(self, req: Request, req_id: str, max_tokens: int, timeline: dict) -> tuple[Request, list[tuple[int, int]]]:
         """A running request's continuation under a name of its own, on the same blocks but for a last one that is not full,
-        and the (from, to) blocks to copy."""
+        and the (from, to) blocks to copy.  It holds its blocks and joins the running set when they have been copied (`join`)."""
         if len(self.running) >= self.max_num_seqs:
             raise RuntimeError(f"{len(self.running)} requests run already, and at most {self.max_num_seqs} may")
         waits = req.num_tokens - req.num_cached > 1  # within its prompt: blocks for all of it
@@ -252,8 +252,10 @@ class Scheduler:
         child = Request(req_id, list(req.prompt), max_tokens, req.stop_ids, timeline, output=list(req.output), block_ids=table,
                         num_cached=req.num_cached, root=req.root, block_hashes=list(req.block_hashes),
                         num_named=min(req.num_named, full), num_cached_tokens=req.num_cached_tokens)
-        self.running.append(child)
         return child, copies
+
+    def join(self, child: Request) -> None:
+        self.running.append(child)
 
     def moved(self, moves: list[tuple[int, int]]) -> None:
         """Rewrites the running requests' tables after blocks have moved (as new lists, which are uploaded whole)."""
