@@ -37,6 +37,7 @@ from .. import _native
 BLOCK_SIZE = 16
 FP4 = torch.float4_e2m1fn_x2
 FP4_BLOCK = 32  # dims per scale of a 4-bit pool
+MAX_PAGE_BYTES = (1 << 23) - 1  # of one tensor, that mllm_copy_pages takes
 FP8 = torch.float8_e4m3fn
 _data_ptr, _nbytes, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.nbytes.__get__, torch.Tensor.is_contiguous
 
@@ -118,7 +119,8 @@ class PagedKVCache:
     def copy_blocks(self, src, dst) -> None:
         """Block dst[i] becomes a copy of block src[i], in every layer's K, V and scales: one call on the current stream of the
         pool's device.  `src` and `dst` are sequences of block ids on the host, of one length.  A block written twice, or read
-        and written, is refused (ValueError), as is one outside the pool; nothing is copied then."""
+        and written, is refused (ValueError), as is one outside the pool; nothing is copied then.  On a GPU a block of one tensor
+        may be of up to 8 MiB - 1."""
         src, dst = _block_ids(src), _block_ids(dst)
         n = len(src)
         if n != len(dst):
@@ -167,6 +169,8 @@ class PagedKVCache:
             if t.shape[0] != self.num_blocks or not t.is_contiguous() or t.device != self.k[0].device:
                 raise ValueError(f"the pools and their scales must be contiguous, of {self.num_blocks} blocks, on one device")
         nbytes = [n // max(1, self.num_blocks) for n in span[1]]
+        if tensors[0].is_cuda and max(nbytes) > MAX_PAGE_BYTES:
+            raise ValueError(f"pages of {max(nbytes)} bytes are too large to copy: at most {MAX_PAGE_BYTES}")
         self._pages = (addresses, span, struct.pack(f"{len(tensors)}Q", *addresses), struct.pack(f"{len(tensors)}q", *nbytes),
                        len(tensors))
         return self._pages[2:]

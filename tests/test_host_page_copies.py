@@ -73,3 +73,32 @@ def test_the_number_of_blocks_counts():
     cache.num_blocks = 16
     with pytest.raises(ValueError, match="of 16 blocks"):
         cache.check_pages()
+
+
+def test_pages_the_library_refuses_are_refused_by_the_check(monkeypatch):
+    # the library's limit and the check's are one; the check applies it to pools on a GPU
+    from minillm import _native
+    from minillm.cache import paged
+
+    def copy(nbytes):
+        _native.lib().call("mllm_copy_pages", struct.pack("Q", 1 << 20), struct.pack("q", nbytes), 1, 4, struct.pack("q", 0),
+                           struct.pack("q", 9), 1, None)
+
+    with pytest.raises(ValueError, match="block 9 is outside"):
+        copy(paged.MAX_PAGE_BYTES)
+    with pytest.raises(ValueError, match="page too large"):
+        copy(paged.MAX_PAGE_BYTES + 1)
+    cache = make_cache()
+    monkeypatch.setattr(paged, "MAX_PAGE_BYTES", 16 * 2 * 128 - 1)
+    cache.check_pages()  # on the host: any size
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    cache = make_cache()
+    cache.k[0] = cache.k[0].as_subclass(OnGpu)
+    for call in (cache.check_pages, lambda: cache.copy_blocks([1], [2])):
+        with pytest.raises(ValueError, match="too large to copy"):
+            call()
+    monkeypatch.setattr(paged, "MAX_PAGE_BYTES", 16 * 2 * 128)
+    cache.check_pages()
