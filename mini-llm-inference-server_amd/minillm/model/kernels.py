@@ -38,6 +38,19 @@ def usable(x: torch.Tensor, dtype: torch.dtype | None = None, grad_ok: bool = Fa
             and x.device.index == torch.cuda.current_device() and _native.available())
 
 
+def for_inference(name: str, *operands: torch.Tensor) -> None:
+    """RuntimeError where a call of the public kernel `name`, which torch does not follow, would lose what torch is asked to
+    follow: a gradient or a forward-mode tangent of an operand, or the operands themselves in a trace."""
+    if torch.is_grad_enabled() and any(x.requires_grad for x in operands):
+        raise RuntimeError(f"{name} is for inference: it has no gradient (call it under no_grad, or the modules)")
+    if torch.compiler.is_compiling():  # breaks its graph around the call
+        return
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in operands):
+        raise RuntimeError(f"{name} is for inference: it has no forward-mode derivative (call it on primals, or the modules)")
+    if torch.jit.is_tracing() or _transform() is not None or any(map(_wrapped, operands)):
+        raise RuntimeError(f"{name} is for inference: it cannot be traced or transformed (call the modules)")
+
+
 def bare(module: torch.nn.Module, cls: type) -> bool:
     d = module.__dict__
     return type(module) is cls and "forward" not in d \
@@ -125,7 +138,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
                  k_weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """RMSNorm of every head of q [B, H, T, Dh] and k [B, Hkv, T, Dh], then their rotation by cos and sin [B, T, Dh], in
     one launch: fp32 arithmetic, one rounding.  Dh a multiple of 16, at most 1024; bfloat16 or float16 throughout.  For
-    inference: operands that need a gradient are refused."""
+    inference: operands that need a gradient or carry a tangent are refused, as are traces and functorch transforms."""
     b, h, t, dh = q.shape
     dtype, device, of_k, table = q.dtype, q.device, k.shape, (b, t, dh)
     if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh:
@@ -134,10 +147,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         raise ValueError(f"cos and sin must be [B, T, Dh] = [{b}, {t}, {dh}]")
     if not (dtype == k.dtype == cos.dtype == sin.dtype and device == k.device == cos.device == sin.device):
         raise ValueError("q, k, cos and sin must share one dtype and device")
+    for_inference("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     if dtype not in _DTYPES or device.type != "cuda":
         raise ValueError("q must be bfloat16 or float16 on a GPU")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        raise RuntimeError("qk_norm_rope is for inference: it has no gradient (call it under no_grad, or the modules)")
     check_norms((q_weight, k_weight, eps), q)
     sq, sk, sc = q.stride(), k.stride(), cos.stride()
     if sq[3] != 1 or sk[3] != 1:
@@ -167,7 +179,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     """q [B, H, T, Dh] and k [B, Hkv, T, Dh] turned by positions [B, T] (int64) times inv_freq [R / 2] (float32), angles in 64
     bits: the first R dims of each head in pairs (i, i + R / 2), or (2 i, 2 i + 1) when `interleaved`, scaled by `factor`;
     dims behind them are copied.  bfloat16 or float16; fp32 arithmetic, one rounding.  The results have the operands' shapes
-    and their order in memory, densely.  For inference: operands that need a gradient are refused."""
+    and their order in memory, densely.  For inference: operands that need a gradient or carry a tangent are refused, as are
+    traces and functorch transforms."""
     b, h, t, dh = q.shape
     dtype, device, of_k = q.dtype, q.device, k.shape
     if len(of_k) != 4 or of_k[0] != b or of_k[2] != t or of_k[3] != dh or of_k[1] < 1:
@@ -178,12 +191,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
         raise ValueError(f"inv_freq must be one row of float32, one to Dh / 2 = {dh // 2} of them")
     if not (dtype == k.dtype and device == k.device == positions.device == inv_freq.device):
         raise ValueError("q and k must share one dtype, and all operands one device")
+    for_inference("rotary", q, k, inv_freq)
     if dtype not in _DTYPES or device.type != "cuda":
         raise ValueError("q must be bfloat16 or float16 on a GPU")
     if not math.isfinite(factor):
         raise ValueError("factor must be finite")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or inv_freq.requires_grad):
-        raise RuntimeError("rotary is for inference: it has no gradient (call it under no_grad)")
     sq, sk, sp = q.stride(), k.stride(), positions.stride()
     if sq[3] != 1 or sk[3] != 1:
         q, k = q.contiguous(), k.contiguous()
