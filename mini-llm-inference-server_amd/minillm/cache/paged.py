@@ -33,6 +33,7 @@ import numpy as np
 import torch
 
 from .. import _native
+from ..attention.hip_backend import check_scales
 
 BLOCK_SIZE = 16
 FP4 = torch.float4_e2m1fn_x2
@@ -103,6 +104,9 @@ class PagedKVCache:
             return got[0], got[1]
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"{'a 4-bit pool' if self.fp4 else 'a pool with block scales'} is read as bfloat16 or float16")
+        if v.shape != k.shape or v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("the pools must be alike and contiguous")
+        check_scales(k, self.k_scale[layer], self.v_scale[layer])
         if device.type != "cuda":
             raise RuntimeError(f"reading {'a 4-bit pool' if self.fp4 else 'a pool with block scales'} needs a GPU device, got "
                                f"{device}")
