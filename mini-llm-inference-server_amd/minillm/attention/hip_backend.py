@@ -304,6 +304,11 @@ def check_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         raise ValueError("q, out and the pools must share one device")
 
 
+def slots_ok(slots: torch.Tensor, n: int, device) -> bool:
+    """Whether the append kernels may read n slots there."""
+    return slots.numel() == n and slots.device == device and slots.dtype == torch.int64 and slots.is_contiguous()
+
+
 def check_norms(qk_norm, q: torch.Tensor, *others: torch.Tensor) -> None:
     """ValueError unless qk_norm is (q weight [Dh], k weight [Dh], eps) for rows like q's, and the `others` are of q's type on its
     device."""
@@ -462,6 +467,8 @@ class HipBackend(AttentionBackend):
             if not q.device == k.device == v.device == k_cache.device == v_cache.device:
                 raise ValueError("q, k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
+            if not slots_ok(meta.slot_mapping, n, q.device):
+                raise ValueError(f"the metadata's slot_mapping must be {n} contiguous int64 on the pools' device")
         elif fp8:
             if isinstance(v_scale, torch.Tensor) and v_scale.dtype == SCALES4:
                 raise ValueError("block scales are for K and V alike")
@@ -571,12 +578,10 @@ class HipBackend(AttentionBackend):
                 dh *= 2
             if len(rows) != 3 or rows[1] != hkv or rows[2] != dh or v.shape != rows or v.dtype != dtype:
                 raise ValueError(f"k and v must be [N, Hkv, Dh] = [N, {hkv}, {dh}] of one dtype")
-            slots = meta.slot_mapping
-            if slots.numel() != rows[0] or slots.device != k_cache.device or slots.dtype != torch.int64 \
-                    or not slots.is_contiguous() or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
+            slots, device = meta.slot_mapping, k_cache.device
+            if not slots_ok(slots, rows[0], device) or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype \
                     or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
                 raise ValueError("the pools must be alike and contiguous, and the metadata describe k's tokens")
-            device = k_cache.device
             if not k.device == v.device == device == v_cache.device:
                 raise ValueError("k, v and the pools must share one device")
             check_scales(k_cache, k_scale, v_scale)
