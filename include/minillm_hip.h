@@ -474,13 +474,14 @@ int mllm_paged_prefill_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride
 
 /*
  * 8-bit KV pool with a scale for each block of tokens and head.  No counterpart in the reference, whose planned fp8 cache has
- * one scale per tensor (docs/distributed_inference_plan.md:310): nothing to calibrate, nothing that saturates.
+ * one scale per tensor (docs/distributed_inference_plan.md:310): nothing to calibrate, and only the 16-bit type's largest
+ * magnitudes saturate (below).
  *   codes               [num_blocks, block_size, Hkv, 128] e4m3fn bytes
  *   k_scales, v_scales  [num_blocks, Hkv] e8m0 bytes, 4-byte aligned, readable up to the next multiple of 4 bytes
  *   value = e4m3fn(code) * 2^(scale - 127); scale 255: NaN
  * A run is a step's consecutive tokens at consecutive slots of one page.  Its exponent is the least e for which the largest
  * finite magnitude of its tokens (of a head's K or V) is at most 448 * 2^(e - 127), kept within the exponents whose values
- * the 16-bit type holds (bf16: 10 .. 246, fp16: 112 .. 134; magnitudes above saturate).  A run at a page's first slot begins
+ * the 16-bit type holds (bf16: 10 .. 246, fp16: 112 .. 134; magnitudes above 448 times the last, 2.98e38 or 57,344, saturate).  A run at a page's first slot begins
  * the page's block anew under e; a run behind earlier tokens of the page takes max(e, scale), and where that grows, the codes
  * of the slots before the run are rounded again to it.  Roundings go to nearest with ties to even; an infinity or a NaN becomes
  * the code of NaN.  A pool is written and read with one 16-bit type.  head_dim 128, block_size 16, 32 or 64.

@@ -20,7 +20,9 @@
 //
 // Bound by launch latency for few tokens (32 rows of 8 heads: 3.6 us, their read back 2.9) and by memory for many: 8,200 tokens
 // of 8 heads, 50 MB, are appended in 12.1 us (4.2 TB/s; 20.9 with windows of 16 tokens that read what else their runs hold again,
-// 14.4 with one routine for all runs, whose registers halve the wavefronts on a CU) and read back in 9.5 (5.3 TB/s).
+// 14.4 with one routine for all runs, whose registers halve the wavefronts on a CU) and read back in 9.5 (5.3 TB/s).  With the
+// rotation and 32 heads of q: 32 rows 3.4 us, with the norms 3.3; 8,200 tokens, 189 MB, 43.5 and 35.7 (4.3 and 5.3 TB/s: the
+// rotation alone rounds each product and sum as torch does), where the same into a 16-bit pool, 206 MB, takes 36.
 #include "kv_common.h"
 
 namespace mllm {
@@ -415,8 +417,11 @@ __global__ __launch_bounds__(256) void read_fp8_blocks_kernel(const char* __rest
 
 // Up to so many tokens a wavefront takes four: few tokens are bound by the latency of a wavefront's chain, many by its
 // instructions and by what is read again.  Of 8 heads, four tokens a wavefront against whole runs: 64 rows of one token 3.0 us
-// against 7.2, 1,024 rows 4.3 against 8.4; 64 tokens in runs of 16 3.5 against 3.4, 1,024 5.2 against 3.7, 8,192 21.2 against
-// 11.4.  A step of up to 1,024 tokens may be decode rows throughout, one of more is prompts for the most part.
+// against 7.2, 1,024 rows 3.9 against 7.9; 64 tokens in runs of 16 3.5 against 3.4, 1,024 4.7 against 3.8, 8,200 20.5 against
+// 10.9.  With rotation and 32 heads of q, which four tokens a wavefront turn up to four times: 1,024 rows 8.8 against 11.9 (with
+// norms 7.1 against 11.0), 1,024 in runs of 16 11.7 against 8.5 (8.5 against 6.6), 4,096 rows 26.7 against 27.9, 8,200 in runs
+// of 16 66 against 44.  A step of up to 1,024 tokens may be decode rows throughout, one of more is prompts for the most part; the
+// number of tokens alone loses up to 3 us to the better split on steps of 512-1,024 prompt tokens.
 constexpr int64_t kSmallStep = 1024;
 
 int check_blocks(const std::string& fn, int32_t dtype, int64_t num_tokens, int64_t num_blocks, int32_t block_size,

@@ -165,7 +165,8 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const int64_t* __restri
 }
 
 // The same for frequencies scaled to long contexts: the angle in 64 bits, reduced to a part of a turn there (in 32 bits it is off
-// by up to 2^-24 of the position), and cos and sin times `factor`.
+// by up to 2^-24 of the position), and cos and sin times `factor`.  A launch and the tables' bytes, as above: 32 positions 2.3 us (the
+// plain one 2.3), 8,196 of 64 frequencies, 4.2 MB written, 3.3 (3.7).
 template <typename T>
 __global__ __launch_bounds__(256) void rope_table_scaled_kernel(const int64_t* __restrict__ pos, int64_t n,
                                                                 const float* __restrict__ inv_freq, int half, float factor,

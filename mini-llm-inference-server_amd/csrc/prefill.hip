@@ -35,12 +35,15 @@
 // is folded into the softmax scale and v_scale into the output.
 //
 // 4-bit pools (kv_fp4.hip) go the same way: a lane loads eight bytes, 16 codes, and the byte of their block's scale, which the
-// conversion to bf16/fp16 applies (exact).  Loads of a quarter of the bytes do not pay here, where the matrix pipes bound the
-// kernel: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 396 us, 391 from an fp8 pool, 370 by DMA
+// conversion to bf16/fp16 applies (exact).  Loads of a quarter of the bytes do not pay here, where matrix, vector and LDS work
+// take turns: 24 rows of up to 700 new tokens behind up to 2,048 (32 heads on 8) take 396 us, 391 from an fp8 pool, 370 by DMA
 // from a 16-bit one.  Without its loads in the loop the 4-bit kernel took 343, with loads but no widening 378: per-lane
 // addresses cost most of the difference (408 with the scale's address made per load, and its pair's products in two parts).
-// P is one 16-bit value in either type, as from the other pools: relative to float64 the output is off by 2.3e-3 in bf16 and
-// 2.9e-4 in fp16, where an output that is rounded alone is off by 1.7e-3 and 2.1e-4; a second part would double the P V products.
+//
+// P is one 16-bit value in either type, from every pool: relative to float64 over the pool's values the output is off by 2.3e-3 in
+// bf16 and 2.9e-4 in fp16, where an output that is rounded alone is off by 1.7e-3 and 2.1e-4.  A second part, for the error of the
+// rounding alone, doubles the P V products: with P kept in fp32 and split under them, 24 such rows from pools of 8-bit blocks took
+// 509-523 us against 403, a mixed step 145 against 128.5.  Those pools' codes, as 4-bit ones, cost 5% of an output and more.
 #include <math.h>
 
 #include <type_traits>
@@ -138,7 +141,9 @@ struct Staged<kPoolFp8Blocks> {
   uint32_t e;  // their page's scale (uniform: a wavefront's rows lie in one page)
 };
 // 24 prompt chunks of up to 700 tokens over up to 2,048, 32 heads on 8, take 408 us from 8-bit blocks, 401 from an fp8 pool and 369
-// from a 16-bit one with the same values: the way through registers.  The codes by DMA into LDS and widened from there took 0.5%
+// from a 16-bit one with the same values in one run (398-418 from 8-bit blocks from card to card): the way through registers, whose
+// widening and LDS stores come behind a phase's other work.  No pipe is near its limit: matrix 34%, vector 39%, LDS 28% of the
+// cycles; all-zero operands, which draw less power, take 3% less.  The codes by DMA into LDS and widened from there took 0.5%
 // less for a ring more; the full operand ring spilled and gave 0.3%.
 
 // fp8 and 4-bit pools: this wavefront's share of a tile (rows 8 w .. 8 w + 7) is one load of 16 values per

@@ -39,10 +39,10 @@ class RMSNorm(nn.Module):
 
 
 class RotaryEmbedding(nn.Module):
-    _factor = None  # see __init__
-
     """The frequency table is derived from the config and kept in float32 on every device it is used on
     (not a module buffer, so casting the model to bf16 never rounds it)."""
+
+    _factor = None  # see __init__
 
     def __init__(self, config: LlamaConfig) -> None:
         super().__init__()
