@@ -47,7 +47,7 @@ def for_inference(name: str, *operands: torch.Tensor) -> None:
         return
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in operands):
         raise RuntimeError(f"{name} is for inference: it has no forward-mode derivative (call it on primals, or the modules)")
-    if torch.jit.is_tracing() or _transform() is not None or any(map(_wrapped, operands)):
+    if torch.jit.is_tracing() or _transform() is not None:  # (a wrapper that outlived its transform has no data pointer to give)
         raise RuntimeError(f"{name} is for inference: it cannot be traced or transformed (call the modules)")
 
 
