@@ -105,6 +105,8 @@ class BlockManager:
         (PagedKVCache.copy_blocks) before either table grows."""
         full = int(num_tokens) // self.block_size
         used = self.blocks_for(num_tokens)
+        if full < 0:
+            raise ValueError(f"a table of {num_tokens} tokens")
         if used > len(table):
             raise ValueError(f"a table of {len(table)} blocks does not hold {num_tokens} tokens")
         fresh = self.allocate(max(used, self.blocks_for(reserve_tokens)) - full)  # first: it raises where none are left
@@ -118,6 +120,8 @@ class BlockManager:
         it loses its name, and ValueError if another table lists it too (`fork` then gives a table with a copy of it).  It keeps
         the scales of a pool that has them (include/minillm_hip.h)."""
         keep = self.blocks_for(num_tokens)
+        if num_tokens < 0:
+            raise ValueError(f"a table of {num_tokens} tokens")
         if keep <= len(table) and int(num_tokens) % self.block_size:
             cut = table[keep - 1]
             if self._holders[cut] > 1:

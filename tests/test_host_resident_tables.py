@@ -129,3 +129,14 @@ def test_a_block_that_is_cut_loses_its_name():
     blocks.trim(table, 16)
     assert prefix.lookup([b"0"]) == table
     blocks.check([table])
+
+
+def test_fewer_than_no_tokens():
+    blocks = BlockManager(6, 16)
+    table = blocks.allocate(3)
+    for n in (-1, -16, -40):
+        for call in (lambda: blocks.fork(table, n), lambda: blocks.trim(table, n)):
+            with pytest.raises(ValueError, match="tokens"):
+                call()
+    assert len(table) == 3 and blocks.num_free == 3
+    blocks.check([table])
