@@ -196,7 +196,9 @@ class DeviceBlockTables:
             sent = prev[1] if prev is not None and prev[0] is ids else []
             start = len(sent)
             if start and prev[2] != cuts or start > len(ids):
-                start = next((j for j, (a, b) in enumerate(zip(sent, ids)) if a != b), min(start, len(ids)))
+                start = min(start, len(ids))
+                if sent[:start] != ids[:start]:
+                    start = next(j for j, (a, b) in enumerate(zip(sent, ids)) if a != b)
                 del sent[start:]
             base = row * self.max_blocks
             if start < len(ids):
